@@ -763,6 +763,94 @@ int lng_drafter_tree_levels(const lng_drafter* D, const int32_t* parent, const i
 int lng_tree_accept(const int32_t* parent, const int64_t* node_tokens, const int64_t* argmax, int32_t n,
                     int32_t* path, int32_t* path_len, int64_t* new_tokens, void* stream);
 
+/* ---------------------------------------------------------------- normalisation, short conv, selective scan */
+/* Layer norm over the last dimension (nn.LayerNorm, the LayerNorm choice of build_lngram_norm,
+ * ffnmem/memory/lngram_v2.py:56-71): y[row] = (x - mean) / sqrt(var + eps) * w + b, var the mean square of
+ * the centred row.  x: `rows` rows of d elements (fp32, bf16 or fp16), x_stride elements apart; y is
+ * contiguous.  w, b [d] in the rows' type or fp32, each may be null (1 and 0).  mean, rstd [rows] fp32, or
+ * both null.  Statistics in fp32, one rounding. */
+int lng_layer_norm(const void* x, int dtype, int64_t rows, int64_t d, int64_t x_stride, const void* w, const void* b,
+                   int w_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
+/* Its backward pass from the rows and the statistics of the forward call: dx [rows, d] contiguous, dw and
+ * db [d] in w_dtype, each may be null (not wanted).  dw and db need the workspace (16-byte aligned); their
+ * sums run in a fixed order, so equal calls give equal bits. */
+size_t lng_layer_norm_grad_workspace_bytes(int64_t rows, int64_t d);
+int lng_layer_norm_grad(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype, int64_t rows,
+                        int64_t d, const void* w, int w_dtype, const float* mean, const float* rstd, void* workspace,
+                        size_t workspace_bytes, void* dx, void* dw, void* db, void* stream);
+
+/* Depthwise causal convolution of 1 to 8 taps: pre[t, c] = bias[c] + sum_j w[c, j] ext[t + j dilation, c],
+ * ext the (K - 1) * dilation rows of hist (zeros where null) and then the sequence; y = silu(pre) (silu 1)
+ * or pre (0).  The conv of DepthwiseCausalConv.forward / forward_incremental
+ * (ffnmem/memory/lngram_v2.py:273-311) on rows that are normalised already, with a bias.
+ * x [B, T, C] (fp32, bf16 or fp16) with batch and token strides in elements, channels contiguous; w [C, K]
+ * and bias [C] in the rows' type or fp32; hist and hist_out [B, (K-1)*dilation, C] in the rows' type, may be
+ * null, and are not the same buffer; y [B, T, C] contiguous.  lengths [B] int32 or null: a sequence's own
+ * tokens; what stands behind them is not read and y is zero there; hist_out follows the last own token. */
+int lng_short_conv(const void* x, int dtype, int64_t B, int64_t T, int32_t C, int64_t x_batch_stride, int64_t x_stride,
+                   const void* w, const void* bias, int w_dtype, int32_t K, int32_t dilation, int silu,
+                   const void* hist, const int32_t* lengths, void* y, void* hist_out, void* stream);
+/* Its backward pass: dx [B, T, C], dhist (the gradient of hist; dhist_out: the gradient of hist_out or
+ * null), dw [C, K], dbias [C], each null where not wanted.  dw and dbias need the workspace; equal calls
+ * give equal bits. */
+size_t lng_short_conv_grad_workspace_bytes(int64_t B, int64_t T, int32_t C, int32_t K, int32_t dilation);
+int lng_short_conv_grad(const void* dy, int64_t dy_batch_stride, int64_t dy_stride, const void* x,
+                        int64_t x_batch_stride, int64_t x_stride, int dtype, int64_t B, int64_t T, int32_t C,
+                        const void* w, const void* bias, int w_dtype, int32_t K, int32_t dilation, int silu,
+                        const void* hist, const int32_t* lengths, const void* dhist_out, void* workspace,
+                        size_t workspace_bytes, void* dx, void* dw, void* dbias, void* dhist, void* stream);
+/* The same for one new token x [B, C] (rows x_stride elements apart) of every sequence; hist_out may be
+ * hist (the history moves on in place). */
+int lng_short_conv_step(const void* x, int dtype, int64_t B, int32_t C, int64_t x_stride, const void* w,
+                        const void* bias, int w_dtype, int32_t K, int32_t dilation, int silu, const void* hist,
+                        void* hist_out, void* y, void* stream);
+
+/* Selective state space scan, N states a channel (the recurrence of ffnmem/memory/ssm.py:58-91 with step
+ * sizes, inputs and outputs per token):
+ *   s = softplus(dt + dt_bias) (softplus 1) or dt + dt_bias (0)
+ *   h[t, c, n] = exp(s A[c, n]) h[t-1, c, n] + s u[t, c] B[t, g, n],   g = c / (C / G)
+ *   y[t, c] = (sum_n C[t, g, n] h[t, c, n] + D[c] u[t, c]) * silu(z[t, c])
+ * u, dt, z [B, T, C] and B, C [B, T, G, N] in `dtype` (fp32, bf16 or fp16), innermost dimension contiguous,
+ * the other strides in elements; y contiguous.  A [C, N], D [C], dt_bias [C], states [B, C, N]: fp32,
+ * contiguous.  z, D, dt_bias, state (zeros), state_out, lengths may be null.  lengths [B] int32: a
+ * sequence's own tokens; what stands behind them is not read, y is zero there and state_out is the state
+ * after the last own one.  1 to 256 states.  States and sums are fp32. */
+typedef struct lng_selective {
+  int64_t B, T;
+  int32_t C, N, G, dtype, softplus, reserved;
+  const void *u, *dt, *z, *Bm, *Cm;
+  int64_t u_batch, u_token, dt_batch, dt_token, z_batch, z_token;
+  int64_t B_batch, B_token, B_group, C_batch, C_token, C_group;
+  const float *A, *D, *dt_bias, *state;
+  const int32_t* lengths;
+  void* y;
+  float* state_out;
+  float* checkpoints;           /* lng_selective_checkpoints() floats for the backward pass, or null */
+  const float* checkpoints_in;  /* lng_selective_scan_grad: what the forward call left in `checkpoints` */
+} lng_selective;
+/* Gradients: dy [B, T, C] (strided) and dstate_out [B, C, N] or null in; du, ddt, dz [B, T, C], dB and dC
+ * [B, T, G, N] contiguous in the tensors' type, dA [C, N], dD, ddt_bias [C], dstate [B, C, N] fp32 (these
+ * four may be null) out. */
+typedef struct lng_selective_grad {
+  const void* dy;
+  int64_t dy_batch, dy_token;
+  const float* dstate_out;
+  void *du, *ddt, *dz, *dB, *dC;
+  float *dA, *dD, *ddt_bias, *dstate;
+} lng_selective_grad;
+size_t lng_selective_size(void);      /* sizeof(lng_selective) */
+size_t lng_selective_grad_size(void); /* sizeof(lng_selective_grad) */
+size_t lng_selective_workspace_bytes(int64_t B, int64_t T, int32_t C, int32_t N, int32_t G, int grad);
+int64_t lng_selective_checkpoints(int64_t B, int64_t T, int32_t C, int32_t N);
+/* Prompts and training.  workspace: lng_selective_workspace_bytes(.., grad 0 / 1), 64-byte aligned, its
+ * contents need not outlive the call.  Equal calls give equal bits. */
+int lng_selective_scan(const lng_selective* args, void* workspace, size_t workspace_bytes, void* stream);
+int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad* grads, void* workspace,
+                            size_t workspace_bytes, void* stream);
+/* One new token of every sequence (T = 1; the token strides and lengths are not read): state_out may be
+ * state. */
+int lng_selective_step(const lng_selective* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

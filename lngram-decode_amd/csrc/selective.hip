@@ -1,0 +1,775 @@
+// Selective state space scan: the diagonal recurrence of DiagonalSSM (ffnmem/memory/ssm.py:22-91) with N
+// states a channel and with step sizes, inputs and outputs that the token chooses, its backward pass, and
+// its step for one new token of every sequence.
+//
+//   s[t, c] = softplus(dt[t, c] + dt_bias[c])  (or dt + dt_bias)
+//   h[t, c, n] = exp(s[t, c] A[c, n]) h[t-1, c, n] + s[t, c] u[t, c] B[t, g, n]      (g: the channel's group)
+//   y[t, c] = (sum_n C[t, g, n] h[t, c, n] + D[c] u[t, c]) * silu(z[t, c])
+//
+// Backward, with e = dy silu(z) and q the gradient of h (q[t] = e[t] C[t] + exp(s[t+1] A) q[t+1]):
+//   dC[t, n] = sum_c e h,  dB[t, n] = sum_c q s u,  du = s sum_n q B + e D,
+//   ds = u sum_n q B + sum_n q exp(s A) h[t-1] A,  dA = sum_t q exp(s A) h[t-1] s,  d dt = ds softplus'(dt)
+//
+// Bound by the vector ALU: an exponential and some five multiply-adds for every (token, channel, state), on
+// 8 bytes a (token, channel).  A lane holds one channel, so u, dt, z and y move as whole rows, and what all
+// of a wave's channels share (B and C of a token) comes through the scalar unit: k_sel_tiles lays B and C
+// out as fp32 tiles of SEG tokens per state, and a tile's row of 2 * SEG values is one scalar load for
+// 64 * SEG state updates.  A segment of SEG tokens stays in registers (step sizes, inputs, outputs) while
+// the loop runs over the states, whose values rest in LDS in between, so every N runs in the same registers.
+// All sums and states are fp32.
+//
+// Where batch * channels gives too few waves, the time axis is cut into chunks: the chunks' own end states
+// (from zero) and total step sizes, then their start states from one short pass over the chunks, then every
+// chunk from its start.  The backward pass does the same for q, backwards, and takes the states of a
+// segment's start from the forward pass (N / SEG floats a (token, channel)).
+#include "common.h"
+
+namespace lng {
+namespace {
+
+constexpr int SEG = 16;   // tokens of a segment
+constexpr int WAVES = 4;  // waves of a block: neighbouring channels of one chunk
+constexpr int MAX_N = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+
+typedef const float __attribute__((address_space(4))) cfloat;  // read through the scalar unit where uniform
+
+struct Dims {
+  int64_t B, T, chunk, segs;  // chunk: tokens of a chunk, a multiple of SEG; segs: segments of a sequence
+  int C, N, G, chunks, cbg;   // cbg: channel blocks of 64 in a group
+  int softplus;
+};
+
+struct Ptrs {
+  const void *u, *dt, *z, *Bm, *Cm, *dy;
+  int64_t ub, ut, dtb, dtt, zb, zt, Bb, Bt, Bg, Cb, Ct, Cg, dyb, dyt;
+  const float *A, *D, *bias, *start, *dend;
+  const int32_t* lengths;
+  void* y;
+  float *end, *ckpt;
+  const float* ckpt_in;
+  // workspace
+  float *tiles, *at, *hloc, *ssum, *pA, *pD, *pBC;
+  void *du, *ddt, *dz;
+  float* dstart;
+};
+
+// log(1 + exp(x)) with log1p by 2 atanh(e / (2 + e)): exact to about an ulp over the whole range, which
+// log(1 + e) is not for the small steps that training starts from.
+__device__ __forceinline__ float softplus(float x) {
+  const float e = expf(-fabsf(x)), s = e / (2.f + e), q = s * s;
+  float p = 1.f / 17.f;
+  p = fmaf(p, q, 1.f / 15.f);
+  p = fmaf(p, q, 1.f / 13.f);
+  p = fmaf(p, q, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  return fmaxf(x, 0.f) + 2.f * s * p;
+}
+__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+
+__device__ __forceinline__ int64_t seq_len(const int32_t* lengths, int64_t b, int64_t T) {
+  if (!lengths) return T;
+  const int64_t n = lengths[b];
+  return n < 0 ? 0 : n > T ? T : n;
+}
+
+// B and C as fp32 tiles [b][g][seg][n][B: SEG, C: SEG] (zeros behind a sequence), and A transposed [N][C].
+template <typename T>
+__global__ __launch_bounds__(256) void k_sel_tiles(Dims d, Ptrs p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t n_tiles = d.B * d.G * d.segs * SEG * d.N;
+  if (i < n_tiles) {
+    const int n = static_cast<int>(i % d.N), k = static_cast<int>(i / d.N % SEG);
+    const int64_t seg = i / d.N / SEG % d.segs, bg = i / d.N / SEG / d.segs, g = bg % d.G, b = bg / d.G;
+    const int64_t t = seg * SEG + k;
+    float bv = 0.f, cv = 0.f;
+    if (t < seq_len(p.lengths, b, d.T)) {
+      bv = to_f32(static_cast<const T*>(p.Bm)[b * p.Bb + t * p.Bt + g * p.Bg + n]);
+      cv = to_f32(static_cast<const T*>(p.Cm)[b * p.Cb + t * p.Ct + g * p.Cg + n]);
+    }
+    float* const o = p.tiles + ((bg * d.segs + seg) * d.N + n) * 2 * SEG + k;
+    o[0] = bv;
+    o[SEG] = cv;
+  } else if (i - n_tiles < static_cast<int64_t>(d.C) * d.N) {
+    const int64_t j = i - n_tiles, c = j % d.C, n = j / d.C;
+    p.at[j] = p.A[c * d.N + n];
+  }
+}
+
+// A wave's share of a launch: 64 channels of one group, one sequence, one chunk.
+struct Unit {
+  int64_t b, bg, t0, t1, end, u;  // tokens [t0, t1) of the chunk; end: the sequence's length
+  int g, c, lane, wave, chunk;
+  bool ok;   // this lane has a channel
+  bool any;  // the wave has one
+  __device__ __forceinline__ Unit(const Dims& d, const int32_t* lengths) {
+    // blocks: channel block groups fastest, then chunks, then sequences
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6, bpg = (d.cbg + waves - 1) / waves;  // blocks of a group's channels
+    const int64_t per = static_cast<int64_t>(bpg) * d.G;
+    const int64_t x = blockIdx.x, cb = x % per, bs = x / per;
+    g = static_cast<int>(cb / bpg);
+    chunk = static_cast<int>(bs % d.chunks);
+    b = bs / d.chunks;
+    bg = b * d.G + g;
+    u = b * d.chunks + chunk;
+    const int cg = d.C / d.G, in = (static_cast<int>(cb % bpg) * waves + wave) * 64;
+    any = in < cg;
+    ok = in + lane < cg;
+    c = g * cg + (ok ? in + lane : cg - 1);
+    t0 = chunk * d.chunk;
+    t1 = t0 + d.chunk < d.T ? t0 + d.chunk : d.T;
+    end = seq_len(lengths, b, d.T);
+  }
+};
+
+// A segment's values of one tensor in fp32; zeros at and behind `end`.
+template <typename T>
+__device__ __forceinline__ void load_seg(const void* base, int64_t row, int64_t stride, int64_t t, int64_t end, int c,
+                                         float (&v)[SEG]) {
+  const T* const p = static_cast<const T*>(base) + row + c;
+#pragma unroll
+  for (int i = 0; i < SEG; ++i) v[i] = t + i < end ? to_f32(p[(t + i) * stride]) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_steps(const Dims& d, const Ptrs& p, int64_t b, int64_t t, int64_t end, int c,
+                                           float bias, float (&s)[SEG]) {
+  load_seg<T>(p.dt, b * p.dtb, p.dtt, t, end, c, s);
+#pragma unroll
+  for (int i = 0; i < SEG; ++i) {
+    const float x = s[i] + bias;
+    s[i] = t + i < end ? (d.softplus ? softplus(x) : x) : 0.f;  // no time passes behind a sequence's end
+  }
+}
+
+struct Row {  // B and C of one state over a segment's tokens
+  float B[SEG], C[SEG];
+};
+__device__ __forceinline__ Row load_row(const float* tiles, int64_t at) {
+  cfloat* const q = (cfloat*)(uintptr_t)(tiles + at);
+  Row r;
+#pragma unroll
+  for (int i = 0; i < SEG; ++i) r.B[i] = q[i], r.C[i] = q[SEG + i];
+  return r;
+}
+
+// AGG: the chunk's end state from zero and its total step size.  Else: y, the final state (its last chunk)
+// and, where wanted, the states at every segment's start.
+template <typename T, bool AGG>
+__global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
+  extern __shared__ float lds[];
+  const Unit w(d, p.lengths);
+  if (!w.any || (AGG && w.chunk == d.chunks - 1)) return;
+  float* const hs = lds + w.wave * 2 * d.N * 64 + w.lane;  // states and decay exponents [N][64]
+  float* const as = hs + d.N * 64;
+  for (int n = 0; n < d.N; ++n) {
+    const int64_t at = static_cast<int64_t>(n) * d.C + w.c;
+    as[n * 64] = p.at[at] * LOG2E;
+    float h = 0.f;
+    if (!AGG) {
+      if (d.chunks > 1)
+        h = p.hloc[w.u * d.N * d.C + at];
+      else if (p.start)
+        h = p.start[(w.b * d.C + w.c) * d.N + n];
+    }
+    hs[n * 64] = h;
+  }
+  const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = !AGG && p.D ? p.D[w.c] : 0.f;
+  float total = 0.f;
+  for (int64_t t = w.t0; t < w.t1; t += SEG) {
+    if (t >= w.end) {  // behind the sequence: zeros, and the states stay
+      if constexpr (!AGG) {
+        if (w.ok)
+          for (int i = 0; i < SEG && t + i < w.t1; ++i)
+            static_cast<T*>(p.y)[(w.b * d.T + t + i) * d.C + w.c] = from_f32<T>(0.f);
+        continue;
+      } else {
+        break;
+      }
+    }
+    float s[SEG], x[SEG], y[SEG];
+    load_seg<T>(p.u, w.b * p.ub, p.ut, t, w.end, w.c, x);
+    load_steps<T>(d, p, w.b, t, w.end, w.c, bias, s);
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) {
+      if constexpr (AGG) total += s[i];
+      y[i] = dskip * x[i];
+      x[i] *= s[i];
+    }
+    const int64_t seg = t / SEG, tile = (w.bg * d.segs + seg) * d.N * 2 * SEG;
+    for (int n = 0; n < d.N; ++n) {
+      const Row r = load_row(p.tiles, tile + n * 2 * SEG);
+      float h = hs[n * 64];
+      const float a = as[n * 64];
+      if (!AGG && p.ckpt && w.ok) p.ckpt[((w.b * d.segs + seg) * d.N + n) * d.C + w.c] = h;
+#pragma unroll
+      for (int i = 0; i < SEG; ++i) {
+        h = fmaf(__builtin_amdgcn_exp2f(s[i] * a), h, x[i] * r.B[i]);
+        if constexpr (!AGG) y[i] = fmaf(r.C[i], h, y[i]);
+      }
+      hs[n * 64] = h;
+    }
+    if constexpr (!AGG) {
+      if (p.z) {
+        float z[SEG];
+        load_seg<T>(p.z, w.b * p.zb, p.zt, t, w.end, w.c, z);
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) y[i] *= z[i] * sigmoid(z[i]);
+      }
+      if (w.ok) {
+        T* const out = static_cast<T*>(p.y) + (w.b * d.T + t) * d.C + w.c;
+#pragma unroll
+        for (int i = 0; i < SEG; ++i)
+          if (t + i < w.t1) out[static_cast<int64_t>(i) * d.C] = from_f32<T>(t + i < w.end ? y[i] : 0.f);
+      }
+    }
+  }
+  if (!w.ok) return;
+  if constexpr (AGG) {
+    for (int n = 0; n < d.N; ++n) p.hloc[(w.u * d.N + n) * d.C + w.c] = hs[n * 64];
+    p.ssum[w.u * d.C + w.c] = total;
+  } else if (p.end && w.chunk == d.chunks - 1) {
+    for (int n = 0; n < d.N; ++n) p.end[(w.b * d.C + w.c) * d.N + n] = hs[n * 64];
+  }
+}
+
+// The chunks' start values from their own ends, in place: hloc[b, chunk, n, c] <- the value that enters the
+// chunk.  Forward: from the first chunk on, starting with the given state.  BACK: the gradient that enters
+// a chunk from behind, from the last chunk on, starting with the final state's gradient.
+template <bool BACK>
+__global__ __launch_bounds__(256) void k_sel_join(Dims d, Ptrs p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= d.B * d.N * d.C) return;
+  const int64_t c = i % d.C, n = i / d.C % d.N, b = i / d.C / d.N;
+  const float a = p.at[n * d.C + c] * LOG2E;
+  const float* const first = BACK ? p.dend : p.start;
+  float h = first ? first[(b * d.C + c) * d.N + n] : 0.f;
+  for (int k = 0; k < d.chunks; ++k) {
+    const int64_t u = b * d.chunks + (BACK ? d.chunks - 1 - k : k);
+    float* const at = p.hloc + (u * d.N + n) * d.C + c;
+    const bool last = k == d.chunks - 1;
+    const float own = last ? 0.f : *at, decay = last ? 0.f : __builtin_amdgcn_exp2f(p.ssum[u * d.C + c] * a);
+    *at = h;
+    h = fmaf(decay, h, own);
+  }
+}
+
+// A segment's e = dy silu(z).
+template <typename T>
+__device__ __forceinline__ void load_gated(const Ptrs& p, int64_t b, int64_t t, int64_t end, int c, float (&e)[SEG]) {
+  load_seg<T>(p.dy, b * p.dyb, p.dyt, t, end, c, e);
+  if (p.z) {
+    float z[SEG];
+    load_seg<T>(p.z, b * p.zb, p.zt, t, end, c, z);
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) e[i] *= z[i] * sigmoid(z[i]);
+  }
+}
+
+// A chunk's own gradient of the state in front of it (nothing from behind) and its total step size.
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
+  extern __shared__ float lds[];
+  const Unit w(d, p.lengths);
+  if (!w.any || w.chunk == 0) return;
+  float* const qs = lds + w.wave * 2 * d.N * 64 + w.lane;
+  float* const as = qs + d.N * 64;
+  for (int n = 0; n < d.N; ++n) qs[n * 64] = 0.f, as[n * 64] = p.at[static_cast<int64_t>(n) * d.C + w.c] * LOG2E;
+  const float bias = p.bias ? p.bias[w.c] : 0.f;
+  float total = 0.f;
+  const int64_t stop = w.t1 < w.end ? w.t1 : w.end;
+  for (int64_t t = (stop - 1) / SEG * SEG; stop > w.t0 && t >= w.t0; t -= SEG) {
+    float s[SEG], e[SEG];
+    load_gated<T>(p, w.b, t, w.end, w.c, e);
+    load_steps<T>(d, p, w.b, t, w.end, w.c, bias, s);
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) total += s[i];
+    const int64_t tile = (w.bg * d.segs + t / SEG) * d.N * 2 * SEG;
+    for (int n = 0; n < d.N; ++n) {
+      const Row r = load_row(p.tiles, tile + n * 2 * SEG);
+      float q = qs[n * 64];
+      const float a = as[n * 64];
+#pragma unroll
+      for (int i = SEG - 1; i >= 0; --i) q = fmaf(e[i], r.C[i], q) * __builtin_amdgcn_exp2f(s[i] * a);
+      qs[n * 64] = q;
+    }
+  }
+  if (!w.ok) return;
+  for (int n = 0; n < d.N; ++n) p.hloc[(w.u * d.N + n) * d.C + w.c] = qs[n * 64];
+  p.ssum[w.u * d.C + w.c] = total;
+}
+
+// The sum over the wave's 64 lanes of each of 32 values, in 70 operations instead of 32 * 7: every round
+// halves the values that a lane carries by handing the other half to its partner.  Lane l receives the sum
+// of value l / 2.
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ float swap_add(bool high, float a, float b) {  // low lanes keep a's sum, high lanes b's
+  const float keep = high ? b : a, give = high ? a : b;
+  return keep + dpp_move<CTRL>(give);
+}
+// The two halves of a swap's result, added.  (Through integers of their own: a bit cast of a vector's element
+// takes the vector's first one.)
+__device__ __forceinline__ float sum_of(unsigned a, unsigned b) {
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[i]),
+                                                    __builtin_bit_cast(unsigned, v[i + 16]), false, false);
+    v[i] = sum_of(r[0], r[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v[i]),
+                                                    __builtin_bit_cast(unsigned, v[i + 8]), false, false);
+    v[i] = sum_of(r[0], r[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = swap_add<0x128>(lane & 8, v[i], v[i + 4]);  // row_ror:8
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = swap_add<0x141>(lane & 4, v[i], v[i + 2]);  // row_half_mirror
+  v[0] = swap_add<0x4E>(lane & 2, v[0], v[1]);                                   // quad_perm 2 3 0 1
+  return v[0] + dpp_move<0xB1>(v[0]);                                            // quad_perm 1 0 3 2
+}
+
+// The backward pass of one chunk, segment by segment from its end.  pBC[cb][b][g][t][2][N] receives the
+// block's share of dB and dC (its channels' sum), pA[unit][n][c] and pD[unit][2][c] the chunk's share of dA,
+// dD and d dt_bias.
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
+  extern __shared__ float lds[];
+  const Unit w(d, p.lengths);
+  const int waves = blockDim.x >> 6, N = d.N;
+  float* const qs = lds + w.wave * 2 * N * 64 + w.lane;  // gradients from behind and dA [N][64]
+  float* const ga = qs + N * 64;
+  float* const sums = lds + waves * 2 * N * 64;          // [wave][n][B: SEG, C: SEG]
+  const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = p.D ? p.D[w.c] : 0.f;
+  float dD = 0.f, dbias = 0.f;
+  for (int n = 0; n < N; ++n) {
+    const int64_t at = static_cast<int64_t>(n) * d.C + w.c;
+    float q = 0.f;
+    if (d.chunks > 1)
+      q = p.hloc[w.u * N * d.C + at];
+    else if (p.dend)
+      q = p.dend[(w.b * d.C + w.c) * N + n];
+    qs[n * 64] = w.ok ? q : 0.f;
+    ga[n * 64] = 0.f;
+  }
+  const int bpg = (d.cbg + waves - 1) / waves;
+  const int64_t cb = blockIdx.x % bpg;  // this block's place among those of its group
+  for (int64_t t = (w.t1 - 1) / SEG * SEG; t >= w.t0; t -= SEG) {
+    const int64_t seg = t / SEG;
+    const int live = static_cast<int>(w.t1 - t < SEG ? w.t1 - t : SEG);  // tokens that the tensors have
+    if (t < w.end) {
+      if (w.any) {
+        float u[SEG], s[SEG], e[SEG], y[SEG], gb[SEG], gs[SEG];
+        load_seg<T>(p.u, w.b * p.ub, p.ut, t, w.end, w.c, u);
+        load_steps<T>(d, p, w.b, t, w.end, w.c, bias, s);
+        load_gated<T>(p, w.b, t, w.end, w.c, e);
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) {
+          e[i] = w.ok ? e[i] : 0.f;  // lanes without a channel add nothing to the sums over channels
+          y[i] = gb[i] = gs[i] = 0.f;
+        }
+        const int64_t tile = (w.bg * d.segs + seg) * N * 2 * SEG;
+        const float* const ck = p.ckpt_in + (w.b * d.segs + seg) * N * d.C + w.c;
+        for (int n = 0; n < N; ++n) {
+          const Row r = load_row(p.tiles, tile + n * 2 * SEG);
+          const float an = p.at[static_cast<int64_t>(n) * d.C + w.c], a2 = an * LOG2E;
+          const float h0 = ck[static_cast<int64_t>(n) * d.C];
+          float a[SEG], h[SEG], v[2 * SEG];
+#pragma unroll
+          for (int i = 0; i < SEG; ++i) {
+            a[i] = __builtin_amdgcn_exp2f(s[i] * a2);
+            h[i] = fmaf(a[i], i ? h[i - 1] : h0, s[i] * u[i] * r.B[i]);
+            y[i] = fmaf(r.C[i], h[i], y[i]);
+            v[SEG + i] = e[i] * h[i];
+          }
+          float q = qs[n * 64], dA = ga[n * 64];
+#pragma unroll
+          for (int i = SEG - 1; i >= 0; --i) {
+            q = fmaf(e[i], r.C[i], q);
+            v[i] = q * (s[i] * u[i]);
+            gb[i] = fmaf(q, r.B[i], gb[i]);
+            q *= a[i];
+            const float through = q * (i ? h[i - 1] : h0);
+            gs[i] = fmaf(through, an, gs[i]);
+            dA = fmaf(through, s[i], dA);
+          }
+          qs[n * 64] = q;
+          ga[n * 64] = dA;
+          const float total = lane_sums(v, w.lane);
+          if ((w.lane & 1) == 0) sums[(w.wave * N + n) * 2 * SEG + (w.lane >> 1)] = total;
+        }
+        // what needs dy, z and dt once more reads them again (from the caches)
+        float raw[SEG], dy[SEG], z[SEG];
+        load_seg<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, w.c, raw);
+        load_seg<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, w.c, dy);
+        if (p.z) load_seg<T>(p.z, w.b * p.zb, p.zt, t, w.end, w.c, z);
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) {
+          const bool in = t + i < w.end;
+          const float du = fmaf(gb[i], s[i], e[i] * dskip);
+          float ds = fmaf(gb[i], u[i], gs[i]);
+          if (d.softplus) ds *= sigmoid(raw[i] + bias);
+          dD += e[i] * u[i];
+          dbias += in ? ds : 0.f;
+          if (i < live && w.ok) {
+            const int64_t at = (w.b * d.T + t + i) * d.C + w.c;
+            static_cast<T*>(p.du)[at] = from_f32<T>(in ? du : 0.f);
+            static_cast<T*>(p.ddt)[at] = from_f32<T>(in ? ds : 0.f);
+            if (p.z) {
+              const float sg = sigmoid(z[i]), yv = fmaf(dskip, u[i], y[i]);
+              static_cast<T*>(p.dz)[at] = from_f32<T>(in ? dy[i] * yv * sg * (1.f + z[i] * (1.f - sg)) : 0.f);
+            }
+          }
+        }
+      } else {
+        for (int i = w.lane; i < N * 2 * SEG; i += 64) sums[w.wave * N * 2 * SEG + i] = 0.f;
+      }
+    } else if (w.ok) {
+      for (int i = 0; i < live; ++i) {
+        const int64_t at = (w.b * d.T + t + i) * d.C + w.c;
+        static_cast<T*>(p.du)[at] = from_f32<T>(0.f);
+        static_cast<T*>(p.ddt)[at] = from_f32<T>(0.f);
+        if (p.z) static_cast<T*>(p.dz)[at] = from_f32<T>(0.f);
+      }
+    }
+    __syncthreads();
+    float* const out = p.pBC + (cb * d.B * d.G + w.bg) * d.T * 2 * N + t * 2 * N;
+    for (int j = threadIdx.x; j < live * 2 * N; j += blockDim.x) {
+      const int n = j % N, which = j / N & 1, i = j / N / 2;
+      float v = 0.f;
+      if (t + i < w.end)
+        for (int k = 0; k < waves; ++k) v += sums[(k * N + n) * 2 * SEG + which * SEG + i];
+      out[j] = v;
+    }
+    __syncthreads();
+  }
+  if (!w.ok) return;
+  for (int n = 0; n < N; ++n) {
+    p.pA[(w.u * N + n) * d.C + w.c] = ga[n * 64];
+    if (p.dstart && w.chunk == 0) p.dstart[(w.b * d.C + w.c) * N + n] = qs[n * 64];
+  }
+  p.pD[w.u * 2 * d.C + w.c] = dD;
+  p.pD[(w.u * 2 + 1) * d.C + w.c] = dbias;
+}
+
+// dB, dC [B, T, G, N] from the channel blocks' shares.
+template <typename T>
+__global__ __launch_bounds__(256) void k_sel_grad_bc(Dims d, const float* __restrict__ pBC, int parts,
+                                                     T* __restrict__ dB, T* __restrict__ dC) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t total = d.B * d.G * d.T * 2 * d.N;
+  if (i >= total) return;
+  float v = 0.f;
+  for (int k = 0; k < parts; ++k) v += pBC[k * total + i];
+  const int64_t n = i % d.N, which = i / d.N & 1, t = i / d.N / 2 % d.T, bg = i / d.N / 2 / d.T, g = bg % d.G;
+  (which ? dC : dB)[((bg / d.G * d.T + t) * d.G + g) * d.N + n] = from_f32<T>(v);
+}
+
+// dA [C, N], dD [C] and d dt_bias [C] from the chunks' shares: 64 columns a block, 4 threads a column.
+__global__ __launch_bounds__(256) void k_sel_grad_a(Dims d, const float* __restrict__ pA, const float* __restrict__ pD,
+                                                    float* __restrict__ dA, float* __restrict__ dD,
+                                                    float* __restrict__ dbias) {
+  __shared__ float part[4][64];
+  const int col = threadIdx.x & 63, grp = threadIdx.x >> 6;
+  const int64_t NC = static_cast<int64_t>(d.N) * d.C, m = static_cast<int64_t>(blockIdx.x) * 64 + col;
+  const int64_t units = d.B * d.chunks;
+  float s = 0.f;
+  if (m < NC) {
+#pragma unroll 8
+    for (int64_t k = grp; k < units; k += 4) s += pA[k * NC + m];
+  } else if (m < NC + 2 * d.C) {
+#pragma unroll 8
+    for (int64_t k = grp; k < units; k += 4) s += pD[k * 2 * d.C + m - NC];
+  }
+  part[grp][col] = s;
+  __syncthreads();
+  if (grp || m >= NC + 2 * d.C) return;
+  s = (part[0][col] + part[1][col]) + (part[2][col] + part[3][col]);
+  if (m < NC) {
+    if (dA) dA[m % d.C * d.N + m / d.C] = s;
+  } else if (m < NC + d.C) {
+    if (dD) dD[m - NC] = s;
+  } else if (dbias) {
+    dbias[m - NC - d.C] = s;
+  }
+}
+
+// One new token of every sequence: LPC neighbouring lanes hold a channel, four states (16 bytes) each and a
+// round; the output is summed over the lanes.  `end` may be the state that is read.
+template <typename T, int LPC, bool VEC>
+__global__ __launch_bounds__(256) void k_sel_step(Dims d, Ptrs p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t total = d.B * d.C, j = i / LPC < total ? i / LPC : total - 1;
+  const bool ok = i / LPC < total;
+  const int part = static_cast<int>(i % LPC);
+  const int64_t b = j / d.C;
+  const int c = static_cast<int>(j % d.C), g = c / (d.C / d.G);
+  const float u = to_f32(static_cast<const T*>(p.u)[b * p.ub + c]);
+  float s = to_f32(static_cast<const T*>(p.dt)[b * p.dtb + c]) + (p.bias ? p.bias[c] : 0.f);
+  if (d.softplus) s = softplus(s);
+  const float x = s * u;
+  const float *h = p.start + j * d.N, *A = p.A + static_cast<int64_t>(c) * d.N;
+  float* const out = p.end + j * d.N;
+  const T *Bm = static_cast<const T*>(p.Bm) + b * p.Bb + g * p.Bg, *Cm = static_cast<const T*>(p.Cm) + b * p.Cb + g * p.Cg;
+  float y = 0.f;
+  for (int n0 = part * 4; n0 < d.N; n0 += LPC * 4) {
+    float hv[4], av[4];
+    if constexpr (VEC) {
+      const f32x4 hq = *reinterpret_cast<const f32x4*>(h + n0), aq = *reinterpret_cast<const f32x4*>(A + n0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) hv[k] = hq[k], av[k] = aq[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) hv[k] = n0 + k < d.N ? h[n0 + k] : 0.f, av[k] = n0 + k < d.N ? A[n0 + k] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (VEC || n0 + k < d.N) {
+        hv[k] = fmaf(__builtin_amdgcn_exp2f(s * (av[k] * LOG2E)), hv[k], x * to_f32(Bm[n0 + k]));
+        y = fmaf(to_f32(Cm[n0 + k]), hv[k], y);
+      }
+    }
+    if (!ok) continue;
+    if constexpr (VEC) {
+      f32x4 hq;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) hq[k] = hv[k];
+      *reinterpret_cast<f32x4*>(out + n0) = hq;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n0 + k < d.N) out[n0 + k] = hv[k];
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < LPC; m *= 2) y += __shfl_xor(y, m);
+  if (!ok || part) return;
+  if (p.D) y = fmaf(p.D[c], u, y);
+  if (p.z) {
+    const float z = to_f32(static_cast<const T*>(p.z)[b * p.zb + c]);
+    y *= z * sigmoid(z);
+  }
+  static_cast<T*>(p.y)[j] = from_f32<T>(y);
+}
+
+// ------------------------------------------------------------------ host
+int waves_for(const Dims& d, bool grad) {
+  // a wave's states take 512 N bytes of LDS (the backward pass 128 N more): blocks of two waves past 32
+  // states, of one past 128, leave a CU several blocks
+  const int by_n = d.N <= 32 ? WAVES : d.N <= 128 ? 2 : 1;
+  return std::min(by_n, d.cbg);
+}
+
+Dims make_dims(const lng_selective& a) {
+  Dims d{};
+  d.B = a.B, d.T = a.T, d.C = a.C, d.N = a.N, d.G = a.G, d.softplus = a.softplus;
+  d.cbg = static_cast<int>(cdiv(a.C / a.G, 64));
+  d.segs = cdiv(a.T, SEG);
+  // chunks: two waves for each of the 1024 SIMDs, of at least four segments
+  const int64_t units = a.B * a.G * d.cbg;
+  const int64_t want = std::min(cdiv(2048, std::max<int64_t>(units, 1)), std::max<int64_t>(1, d.segs / 4));
+  d.chunk = std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1))) * SEG;
+  d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
+  return d;
+}
+
+struct Space {  // workspace offsets in floats
+  int64_t tiles, at, hloc, ssum, pA = 0, pD = 0, pBC = 0, total = 0;
+  int64_t take(int64_t n) {
+    const int64_t p = total;
+    total += (n + 63) & ~int64_t{63};
+    return p;
+  }
+  Space(const Dims& d, bool grad) {
+    const int64_t NC = int64_t{d.N} * d.C, units = d.B * d.chunks;
+    tiles = take(d.B * d.G * d.segs * SEG * 2 * d.N);
+    at = take(NC);
+    hloc = take(d.chunks > 1 ? units * NC : 0);
+    ssum = take(d.chunks > 1 ? units * d.C : 0);
+    if (!grad) return;
+    pA = take(units * NC);
+    pD = take(units * 2 * d.C);
+    pBC = take(cdiv(d.cbg, waves_for(d, true)) * d.B * d.G * d.T * 2 * d.N);
+  }
+};
+
+Ptrs make_ptrs(const lng_selective& a) {
+  Ptrs p{};
+  p.u = a.u, p.dt = a.dt, p.z = a.z, p.Bm = a.Bm, p.Cm = a.Cm;
+  p.ub = a.u_batch, p.ut = a.u_token, p.dtb = a.dt_batch, p.dtt = a.dt_token, p.zb = a.z_batch, p.zt = a.z_token;
+  p.Bb = a.B_batch, p.Bt = a.B_token, p.Bg = a.B_group, p.Cb = a.C_batch, p.Ct = a.C_token, p.Cg = a.C_group;
+  p.A = a.A, p.D = a.D, p.bias = a.dt_bias, p.start = a.state, p.lengths = a.lengths;
+  p.y = a.y, p.end = a.state_out, p.ckpt = a.checkpoints;
+  return p;
+}
+
+int check_args(const char* what, const lng_selective* a) {
+  if (!a) return fail(LNG_E_ARG, std::string(what) + ": null arguments");
+  if (a->dtype != LNG_F32 && a->dtype != LNG_BF16 && a->dtype != LNG_F16)
+    return fail(LNG_E_DTYPE, std::string(what) + ": fp32, bf16 or fp16 tensors");
+  if (a->B < 0 || a->T < 0 || a->C <= 0 || a->N <= 0 || a->N > MAX_N || a->G <= 0 || a->C % a->G ||
+      a->C > (1 << 20) || a->T > (int64_t{1} << 31) || a->B > (int64_t{1} << 24) ||
+      a->B * a->T > (int64_t{1} << 38) / a->C / a->N)
+    return fail(LNG_E_ARG, std::string(what) + ": bad shape (1 to 256 states, groups that divide the channels)");
+  const int64_t lanes = cdiv(a->C / a->G, 64) * 64 * a->G, most = int64_t{1} << 38;  // of any launch's threads
+  if (a->B * a->G * (a->T + SEG) > most / 2 / a->N || a->B * lanes * (a->T / 64 + 1) > most ||
+      a->B * a->C > most / SEG || a->B * lanes > most / a->N)
+    return fail(LNG_E_ARG, std::string(what) + ": too many tokens, groups or channels for one call");
+  if (a->B * a->T > 0 && (!a->u || !a->dt || !a->Bm || !a->Cm || !a->A || (!a->y && !a->checkpoints_in)))
+    return fail(LNG_E_ARG, std::string(what) + ": null pointer");
+  return LNG_OK;
+}
+
+void place(Ptrs& p, const Space& s, void* ws) {
+  float* const w = static_cast<float*>(ws);
+  p.tiles = w + s.tiles, p.at = w + s.at, p.hloc = w + s.hloc, p.ssum = w + s.ssum, p.pA = w + s.pA, p.pD = w + s.pD;
+  p.pBC = w + s.pBC;
+}
+
+unsigned grid256(int64_t n) { return static_cast<unsigned>(cdiv(n, 256)); }
+unsigned unit_blocks(const Dims& d, int waves) {
+  return static_cast<unsigned>(cdiv(d.cbg, waves) * d.G * d.chunks * d.B);
+}
+
+template <typename T>
+int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
+  const int waves = waves_for(d, false);
+  const unsigned blocks = unit_blocks(d, waves), lds = waves * 2 * d.N * 64 * 4;
+  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.N + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+  if (d.chunks > 1) {
+    k_sel_scan<T, true><<<blocks, 64 * waves, lds, st>>>(d, p);
+    k_sel_join<false><<<grid256(d.B * d.N * d.C), 256, 0, st>>>(d, p);
+  }
+  k_sel_scan<T, false><<<blocks, 64 * waves, lds, st>>>(d, p);
+  return check_launch("selective_scan");
+}
+
+template <typename T>
+int run_grad(const Dims& d, Ptrs p, const lng_selective_grad& g, hipStream_t st) {
+  const int waves = waves_for(d, true);
+  const unsigned blocks = unit_blocks(d, waves), lds = waves * 2 * d.N * 64 * 4;
+  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.N + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+  if (d.chunks > 1) {
+    k_sel_grad_ends<T><<<blocks, 64 * waves, lds, st>>>(d, p);
+    k_sel_join<true><<<grid256(d.B * d.N * d.C), 256, 0, st>>>(d, p);
+  }
+  k_sel_grad<T><<<blocks, 64 * waves, lds + waves * d.N * 2 * SEG * 4, st>>>(d, p);
+  k_sel_grad_bc<T><<<grid256(d.B * d.G * d.T * 2 * d.N), 256, 0, st>>>(
+      d, p.pBC, static_cast<int>(cdiv(d.cbg, waves)), static_cast<T*>(g.dB), static_cast<T*>(g.dC));
+  k_sel_grad_a<<<static_cast<unsigned>(cdiv(int64_t{d.N + 2} * d.C, 64)), 256, 0, st>>>(d, p.pA, p.pD, g.dA, g.dD,
+                                                                                       g.ddt_bias);
+  return check_launch("selective_scan_grad");
+}
+
+template <typename T>
+int run_step(const Dims& d, const Ptrs& p, hipStream_t st) {
+  const bool vec = d.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.start) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(p.end) % 16 == 0 && reinterpret_cast<uintptr_t>(p.A) % 16 == 0;
+  int lpc = 1;
+  while (lpc < 16 && lpc * 4 < d.N) lpc *= 2;
+  const unsigned blocks = grid256(d.B * d.C * lpc);
+#define LNG_SEL_STEP(L)                                       \
+  if (lpc == L) {                                             \
+    if (vec)                                                  \
+      k_sel_step<T, L, true><<<blocks, 256, 0, st>>>(d, p);   \
+    else                                                      \
+      k_sel_step<T, L, false><<<blocks, 256, 0, st>>>(d, p);  \
+  }
+  LNG_SEL_STEP(1)
+  LNG_SEL_STEP(2)
+  LNG_SEL_STEP(4)
+  LNG_SEL_STEP(8)
+  LNG_SEL_STEP(16)
+#undef LNG_SEL_STEP
+  return check_launch("selective_step");
+}
+
+template <typename F>
+int with_type(int dtype, F f) {
+  if (dtype == LNG_F32) return f(float{});
+  if (dtype == LNG_BF16) return f(bf16{});
+  return f(_Float16{});
+}
+
+}  // namespace
+}  // namespace lng
+
+using namespace lng;
+
+extern "C" {
+
+size_t lng_selective_size(void) { return sizeof(lng_selective); }
+size_t lng_selective_grad_size(void) { return sizeof(lng_selective_grad); }
+
+size_t lng_selective_workspace_bytes(int64_t B, int64_t T, int32_t C, int32_t N, int32_t G, int grad) {
+  lng_selective a{};
+  a.B = B, a.T = T, a.C = C, a.N = N, a.G = G, a.dtype = LNG_F32;
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > MAX_N || G <= 0 || C % G) return 0;
+  return static_cast<size_t>(Space(make_dims(a), grad != 0).total) * 4;
+}
+
+int64_t lng_selective_checkpoints(int64_t B, int64_t T, int32_t C, int32_t N) {
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0) return 0;
+  return B * cdiv(T, SEG) * N * C;
+}
+
+int lng_selective_scan(const lng_selective* args, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_args("selective_scan", args)) return rc;
+  const lng_selective& a = *args;
+  if (a.B == 0 || a.T == 0) return LNG_OK;
+  if (!a.y) return fail(LNG_E_ARG, "selective_scan: null pointer");
+  const Dims d = make_dims(a);
+  const Space s(d, false);
+  if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)
+    return fail(LNG_E_ARG, "selective_scan: the workspace is too small or not 64-byte aligned");
+  Ptrs p = make_ptrs(a);
+  place(p, s, workspace);
+  return with_type(a.dtype, [&](auto t) { return run_scan<decltype(t)>(d, p, as_stream(stream)); });
+}
+
+int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad* grads, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  if (int rc = check_args("selective_scan_grad", args)) return rc;
+  const lng_selective& a = *args;
+  if (!grads) return fail(LNG_E_ARG, "selective_scan_grad: null arguments");
+  const lng_selective_grad& g = *grads;
+  if (a.B == 0 || a.T == 0) return fail(LNG_E_ARG, "selective_scan_grad: no tokens");
+  if (!a.checkpoints_in || !g.dy || !g.du || !g.ddt || !g.dB || !g.dC || (a.z && !g.dz))
+    return fail(LNG_E_ARG, "selective_scan_grad: null pointer");
+  const Dims d = make_dims(a);
+  const Space s(d, true);
+  if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)
+    return fail(LNG_E_ARG, "selective_scan_grad: the workspace is too small or not 64-byte aligned");
+  Ptrs p = make_ptrs(a);
+  place(p, s, workspace);
+  p.ckpt_in = a.checkpoints_in, p.dy = g.dy, p.dyb = g.dy_batch, p.dyt = g.dy_token, p.dend = g.dstate_out;
+  p.du = g.du, p.ddt = g.ddt, p.dz = g.dz, p.dstart = g.dstate;
+  return with_type(a.dtype, [&](auto t) { return run_grad<decltype(t)>(d, p, g, as_stream(stream)); });
+}
+
+int lng_selective_step(const lng_selective* args, void* stream) {
+  if (int rc = check_args("selective_step", args)) return rc;
+  const lng_selective& a = *args;
+  if (a.T != 1) return fail(LNG_E_ARG, "selective_step: one token of every sequence (T = 1)");
+  if (a.B == 0) return LNG_OK;
+  if (!a.state || !a.state_out || !a.y) return fail(LNG_E_ARG, "selective_step: null pointer");
+  const Dims d = make_dims(a);
+  const Ptrs p = make_ptrs(a);
+  return with_type(a.dtype, [&](auto t) { return run_step<decltype(t)>(d, p, as_stream(stream)); });
+}
+
+}  // extern "C"

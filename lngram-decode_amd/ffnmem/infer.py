@@ -102,10 +102,18 @@ def memory_model(mem, tok_emb=None, ssm=None):
 
 
 # ------------------------------------------------------------------ pieces
+def _diagonal(model, what: str):
+    """The model's SSM, whose state is the feature row that ``DecodeState.ssm`` caches."""
+    if not hasattr(model.ssm, "decay"):
+        raise NotImplementedError(f"{what}: the features of a {type(model.ssm).__name__} are not its state; call its "
+                                  "forward or step with the state that it returned")
+    return model.ssm
+
+
 def ssm_continue(model, emb: Tensor, s_prev: Tensor | None) -> Tensor:
     """SSM states of new positions from the state before them (``infer.py:125-137``):
     ``lng_ssm_scan`` with the carried state as ``s0``."""
-    ssm = model.ssm
+    ssm = _diagonal(model, "ssm_continue")
     return ops.ssm_scan(ssm.decay(), ssm.inputs(emb), s_prev)
 
 
@@ -120,6 +128,12 @@ def router_input_at(model, mem, state: DecodeState, emb: Tensor, s_new: Tensor |
     if s_new is not None:
         s_cat = torch.cat((state.ssm[:, L - 1:L], s_new), dim=1)
     return mem.router_features(torch.cat((prev, emb), dim=1), s_cat)[:, 1:]
+
+
+def _need_one_kernel_conv(m, what: str) -> None:
+    if not m.short_conv.one_kernel:
+        raise NotImplementedError(f"{what}: a short conv with LayerNorm or a bias runs at lengths that the host knows "
+                                  "(memory_step), not from a device length or over a tree's windows")
 
 
 def _readout_head(m, h: Tensor, codes: Tensor, pos0: int, pos0_dev: Tensor | None, q_raw: Tensor | None = None) -> Tensor:
@@ -146,8 +160,6 @@ def _oproj_to_cache(m, head: Tensor, conv_in: Tensor, L: int, n: int, L_dev: Ten
     x = head.reshape(b, n, m.readout_inner_dim)
     w_o = m.readout_o_proj.weight
     conv = m.short_conv
-    if conv.conv.bias is not None:
-        raise NotImplementedError("conv bias is not supported by lng_causal_conv")
     if _skinny_ok(x, w_o) and conv_in.dtype == torch.bfloat16:
         ops.linear_at(x, w_o, conv_in, L, L_dev)     # the projection writes the cache rows
     else:
@@ -164,6 +176,11 @@ def _finish_cached(m, head: Tensor, conv_in: Tensor, L: int, n: int, L_dev: Tens
     ``mixed + short_conv`` over the cached window (``infer.py:175-182``)."""
     _oproj_to_cache(m, head, conv_in, L, n, L_dev)
     conv = m.short_conv
+    if not conv.one_kernel:
+        # the window's rows normalised once more, the conv over them, and the new positions of it
+        lo = max(0, L - conv.left_padding)
+        rows = conv_in[:, lo:L + n]
+        return (rows + conv(rows))[:, L - lo:].detach().contiguous()
     length = L + n if L_dev is None else conv_in.shape[1]
     return ops.causal_conv_at(conv_in, conv.norm.weight, conv.conv.weight, conv.dilation, conv.norm.eps,
                               pos0=L, n=n, length=length, pos0_dev=L_dev, residual=True)
@@ -226,6 +243,7 @@ def static_memory_step(model, pos: int, state: DecodeState, h: Tensor, codes_new
     The caller advances ``state.length`` (and ``L_t``) afterwards."""
     mem = model.blocks[pos].memory
     m = mem.module
+    _need_one_kernel_conv(m, "static_memory_step")
     n = h.shape[1]
     dev = h.device
     L32 = (L_t if L_t.dtype == torch.int32 else L_t.to(torch.int32)).reshape(1)
@@ -275,7 +293,7 @@ def tree_ssm_states(model, state: DecodeState, emb: Tensor, parent) -> Tensor:
     (``tree_verify_step``, ``drafting/tree.py:153-161``): each node continues from its parent's
     state, the root from the cached state at ``L - 1`` (zero at ``L = 0``); ``lng_ssm_tree``.
     The caller writes them into ``state.ssm`` after the step, as the reference does."""
-    ssm = model.ssm
+    ssm = _diagonal(model, "tree_ssm_states")
     L = state.length
     root = state.ssm[:, L - 1] if L > 0 else None
     return ops.ssm_tree(ssm.decay(), ssm.inputs(emb), _parent_index(parent, emb.device)[0], root)
@@ -337,6 +355,7 @@ def _tree_memory(model, pos: int, state: DecodeState, h: Tensor, codes: Tensor, 
     dev = h.device
     if len(parent) != n:
         raise ValueError(f"tree_memory_step: {len(parent)} parents for {n} nodes")
+    _need_one_kernel_conv(m, "tree_memory_step")
     cache = state.codes[pos]
     hist = m.route_history_length
     conv = m.short_conv

@@ -27,6 +27,9 @@ from torch import Tensor, nn
 
 from lngram_hip import ops
 
+from .norm import LayerNorm
+from .short_conv import short_conv
+
 
 @torch.no_grad()
 def _normal_init(weight: Tensor, std: float) -> None:
@@ -148,12 +151,12 @@ class RMSNorm(nn.Module):
 
 
 def build_lngram_norm(normalization: str, hidden_size: int, eps: float, device=None, dtype=None) -> nn.Module:
-    """``lngram_v2.py:56-71``.  Only RMSNorm has a kernel; LayerNorm is rejected."""
+    """``lngram_v2.py:56-71``."""
     name = str(normalization).lower().replace("_", "")
     if name == "rmsnorm":
         return RMSNorm(hidden_size, eps=eps, device=device, dtype=dtype)
     if name == "layernorm":
-        raise NotImplementedError("LNGram LayerNorm readout has no MI355X kernel; use RMSNorm")
+        return LayerNorm(hidden_size, eps=eps, device=device, dtype=dtype)
     raise ValueError(f"Unsupported LNGram normalization {normalization!r}; expected RMSNorm or LayerNorm")
 
 
@@ -189,10 +192,11 @@ def _aligned_ngram_address(codes: Tensor, order: int, bits: int) -> Tensor:
 
 
 class DepthwiseCausalConv(nn.Module):
-    """Zero-left-padded depthwise causal conv (``lngram_v2.py:207-286``): ``SiLU(conv(RMSNorm(x)))``.
+    """Zero-left-padded depthwise causal conv (``lngram_v2.py:207-286``): ``SiLU(conv(norm(x)))``.
 
-    Parameters ``norm.weight`` and ``conv.weight [d, 1, K]`` as in the reference; the
-    forward runs ``lng_causal_conv``."""
+    Parameters ``norm.weight`` and ``conv.weight [d, 1, K]`` as in the reference.  With RMSNorm and no bias
+    the forward is one kernel (``lng_causal_conv``); with LayerNorm or a bias the norm and the conv
+    (``lng_short_conv``, up to 8 taps) are a kernel each, and with LayerNorm the pair is differentiable."""
 
     def __init__(self, hidden_size: int, kernel_size: int, dilation: int, eps: float, normalization: str = "RMSNorm",
                  bias: bool = False, zero_init: bool = True, device=None, dtype=None):
@@ -215,11 +219,17 @@ class DepthwiseCausalConv(nn.Module):
             raise ValueError(f"causal conv expects [B,T,{self.hidden_size}], got {tuple(values.shape)}")
         if segment_ids is not None:
             raise NotImplementedError("packed-segment causal conv is not part of the MI355X path")
-        if self.conv.bias is not None:
-            raise NotImplementedError("conv bias is not supported by lng_causal_conv")
+
+    @property
+    def one_kernel(self) -> bool:
+        """Whether the norm is part of the conv's kernel (RMSNorm, no bias): those forms also read a cache
+        at a position that the device holds, and a tree's windows."""
+        return self.conv.bias is None and not isinstance(self.norm, LayerNorm)
 
     def forward(self, values: Tensor, segment_ids: Optional[Tensor] = None) -> Tensor:
         self._check(values, segment_ids)
+        if not self.one_kernel:
+            return short_conv(self.norm(values), self.conv.weight, self.conv.bias, dilation=self.dilation)
         return ops.causal_conv(values, self.norm.weight, self.conv.weight, self.dilation, self.norm.eps,
                                residual=False)
 
@@ -229,10 +239,19 @@ class DepthwiseCausalConv(nn.Module):
         of the next call.  Here the history holds the last ``left_padding`` input rows before their
         RMSNorm: ``lng_causal_conv_at`` normalises every row it reads exactly as the whole-sequence
         conv does, so chained calls give the whole sequence's output bit for bit (a zero row
-        normalises to zero, the left padding)."""
+        normalises to zero, the left padding).  With LayerNorm or a bias it holds the normalised rows, as
+        the reference's does (a zero row does not normalise to zero there)."""
         self._check(values, None)
         b, n, d = values.shape
         lp = self.left_padding
+        if not self.one_kernel:
+            if history is not None:
+                if tuple(history.shape) != (b, d, lp):
+                    raise ValueError(f"conv history shape={tuple(history.shape)}, expected {(b, d, lp)}")
+                history = history.transpose(1, 2).to(values.dtype)
+            out, rows = short_conv(self.norm(values), self.conv.weight, self.conv.bias, dilation=self.dilation,
+                                   history=history, return_history=True)
+            return out, rows.transpose(1, 2).contiguous()
         if lp == 0:
             return self.forward(values), values.new_zeros(b, d, 0)
         if history is None:
@@ -247,15 +266,17 @@ class DepthwiseCausalConv(nn.Module):
         return out, window[:, -lp:].transpose(1, 2).contiguous()
 
     def forward_residual(self, values: Tensor) -> Tensor:
-        """``values + forward(values)`` in one kernel (the ``_finish`` residual)."""
+        """``values + forward(values)`` (the ``_finish`` residual), in the conv's one kernel where it has one."""
         self._check(values, None)
+        if not self.one_kernel:
+            return values + self.forward(values)
         return ops.causal_conv(values, self.norm.weight, self.conv.weight, self.dilation, self.norm.eps,
                                residual=True)
 
     def takes_row_stats(self, dtype: torch.dtype) -> bool:
-        """Whether :meth:`forward_residual_stats` applies (bf16, kernel 4, dilation 3, no bias)."""
+        """Whether :meth:`forward_residual_stats` applies (bf16, kernel 4, dilation 3, RMSNorm, no bias)."""
         return (dtype == torch.bfloat16 and self.kernel_size == 4 and self.dilation == 3
-                and self.conv.bias is None and self.hidden_size % 8 == 0 and self.hidden_size <= 2048)
+                and self.one_kernel and self.hidden_size % 8 == 0 and self.hidden_size <= 2048)
 
     def forward_residual_stats(self, values: Tensor, rowsq: Tensor) -> Tensor:
         """:meth:`forward_residual` with the RMSNorm row statistics computed by the producing
@@ -458,13 +479,13 @@ class _RouteNgramMemoryBase(nn.Module):
 
     # ------------------------------------------------------------------ projections
     def _project_query(self, hidden_states: Tensor) -> Tensor:
-        """``W_q RMSNorm(h)`` -> ``[B, T, H, hd]`` (``lngram_v2.py:1115-1118``)."""
+        """``W_q norm(h)`` -> ``[B, T, H, hd]`` (``lngram_v2.py:1115-1118``)."""
         b, t, _ = hidden_states.shape
         q = ops.linear(self.readout_query_norm(hidden_states), self.readout_q_proj.weight)
         return q.view(b, t, self.readout_num_heads, self.readout_head_dim)
 
     def _project_memory(self, route_tokens: Tensor) -> Tuple[Tensor, Tensor]:
-        """Memory RMSNorm + KV projection -> key, value ``[B, T, KV, R, hd]`` views (``lngram_v2.py:1120-1131``)."""
+        """Memory norm + KV projection -> key, value ``[B, T, KV, R, hd]`` views (``lngram_v2.py:1120-1131``)."""
         kv = ops.linear(self.readout_memory_norm(route_tokens), self.readout_kv_proj.weight)
         key, value = kv.split(self.readout_kv_inner_dim, dim=-1)
         b, t, r, _ = key.shape
@@ -494,7 +515,8 @@ class _RouteNgramMemoryBase(nn.Module):
         # other dtypes and widths: the projection, then the single-pass conv (row statistics formed
         # inside its blocks)
         mixed = ops.linear(flat, self.readout_o_proj.weight)
-        return self.short_conv.forward_residual(mixed)
+        # the readout in front of it has no backward pass: a conv that has one leaves no part of a graph
+        return self.short_conv.forward_residual(mixed).detach()
 
     # ------------------------------------------------------------------ fused path
     # Layers whose intermediates fit this run as one call (lng_memory_forward); past it the host's share
@@ -508,6 +530,8 @@ class _RouteNgramMemoryBase(nn.Module):
               and self.bits_per_route == 4 and self.num_routes <= 256
               and self.readout_num_heads == 16 and self.readout_head_dim == 64
               and self.readout_num_kv_heads == 4 and self.readout_kv_proj.weight.dtype == torch.bfloat16
+              and not isinstance(self.readout_query_norm, LayerNorm)
+              and not isinstance(self.readout_memory_norm, LayerNorm)
               and all(t.weight.dtype == torch.bfloat16 for t in self.tables.values()))
         if ok and tables:
             ok = all(t.weight.device.type == "cuda" for t in self.tables.values())
@@ -551,7 +575,9 @@ class _RouteNgramMemoryBase(nn.Module):
             tables = [mods["tables"]._modules[f"ngram_{n}"]._parameters["weight"] for n in self.ngrams]
         except KeyError:                                   # a parametrised weight
             return None
-        if bias is not None or len(tables) > 4 or any(x is None for x in (wq, qn, kv, mn, wo, cn, cw, *tables)):
+        if bias is not None or any(isinstance(n, LayerNorm) for n in (*norms, conv._modules["norm"])):
+            return None                                    # the norms of these launches are RMSNorms
+        if len(tables) > 4 or any(x is None for x in (wq, qn, kv, mn, wo, cn, cw, *tables)):
             return None
         if not fused and (torch.nn.modules.module._has_any_global_hook()
                           or any(n._forward_hooks or n._forward_pre_hooks or type(n) is not RMSNorm for n in norms)):

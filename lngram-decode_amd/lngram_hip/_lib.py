@@ -77,6 +77,28 @@ class MemoryLayer(ctypes.Structure):
 
 _PL = ctypes.POINTER(MemoryLayer)
 
+class Selective(ctypes.Structure):
+    """``lng_selective`` (include/lngram_hip.h): shapes, strides and pointers of a selective scan."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("B", "T")] + [
+        (n, ctypes.c_int32) for n in ("C", "N", "G", "dtype", "softplus", "reserved")] + [
+        (n, ctypes.c_void_p) for n in ("u", "dt", "z", "Bm", "Cm")] + [
+        (n, ctypes.c_int64) for n in ("u_batch", "u_token", "dt_batch", "dt_token", "z_batch", "z_token", "B_batch",
+                                      "B_token", "B_group", "C_batch", "C_token", "C_group")] + [
+        (n, ctypes.c_void_p) for n in ("A", "D", "dt_bias", "state", "lengths", "y", "state_out", "checkpoints",
+                                       "checkpoints_in")]
+
+
+class SelectiveGrad(ctypes.Structure):
+    """``lng_selective_grad`` (include/lngram_hip.h): the gradients of a selective scan."""
+
+    _fields_ = [("dy", ctypes.c_void_p), ("dy_batch", ctypes.c_int64), ("dy_token", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("dstate_out", "du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate")]
+
+
+_PSel = ctypes.POINTER(Selective)
+_PSelG = ctypes.POINTER(SelectiveGrad)
+
 # name -> (restype, argtypes); must cover every function declared in the header
 SIGNATURES = {
     "lng_abi_version": (_int, []),
@@ -143,6 +165,23 @@ SIGNATURES = {
     "lng_memory_forward_workspace_bytes": (ctypes.c_size_t, [_PL, _i64, _i64]),
     "lng_memory_forward": (_int, [_PL, _p, _p, _int, _i64, _i64, _p, ctypes.c_size_t, _p, _p]),
     "lng_memory_step": (_int, [_PL, _p, _p, _int, _i64, _i64, _i64, _p, _p, _i64, _p, ctypes.c_size_t, _p, _p]),
+    "lng_layer_norm": (_int, [_p, _int, _i64, _i64, _i64, _p, _p, _int, _f, _p, _p, _p, _p]),
+    "lng_layer_norm_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "lng_layer_norm_grad": (_int, [_p, _i64, _p, _i64, _int, _i64, _i64, _p, _int, _p, _p, _p, ctypes.c_size_t, _p, _p,
+                                   _p, _p]),
+    "lng_short_conv": (_int, [_p, _int, _i64, _i64, _i32, _i64, _i64, _p, _p, _int, _i32, _i32, _int, _p, _p, _p, _p,
+                              _p]),
+    "lng_short_conv_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i32, _i32]),
+    "lng_short_conv_grad": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i32, _p, _p, _int, _i32, _i32,
+                                   _int, _p, _p, _p, _p, ctypes.c_size_t, _p, _p, _p, _p, _p]),
+    "lng_short_conv_step": (_int, [_p, _int, _i64, _i32, _i64, _p, _p, _int, _i32, _i32, _int, _p, _p, _p, _p]),
+    "lng_selective_size": (ctypes.c_size_t, []),
+    "lng_selective_grad_size": (ctypes.c_size_t, []),
+    "lng_selective_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i32, _i32, _int]),
+    "lng_selective_checkpoints": (_i64, [_i64, _i64, _i32, _i32]),
+    "lng_selective_scan": (_int, [_PSel, _p, ctypes.c_size_t, _p]),
+    "lng_selective_scan_grad": (_int, [_PSel, _PSelG, _p, ctypes.c_size_t, _p]),
+    "lng_selective_step": (_int, [_PSel, _p]),
     "lng_host_device_pointer": (_int, [_p, ctypes.POINTER(_p)]),
     "lng_permute_table": (_int, [_p, _p, _int, _i32, _i32, _i32, _i32, _p]),
     "lng_serving_address": (_int, [_p, _int, _i64, _i64, _i32, _i32, _i32, _p, _p]),

@@ -7,6 +7,7 @@ are rejected: there is no CPU path in the product.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -1330,6 +1331,354 @@ def ssm_scan_status(dev: torch.device) -> int:
     v = int(word.item())
     word.zero_()
     return v
+
+
+# ----------------------------------------------------------------------------- norm, short conv, selective scan
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _on(dev: torch.device):
+    """The tensors' device as the current one while a call is made on it."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _float_rows(what: str, x: torch.Tensor, *weights) -> None:
+    """fp32, bf16 or fp16 rows with weights of one type, the rows' own or fp32."""
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"{what}: fp32, bf16 or fp16 tensors, got {x.dtype}")
+    types = {w.dtype for w in weights if w is not None}
+    if len(types) > 1 or not types <= {x.dtype, torch.float32}:
+        raise TypeError(f"{what}: weights of one type, {x.dtype} as the rows or float32, got "
+                        f"{', '.join(str(t) for t in types)}")
+
+
+def _as_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x [..., d]`` as ``[rows, d]`` with contiguous rows, without a copy where its strides allow it."""
+    d = x.shape[-1]
+    rows = x.reshape(x.numel() // d, d)
+    return rows if rows.stride(1) == 1 or d == 1 else rows.contiguous()
+
+
+def _last_contiguous(x: torch.Tensor) -> torch.Tensor:
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _expect(what: str, name: str, t: torch.Tensor | None, *shape) -> None:
+    if t is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {shape}")
+
+
+def _lengths32(what: str, lengths: torch.Tensor | None, batch: int) -> torch.Tensor | None:
+    if lengths is None:
+        return None
+    _expect(what, "lengths", lengths, batch)
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: int32 or int64 lengths, got {lengths.dtype}")
+    return lengths.to(torch.int32).contiguous()
+
+
+def _separate(what: str, name: str, out: torch.Tensor, src: torch.Tensor) -> None:
+    """``out`` is ``src`` itself or shares no memory with it."""
+    lo, n = src.data_ptr(), src.numel() * src.element_size()
+    at = out.data_ptr()
+    if at != lo and at < lo + n and lo < at + n:
+        raise ValueError(f"{what}: {name} overlaps what it is computed from")
+
+
+def layer_norm(x: torch.Tensor, w: torch.Tensor | None, b: torch.Tensor | None, eps: float, want_stats: bool = False):
+    """Layer norm over the last dimension (``lng_layer_norm``); w, b ``[d]`` in x's type or fp32, or None.
+    ``want_stats``: returns ``(y, mean, rstd)`` for :func:`layer_norm_grad`, fp32 ``[rows]``."""
+    dev = _dev(x, w, b)
+    _float_rows("layer_norm", x, w, b)
+    d = x.shape[-1] if x.dim() else 0
+    if d == 0:
+        raise ValueError("layer_norm: the last dimension is empty")
+    _expect("layer_norm", "weight", w, d)
+    _expect("layer_norm", "bias", b, d)
+    rows = _as_rows(x)
+    wc, bc = (None if t is None else t.contiguous() for t in (w, b))
+    n = rows.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=dev)
+    wt = next((t.dtype for t in (w, b) if t is not None), x.dtype)
+    with _on(dev):
+        check(_timed("layer_norm", dev, lambda: lib().lng_layer_norm(
+            _ptr(rows), dtype_code(x.dtype), n, d, rows.stride(0), _ptr(wc), _ptr(bc), dtype_code(wt), float(eps), _ptr(y),
+            _ptr(mean), _ptr(rstd), _stream(dev))), "layer_norm")
+    return (y, mean, rstd) if want_stats else y
+
+
+def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, mean: torch.Tensor, rstd: torch.Tensor,
+                    want=(True, True, True), w_dtype: torch.dtype | None = None) -> tuple:
+    """``(dx, dw, db)`` of :func:`layer_norm` (``lng_layer_norm_grad``), None where not wanted; dw and db in
+    ``w_dtype`` (None: the weight's type)."""
+    dev = _dev(dy, x, w, mean, rstd)
+    d = x.shape[-1]
+    _expect("layer_norm_grad", "dy", dy, *x.shape)
+    if dy.dtype != x.dtype:
+        raise TypeError(f"layer_norm_grad: dy {dy.dtype} for rows in {x.dtype}")
+    wt = w_dtype or (x.dtype if w is None else w.dtype)
+    _float_rows("layer_norm_grad", x, w, torch.empty(0, dtype=wt))
+    rows, grads = _as_rows(x), _as_rows(dy)
+    n = rows.shape[0]
+    _expect("layer_norm_grad", "mean", mean, n)
+    _expect("layer_norm_grad", "rstd", rstd, n)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    dw, db = (torch.empty(d, dtype=wt, device=dev) if k else None for k in want[1:])
+    ws = None
+    if want[1] or want[2]:
+        ws = torch.empty(lib().lng_layer_norm_grad_workspace_bytes(n, d), dtype=torch.uint8, device=dev)
+    wc = None if w is None else w.contiguous()
+    with _on(dev):
+        check(_timed("layer_norm_grad", dev, lambda: lib().lng_layer_norm_grad(
+            _ptr(grads), grads.stride(0), _ptr(rows), rows.stride(0), dtype_code(x.dtype), n, d, _ptr(wc), dtype_code(wt),
+            _ptr(mean), _ptr(rstd), _ptr(ws), 0 if ws is None else ws.numel(), _ptr(dx), _ptr(dw), _ptr(db),
+            _stream(dev))), "layer_norm_grad")
+    return dx, dw, db
+
+
+def _conv_check(what: str, x, w, bias, dilation: int, hist, dims: int) -> tuple:
+    """``(C, K, rows of a history)`` of a short conv's checked arguments."""
+    if x.dim() != dims:
+        raise ValueError(f"{what}: x is {'[B, T, C]' if dims == 3 else '[B, C]'}, got {tuple(x.shape)}")
+    _float_rows(what, x, w, bias)
+    c = x.shape[-1]
+    if w.dim() != 2 or w.shape[0] != c or not 1 <= w.shape[1] <= 8:
+        raise ValueError(f"{what}: weight [C, K] with C = {c} and 1 to 8 taps, got {tuple(w.shape)}")
+    if int(dilation) < 1:
+        raise ValueError(f"{what}: dilation must be positive")
+    _expect(what, "bias", bias, c)
+    back = (w.shape[1] - 1) * int(dilation)
+    if hist is not None:
+        _expect(what, "history", hist, x.shape[0], back, c)
+        if hist.dtype != x.dtype:
+            raise TypeError(f"{what}: history {hist.dtype} for rows in {x.dtype}")
+    return c, w.shape[1], back
+
+
+def short_conv(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, dilation: int = 1,
+               silu: bool = True, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+               want_history: bool = False):
+    """Depthwise causal conv of x ``[B, T, C]`` with w ``[C, K]`` (``lng_short_conv``).  ``history``
+    ``[B, (K - 1) * dilation, C]``: the rows before the first position (None: zeros); ``lengths [B]``: each
+    sequence's own tokens (zeros behind them).  ``want_history``: returns ``(y, next history)``."""
+    dev = _dev(x, w, bias, history, lengths)
+    c, k, back = _conv_check("short_conv", x, w, bias, dilation, history, 3)
+    b, t, _ = x.shape
+    n = _lengths32("short_conv", lengths, b)
+    xc, wc, bc, hc = _last_contiguous(x), _c(w), None if bias is None else bias.contiguous(),         None if history is None else history.contiguous()
+    y = torch.empty(b, t, c, dtype=x.dtype, device=dev)
+    out = torch.empty(b, back, c, dtype=x.dtype, device=dev) if want_history else None
+    if c:
+        with _on(dev):
+            check(_timed("short_conv", dev, lambda: lib().lng_short_conv(
+                _ptr(xc), dtype_code(x.dtype), b, t, c, xc.stride(0), xc.stride(1), _ptr(wc), _ptr(bc),
+                dtype_code(w.dtype), k, int(dilation), int(bool(silu)), _ptr(hc) if back else None, _ptr(n), _ptr(y),
+                _ptr(out) if back else None, _stream(dev))), "short_conv")
+    return (y, out) if want_history else y
+
+
+def short_conv_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, dilation: int,
+                    silu: bool, history: torch.Tensor | None, lengths: torch.Tensor | None,
+                    dhistory: torch.Tensor | None = None, want=(True, True, True, True)) -> tuple:
+    """``(dx, dw, dbias, dhistory)`` of :func:`short_conv` (``lng_short_conv_grad``), None where not wanted;
+    ``dhistory``: the gradient of the next history, or None."""
+    dev = _dev(dy, x, w, bias, history, lengths, dhistory)
+    c, k, back = _conv_check("short_conv_grad", x, w, bias, dilation, history, 3)
+    b, t, _ = x.shape
+    _expect("short_conv_grad", "dy", dy, b, t, c)
+    _expect("short_conv_grad", "the next history's gradient", dhistory, b, back, c)
+    if dy.dtype != x.dtype or (dhistory is not None and dhistory.dtype != x.dtype):
+        raise TypeError(f"short_conv_grad: gradients in the rows' type {x.dtype}")
+    n = _lengths32("short_conv_grad", lengths, b)
+    dyc, xc, wc = _last_contiguous(dy), _last_contiguous(x), _c(w)
+    bc, hc, dhc = (None if v is None else v.contiguous() for v in (bias, history, dhistory))
+    dx = torch.empty(b, t, c, dtype=x.dtype, device=dev) if want[0] else None
+    dw = torch.empty(c, k, dtype=w.dtype, device=dev) if want[1] else None
+    db = torch.empty(c, dtype=w.dtype, device=dev) if want[2] else None
+    dh = torch.empty(b, back, c, dtype=x.dtype, device=dev) if want[3] else None
+    ws = None
+    if want[1] or want[2]:
+        ws = torch.empty(lib().lng_short_conv_grad_workspace_bytes(b, t, c, k, int(dilation)), dtype=torch.uint8,
+                         device=dev)
+    if c:
+        with _on(dev):
+            check(_timed("short_conv_grad", dev, lambda: lib().lng_short_conv_grad(
+                _ptr(dyc), dyc.stride(0), dyc.stride(1), _ptr(xc), xc.stride(0), xc.stride(1), dtype_code(x.dtype), b, t,
+                c, _ptr(wc), _ptr(bc), dtype_code(w.dtype), k, int(dilation), int(bool(silu)),
+                _ptr(hc) if back else None, _ptr(n), _ptr(dhc) if back else None, _ptr(ws),
+                0 if ws is None else ws.numel(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(dh) if back else None,
+                _stream(dev))), "short_conv_grad")
+    return dx, dw, db, dh
+
+
+def short_conv_step(x: torch.Tensor, history: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
+                    dilation: int = 1, silu: bool = True, out_history: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`short_conv` of one new token x ``[B, C]`` of every sequence (``lng_short_conv_step``).  The
+    history moves on in place, or into ``out_history``."""
+    out = history if out_history is None else out_history
+    dev = _dev(x, history, w, bias, out)
+    c, k, back = _conv_check("short_conv_step", x, w, bias, dilation, history, 2)
+    _expect("short_conv_step", "out_history", out, x.shape[0], back, c)
+    if out.dtype != x.dtype or not (history.is_contiguous() and out.is_contiguous()):
+        raise ValueError("short_conv_step: histories are contiguous, in the rows' type")
+    _separate("short_conv_step", "out_history", out, history)
+    xc, wc, bc = _last_contiguous(x), _c(w), None if bias is None else bias.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if c:
+        with _on(dev):
+            check(_timed("short_conv_step", dev, lambda: lib().lng_short_conv_step(
+                _ptr(xc), dtype_code(x.dtype), x.shape[0], c, xc.stride(0), _ptr(wc), _ptr(bc), dtype_code(w.dtype), k,
+                int(dilation), int(bool(silu)), _ptr(history), _ptr(out), _ptr(y), _stream(dev))), "short_conv_step")
+    return y
+
+
+def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool, state, lengths, dims: int):
+    """``(lng_selective, tensors to keep alive)`` of a selective scan's checked arguments; dims 3: ``[B, T, C]``
+    tensors, 2: ``[B, C]`` (one token)."""
+    if u.dim() != dims or u.shape[-1] == 0:
+        raise ValueError(f"{what}: u is {'[B, T, C]' if dims == 3 else '[B, C]'}, got {tuple(u.shape)}")
+    lead, c = tuple(u.shape[:-1]), u.shape[-1]
+    if u.dtype not in _FLOATS or any(t is not None and t.dtype != u.dtype for t in (dt, B, C, z)):
+        raise TypeError(f"{what}: u, dt, B, C and z in one type, fp32, bf16 or fp16")
+    _expect(what, "dt", dt, *lead, c)
+    _expect(what, "z", z, *lead, c)
+    if A.dim() != 2 or A.shape[0] != c or not 1 <= A.shape[1] <= 256:
+        raise ValueError(f"{what}: A is [C, N] with C = {c} and 1 to 256 states, got {tuple(A.shape)}")
+    n = A.shape[1]
+    if B.dim() == dims:
+        B = B.unsqueeze(-2)
+    if C.dim() == dims:
+        C = C.unsqueeze(-2)
+    if B.dim() != dims + 1 or B.shape[-2] == 0 or c % B.shape[-2]:
+        raise ValueError(f"{what}: B and C are [.., N] or [.., G, N] with G a divisor of {c}")
+    g = B.shape[-2]
+    _expect(what, "B", B, *lead, g, n)
+    _expect(what, "C", C, *lead, g, n)
+    _expect(what, "D", D, c)
+    _expect(what, "dt_bias", dt_bias, c)
+    _expect(what, "state", state, lead[0], c, n)
+    if any(t is not None and t.dtype != torch.float32 for t in (A, D, dt_bias, state)):
+        raise TypeError(f"{what}: A, D, dt_bias and states are float32")
+    ln = _lengths32(what, lengths, lead[0])
+    u, dt, B, C = (_last_contiguous(t) for t in (u, dt, B, C))
+    z = None if z is None else _last_contiguous(z)
+    A, D, dt_bias, state = (None if t is None else t.contiguous() for t in (A, D, dt_bias, state))
+
+    def strides(t):
+        s = t.stride()
+        return (s[0], s[1] if dims == 3 else 0)
+
+    a = _lib.Selective(B=lead[0], T=lead[1] if dims == 3 else 1, C=c, N=n, G=g, dtype=dtype_code(u.dtype),
+                       softplus=int(bool(dt_softplus)), u=_ptr(u), dt=_ptr(dt), z=_ptr(z), Bm=_ptr(B), Cm=_ptr(C),
+                       A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias), state=_ptr(state), lengths=_ptr(ln))
+    a.u_batch, a.u_token = strides(u)
+    a.dt_batch, a.dt_token = strides(dt)
+    if z is not None:
+        a.z_batch, a.z_token = strides(z)
+    a.B_batch, a.B_token, a.B_group = *strides(B), B.stride(-2)
+    a.C_batch, a.C_token, a.C_group = *strides(C), C.stride(-2)
+    return a, (u, dt, z, B, C, A, D, dt_bias, state, ln)
+
+
+def _selective_workspace(a, grad: bool, dev: torch.device) -> torch.Tensor:
+    return torch.empty(lib().lng_selective_workspace_bytes(a.B, a.T, a.C, a.N, a.G, int(grad)), dtype=torch.uint8,
+                       device=dev)
+
+
+def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                   D: torch.Tensor | None = None, z: torch.Tensor | None = None, dt_bias: torch.Tensor | None = None,
+                   dt_softplus: bool = False, state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   want_state: bool = False, want_checkpoints: bool = False) -> tuple:
+    """``(y, final state or None, checkpoints or None)`` of the selective scan (``lng_selective_scan``) of
+    u, dt, z ``[B, T, C]`` with A ``[C, N]`` and B, C ``[B, T, N]`` or ``[B, T, G, N]``; the checkpoints are
+    what :func:`selective_scan_grad` takes."""
+    dev = _dev(u, dt, A, B, C, D, z, dt_bias, state, lengths)
+    a, keep = _selective_args("selective_scan", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, 3)
+    y = torch.empty(u.shape, dtype=u.dtype, device=dev)
+    end = ckpt = None
+    if want_state:
+        if a.T == 0:
+            end = torch.zeros(a.B, a.C, a.N, device=dev) if state is None else state.clone()
+        else:
+            end = torch.empty(a.B, a.C, a.N, dtype=torch.float32, device=dev)
+    if want_checkpoints:
+        ckpt = torch.empty(lib().lng_selective_checkpoints(a.B, a.T, a.C, a.N), dtype=torch.float32, device=dev)
+    a.y, a.state_out, a.checkpoints = _ptr(y), _ptr(end), _ptr(ckpt)
+    ws = _selective_workspace(a, False, dev)
+    if y.numel():
+        with _on(dev):
+            check(_timed("selective_scan", dev, lambda: lib().lng_selective_scan(
+                ctypes.byref(a), _ptr(ws), ws.numel(), _stream(dev))), "selective_scan")
+    del keep
+    return y, end, ckpt
+
+
+def selective_scan_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoints: torch.Tensor, u: torch.Tensor,
+                        dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: torch.Tensor | None,
+                        z: torch.Tensor | None, dt_bias: torch.Tensor | None, dt_softplus: bool,
+                        state: torch.Tensor | None, lengths: torch.Tensor | None) -> dict:
+    """The gradients of :func:`selective_scan` (``lng_selective_scan_grad``) by their inputs' names, given
+    those of y and of the final state (None: zero)."""
+    dev = _dev(dy, dstate, checkpoints, u, dt, A, B, C, D, z, dt_bias, state, lengths)
+    a, keep = _selective_args("selective_scan_grad", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, 3)
+    _expect("selective_scan_grad", "dy", dy, *u.shape)
+    _expect("selective_scan_grad", "dstate", dstate, a.B, a.C, a.N)
+    if dy.dtype != u.dtype or (dstate is not None and dstate.dtype != torch.float32):
+        raise TypeError("selective_scan_grad: dy in u's type, dstate in float32")
+    _expect("selective_scan_grad", "checkpoints", checkpoints, lib().lng_selective_checkpoints(a.B, a.T, a.C, a.N))
+    f32 = torch.float32
+    out = {"u": torch.empty(u.shape, dtype=u.dtype, device=dev), "dt": torch.empty(u.shape, dtype=u.dtype, device=dev),
+           "A": torch.empty(A.shape, dtype=f32, device=dev), "B": torch.empty(B.shape, dtype=u.dtype, device=dev),
+           "C": torch.empty(C.shape, dtype=u.dtype, device=dev)}
+    if D is not None:
+        out["D"] = torch.empty(D.shape, dtype=f32, device=dev)
+    if z is not None:
+        out["z"] = torch.empty(u.shape, dtype=u.dtype, device=dev)
+    if dt_bias is not None:
+        out["dt_bias"] = torch.empty(dt_bias.shape, dtype=f32, device=dev)
+    if state is not None:
+        out["state"] = torch.empty(a.B, a.C, a.N, dtype=f32, device=dev)
+    if not u.numel():                                    # no tokens: the state's gradient passes through
+        for k, v in out.items():
+            v.zero_() if k != "state" or dstate is None else v.copy_(dstate)
+        return out
+    dyc, dsc = _last_contiguous(dy), None if dstate is None else dstate.contiguous()
+    a.checkpoints_in = _ptr(checkpoints)
+    g = _lib.SelectiveGrad(dy=_ptr(dyc), dy_batch=dyc.stride(0), dy_token=dyc.stride(1), dstate_out=_ptr(dsc),
+                           du=_ptr(out["u"]), ddt=_ptr(out["dt"]), dz=_ptr(out.get("z")), dB=_ptr(out["B"]),
+                           dC=_ptr(out["C"]), dA=_ptr(out["A"]), dD=_ptr(out.get("D")),
+                           ddt_bias=_ptr(out.get("dt_bias")), dstate=_ptr(out.get("state")))
+    ws = _selective_workspace(a, True, dev)
+    with _on(dev):
+        check(_timed("selective_scan_grad", dev, lambda: lib().lng_selective_scan_grad(
+            ctypes.byref(a), ctypes.byref(g), _ptr(ws), ws.numel(), _stream(dev))), "selective_scan_grad")
+    del keep
+    return out
+
+
+def selective_step(state: torch.Tensor, u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+                   C: torch.Tensor, D: torch.Tensor | None = None, z: torch.Tensor | None = None,
+                   dt_bias: torch.Tensor | None = None, dt_softplus: bool = False,
+                   out_state: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`selective_scan` of one new token u ``[B, C]`` of every sequence (``lng_selective_step``).  The
+    state moves on in place, or into ``out_state``."""
+    out = state if out_state is None else out_state
+    dev = _dev(state, u, dt, A, B, C, D, z, dt_bias, out)
+    if not state.is_contiguous() or not out.is_contiguous() or out.dtype != torch.float32:
+        raise ValueError("selective_step: states are contiguous float32 [B, C, N]")
+    a, keep = _selective_args("selective_step", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, None, 2)
+    _expect("selective_step", "out_state", out, a.B, a.C, a.N)
+    _separate("selective_step", "out_state", out, state)
+    y = torch.empty(u.shape, dtype=u.dtype, device=dev)
+    a.y, a.state_out = _ptr(y), _ptr(out)
+    with _on(dev):
+        check(_timed("selective_step", dev, lambda: lib().lng_selective_step(ctypes.byref(a), _stream(dev))),
+              "selective_step")
+    del keep
+    return y
 
 
 def tree_accept(parent: torch.Tensor, node_tokens: torch.Tensor, argmax: torch.Tensor, out=None):
