@@ -35,8 +35,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 typedef const float __attribute__((address_space(4))) cfloat;  // read through the scalar unit where uniform
 
 struct Dims {
-  int64_t B, T, chunk, segs;  // chunk: tokens of a chunk, a multiple of SEG; segs: segments of a sequence
-  int C, N, G, chunks, cbg;   // cbg: channel blocks of 64 in a group
+  int64_t B;
+  int T, chunk, segs;        // chunk: tokens of a chunk, a multiple of SEG; segs: segments of a sequence
+  int C, N, G, chunks, cbg;  // cbg: channel blocks of 64 in a group
   int softplus;
 };
 
@@ -71,9 +72,10 @@ __device__ __forceinline__ float softplus(float x) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 
-__device__ __forceinline__ int64_t seq_len(const int32_t* lengths, int64_t b, int64_t T) {
+// The own tokens of sequence b (the same in every lane that asks for the same b).
+__device__ __forceinline__ int seq_len(const int32_t* lengths, int64_t b, int T) {
   if (!lengths) return T;
-  const int64_t n = lengths[b];
+  const int n = lengths[b];
   return n < 0 ? 0 : n > T ? T : n;
 }
 
@@ -102,49 +104,100 @@ __global__ __launch_bounds__(256) void k_sel_tiles(Dims d, Ptrs p) {
 
 // A wave's share of a launch: 64 channels of one group, one sequence, one chunk.
 struct Unit {
-  int64_t b, bg, t0, t1, end, u;  // tokens [t0, t1) of the chunk; end: the sequence's length
-  int g, c, lane, wave, chunk;
+  int64_t b, bg, u;       // sequence, sequence and group, sequence and chunk
+  int t0, t1, end;        // tokens [t0, t1) of the chunk; end: the sequence's length
+  int c, lane, wave, chunk;
   bool ok;   // this lane has a channel
   bool any;  // the wave has one
   __device__ __forceinline__ Unit(const Dims& d, const int32_t* lengths) {
     // blocks: channel block groups fastest, then chunks, then sequences
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int waves = blockDim.x >> 6, bpg = (d.cbg + waves - 1) / waves;  // blocks of a group's channels
-    const int64_t per = static_cast<int64_t>(bpg) * d.G;
-    const int64_t x = blockIdx.x, cb = x % per, bs = x / per;
-    g = static_cast<int>(cb / bpg);
-    chunk = static_cast<int>(bs % d.chunks);
+    const unsigned waves = blockDim.x >> 6, bpg = (d.cbg + waves - 1) / waves;  // blocks of a group's channels
+    const unsigned x = blockIdx.x, cb = x % (bpg * d.G), bs = x / (bpg * d.G);
+    const int g = cb / bpg;
+    chunk = bs % d.chunks;
     b = bs / d.chunks;
     bg = b * d.G + g;
-    u = b * d.chunks + chunk;
-    const int cg = d.C / d.G, in = (static_cast<int>(cb % bpg) * waves + wave) * 64;
+    u = bs;
+    const int cg = d.C / d.G, in = ((cb % bpg) * waves + wave) * 64;
     any = in < cg;
     ok = in + lane < cg;
     c = g * cg + (ok ? in + lane : cg - 1);
     t0 = chunk * d.chunk;
     t1 = t0 + d.chunk < d.T ? t0 + d.chunk : d.T;
-    end = seq_len(lengths, b, d.T);
+    end = __builtin_amdgcn_readfirstlane(seq_len(lengths, b, d.T));
+  }
+  // The lane's byte offset in a row of T; lanes without a channel write nowhere (past every buffer's end).
+  template <typename T>
+  __device__ __forceinline__ int in(bool store = false) const {
+    return store && !ok ? static_cast<int>(0x80000000u) : c * static_cast<int>(sizeof(T));
   }
 };
 
-// A segment's values of one tensor in fp32; zeros at and behind `end`.
+// Rows of C channels behind one scalar address, reached by a lane's offset and a scalar one, so that no lane
+// holds addresses.  The buffer's bounds hold a lane's offset, not the scalar one: `load` and `store` take rows
+// that exist, `store_in` adds the row to the lane's offset and does nothing past the last one.
 template <typename T>
-__device__ __forceinline__ void load_seg(const void* base, int64_t row, int64_t stride, int64_t t, int64_t end, int c,
-                                         float (&v)[SEG]) {
-  const T* const p = static_cast<const T*>(base) + row + c;
+struct Rows {
+  __amdgpu_buffer_rsrc_t buf;
+  int stride;  // bytes
+  // `rows` rows from `row` on, `token` elements apart
+  __device__ __forceinline__ Rows(const void* row, int64_t token, int rows, int C)
+      : stride(static_cast<int>(token) * static_cast<int>(sizeof(T))) {
+    buf = dev_buf(row, static_cast<uint32_t>((rows - 1) * stride + C * static_cast<int>(sizeof(T))));
+  }
+  __device__ __forceinline__ T load(int lane, int i) const {
+    if constexpr (sizeof(T) == 2)
+      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(buf, lane, i * stride, 0));
+    else
+      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(buf, lane, i * stride, 0));
+  }
+  __device__ __forceinline__ void put(int lane, int scalar, float v) const {
+    const T t = from_f32<T>(v);
+    if constexpr (sizeof(T) == 2)
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t), buf, lane, scalar, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, t), buf, lane, scalar, 0);
+  }
+  __device__ __forceinline__ void store(int lane, int i, float v) const { put(lane, i * stride, v); }
+  __device__ __forceinline__ void store_in(int lane, int i, float v) const { put(lane + i * stride, 0, v); }
+};
+
+__device__ __forceinline__ int live(int t, int end) { return end - t < SEG ? end - t : SEG; }
+
+// A segment's values of one tensor, as stored: SEG loads that go out together.  Tokens at and behind `end`
+// (which is past t) read the last own one; `widen` and `steps` put zeros in their place.
+template <typename T>
+__device__ __forceinline__ void fetch(const void* base, int64_t batch, int64_t token, int t, int end, int C, int lane,
+                                      T (&v)[SEG]) {
+  const int n = live(t, end);
+  const Rows<T> rows(static_cast<const T*>(base) + batch + t * token, token, n, C);
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) v[i] = t + i < end ? to_f32(p[(t + i) * stride]) : 0.f;
+  for (int i = 0; i < SEG; ++i) v[i] = rows.load(lane, i < n ? i : n - 1);
+}
+template <typename T>
+__device__ __forceinline__ void widen(const T (&r)[SEG], int t, int end, float (&v)[SEG]) {
+#pragma unroll
+  for (int i = 0; i < SEG; ++i) v[i] = to_f32(r[i]);
+  if (t + SEG > end) {
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) v[i] = t + i < end ? v[i] : 0.f;
+  }
 }
 
+// Step sizes from dt; no time passes behind a sequence's end.
 template <typename T>
-__device__ __forceinline__ void load_steps(const Dims& d, const Ptrs& p, int64_t b, int64_t t, int64_t end, int c,
-                                           float bias, float (&s)[SEG]) {
-  load_seg<T>(p.dt, b * p.dtb, p.dtt, t, end, c, s);
+__device__ __forceinline__ void steps(const Dims& d, const T (&r)[SEG], int t, int end, float bias, float (&s)[SEG]) {
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) {
-    const float x = s[i] + bias;
-    s[i] = t + i < end ? (d.softplus ? softplus(x) : x) : 0.f;  // no time passes behind a sequence's end
+  for (int i = 0; i < SEG; ++i) s[i] = to_f32(r[i]) + bias;
+  if (d.softplus) {
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) s[i] = softplus(s[i]);
+  }
+  if (t + SEG > end) {
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) s[i] = t + i < end ? s[i] : 0.f;
   }
 }
 
@@ -182,53 +235,62 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
   }
   const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = !AGG && p.D ? p.D[w.c] : 0.f;
   float total = 0.f;
-  for (int64_t t = w.t0; t < w.t1; t += SEG) {
-    if (t >= w.end) {  // behind the sequence: zeros, and the states stay
-      if constexpr (!AGG) {
-        if (w.ok)
-          for (int i = 0; i < SEG && t + i < w.t1; ++i)
-            static_cast<T*>(p.y)[(w.b * d.T + t + i) * d.C + w.c] = from_f32<T>(0.f);
-        continue;
-      } else {
-        break;
-      }
-    }
-    float s[SEG], x[SEG], y[SEG];
-    load_seg<T>(p.u, w.b * p.ub, p.ut, t, w.end, w.c, x);
-    load_steps<T>(d, p, w.b, t, w.end, w.c, bias, s);
+  const int stop = w.t1 < w.end ? w.t1 : w.end;  // behind it: zeros, and the states stay
+  const int in = w.in<T>(), out = w.in<T>(true), out32 = w.in<float>(true);
+  T ur[SEG], dr[SEG], zr[SEG];
+  auto read = [&](int t) {
+    fetch<T>(p.u, w.b * p.ub, p.ut, t, stop, d.C, in, ur);
+    fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, stop, d.C, in, dr);
+    if constexpr (!AGG)
+      if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, stop, d.C, in, zr);
+  };
+  if (w.t0 < stop) read(w.t0);
+  for (int t = w.t0; t < stop; t += SEG) {
+    float s[SEG], x[SEG], y[SEG], gate[SEG];
+    widen<T>(ur, t, stop, x);
+    steps<T>(d, dr, t, stop, bias, s);
 #pragma unroll
     for (int i = 0; i < SEG; ++i) {
       if constexpr (AGG) total += s[i];
       y[i] = dskip * x[i];
       x[i] *= s[i];
+      gate[i] = 1.f;
     }
-    const int64_t seg = t / SEG, tile = (w.bg * d.segs + seg) * d.N * 2 * SEG;
+    if constexpr (!AGG) {
+      if (p.z) {
+        widen<T>(zr, t, stop, gate);
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) gate[i] *= sigmoid(gate[i]);
+      }
+    }
+    if (t + SEG < stop) read(t + SEG);  // the next segment's values arrive while this one is computed
+    const int64_t tile = (w.bg * d.segs + t / SEG) * d.N * 2 * SEG;
+    const Rows<float> ckpt(p.ckpt + (w.b * d.segs + t / SEG) * d.N * d.C, d.C, d.N, d.C);
+    Row r = load_row(p.tiles, tile);
+    float h = hs[0], a = as[0];
     for (int n = 0; n < d.N; ++n) {
-      const Row r = load_row(p.tiles, tile + n * 2 * SEG);
-      float h = hs[n * 64];
-      const float a = as[n * 64];
-      if (!AGG && p.ckpt && w.ok) p.ckpt[((w.b * d.segs + seg) * d.N + n) * d.C + w.c] = h;
+      const int m = n + 1 < d.N ? n + 1 : n;  // the next state's values likewise
+      const Row rn = load_row(p.tiles, tile + m * 2 * SEG);
+      const float hn = hs[m * 64], an = as[m * 64];
+      if (!AGG && p.ckpt) ckpt.store(out32, n, h);
 #pragma unroll
       for (int i = 0; i < SEG; ++i) {
         h = fmaf(__builtin_amdgcn_exp2f(s[i] * a), h, x[i] * r.B[i]);
         if constexpr (!AGG) y[i] = fmaf(r.C[i], h, y[i]);
       }
       hs[n * 64] = h;
+      r = rn, h = hn, a = an;
     }
     if constexpr (!AGG) {
-      if (p.z) {
-        float z[SEG];
-        load_seg<T>(p.z, w.b * p.zb, p.zt, t, w.end, w.c, z);
+      const Rows<T> rows(static_cast<T*>(p.y) + (w.b * d.T + t) * d.C, d.C, live(t, stop), d.C);
 #pragma unroll
-        for (int i = 0; i < SEG; ++i) y[i] *= z[i] * sigmoid(z[i]);
-      }
-      if (w.ok) {
-        T* const out = static_cast<T*>(p.y) + (w.b * d.T + t) * d.C + w.c;
-#pragma unroll
-        for (int i = 0; i < SEG; ++i)
-          if (t + i < w.t1) out[static_cast<int64_t>(i) * d.C] = from_f32<T>(t + i < w.end ? y[i] : 0.f);
-      }
+      for (int i = 0; i < SEG; ++i) rows.store_in(out, i, y[i] * gate[i]);
     }
+  }
+  if constexpr (!AGG) {
+    if (w.ok)
+      for (int64_t t = w.t0 < stop ? stop : w.t0; t < w.t1; ++t)
+        static_cast<T*>(p.y)[(w.b * d.T + t) * d.C + w.c] = from_f32<T>(0.f);
   }
   if (!w.ok) return;
   if constexpr (AGG) {
@@ -250,25 +312,22 @@ __global__ __launch_bounds__(256) void k_sel_join(Dims d, Ptrs p) {
   const float a = p.at[n * d.C + c] * LOG2E;
   const float* const first = BACK ? p.dend : p.start;
   float h = first ? first[(b * d.C + c) * d.N + n] : 0.f;
-  for (int k = 0; k < d.chunks; ++k) {
-    const int64_t u = b * d.chunks + (BACK ? d.chunks - 1 - k : k);
-    float* const at = p.hloc + (u * d.N + n) * d.C + c;
-    const bool last = k == d.chunks - 1;
-    const float own = last ? 0.f : *at, decay = last ? 0.f : __builtin_amdgcn_exp2f(p.ssum[u * d.C + c] * a);
-    *at = h;
-    h = fmaf(decay, h, own);
-  }
-}
-
-// A segment's e = dy silu(z).
-template <typename T>
-__device__ __forceinline__ void load_gated(const Ptrs& p, int64_t b, int64_t t, int64_t end, int c, float (&e)[SEG]) {
-  load_seg<T>(p.dy, b * p.dyb, p.dyt, t, end, c, e);
-  if (p.z) {
-    float z[SEG];
-    load_seg<T>(p.z, b * p.zb, p.zt, t, end, c, z);
+  constexpr int AHEAD = 16;  // chunks whose values are read together: the chain itself is short
+  for (int k0 = 0; k0 < d.chunks; k0 += AHEAD) {
+    float own[AHEAD], decay[AHEAD];
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) e[i] *= z[i] * sigmoid(z[i]);
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j < d.chunks - 1 ? k0 + j : d.chunks - 2;  // the last chunk's own values are not used
+      const int64_t u = b * d.chunks + (BACK ? d.chunks - 1 - k : k);
+      own[j] = p.hloc[(u * d.N + n) * d.C + c];
+      decay[j] = p.ssum[u * d.C + c];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j;
+      if (k < d.chunks) p.hloc[((b * d.chunks + (BACK ? d.chunks - 1 - k : k)) * d.N + n) * d.C + c] = h;
+      h = fmaf(__builtin_amdgcn_exp2f(decay[j] * a), h, own[j]);
+    }
   }
 }
 
@@ -283,21 +342,39 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
   for (int n = 0; n < d.N; ++n) qs[n * 64] = 0.f, as[n * 64] = p.at[static_cast<int64_t>(n) * d.C + w.c] * LOG2E;
   const float bias = p.bias ? p.bias[w.c] : 0.f;
   float total = 0.f;
-  const int64_t stop = w.t1 < w.end ? w.t1 : w.end;
-  for (int64_t t = (stop - 1) / SEG * SEG; stop > w.t0 && t >= w.t0; t -= SEG) {
+  const int stop = w.t1 < w.end ? w.t1 : w.end, in = w.in<T>();
+  T er[SEG], dr[SEG], zr[SEG];
+  auto read = [&](int t) {
+    fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, stop, d.C, in, er);
+    fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, stop, d.C, in, dr);
+    if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, stop, d.C, in, zr);
+  };
+  const int last = stop > w.t0 ? (stop - 1) / SEG * SEG : w.t0 - SEG;
+  if (last >= w.t0) read(last);
+  for (int t = last; t >= w.t0; t -= SEG) {
     float s[SEG], e[SEG];
-    load_gated<T>(p, w.b, t, w.end, w.c, e);
-    load_steps<T>(d, p, w.b, t, w.end, w.c, bias, s);
+    widen<T>(er, t, stop, e);
+    steps<T>(d, dr, t, stop, bias, s);
+    if (p.z) {
+      float z[SEG];
+      widen<T>(zr, t, stop, z);
+#pragma unroll
+      for (int i = 0; i < SEG; ++i) e[i] *= z[i] * sigmoid(z[i]);
+    }
+    if (t > w.t0) read(t - SEG);
 #pragma unroll
     for (int i = 0; i < SEG; ++i) total += s[i];
     const int64_t tile = (w.bg * d.segs + t / SEG) * d.N * 2 * SEG;
+    Row r = load_row(p.tiles, tile);
+    float q = qs[0], a = as[0];
     for (int n = 0; n < d.N; ++n) {
-      const Row r = load_row(p.tiles, tile + n * 2 * SEG);
-      float q = qs[n * 64];
-      const float a = as[n * 64];
+      const int m = n + 1 < d.N ? n + 1 : n;
+      const Row rn = load_row(p.tiles, tile + m * 2 * SEG);
+      const float qn = qs[m * 64], an = as[m * 64];
 #pragma unroll
       for (int i = SEG - 1; i >= 0; --i) q = fmaf(e[i], r.C[i], q) * __builtin_amdgcn_exp2f(s[i] * a);
       qs[n * 64] = q;
+      r = rn, q = qn, a = an;
     }
   }
   if (!w.ok) return;
@@ -368,26 +445,46 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
   }
   const int bpg = (d.cbg + waves - 1) / waves;
   const int64_t cb = blockIdx.x % bpg;  // this block's place among those of its group
-  for (int64_t t = (w.t1 - 1) / SEG * SEG; t >= w.t0; t -= SEG) {
-    const int64_t seg = t / SEG;
-    const int live = static_cast<int>(w.t1 - t < SEG ? w.t1 - t : SEG);  // tokens that the tensors have
+  const int in = w.in<T>(), out_t = w.in<T>(true), in32 = w.in<float>();
+  const Rows<float> at(p.at, d.C, N, d.C);
+  for (int t = (w.t1 - 1) / SEG * SEG; t >= w.t0; t -= SEG) {
+    const int64_t seg = t / SEG, row = (w.b * d.T + t) * d.C;
+    const int rows = live(t, w.t1);  // tokens that the tensors have
+    const Rows<T> du_out(static_cast<T*>(p.du) + row, d.C, rows, d.C);
+    const Rows<T> ddt_out(static_cast<T*>(p.ddt) + row, d.C, rows, d.C);
+    const Rows<T> dz_out(static_cast<T*>(p.dz) + row, d.C, p.z ? rows : 1, d.C);
     if (t < w.end) {
       if (w.any) {
         float u[SEG], s[SEG], e[SEG], y[SEG], gb[SEG], gs[SEG];
-        load_seg<T>(p.u, w.b * p.ub, p.ut, t, w.end, w.c, u);
-        load_steps<T>(d, p, w.b, t, w.end, w.c, bias, s);
-        load_gated<T>(p, w.b, t, w.end, w.c, e);
+        {
+          T ur[SEG], dr[SEG], er[SEG], zr[SEG];
+          fetch<T>(p.u, w.b * p.ub, p.ut, t, w.end, d.C, in, ur);
+          fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, d.C, in, dr);
+          fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, d.C, in, er);
+          if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, w.end, d.C, in, zr);
+          widen<T>(ur, t, w.end, u);
+          steps<T>(d, dr, t, w.end, bias, s);
+          widen<T>(er, t, w.end, e);
+          if (p.z) {
+            widen<T>(zr, t, w.end, y);
+#pragma unroll
+            for (int i = 0; i < SEG; ++i) e[i] *= y[i] * sigmoid(y[i]);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < SEG; ++i) {
           e[i] = w.ok ? e[i] : 0.f;  // lanes without a channel add nothing to the sums over channels
           y[i] = gb[i] = gs[i] = 0.f;
         }
         const int64_t tile = (w.bg * d.segs + seg) * N * 2 * SEG;
-        const float* const ck = p.ckpt_in + (w.b * d.segs + seg) * N * d.C + w.c;
+        const Rows<float> ckpt(p.ckpt_in + (w.b * d.segs + seg) * N * d.C, d.C, N, d.C);
+        Row r = load_row(p.tiles, tile);
+        float an = at.load(in32, 0), h0 = ckpt.load(in32, 0);
         for (int n = 0; n < N; ++n) {
-          const Row r = load_row(p.tiles, tile + n * 2 * SEG);
-          const float an = p.at[static_cast<int64_t>(n) * d.C + w.c], a2 = an * LOG2E;
-          const float h0 = ck[static_cast<int64_t>(n) * d.C];
+          const int m = n + 1 < N ? n + 1 : n;  // the next state's values arrive while this one is computed
+          const Row rn = load_row(p.tiles, tile + m * 2 * SEG);
+          const float ann = at.load(in32, m), hn = ckpt.load(in32, m);
+          const float a2 = an * LOG2E;
           float a[SEG], h[SEG], v[2 * SEG];
 #pragma unroll
           for (int i = 0; i < SEG; ++i) {
@@ -411,44 +508,45 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
           ga[n * 64] = dA;
           const float total = lane_sums(v, w.lane);
           if ((w.lane & 1) == 0) sums[(w.wave * N + n) * 2 * SEG + (w.lane >> 1)] = total;
+          r = rn, an = ann, h0 = hn;
         }
-        // what needs dy, z and dt once more reads them again (from the caches)
-        float raw[SEG], dy[SEG], z[SEG];
-        load_seg<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, w.c, raw);
-        load_seg<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, w.c, dy);
-        if (p.z) load_seg<T>(p.z, w.b * p.zb, p.zt, t, w.end, w.c, z);
+        // what needs dy, z and dt once more reads them again (from the caches), not earlier than here: the
+        // loop over the states needs the registers
+        asm volatile("" ::: "memory");
+        T raw[SEG], dy[SEG], zr[SEG];
+        fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, d.C, in, raw);
+        fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, d.C, in, dy);
+        if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, w.end, d.C, in, zr);
 #pragma unroll
         for (int i = 0; i < SEG; ++i) {
-          const bool in = t + i < w.end;
+          const bool own = t + i < w.end;
           const float du = fmaf(gb[i], s[i], e[i] * dskip);
           float ds = fmaf(gb[i], u[i], gs[i]);
-          if (d.softplus) ds *= sigmoid(raw[i] + bias);
+          if (d.softplus) ds *= sigmoid(to_f32(raw[i]) + bias);
           dD += e[i] * u[i];
-          dbias += in ? ds : 0.f;
-          if (i < live && w.ok) {
-            const int64_t at = (w.b * d.T + t + i) * d.C + w.c;
-            static_cast<T*>(p.du)[at] = from_f32<T>(in ? du : 0.f);
-            static_cast<T*>(p.ddt)[at] = from_f32<T>(in ? ds : 0.f);
-            if (p.z) {
-              const float sg = sigmoid(z[i]), yv = fmaf(dskip, u[i], y[i]);
-              static_cast<T*>(p.dz)[at] = from_f32<T>(in ? dy[i] * yv * sg * (1.f + z[i] * (1.f - sg)) : 0.f);
-            }
+          dbias += own ? ds : 0.f;
+          du_out.store_in(out_t, i, own ? du : 0.f);
+          ddt_out.store_in(out_t, i, own ? ds : 0.f);
+          if (p.z) {
+            const float z = to_f32(zr[i]), sg = sigmoid(z), yv = fmaf(dskip, u[i], y[i]);
+            const float dz = to_f32(dy[i]) * yv * sg * (1.f + z * (1.f - sg));
+            dz_out.store_in(out_t, i, own ? dz : 0.f);
           }
         }
       } else {
         for (int i = w.lane; i < N * 2 * SEG; i += 64) sums[w.wave * N * 2 * SEG + i] = 0.f;
       }
-    } else if (w.ok) {
-      for (int i = 0; i < live; ++i) {
-        const int64_t at = (w.b * d.T + t + i) * d.C + w.c;
-        static_cast<T*>(p.du)[at] = from_f32<T>(0.f);
-        static_cast<T*>(p.ddt)[at] = from_f32<T>(0.f);
-        if (p.z) static_cast<T*>(p.dz)[at] = from_f32<T>(0.f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < SEG; ++i) {
+        du_out.store_in(out_t, i, 0.f);
+        ddt_out.store_in(out_t, i, 0.f);
+        if (p.z) dz_out.store_in(out_t, i, 0.f);
       }
     }
     __syncthreads();
-    float* const out = p.pBC + (cb * d.B * d.G + w.bg) * d.T * 2 * N + t * 2 * N;
-    for (int j = threadIdx.x; j < live * 2 * N; j += blockDim.x) {
+    float* const out = p.pBC + ((cb * d.B * d.G + w.bg) * d.T + t) * 2 * N;
+    for (int j = threadIdx.x; j < rows * 2 * N; j += blockDim.x) {
       const int n = j % N, which = j / N & 1, i = j / N / 2;
       float v = 0.f;
       if (t + i < w.end)
@@ -576,13 +674,13 @@ int waves_for(const Dims& d, bool grad) {
 
 Dims make_dims(const lng_selective& a) {
   Dims d{};
-  d.B = a.B, d.T = a.T, d.C = a.C, d.N = a.N, d.G = a.G, d.softplus = a.softplus;
+  d.B = a.B, d.T = static_cast<int>(a.T), d.C = a.C, d.N = a.N, d.G = a.G, d.softplus = a.softplus;
   d.cbg = static_cast<int>(cdiv(a.C / a.G, 64));
-  d.segs = cdiv(a.T, SEG);
+  d.segs = static_cast<int>(cdiv(a.T, SEG));
   // chunks: two waves for each of the 1024 SIMDs, of at least four segments
   const int64_t units = a.B * a.G * d.cbg;
-  const int64_t want = std::min(cdiv(2048, std::max<int64_t>(units, 1)), std::max<int64_t>(1, d.segs / 4));
-  d.chunk = std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1))) * SEG;
+  const int64_t want = std::min<int64_t>(cdiv(2048, std::max<int64_t>(units, 1)), std::max(1, d.segs / 4));
+  d.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1)))) * SEG;
   d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
   return d;
 }
@@ -622,13 +720,18 @@ int check_args(const char* what, const lng_selective* a) {
   if (a->dtype != LNG_F32 && a->dtype != LNG_BF16 && a->dtype != LNG_F16)
     return fail(LNG_E_DTYPE, std::string(what) + ": fp32, bf16 or fp16 tensors");
   if (a->B < 0 || a->T < 0 || a->C <= 0 || a->N <= 0 || a->N > MAX_N || a->G <= 0 || a->C % a->G ||
-      a->C > (1 << 20) || a->T > (int64_t{1} << 31) || a->B > (int64_t{1} << 24) ||
+      a->C > (1 << 20) || a->T > (int64_t{1} << 30) || a->B > (int64_t{1} << 24) ||
       a->B * a->T > (int64_t{1} << 38) / a->C / a->N)
     return fail(LNG_E_ARG, std::string(what) + ": bad shape (1 to 256 states, groups that divide the channels)");
   const int64_t lanes = cdiv(a->C / a->G, 64) * 64 * a->G, most = int64_t{1} << 38;  // of any launch's threads
   if (a->B * a->G * (a->T + SEG) > most / 2 / a->N || a->B * lanes * (a->T / 64 + 1) > most ||
       a->B * a->C > most / SEG || a->B * lanes > most / a->N)
     return fail(LNG_E_ARG, std::string(what) + ": too many tokens, groups or channels for one call");
+  // a segment's rows are reached by 32-bit offsets from its first one
+  const int64_t far = (int64_t{1} << 26) / dtype_size(a->dtype);
+  for (const int64_t token : {a->u_token, a->dt_token, a->z_token})
+    if (token < 0 || token > far)
+      return fail(LNG_E_ARG, std::string(what) + ": rows of u, dt and z are 0 to 2^26 bytes apart");
   if (a->B * a->T > 0 && (!a->u || !a->dt || !a->Bm || !a->Cm || !a->A || (!a->y && !a->checkpoints_in)))
     return fail(LNG_E_ARG, std::string(what) + ": null pointer");
   return LNG_OK;
@@ -750,6 +853,8 @@ int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad*
   if (a.B == 0 || a.T == 0) return fail(LNG_E_ARG, "selective_scan_grad: no tokens");
   if (!a.checkpoints_in || !g.dy || !g.du || !g.ddt || !g.dB || !g.dC || (a.z && !g.dz))
     return fail(LNG_E_ARG, "selective_scan_grad: null pointer");
+  if (g.dy_token < 0 || g.dy_token > (int64_t{1} << 26) / dtype_size(a.dtype))
+    return fail(LNG_E_ARG, "selective_scan_grad: rows of dy are 0 to 2^26 bytes apart");
   const Dims d = make_dims(a);
   const Space s(d, true);
   if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)

@@ -1363,6 +1363,12 @@ def _last_contiguous(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
 
 
+def _near_rows(x: torch.Tensor) -> torch.Tensor:
+    """``[B, T, C]`` with contiguous channels and rows at most 2^26 bytes apart (the scan's row offsets)."""
+    x = _last_contiguous(x)
+    return x if x.dim() < 3 or x.stride(1) * x.element_size() <= 1 << 26 else x.contiguous()
+
+
 def _expect(what: str, name: str, t: torch.Tensor | None, *shape) -> None:
     if t is not None and tuple(t.shape) != shape:
         raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {shape}")
@@ -1563,8 +1569,8 @@ def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool,
     if any(t is not None and t.dtype != torch.float32 for t in (A, D, dt_bias, state)):
         raise TypeError(f"{what}: A, D, dt_bias and states are float32")
     ln = _lengths32(what, lengths, lead[0])
-    u, dt, B, C = (_last_contiguous(t) for t in (u, dt, B, C))
-    z = None if z is None else _last_contiguous(z)
+    u, dt, B, C = _near_rows(u), _near_rows(dt), _last_contiguous(B), _last_contiguous(C)
+    z = None if z is None else _near_rows(z)
     A, D, dt_bias, state = (None if t is None else t.contiguous() for t in (A, D, dt_bias, state))
 
     def strides(t):
@@ -1645,7 +1651,7 @@ def selective_scan_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoin
         for k, v in out.items():
             v.zero_() if k != "state" or dstate is None else v.copy_(dstate)
         return out
-    dyc, dsc = _last_contiguous(dy), None if dstate is None else dstate.contiguous()
+    dyc, dsc = _near_rows(dy), None if dstate is None else dstate.contiguous()
     a.checkpoints_in = _ptr(checkpoints)
     g = _lib.SelectiveGrad(dy=_ptr(dyc), dy_batch=dyc.stride(0), dy_token=dyc.stride(1), dstate_out=_ptr(dsc),
                            du=_ptr(out["u"]), ddt=_ptr(out["dt"]), dz=_ptr(out.get("z")), dB=_ptr(out["B"]),
