@@ -55,22 +55,37 @@ struct Ptrs {
   float* dstart;
 };
 
+// exp(-|x|), to about an ulp: the product with log2 e is corrected for its own rounding (r), which the plain
+// exp2(x log2 e) magnifies by |x|.  Past 88 the result is that of 88 (below the smallest normal number); NaN
+// stays NaN.  Seven operations and the exponential, where expf takes some twenty, and every token of a
+// channel needs two or three.
+__device__ __forceinline__ float exp_minus_abs(float x) {
+  constexpr float LOG2E_REST = 1.92596303e-8f;  // log2 e - LOG2E
+  constexpr float LN2 = 0.69314718f;
+  float a = fabsf(x);
+  a = a > 88.f ? 88.f : a;
+  const float t = -a * LOG2E, r = fmaf(-a, LOG2E_REST, fmaf(-a, LOG2E, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, r * LN2, e);
+}
 // log(1 + exp(x)) with log1p by 2 atanh(e / (2 + e)): exact to about an ulp over the whole range, which
-// log(1 + e) is not for the small steps that training starts from.
+// log(1 + e) is not for the small steps that training starts from.  The series' first term left out is below
+// 2^-26 at e = 1.
 __device__ __forceinline__ float softplus(float x) {
-  const float e = expf(-fabsf(x)), s = e / (2.f + e), q = s * s;
-  float p = 1.f / 17.f;
-  p = fmaf(p, q, 1.f / 15.f);
-  p = fmaf(p, q, 1.f / 13.f);
+  const float e = exp_minus_abs(x), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+  float p = 1.f / 13.f;
   p = fmaf(p, q, 1.f / 11.f);
   p = fmaf(p, q, 1.f / 9.f);
   p = fmaf(p, q, 1.f / 7.f);
   p = fmaf(p, q, 1.f / 5.f);
   p = fmaf(p, q, 1.f / 3.f);
   p = fmaf(p, q, 1.f);
-  return fmaxf(x, 0.f) + 2.f * s * p;
+  return fmaf(2.f * s, p, fmaxf(x, 0.f));
 }
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+__device__ __forceinline__ float sigmoid(float x) {
+  const float e = exp_minus_abs(x);
+  return (x < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+}
 
 // The own tokens of sequence b (the same in every lane that asks for the same b).
 __device__ __forceinline__ int seq_len(const int32_t* lengths, int64_t b, int T) {
@@ -136,8 +151,8 @@ struct Unit {
 };
 
 // Rows of C channels behind one scalar address, reached by a lane's offset and a scalar one, so that no lane
-// holds addresses.  The buffer's bounds hold a lane's offset, not the scalar one: `load` and `store` take rows
-// that exist, `store_in` adds the row to the lane's offset and does nothing past the last one.
+// holds addresses.  The buffer's bounds hold a lane's offset (which is how lanes without a channel write
+// nothing), not the scalar one: `load` and `store` take rows that exist.
 template <typename T>
 struct Rows {
   __amdgpu_buffer_rsrc_t buf;
@@ -147,22 +162,43 @@ struct Rows {
       : stride(static_cast<int>(token) * static_cast<int>(sizeof(T))) {
     buf = dev_buf(row, static_cast<uint32_t>((rows - 1) * stride + C * static_cast<int>(sizeof(T))));
   }
-  __device__ __forceinline__ T load(int lane, int i) const {
+  // The value's bits in a register of its own: a load into half a register would be waited for at once.
+  __device__ __forceinline__ unsigned load(int lane, int i) const {
     if constexpr (sizeof(T) == 2)
-      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(buf, lane, i * stride, 0));
+      return static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(buf, lane, i * stride, 0));
     else
-      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(buf, lane, i * stride, 0));
+      return __builtin_amdgcn_raw_buffer_load_b32(buf, lane, i * stride, 0);
   }
-  __device__ __forceinline__ void put(int lane, int scalar, float v) const {
+  __device__ __forceinline__ void store(int lane, int i, float v) const {
     const T t = from_f32<T>(v);
     if constexpr (sizeof(T) == 2)
-      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t), buf, lane, scalar, 0);
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t), buf, lane, i * stride, 0);
     else
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, t), buf, lane, scalar, 0);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, t), buf, lane, i * stride, 0);
   }
-  __device__ __forceinline__ void store(int lane, int i, float v) const { put(lane, i * stride, v); }
-  __device__ __forceinline__ void store_in(int lane, int i, float v) const { put(lane + i * stride, 0, v); }
 };
+
+// The first n of a segment's values into contiguous rows from `row` on.
+template <typename T>
+__device__ __forceinline__ void put_seg(void* base, int64_t row, int n, int C, int lane, const float (&v)[SEG]) {
+  const Rows<T> rows(static_cast<T*>(base) + row, C, n, C);
+  if (n == SEG) {
+#pragma unroll
+    for (int i = 0; i < SEG; ++i) rows.store(lane, i, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < SEG; ++i)
+      if (i < n) rows.store(lane, i, v[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float value(unsigned bits) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_bit_cast(float, bits);
+  else
+    return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+}
 
 __device__ __forceinline__ int live(int t, int end) { return end - t < SEG ? end - t : SEG; }
 
@@ -170,16 +206,16 @@ __device__ __forceinline__ int live(int t, int end) { return end - t < SEG ? end
 // (which is past t) read the last own one; `widen` and `steps` put zeros in their place.
 template <typename T>
 __device__ __forceinline__ void fetch(const void* base, int64_t batch, int64_t token, int t, int end, int C, int lane,
-                                      T (&v)[SEG]) {
+                                      unsigned (&v)[SEG]) {
   const int n = live(t, end);
   const Rows<T> rows(static_cast<const T*>(base) + batch + t * token, token, n, C);
 #pragma unroll
   for (int i = 0; i < SEG; ++i) v[i] = rows.load(lane, i < n ? i : n - 1);
 }
 template <typename T>
-__device__ __forceinline__ void widen(const T (&r)[SEG], int t, int end, float (&v)[SEG]) {
+__device__ __forceinline__ void widen(const unsigned (&r)[SEG], int t, int end, float (&v)[SEG]) {
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) v[i] = to_f32(r[i]);
+  for (int i = 0; i < SEG; ++i) v[i] = value<T>(r[i]);
   if (t + SEG > end) {
 #pragma unroll
     for (int i = 0; i < SEG; ++i) v[i] = t + i < end ? v[i] : 0.f;
@@ -188,9 +224,9 @@ __device__ __forceinline__ void widen(const T (&r)[SEG], int t, int end, float (
 
 // Step sizes from dt; no time passes behind a sequence's end.
 template <typename T>
-__device__ __forceinline__ void steps(const Dims& d, const T (&r)[SEG], int t, int end, float bias, float (&s)[SEG]) {
+__device__ __forceinline__ void steps(const Dims& d, const unsigned (&r)[SEG], int t, int end, float bias, float (&s)[SEG]) {
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) s[i] = to_f32(r[i]) + bias;
+  for (int i = 0; i < SEG; ++i) s[i] = value<T>(r[i]) + bias;
   if (d.softplus) {
 #pragma unroll
     for (int i = 0; i < SEG; ++i) s[i] = softplus(s[i]);
@@ -212,6 +248,67 @@ __device__ __forceinline__ Row load_row(const float* tiles, int64_t at) {
   return r;
 }
 
+// Reads a word of each of a tile's 128-byte rows through the vector unit, a segment ahead of their scalar
+// loads: those then find them in the XCD's L2 and not 2000 cycles away in memory, longer than a row's SEG
+// tokens take.  `done` uses the words once they are there.
+struct Warm {
+  float got = 0.f;
+  __device__ __forceinline__ void start(const float* tiles, int64_t tile, int N, int lane) {
+    got = 0.f;
+    for (int n = lane; n < N; n += 64) got += tiles[tile + n * 2 * SEG];
+  }
+  __device__ __forceinline__ void done() {
+    asm volatile("" ::"v"(got));
+  }
+};
+
+// Scalar loads come back in any order, so a wait for one is a wait for all: it stands in front of the next
+// row's load, where what it waits for was asked for a whole row's work ago (behind that load, where the
+// compiler would put it, every row waits for memory: 75 us instead of 55 for the outputs of 8 x 4096 x 256).
+constexpr int WAITCNT_LGKM0 = 0xC07F;  // s_waitcnt lgkmcnt(0), the other counts left open
+__device__ __forceinline__ void rows_arrived() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(WAITCNT_LGKM0);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A lane's per-state values (a state or its gradient, and the decay exponent A log2 e): the lane's columns of
+// [N][64] arrays in LDS.  They could stay in registers only with the walk over the states unrolled, and that
+// is slower: some 20 KB of code, which a wave runs through once a segment, are fetched slower than they run.
+struct States {
+  float *v, *a;
+  __device__ __forceinline__ States(float* lds, int wave, int lane, int N) {
+    v = lds + wave * 2 * N * 64 + lane;
+    a = v + N * 64;
+  }
+  // f(row, value, exponent, n) for every state, which updates the value: two rows in turn, the next state's
+  // row and values on their way while f runs over SEG tokens, and the last state's value on its way back.
+  template <typename F>
+  __device__ __forceinline__ void walk(const float* tiles, int64_t tile, int N, F f) {
+    Row r0 = load_row(tiles, tile), r1;
+    float v0 = v[0], a0 = a[0], v1, a1, done = v0;
+    float* back = v;
+    for (int n = 0; n < N; n += 2) {
+      int m = n + 1 < N ? n + 1 : n;
+      rows_arrived();
+      r1 = load_row(tiles, tile + m * 2 * SEG);
+      v1 = v[m * 64], a1 = a[m * 64];
+      *back = done;
+      f(r0, v0, a0, n);
+      done = v0, back = v + n * 64;
+      if (n + 1 >= N) break;
+      m = n + 2 < N ? n + 2 : n;
+      rows_arrived();
+      r0 = load_row(tiles, tile + m * 2 * SEG);
+      v0 = v[m * 64], a0 = a[m * 64];
+      *back = done;
+      f(r1, v1, a1, n + 1);
+      done = v1, back = v + (n + 1) * 64;
+    }
+    *back = done;
+  }
+};
+
 // AGG: the chunk's end state from zero and its total step size.  Else: y, the final state (its last chunk)
 // and, where wanted, the states at every segment's start.
 template <typename T, bool AGG>
@@ -219,32 +316,37 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
   extern __shared__ float lds[];
   const Unit w(d, p.lengths);
   if (!w.any || (AGG && w.chunk == d.chunks - 1)) return;
-  float* const hs = lds + w.wave * 2 * d.N * 64 + w.lane;  // states and decay exponents [N][64]
-  float* const as = hs + d.N * 64;
-  for (int n = 0; n < d.N; ++n) {
-    const int64_t at = static_cast<int64_t>(n) * d.C + w.c;
-    as[n * 64] = p.at[at] * LOG2E;
-    float h = 0.f;
-    if (!AGG) {
-      if (d.chunks > 1)
-        h = p.hloc[w.u * d.N * d.C + at];
-      else if (p.start)
-        h = p.start[(w.b * d.C + w.c) * d.N + n];
-    }
-    hs[n * 64] = h;
-  }
-  const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = !AGG && p.D ? p.D[w.c] : 0.f;
-  float total = 0.f;
   const int stop = w.t1 < w.end ? w.t1 : w.end;  // behind it: zeros, and the states stay
   const int in = w.in<T>(), out = w.in<T>(true), out32 = w.in<float>(true);
-  T ur[SEG], dr[SEG], zr[SEG];
+  unsigned ur[SEG], dr[SEG], zr[SEG];
   auto read = [&](int t) {
     fetch<T>(p.u, w.b * p.ub, p.ut, t, stop, d.C, in, ur);
     fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, stop, d.C, in, dr);
     if constexpr (!AGG)
       if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, stop, d.C, in, zr);
   };
-  if (w.t0 < stop) read(w.t0);
+  Warm warm;
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.N * 2 * SEG; };
+  if (w.t0 < stop) {
+    warm.start(p.tiles, tile_of(w.t0), d.N, w.lane);
+    read(w.t0);
+  }
+  States states(lds, w.wave, w.lane, d.N);
+#pragma unroll 8
+  for (int n = 0; n < d.N; ++n) {
+    const int64_t at = static_cast<int64_t>(n) * d.C + w.c;
+    float h = 0.f;
+    if constexpr (!AGG) {
+      if (d.chunks > 1)
+        h = p.hloc[w.u * d.N * d.C + at];
+      else if (p.start)
+        h = p.start[(w.b * d.C + w.c) * d.N + n];
+    }
+    states.v[n * 64] = h;
+    states.a[n * 64] = p.at[at] * LOG2E;
+  }
+  const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = !AGG && p.D ? p.D[w.c] : 0.f;
+  float total = 0.f;
   for (int t = w.t0; t < stop; t += SEG) {
     float s[SEG], x[SEG], y[SEG], gate[SEG];
     widen<T>(ur, t, stop, x);
@@ -263,71 +365,93 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
         for (int i = 0; i < SEG; ++i) gate[i] *= sigmoid(gate[i]);
       }
     }
-    if (t + SEG < stop) read(t + SEG);  // the next segment's values arrive while this one is computed
-    const int64_t tile = (w.bg * d.segs + t / SEG) * d.N * 2 * SEG;
+    warm.done();
+    if (t + SEG < stop) {  // the next segment's values arrive while this one is computed
+      warm.start(p.tiles, tile_of(t + SEG), d.N, w.lane);
+      read(t + SEG);
+    }
     const Rows<float> ckpt(p.ckpt + (w.b * d.segs + t / SEG) * d.N * d.C, d.C, d.N, d.C);
-    Row r = load_row(p.tiles, tile);
-    float h = hs[0], a = as[0];
-    for (int n = 0; n < d.N; ++n) {
-      const int m = n + 1 < d.N ? n + 1 : n;  // the next state's values likewise
-      const Row rn = load_row(p.tiles, tile + m * 2 * SEG);
-      const float hn = hs[m * 64], an = as[m * 64];
+    states.walk(p.tiles, tile_of(t), d.N, [&](const Row& r, float& h, float a, int n) {
       if (!AGG && p.ckpt) ckpt.store(out32, n, h);
 #pragma unroll
       for (int i = 0; i < SEG; ++i) {
         h = fmaf(__builtin_amdgcn_exp2f(s[i] * a), h, x[i] * r.B[i]);
         if constexpr (!AGG) y[i] = fmaf(r.C[i], h, y[i]);
       }
-      hs[n * 64] = h;
-      r = rn, h = hn, a = an;
-    }
+    });
     if constexpr (!AGG) {
-      const Rows<T> rows(static_cast<T*>(p.y) + (w.b * d.T + t) * d.C, d.C, live(t, stop), d.C);
 #pragma unroll
-      for (int i = 0; i < SEG; ++i) rows.store_in(out, i, y[i] * gate[i]);
+      for (int i = 0; i < SEG; ++i) y[i] *= gate[i];
+      put_seg<T>(p.y, (w.b * d.T + t) * d.C, live(t, stop), d.C, out, y);
     }
-  }
-  if constexpr (!AGG) {
-    if (w.ok)
-      for (int64_t t = w.t0 < stop ? stop : w.t0; t < w.t1; ++t)
-        static_cast<T*>(p.y)[(w.b * d.T + t) * d.C + w.c] = from_f32<T>(0.f);
   }
   if (!w.ok) return;
   if constexpr (AGG) {
-    for (int n = 0; n < d.N; ++n) p.hloc[(w.u * d.N + n) * d.C + w.c] = hs[n * 64];
+    for (int n = 0; n < d.N; ++n) p.hloc[(w.u * d.N + n) * d.C + w.c] = states.v[n * 64];
     p.ssum[w.u * d.C + w.c] = total;
-  } else if (p.end && w.chunk == d.chunks - 1) {
-    for (int n = 0; n < d.N; ++n) p.end[(w.b * d.C + w.c) * d.N + n] = hs[n * 64];
+  } else {
+    for (int64_t t = w.t0 < stop ? stop : w.t0; t < w.t1; ++t)
+      static_cast<T*>(p.y)[(w.b * d.T + t) * d.C + w.c] = from_f32<T>(0.f);
+    if (p.end && w.chunk == d.chunks - 1)
+      for (int n = 0; n < d.N; ++n) p.end[(w.b * d.C + w.c) * d.N + n] = states.v[n * 64];
   }
 }
 
 // The chunks' start values from their own ends, in place: hloc[b, chunk, n, c] <- the value that enters the
 // chunk.  Forward: from the first chunk on, starting with the given state.  BACK: the gradient that enters
-// a chunk from behind, from the last chunk on, starting with the final state's gradient.
+// a chunk from behind, from the last chunk on, starting with the final state's gradient.  Block: 64 (b, n, c)
+// by up to 16 waves, each of which holds the values of JOIN neighbouring chunks in registers: their loads go
+// out together, their joint end and decay meet the other waves' in LDS, and longer sequences take another
+// round (22 us for 64 chunks one after the other, 9 with 16 loads at a time).
+constexpr int JOIN = 8;
 template <bool BACK>
-__global__ __launch_bounds__(256) void k_sel_join(Dims d, Ptrs p) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= d.B * d.N * d.C) return;
+__global__ __launch_bounds__(1024) void k_sel_join(Dims d, Ptrs p) {
+  __shared__ float ends[16][64], decays[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int64_t total = d.B * d.N * d.C, i0 = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  const int64_t i = i0 < total ? i0 : total - 1;
   const int64_t c = i % d.C, n = i / d.C % d.N, b = i / d.C / d.N;
   const float a = p.at[n * d.C + c] * LOG2E;
   const float* const first = BACK ? p.dend : p.start;
-  float h = first ? first[(b * d.C + c) * d.N + n] : 0.f;
-  constexpr int AHEAD = 16;  // chunks whose values are read together: the chain itself is short
-  for (int k0 = 0; k0 < d.chunks; k0 += AHEAD) {
-    float own[AHEAD], decay[AHEAD];
+  float carry = first ? first[(b * d.C + c) * d.N + n] : 0.f;
+  for (int k0 = 0; k0 < d.chunks; k0 += waves * JOIN) {
+    float own[JOIN], decay[JOIN];
+    auto unit = [&](int j) {
+      const int k = k0 + wave * JOIN + j;
+      return b * d.chunks + (BACK ? d.chunks - 1 - k : k);
+    };
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int k = k0 + j < d.chunks - 1 ? k0 + j : d.chunks - 2;  // the last chunk's own values are not used
-      const int64_t u = b * d.chunks + (BACK ? d.chunks - 1 - k : k);
-      own[j] = p.hloc[(u * d.N + n) * d.C + c];
-      decay[j] = p.ssum[u * d.C + c];
+    for (int j = 0; j < JOIN; ++j) {
+      own[j] = 0.f, decay[j] = 0.f;  // the last chunk's own values are not used
+      if (k0 + wave * JOIN + j < d.chunks - 1) {
+        own[j] = p.hloc[(unit(j) * d.N + n) * d.C + c];
+        decay[j] = p.ssum[unit(j) * d.C + c];
+      }
     }
+    float h = 0.f, steps = 0.f;
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int k = k0 + j;
-      if (k < d.chunks) p.hloc[((b * d.chunks + (BACK ? d.chunks - 1 - k : k)) * d.N + n) * d.C + c] = h;
-      h = fmaf(__builtin_amdgcn_exp2f(decay[j] * a), h, own[j]);
+    for (int j = 0; j < JOIN; ++j) {
+      steps += decay[j];
+      decay[j] = __builtin_amdgcn_exp2f(decay[j] * a);
+      h = fmaf(decay[j], h, own[j]);
     }
+    ends[wave][lane] = h;
+    decays[wave][lane] = __builtin_amdgcn_exp2f(steps * a);
+    __syncthreads();
+    h = carry;
+    for (int k = 0; k < waves; ++k) {
+      if (k == wave) {
+        float g = h;
+#pragma unroll
+        for (int j = 0; j < JOIN; ++j) {
+          if (k0 + wave * JOIN + j < d.chunks && i0 < total) p.hloc[(unit(j) * d.N + n) * d.C + c] = g;
+          g = fmaf(decay[j], g, own[j]);
+        }
+      }
+      h = fmaf(decays[k][lane], h, ends[k][lane]);
+    }
+    carry = h;
+    __syncthreads();
   }
 }
 
@@ -337,20 +461,28 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
   extern __shared__ float lds[];
   const Unit w(d, p.lengths);
   if (!w.any || w.chunk == 0) return;
-  float* const qs = lds + w.wave * 2 * d.N * 64 + w.lane;
-  float* const as = qs + d.N * 64;
-  for (int n = 0; n < d.N; ++n) qs[n * 64] = 0.f, as[n * 64] = p.at[static_cast<int64_t>(n) * d.C + w.c] * LOG2E;
-  const float bias = p.bias ? p.bias[w.c] : 0.f;
-  float total = 0.f;
   const int stop = w.t1 < w.end ? w.t1 : w.end, in = w.in<T>();
-  T er[SEG], dr[SEG], zr[SEG];
+  unsigned er[SEG], dr[SEG], zr[SEG];
   auto read = [&](int t) {
     fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, stop, d.C, in, er);
     fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, stop, d.C, in, dr);
     if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, stop, d.C, in, zr);
   };
   const int last = stop > w.t0 ? (stop - 1) / SEG * SEG : w.t0 - SEG;
-  if (last >= w.t0) read(last);
+  Warm warm;
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.N * 2 * SEG; };
+  if (last >= w.t0) {
+    warm.start(p.tiles, tile_of(last), d.N, w.lane);
+    read(last);
+  }
+  States states(lds, w.wave, w.lane, d.N);
+#pragma unroll 8
+  for (int n = 0; n < d.N; ++n) {
+    states.v[n * 64] = 0.f;
+    states.a[n * 64] = p.at[static_cast<int64_t>(n) * d.C + w.c] * LOG2E;
+  }
+  const float bias = p.bias ? p.bias[w.c] : 0.f;
+  float total = 0.f;
   for (int t = last; t >= w.t0; t -= SEG) {
     float s[SEG], e[SEG];
     widen<T>(er, t, stop, e);
@@ -361,24 +493,20 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
 #pragma unroll
       for (int i = 0; i < SEG; ++i) e[i] *= z[i] * sigmoid(z[i]);
     }
-    if (t > w.t0) read(t - SEG);
+    warm.done();
+    if (t > w.t0) {
+      warm.start(p.tiles, tile_of(t - SEG), d.N, w.lane);
+      read(t - SEG);
+    }
 #pragma unroll
     for (int i = 0; i < SEG; ++i) total += s[i];
-    const int64_t tile = (w.bg * d.segs + t / SEG) * d.N * 2 * SEG;
-    Row r = load_row(p.tiles, tile);
-    float q = qs[0], a = as[0];
-    for (int n = 0; n < d.N; ++n) {
-      const int m = n + 1 < d.N ? n + 1 : n;
-      const Row rn = load_row(p.tiles, tile + m * 2 * SEG);
-      const float qn = qs[m * 64], an = as[m * 64];
+    states.walk(p.tiles, tile_of(t), d.N, [&](const Row& r, float& q, float a, int) {
 #pragma unroll
       for (int i = SEG - 1; i >= 0; --i) q = fmaf(e[i], r.C[i], q) * __builtin_amdgcn_exp2f(s[i] * a);
-      qs[n * 64] = q;
-      r = rn, q = qn, a = an;
-    }
+    });
   }
   if (!w.ok) return;
-  for (int n = 0; n < d.N; ++n) p.hloc[(w.u * d.N + n) * d.C + w.c] = qs[n * 64];
+  for (int n = 0; n < d.N; ++n) p.hloc[(w.u * d.N + n) * d.C + w.c] = states.v[n * 64];
   p.ssum[w.u * d.C + w.c] = total;
 }
 
@@ -428,8 +556,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
   extern __shared__ float lds[];
   const Unit w(d, p.lengths);
   const int waves = blockDim.x >> 6, N = d.N;
-  float* const qs = lds + w.wave * 2 * N * 64 + w.lane;  // gradients from behind and dA [N][64]
-  float* const ga = qs + N * 64;
+  States grads(lds, w.wave, w.lane, N);  // the gradients from behind, and dA in the place of the exponents
+  float *const qs = grads.v, *const ga = grads.a;
   float* const sums = lds + waves * 2 * N * 64;          // [wave][n][B: SEG, C: SEG]
   const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = p.D ? p.D[w.c] : 0.f;
   float dD = 0.f, dbias = 0.f;
@@ -447,17 +575,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
   const int64_t cb = blockIdx.x % bpg;  // this block's place among those of its group
   const int in = w.in<T>(), out_t = w.in<T>(true), in32 = w.in<float>();
   const Rows<float> at(p.at, d.C, N, d.C);
+  Warm warm;
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * N * 2 * SEG; };
+  warm.start(p.tiles, tile_of(w.t1 - 1), N, w.lane);
   for (int t = (w.t1 - 1) / SEG * SEG; t >= w.t0; t -= SEG) {
     const int64_t seg = t / SEG, row = (w.b * d.T + t) * d.C;
     const int rows = live(t, w.t1);  // tokens that the tensors have
-    const Rows<T> du_out(static_cast<T*>(p.du) + row, d.C, rows, d.C);
-    const Rows<T> ddt_out(static_cast<T*>(p.ddt) + row, d.C, rows, d.C);
-    const Rows<T> dz_out(static_cast<T*>(p.dz) + row, d.C, p.z ? rows : 1, d.C);
     if (t < w.end) {
       if (w.any) {
         float u[SEG], s[SEG], e[SEG], y[SEG], gb[SEG], gs[SEG];
         {
-          T ur[SEG], dr[SEG], er[SEG], zr[SEG];
+          unsigned ur[SEG], dr[SEG], er[SEG], zr[SEG];
           fetch<T>(p.u, w.b * p.ub, p.ut, t, w.end, d.C, in, ur);
           fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, d.C, in, dr);
           fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, d.C, in, er);
@@ -476,15 +604,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
           e[i] = w.ok ? e[i] : 0.f;  // lanes without a channel add nothing to the sums over channels
           y[i] = gb[i] = gs[i] = 0.f;
         }
-        const int64_t tile = (w.bg * d.segs + seg) * N * 2 * SEG;
+        warm.done();
+        if (t > w.t0) warm.start(p.tiles, tile_of(t - SEG), N, w.lane);
+        const int64_t tile = tile_of(t);
         const Rows<float> ckpt(p.ckpt_in + (w.b * d.segs + seg) * N * d.C, d.C, N, d.C);
-        Row r = load_row(p.tiles, tile);
-        float an = at.load(in32, 0), h0 = ckpt.load(in32, 0);
-        for (int n = 0; n < N; ++n) {
-          const int m = n + 1 < N ? n + 1 : n;  // the next state's values arrive while this one is computed
-          const Row rn = load_row(p.tiles, tile + m * 2 * SEG);
-          const float ann = at.load(in32, m), hn = ckpt.load(in32, m);
-          const float a2 = an * LOG2E;
+        float an_next = value<float>(at.load(in32, 0)), h0_next = value<float>(ckpt.load(in32, 0));
+        grads.walk(p.tiles, tile, N, [&](const Row& r, float& q, float dA, int n) {
+          const int m = n + 1 < N ? n + 1 : n;
+          const float an = an_next, h0 = h0_next, a2 = an * LOG2E;
+          an_next = value<float>(at.load(in32, m)), h0_next = value<float>(ckpt.load(in32, m));
           float a[SEG], h[SEG], v[2 * SEG];
 #pragma unroll
           for (int i = 0; i < SEG; ++i) {
@@ -493,7 +621,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
             y[i] = fmaf(r.C[i], h[i], y[i]);
             v[SEG + i] = e[i] * h[i];
           }
-          float q = qs[n * 64], dA = ga[n * 64];
 #pragma unroll
           for (int i = SEG - 1; i >= 0; --i) {
             q = fmaf(e[i], r.C[i], q);
@@ -504,45 +631,53 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
             gs[i] = fmaf(through, an, gs[i]);
             dA = fmaf(through, s[i], dA);
           }
-          qs[n * 64] = q;
           ga[n * 64] = dA;
           const float total = lane_sums(v, w.lane);
           if ((w.lane & 1) == 0) sums[(w.wave * N + n) * 2 * SEG + (w.lane >> 1)] = total;
-          r = rn, an = ann, h0 = hn;
-        }
+        });
         // what needs dy, z and dt once more reads them again (from the caches), not earlier than here: the
         // loop over the states needs the registers
         asm volatile("" ::: "memory");
-        T raw[SEG], dy[SEG], zr[SEG];
+        unsigned raw[SEG], dy[SEG], zr[SEG];
         fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, d.C, in, raw);
         fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, d.C, in, dy);
         if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, w.end, d.C, in, zr);
 #pragma unroll
         for (int i = 0; i < SEG; ++i) {
-          const bool own = t + i < w.end;
-          const float du = fmaf(gb[i], s[i], e[i] * dskip);
-          float ds = fmaf(gb[i], u[i], gs[i]);
-          if (d.softplus) ds *= sigmoid(to_f32(raw[i]) + bias);
-          dD += e[i] * u[i];
-          dbias += own ? ds : 0.f;
-          du_out.store_in(out_t, i, own ? du : 0.f);
-          ddt_out.store_in(out_t, i, own ? ds : 0.f);
-          if (p.z) {
-            const float z = to_f32(zr[i]), sg = sigmoid(z), yv = fmaf(dskip, u[i], y[i]);
-            const float dz = to_f32(dy[i]) * yv * sg * (1.f + z * (1.f - sg));
-            dz_out.store_in(out_t, i, own ? dz : 0.f);
+          dD = fmaf(e[i], u[i], dD);
+          y[i] = fmaf(dskip, u[i], y[i]);
+          gs[i] = fmaf(gb[i], u[i], gs[i]);                // d step
+          gb[i] = fmaf(gb[i], s[i], e[i] * dskip);         // du
+        }
+        if (d.softplus) {
+#pragma unroll
+          for (int i = 0; i < SEG; ++i) gs[i] *= sigmoid(value<T>(raw[i]) + bias);
+        }
+        if (p.z) {
+#pragma unroll
+          for (int i = 0; i < SEG; ++i) {
+            const float z = value<T>(zr[i]), sg = sigmoid(z);
+            y[i] *= value<T>(dy[i]) * sg * fmaf(z, 1.f - sg, 1.f);  // dz
           }
         }
+        if (t + SEG > w.end) {
+#pragma unroll
+          for (int i = 0; i < SEG; ++i)
+            if (t + i >= w.end) gb[i] = gs[i] = y[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) dbias += gs[i];
+        put_seg<T>(p.du, row, rows, d.C, out_t, gb);
+        put_seg<T>(p.ddt, row, rows, d.C, out_t, gs);
+        if (p.z) put_seg<T>(p.dz, row, rows, d.C, out_t, y);
       } else {
         for (int i = w.lane; i < N * 2 * SEG; i += 64) sums[w.wave * N * 2 * SEG + i] = 0.f;
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < SEG; ++i) {
-        du_out.store_in(out_t, i, 0.f);
-        ddt_out.store_in(out_t, i, 0.f);
-        if (p.z) dz_out.store_in(out_t, i, 0.f);
-      }
+      const float none[SEG] = {};
+      put_seg<T>(p.du, row, rows, d.C, out_t, none);
+      put_seg<T>(p.ddt, row, rows, d.C, out_t, none);
+      if (p.z) put_seg<T>(p.dz, row, rows, d.C, out_t, none);
     }
     __syncthreads();
     float* const out = p.pBC + ((cb * d.B * d.G + w.bg) * d.T + t) * 2 * N;
@@ -748,29 +883,37 @@ unsigned unit_blocks(const Dims& d, int waves) {
   return static_cast<unsigned>(cdiv(d.cbg, waves) * d.G * d.chunks * d.B);
 }
 
+unsigned states_lds(const Dims& d, int waves) { return waves * 2 * d.N * 64 * 4; }
+
+template <bool BACK>
+void launch_join(const Dims& d, const Ptrs& p, hipStream_t st) {
+  const int waves = static_cast<int>(std::min<int64_t>(16, cdiv(d.chunks, JOIN)));
+  k_sel_join<BACK><<<static_cast<unsigned>(cdiv(d.B * d.N * d.C, 64)), 64 * waves, 0, st>>>(d, p);
+}
+
 template <typename T>
 int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
   const int waves = waves_for(d, false);
-  const unsigned blocks = unit_blocks(d, waves), lds = waves * 2 * d.N * 64 * 4;
+  const unsigned blocks = unit_blocks(d, waves);
   k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.N + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
   if (d.chunks > 1) {
-    k_sel_scan<T, true><<<blocks, 64 * waves, lds, st>>>(d, p);
-    k_sel_join<false><<<grid256(d.B * d.N * d.C), 256, 0, st>>>(d, p);
+    k_sel_scan<T, true><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
+    launch_join<false>(d, p, st);
   }
-  k_sel_scan<T, false><<<blocks, 64 * waves, lds, st>>>(d, p);
+  k_sel_scan<T, false><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
   return check_launch("selective_scan");
 }
 
 template <typename T>
 int run_grad(const Dims& d, Ptrs p, const lng_selective_grad& g, hipStream_t st) {
   const int waves = waves_for(d, true);
-  const unsigned blocks = unit_blocks(d, waves), lds = waves * 2 * d.N * 64 * 4;
+  const unsigned blocks = unit_blocks(d, waves);
   k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.N + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
   if (d.chunks > 1) {
-    k_sel_grad_ends<T><<<blocks, 64 * waves, lds, st>>>(d, p);
-    k_sel_join<true><<<grid256(d.B * d.N * d.C), 256, 0, st>>>(d, p);
+    k_sel_grad_ends<T><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
+    launch_join<true>(d, p, st);
   }
-  k_sel_grad<T><<<blocks, 64 * waves, lds + waves * d.N * 2 * SEG * 4, st>>>(d, p);
+  k_sel_grad<T><<<blocks, 64 * waves, states_lds(d, waves) + waves * d.N * 2 * SEG * 4, st>>>(d, p);
   k_sel_grad_bc<T><<<grid256(d.B * d.G * d.T * 2 * d.N), 256, 0, st>>>(
       d, p.pBC, static_cast<int>(cdiv(d.cbg, waves)), static_cast<T*>(g.dB), static_cast<T*>(g.dC));
   k_sel_grad_a<<<static_cast<unsigned>(cdiv(int64_t{d.N + 2} * d.C, 64)), 256, 0, st>>>(d, p.pA, p.pD, g.dA, g.dD,
