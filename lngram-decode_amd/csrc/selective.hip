@@ -20,14 +20,15 @@
 //
 // Where batch * channels gives too few waves, the time axis is cut into chunks: the chunks' own end states
 // (from zero) and total step sizes, then their start states from one short pass over the chunks, then every
-// chunk from its start.  The backward pass does the same for q, backwards, and takes the states of a
-// segment's start from the forward pass (N / SEG floats a (token, channel)).
+// chunk from its start.  The backward pass does the same for q, backwards, and takes the states of
+// every GSEG tokens' start from the forward pass (N / GSEG floats a (token, channel)).
 #include "common.h"
 
 namespace lng {
 namespace {
 
-constexpr int SEG = 16;   // tokens of a segment
+constexpr int SEG = 16;   // tokens of a tile, and of the forward pass's segments
+constexpr int GSEG = 8;   // tokens of the backward pass's segments, whose first states the forward pass leaves
 constexpr int WAVES = 4;  // waves of a block: neighbouring channels of one chunk
 constexpr int MAX_N = 256;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -36,7 +37,7 @@ typedef const float __attribute__((address_space(4))) cfloat;  // read through t
 
 struct Dims {
   int64_t B;
-  int T, chunk, segs;        // chunk: tokens of a chunk, a multiple of SEG; segs: segments of a sequence
+  int T, chunk, segs, gsegs;  // chunk: tokens of a chunk, a multiple of SEG; segs, gsegs: a sequence's segments
   int C, N, G, chunks, cbg;  // cbg: channel blocks of 64 in a group
   int softplus;
 };
@@ -179,15 +180,15 @@ struct Rows {
 };
 
 // The first n of a segment's values into contiguous rows from `row` on.
-template <typename T>
-__device__ __forceinline__ void put_seg(void* base, int64_t row, int n, int C, int lane, const float (&v)[SEG]) {
+template <typename T, int S>
+__device__ __forceinline__ void put_seg(void* base, int64_t row, int n, int C, int lane, const float (&v)[S]) {
   const Rows<T> rows(static_cast<T*>(base) + row, C, n, C);
-  if (n == SEG) {
+  if (n == S) {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) rows.store(lane, i, v[i]);
+    for (int i = 0; i < S; ++i) rows.store(lane, i, v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i)
+    for (int i = 0; i < S; ++i)
       if (i < n) rows.store(lane, i, v[i]);
   }
 }
@@ -200,51 +201,56 @@ __device__ __forceinline__ float value(unsigned bits) {
     return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
 }
 
-__device__ __forceinline__ int live(int t, int end) { return end - t < SEG ? end - t : SEG; }
+template <int S>
+__device__ __forceinline__ int live(int t, int end) {
+  return end - t < S ? end - t : S;
+}
 
-// A segment's values of one tensor, as stored: SEG loads that go out together.  Tokens at and behind `end`
+// A segment's values of one tensor, as stored: loads that go out together.  Tokens at and behind `end`
 // (which is past t) read the last own one; `widen` and `steps` put zeros in their place.
-template <typename T>
+template <typename T, int S>
 __device__ __forceinline__ void fetch(const void* base, int64_t batch, int64_t token, int t, int end, int C, int lane,
-                                      unsigned (&v)[SEG]) {
-  const int n = live(t, end);
+                                      unsigned (&v)[S]) {
+  const int n = live<S>(t, end);
   const Rows<T> rows(static_cast<const T*>(base) + batch + t * token, token, n, C);
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) v[i] = rows.load(lane, i < n ? i : n - 1);
+  for (int i = 0; i < S; ++i) v[i] = rows.load(lane, i < n ? i : n - 1);
 }
-template <typename T>
-__device__ __forceinline__ void widen(const unsigned (&r)[SEG], int t, int end, float (&v)[SEG]) {
+template <typename T, int S>
+__device__ __forceinline__ void widen(const unsigned (&r)[S], int t, int end, float (&v)[S]) {
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) v[i] = value<T>(r[i]);
-  if (t + SEG > end) {
+  for (int i = 0; i < S; ++i) v[i] = value<T>(r[i]);
+  if (t + S > end) {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) v[i] = t + i < end ? v[i] : 0.f;
+    for (int i = 0; i < S; ++i) v[i] = t + i < end ? v[i] : 0.f;
   }
 }
 
 // Step sizes from dt; no time passes behind a sequence's end.
-template <typename T>
-__device__ __forceinline__ void steps(const Dims& d, const unsigned (&r)[SEG], int t, int end, float bias, float (&s)[SEG]) {
+template <typename T, int S>
+__device__ __forceinline__ void steps(const Dims& d, const unsigned (&r)[S], int t, int end, float bias, float (&s)[S]) {
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) s[i] = value<T>(r[i]) + bias;
+  for (int i = 0; i < S; ++i) s[i] = value<T>(r[i]) + bias;
   if (d.softplus) {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) s[i] = softplus(s[i]);
+    for (int i = 0; i < S; ++i) s[i] = softplus(s[i]);
   }
-  if (t + SEG > end) {
+  if (t + S > end) {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) s[i] = t + i < end ? s[i] : 0.f;
+    for (int i = 0; i < S; ++i) s[i] = t + i < end ? s[i] : 0.f;
   }
 }
 
-struct Row {  // B and C of one state over a segment's tokens
-  float B[SEG], C[SEG];
+template <int S>
+struct Row {  // B and C of one state over S of a tile's tokens
+  float B[S], C[S];
 };
-__device__ __forceinline__ Row load_row(const float* tiles, int64_t at) {
+template <int S>
+__device__ __forceinline__ Row<S> load_row(const float* tiles, int64_t at) {
   cfloat* const q = (cfloat*)(uintptr_t)(tiles + at);
-  Row r;
+  Row<S> r;
 #pragma unroll
-  for (int i = 0; i < SEG; ++i) r.B[i] = q[i], r.C[i] = q[SEG + i];
+  for (int i = 0; i < S; ++i) r.B[i] = q[i], r.C[i] = q[SEG + i];
   return r;
 }
 
@@ -282,16 +288,16 @@ struct States {
     a = v + N * 64;
   }
   // f(row, value, exponent, n) for every state, which updates the value: two rows in turn, the next state's
-  // row and values on their way while f runs over SEG tokens, and the last state's value on its way back.
-  template <typename F>
+  // row and values on their way while f runs over the S tokens, and the last state's value on its way back.
+  template <int S, typename F>
   __device__ __forceinline__ void walk(const float* tiles, int64_t tile, int N, F f) {
-    Row r0 = load_row(tiles, tile), r1;
+    Row<S> r0 = load_row<S>(tiles, tile), r1;
     float v0 = v[0], a0 = a[0], v1, a1, done = v0;
     float* back = v;
     for (int n = 0; n < N; n += 2) {
       int m = n + 1 < N ? n + 1 : n;
       rows_arrived();
-      r1 = load_row(tiles, tile + m * 2 * SEG);
+      r1 = load_row<S>(tiles, tile + m * 2 * SEG);
       v1 = v[m * 64], a1 = a[m * 64];
       *back = done;
       f(r0, v0, a0, n);
@@ -299,7 +305,7 @@ struct States {
       if (n + 1 >= N) break;
       m = n + 2 < N ? n + 2 : n;
       rows_arrived();
-      r0 = load_row(tiles, tile + m * 2 * SEG);
+      r0 = load_row<S>(tiles, tile + m * 2 * SEG);
       v0 = v[m * 64], a0 = a[m * 64];
       *back = done;
       f(r1, v1, a1, n + 1);
@@ -370,11 +376,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
       warm.start(p.tiles, tile_of(t + SEG), d.N, w.lane);
       read(t + SEG);
     }
-    const Rows<float> ckpt(p.ckpt + (w.b * d.segs + t / SEG) * d.N * d.C, d.C, d.N, d.C);
-    states.walk(p.tiles, tile_of(t), d.N, [&](const Row& r, float& h, float a, int n) {
-      if (!AGG && p.ckpt) ckpt.store(out32, n, h);
+    const int64_t ck = (w.b * d.gsegs + t / GSEG) * d.N * d.C;
+    const Rows<float> first(p.ckpt + ck, d.C, d.N, d.C), second(p.ckpt + ck + static_cast<int64_t>(d.N) * d.C, d.C, d.N, d.C);
+    const bool both = t + GSEG < stop;
+    states.walk<SEG>(p.tiles, tile_of(t), d.N, [&](const Row<SEG>& r, float& h, float a, int n) {
+      if (!AGG && p.ckpt) first.store(out32, n, h);
 #pragma unroll
       for (int i = 0; i < SEG; ++i) {
+        if (!AGG && i == GSEG && p.ckpt && both) second.store(out32, n, h);
         h = fmaf(__builtin_amdgcn_exp2f(s[i] * a), h, x[i] * r.B[i]);
         if constexpr (!AGG) y[i] = fmaf(r.C[i], h, y[i]);
       }
@@ -382,7 +391,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
     if constexpr (!AGG) {
 #pragma unroll
       for (int i = 0; i < SEG; ++i) y[i] *= gate[i];
-      put_seg<T>(p.y, (w.b * d.T + t) * d.C, live(t, stop), d.C, out, y);
+      put_seg<T>(p.y, (w.b * d.T + t) * d.C, live<SEG>(t, stop), d.C, out, y);
     }
   }
   if (!w.ok) return;
@@ -500,7 +509,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
     }
 #pragma unroll
     for (int i = 0; i < SEG; ++i) total += s[i];
-    states.walk(p.tiles, tile_of(t), d.N, [&](const Row& r, float& q, float a, int) {
+    states.walk<SEG>(p.tiles, tile_of(t), d.N, [&](const Row<SEG>& r, float& q, float a, int) {
 #pragma unroll
       for (int i = SEG - 1; i >= 0; --i) q = fmaf(e[i], r.C[i], q) * __builtin_amdgcn_exp2f(s[i] * a);
     });
@@ -510,9 +519,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
   p.ssum[w.u * d.C + w.c] = total;
 }
 
-// The sum over the wave's 64 lanes of each of 32 values, in 70 operations instead of 32 * 7: every round
+// The sum over the wave's 64 lanes of each of 16 values, in 35 operations instead of 16 * 7: every round
 // halves the values that a lane carries by handing the other half to its partner.  Lane l receives the sum
-// of value l / 2.
+// of value l / 4.
 template <int CTRL>
 __device__ __forceinline__ float dpp_move(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
@@ -527,24 +536,23 @@ __device__ __forceinline__ float swap_add(bool high, float a, float b) {  // low
 __device__ __forceinline__ float sum_of(unsigned a, unsigned b) {
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
-__device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[i]),
-                                                    __builtin_bit_cast(unsigned, v[i + 16]), false, false);
-    v[i] = sum_of(r[0], r[1]);
-  }
+__device__ __forceinline__ float lane_sums(float (&v)[16], int lane) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v[i]),
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[i]),
                                                     __builtin_bit_cast(unsigned, v[i + 8]), false, false);
     v[i] = sum_of(r[0], r[1]);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = swap_add<0x128>(lane & 8, v[i], v[i + 4]);  // row_ror:8
+  for (int i = 0; i < 4; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v[i]),
+                                                    __builtin_bit_cast(unsigned, v[i + 4]), false, false);
+    v[i] = sum_of(r[0], r[1]);
+  }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) v[i] = swap_add<0x141>(lane & 4, v[i], v[i + 2]);  // row_half_mirror
-  v[0] = swap_add<0x4E>(lane & 2, v[0], v[1]);                                   // quad_perm 2 3 0 1
+  for (int i = 0; i < 2; ++i) v[i] = swap_add<0x128>(lane & 8, v[i], v[i + 2]);  // row_ror:8
+  v[0] = swap_add<0x141>(lane & 4, v[0], v[1]);                                  // row_half_mirror
+  v[0] += dpp_move<0x4E>(v[0]);                                                  // quad_perm 2 3 0 1
   return v[0] + dpp_move<0xB1>(v[0]);                                            // quad_perm 1 0 3 2
 }
 
@@ -552,13 +560,13 @@ __device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
 // block's share of dB and dC (its channels' sum), pA[unit][n][c] and pD[unit][2][c] the chunk's share of dA,
 // dD and d dt_bias.
 template <typename T>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
+__global__ __launch_bounds__(64 * WAVES, 3) void k_sel_grad(Dims d, Ptrs p) {
   extern __shared__ float lds[];
   const Unit w(d, p.lengths);
   const int waves = blockDim.x >> 6, N = d.N;
   States grads(lds, w.wave, w.lane, N);  // the gradients from behind, and dA in the place of the exponents
   float *const qs = grads.v, *const ga = grads.a;
-  float* const sums = lds + waves * 2 * N * 64;          // [wave][n][B: SEG, C: SEG]
+  float* const sums = lds + waves * 2 * N * 64;          // [wave][n][B: GSEG, C: GSEG]
   const float bias = p.bias ? p.bias[w.c] : 0.f, dskip = p.D ? p.D[w.c] : 0.f;
   float dD = 0.f, dbias = 0.f;
   for (int n = 0; n < N; ++n) {
@@ -576,16 +584,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
   const int in = w.in<T>(), out_t = w.in<T>(true), in32 = w.in<float>();
   const Rows<float> at(p.at, d.C, N, d.C);
   Warm warm;
-  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * N * 2 * SEG; };
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * N * 2 * SEG + t % SEG; };
   warm.start(p.tiles, tile_of(w.t1 - 1), N, w.lane);
-  for (int t = (w.t1 - 1) / SEG * SEG; t >= w.t0; t -= SEG) {
-    const int64_t seg = t / SEG, row = (w.b * d.T + t) * d.C;
-    const int rows = live(t, w.t1);  // tokens that the tensors have
+  for (int t = (w.t1 - 1) / GSEG * GSEG; t >= w.t0; t -= GSEG) {
+    const int64_t row = (w.b * d.T + t) * d.C;
+    const int rows = live<GSEG>(t, w.t1);  // tokens that the tensors have
     if (t < w.end) {
       if (w.any) {
-        float u[SEG], s[SEG], e[SEG], y[SEG], gb[SEG], gs[SEG];
+        // inputs, step sizes and their slopes, gated gradients, dz without its y; sums over the states
+        float u[GSEG], s[GSEG], slope[GSEG], e[GSEG], dz[GSEG], y[GSEG], gb[GSEG], gs[GSEG];
         {
-          unsigned ur[SEG], dr[SEG], er[SEG], zr[SEG];
+          unsigned ur[GSEG], dr[GSEG], er[GSEG], zr[GSEG];
           fetch<T>(p.u, w.b * p.ub, p.ut, t, w.end, d.C, in, ur);
           fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, d.C, in, dr);
           fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, d.C, in, er);
@@ -593,36 +602,47 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
           widen<T>(ur, t, w.end, u);
           steps<T>(d, dr, t, w.end, bias, s);
           widen<T>(er, t, w.end, e);
-          if (p.z) {
-            widen<T>(zr, t, w.end, y);
 #pragma unroll
-            for (int i = 0; i < SEG; ++i) e[i] *= y[i] * sigmoid(y[i]);
+          for (int i = 0; i < GSEG; ++i) slope[i] = 1.f, dz[i] = 0.f;
+          if (d.softplus) {
+#pragma unroll
+            for (int i = 0; i < GSEG; ++i) slope[i] = sigmoid(value<T>(dr[i]) + bias);
+          }
+          if (p.z) {
+            float z[GSEG];
+            widen<T>(zr, t, w.end, z);
+#pragma unroll
+            for (int i = 0; i < GSEG; ++i) {
+              const float sg = sigmoid(z[i]);
+              dz[i] = e[i] * sg * fmaf(z[i], 1.f - sg, 1.f);
+              e[i] *= z[i] * sg;
+            }
           }
         }
 #pragma unroll
-        for (int i = 0; i < SEG; ++i) {
+        for (int i = 0; i < GSEG; ++i) {
           e[i] = w.ok ? e[i] : 0.f;  // lanes without a channel add nothing to the sums over channels
           y[i] = gb[i] = gs[i] = 0.f;
         }
         warm.done();
-        if (t > w.t0) warm.start(p.tiles, tile_of(t - SEG), N, w.lane);
+        if (t > w.t0) warm.start(p.tiles, tile_of(t - GSEG), N, w.lane);
         const int64_t tile = tile_of(t);
-        const Rows<float> ckpt(p.ckpt_in + (w.b * d.segs + seg) * N * d.C, d.C, N, d.C);
+        const Rows<float> ckpt(p.ckpt_in + (w.b * d.gsegs + t / GSEG) * N * d.C, d.C, N, d.C);
         float an_next = value<float>(at.load(in32, 0)), h0_next = value<float>(ckpt.load(in32, 0));
-        grads.walk(p.tiles, tile, N, [&](const Row& r, float& q, float dA, int n) {
+        grads.walk<GSEG>(p.tiles, tile, N, [&](const Row<GSEG>& r, float& q, float dA, int n) {
           const int m = n + 1 < N ? n + 1 : n;
           const float an = an_next, h0 = h0_next, a2 = an * LOG2E;
           an_next = value<float>(at.load(in32, m)), h0_next = value<float>(ckpt.load(in32, m));
-          float a[SEG], h[SEG], v[2 * SEG];
+          float a[GSEG], h[GSEG], v[2 * GSEG];
 #pragma unroll
-          for (int i = 0; i < SEG; ++i) {
+          for (int i = 0; i < GSEG; ++i) {
             a[i] = __builtin_amdgcn_exp2f(s[i] * a2);
             h[i] = fmaf(a[i], i ? h[i - 1] : h0, s[i] * u[i] * r.B[i]);
             y[i] = fmaf(r.C[i], h[i], y[i]);
-            v[SEG + i] = e[i] * h[i];
+            v[GSEG + i] = e[i] * h[i];
           }
 #pragma unroll
-          for (int i = SEG - 1; i >= 0; --i) {
+          for (int i = GSEG - 1; i >= 0; --i) {
             q = fmaf(e[i], r.C[i], q);
             v[i] = q * (s[i] * u[i]);
             gb[i] = fmaf(q, r.B[i], gb[i]);
@@ -633,48 +653,30 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
           }
           ga[n * 64] = dA;
           const float total = lane_sums(v, w.lane);
-          if ((w.lane & 1) == 0) sums[(w.wave * N + n) * 2 * SEG + (w.lane >> 1)] = total;
+          if ((w.lane & 3) == 0) sums[(w.wave * N + n) * 2 * GSEG + (w.lane >> 2)] = total;
         });
-        // what needs dy, z and dt once more reads them again (from the caches), not earlier than here: the
-        // loop over the states needs the registers
-        asm volatile("" ::: "memory");
-        unsigned raw[SEG], dy[SEG], zr[SEG];
-        fetch<T>(p.dt, w.b * p.dtb, p.dtt, t, w.end, d.C, in, raw);
-        fetch<T>(p.dy, w.b * p.dyb, p.dyt, t, w.end, d.C, in, dy);
-        if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, w.end, d.C, in, zr);
 #pragma unroll
-        for (int i = 0; i < SEG; ++i) {
+        for (int i = 0; i < GSEG; ++i) {
           dD = fmaf(e[i], u[i], dD);
-          y[i] = fmaf(dskip, u[i], y[i]);
-          gs[i] = fmaf(gb[i], u[i], gs[i]);                // d step
-          gb[i] = fmaf(gb[i], s[i], e[i] * dskip);         // du
+          dz[i] *= fmaf(dskip, u[i], y[i]);
+          gs[i] = fmaf(gb[i], u[i], gs[i]) * slope[i];  // d dt
+          gb[i] = fmaf(gb[i], s[i], e[i] * dskip);      // du
         }
-        if (d.softplus) {
+        if (t + GSEG > w.end) {
 #pragma unroll
-          for (int i = 0; i < SEG; ++i) gs[i] *= sigmoid(value<T>(raw[i]) + bias);
-        }
-        if (p.z) {
-#pragma unroll
-          for (int i = 0; i < SEG; ++i) {
-            const float z = value<T>(zr[i]), sg = sigmoid(z);
-            y[i] *= value<T>(dy[i]) * sg * fmaf(z, 1.f - sg, 1.f);  // dz
-          }
-        }
-        if (t + SEG > w.end) {
-#pragma unroll
-          for (int i = 0; i < SEG; ++i)
-            if (t + i >= w.end) gb[i] = gs[i] = y[i] = 0.f;
+          for (int i = 0; i < GSEG; ++i)
+            if (t + i >= w.end) gb[i] = gs[i] = dz[i] = 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < SEG; ++i) dbias += gs[i];
+        for (int i = 0; i < GSEG; ++i) dbias += gs[i];
         put_seg<T>(p.du, row, rows, d.C, out_t, gb);
         put_seg<T>(p.ddt, row, rows, d.C, out_t, gs);
-        if (p.z) put_seg<T>(p.dz, row, rows, d.C, out_t, y);
+        if (p.z) put_seg<T>(p.dz, row, rows, d.C, out_t, dz);
       } else {
-        for (int i = w.lane; i < N * 2 * SEG; i += 64) sums[w.wave * N * 2 * SEG + i] = 0.f;
+        for (int i = w.lane; i < N * 2 * GSEG; i += 64) sums[w.wave * N * 2 * GSEG + i] = 0.f;
       }
     } else {
-      const float none[SEG] = {};
+      const float none[GSEG] = {};
       put_seg<T>(p.du, row, rows, d.C, out_t, none);
       put_seg<T>(p.ddt, row, rows, d.C, out_t, none);
       if (p.z) put_seg<T>(p.dz, row, rows, d.C, out_t, none);
@@ -685,7 +687,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_sel_grad(Dims d, Ptrs p) {
       const int n = j % N, which = j / N & 1, i = j / N / 2;
       float v = 0.f;
       if (t + i < w.end)
-        for (int k = 0; k < waves; ++k) v += sums[(k * N + n) * 2 * SEG + which * SEG + i];
+        for (int k = 0; k < waves; ++k) v += sums[(k * N + n) * 2 * GSEG + which * GSEG + i];
       out[j] = v;
     }
     __syncthreads();
@@ -811,10 +813,10 @@ Dims make_dims(const lng_selective& a) {
   Dims d{};
   d.B = a.B, d.T = static_cast<int>(a.T), d.C = a.C, d.N = a.N, d.G = a.G, d.softplus = a.softplus;
   d.cbg = static_cast<int>(cdiv(a.C / a.G, 64));
-  d.segs = static_cast<int>(cdiv(a.T, SEG));
-  // chunks: two waves for each of the 1024 SIMDs, of at least four segments
+  d.segs = static_cast<int>(cdiv(a.T, SEG)), d.gsegs = static_cast<int>(cdiv(a.T, GSEG));
+  // chunks: four waves for each of the 1024 SIMDs, of at least two segments
   const int64_t units = a.B * a.G * d.cbg;
-  const int64_t want = std::min<int64_t>(cdiv(2048, std::max<int64_t>(units, 1)), std::max(1, d.segs / 4));
+  const int64_t want = std::min<int64_t>(cdiv(4096, std::max<int64_t>(units, 1)), std::max(1, d.segs / 2));
   d.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1)))) * SEG;
   d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
   return d;
@@ -913,7 +915,7 @@ int run_grad(const Dims& d, Ptrs p, const lng_selective_grad& g, hipStream_t st)
     k_sel_grad_ends<T><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
     launch_join<true>(d, p, st);
   }
-  k_sel_grad<T><<<blocks, 64 * waves, states_lds(d, waves) + waves * d.N * 2 * SEG * 4, st>>>(d, p);
+  k_sel_grad<T><<<blocks, 64 * waves, states_lds(d, waves) + waves * d.N * 2 * GSEG * 4, st>>>(d, p);
   k_sel_grad_bc<T><<<grid256(d.B * d.G * d.T * 2 * d.N), 256, 0, st>>>(
       d, p.pBC, static_cast<int>(cdiv(d.cbg, waves)), static_cast<T*>(g.dB), static_cast<T*>(g.dC));
   k_sel_grad_a<<<static_cast<unsigned>(cdiv(int64_t{d.N + 2} * d.C, 64)), 256, 0, st>>>(d, p.pA, p.pD, g.dA, g.dD,
@@ -970,7 +972,7 @@ size_t lng_selective_workspace_bytes(int64_t B, int64_t T, int32_t C, int32_t N,
 
 int64_t lng_selective_checkpoints(int64_t B, int64_t T, int32_t C, int32_t N) {
   if (B <= 0 || T <= 0 || C <= 0 || N <= 0) return 0;
-  return B * cdiv(T, SEG) * N * C;
+  return B * cdiv(T, GSEG) * N * C;
 }
 
 int lng_selective_scan(const lng_selective* args, void* workspace, size_t workspace_bytes, void* stream) {
