@@ -46,6 +46,35 @@ __device__ __forceinline__ _Float16 from_f32<_Float16>(float x) { return static_
 template <typename T>
 __device__ __forceinline__ float round_to(float x) { return to_f32(from_f32<T>(x)); }
 
+// ------------------------------------------------------------------ activations
+constexpr float LOG2E = 1.4426950408889634f;
+
+// exp(-|x|), to about an ulp: the product with log2 e is corrected for its own rounding (r), which the plain
+// exp2(x log2 e) magnifies by |x|.  Past 88 the result is that of 88 (below the smallest normal number); NaN
+// stays NaN.  Seven operations and the exponential, where expf takes some twenty.
+__device__ __forceinline__ float exp_minus_abs(float x) {
+  constexpr float LOG2E_REST = 1.92596303e-8f;  // log2 e - LOG2E
+  constexpr float LN2 = 0.69314718f;
+  float a = fabsf(x);
+  a = a > 88.f ? 88.f : a;
+  const float t = -a * LOG2E, r = fmaf(-a, LOG2E_REST, fmaf(-a, LOG2E, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, r * LN2, e);
+}
+__device__ __forceinline__ float sigmoid(float x) {
+  const float e = exp_minus_abs(x);
+  return (x < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+}
+// v * sigmoid(v) for a result in T.  One that is rounded to 16 bits takes the exponential without its
+// correction: an error of |v| 2^-23 relative, far below half a step of T.
+template <typename T>
+__device__ __forceinline__ float silu(float v) {
+  if constexpr (sizeof(T) == 2)
+    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-v * LOG2E));
+  else
+    return v * sigmoid(v);
+}
+
 // ------------------------------------------------------------------ wave reductions (wave64)
 // Inclusive scans inside each 16-lane row with DPP row_shr:1,2,4,8 (VALU data movement, no LDS
 // round trip), then the four row totals (lanes 15, 31, 47, 63) read as scalars.  Every lane

@@ -31,7 +31,6 @@ constexpr int SEG = 16;   // tokens of a tile, and of the forward pass's segment
 constexpr int GSEG = 8;   // tokens of the backward pass's segments, whose first states the forward pass leaves
 constexpr int WAVES = 4;  // waves of a block: neighbouring channels of one chunk
 constexpr int MAX_N = 256;
-constexpr float LOG2E = 1.4426950408889634f;
 
 typedef const float __attribute__((address_space(4))) cfloat;  // read through the scalar unit where uniform
 
@@ -56,19 +55,6 @@ struct Ptrs {
   float* dstart;
 };
 
-// exp(-|x|), to about an ulp: the product with log2 e is corrected for its own rounding (r), which the plain
-// exp2(x log2 e) magnifies by |x|.  Past 88 the result is that of 88 (below the smallest normal number); NaN
-// stays NaN.  Seven operations and the exponential, where expf takes some twenty, and every token of a
-// channel needs two or three.
-__device__ __forceinline__ float exp_minus_abs(float x) {
-  constexpr float LOG2E_REST = 1.92596303e-8f;  // log2 e - LOG2E
-  constexpr float LN2 = 0.69314718f;
-  float a = fabsf(x);
-  a = a > 88.f ? 88.f : a;
-  const float t = -a * LOG2E, r = fmaf(-a, LOG2E_REST, fmaf(-a, LOG2E, -t));
-  const float e = __builtin_amdgcn_exp2f(t);
-  return fmaf(e, r * LN2, e);
-}
 // log(1 + exp(x)) with log1p by 2 atanh(e / (2 + e)): exact to about an ulp over the whole range, which
 // log(1 + e) is not for the small steps that training starts from.  The series' first term left out is below
 // 2^-26 at e = 1.
@@ -83,11 +69,6 @@ __device__ __forceinline__ float softplus(float x) {
   p = fmaf(p, q, 1.f);
   return fmaf(2.f * s, p, fmaxf(x, 0.f));
 }
-__device__ __forceinline__ float sigmoid(float x) {
-  const float e = exp_minus_abs(x);
-  return (x < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
-}
-
 // The own tokens of sequence b (the same in every lane that asks for the same b).
 __device__ __forceinline__ int seq_len(const int32_t* lengths, int64_t b, int T) {
   if (!lengths) return T;
@@ -368,7 +349,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
       if (p.z) {
         widen<T>(zr, t, stop, gate);
 #pragma unroll
-        for (int i = 0; i < SEG; ++i) gate[i] *= sigmoid(gate[i]);
+        for (int i = 0; i < SEG; ++i) gate[i] = silu<T>(gate[i]);
       }
     }
     warm.done();

@@ -101,11 +101,10 @@ __device__ __forceinline__ void load_weights(const ConvArgs& a, int c, float (&w
   for (int i = 0; i < VEC; ++i) bias[i] = a.bias ? to_f32(static_cast<const W*>(a.bias)[c + i]) : 0.f;
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.f + expf(-v)); }
 // d silu / dv = s (1 + v (1 - s)), s = sigmoid(v)
 __device__ __forceinline__ float silu_grad(float v) {
-  const float s = 1.f / (1.f + expf(-v));
-  return s * (1.f + v * (1.f - s));
+  const float s = sigmoid(v);
+  return s * fmaf(v, 1.f - s, 1.f);
 }
 
 // Threads [0, B * tiles * dil * C / VEC): outputs; behind them B * lp * C / VEC threads copy the next history.
@@ -153,7 +152,7 @@ __global__ __launch_bounds__(256) void k_short_conv(ConvArgs a) {
       for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[j][k], x[m + j][k], v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = pos < n ? (a.act ? silu(v[k]) : v[k]) : 0.f;
+    for (int k = 0; k < VEC; ++k) v[k] = pos < n ? (a.act ? silu<T>(v[k]) : v[k]) : 0.f;
     store_pack<T, VEC>(static_cast<T*>(a.y) + (b * a.T + pos) * a.C + c, v);
   }
 }
@@ -303,8 +302,9 @@ __global__ __launch_bounds__(256) void k_conv_partials(const float* __restrict__
 }
 
 // One new token of every sequence: a thread owns VEC channels of a sequence, so the history may move in
-// place (hist_out == hist): each of its rows is read before the thread writes the row in front of it.
-template <typename T, typename W, int VEC>
+// place (hist_out == hist): each of its rows is read before the thread writes the row in front of it.  NEAR:
+// without dilation the window has at most MAX_TAPS rows, which are all asked for together.
+template <typename T, typename W, int VEC, bool NEAR>
 __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
   const int64_t ncv = a.C / VEC, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= a.B * ncv) return;
@@ -312,27 +312,46 @@ __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
   const int64_t b = i / ncv;
   const T* const h = static_cast<const T*>(a.hist) + b * lp * a.C + c;
   T* const ho = static_cast<T*>(a.hist_out) + b * lp * a.C + c;
-  const W *wp = static_cast<const W*>(a.w) + static_cast<int64_t>(c) * a.K, *bp = static_cast<const W*>(a.bias);
   float x[VEC], v[VEC];
   load_pack<T, VEC>(static_cast<const T*>(a.x) + b * a.xb + c, x);
+  if constexpr (NEAR) {
+    const int skip = MAX_TAPS - a.K;  // row e of the window and its weight in registers e + skip, the token's last
+    float r[MAX_TAPS - 1][VEC], w[MAX_TAPS][VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v[k] = bp ? to_f32(bp[c + k]) : 0.f;
-  for (int e = 0; e <= lp; ++e) {  // the window's rows: the history, then the token
-    float r[VEC];
-    if (e < lp) {
-      load_pack<T, VEC>(h + static_cast<int64_t>(e) * a.C, r);
-    } else {
+    for (int j = 0; j < MAX_TAPS - 1; ++j)
+      if (j >= skip) load_pack<T, VEC>(h + static_cast<int64_t>(j - skip) * a.C, r[j]);
+    load_weights<W, VEC, 0, MAX_TAPS>(a, c, w, v);  // v: the bias
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) r[k] = x[k];
+    for (int j = 0; j < MAX_TAPS - 1; ++j) {
+      if (j < skip) continue;
+      if (j > skip) store_pack<T, VEC>(ho + static_cast<int64_t>(j - skip - 1) * a.C, r[j]);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[j][k], r[j][k], v[k]);
     }
-    if (e > 0) store_pack<T, VEC>(ho + static_cast<int64_t>(e - 1) * a.C, r);
-    if (e % a.dil == 0) {
+    if (lp > 0) store_pack<T, VEC>(ho + static_cast<int64_t>(lp - 1) * a.C, x);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = fmaf(to_f32(wp[k * a.K + e / a.dil]), r[k], v[k]);
+    for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[MAX_TAPS - 1][k], x[k], v[k]);
+  } else {
+    const W *wp = static_cast<const W*>(a.w) + static_cast<int64_t>(c) * a.K, *bp = static_cast<const W*>(a.bias);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = bp ? to_f32(bp[c + k]) : 0.f;
+    for (int e = 0; e <= lp; ++e) {  // the window's rows: the history, then the token
+      float r[VEC];
+      if (e < lp) {
+        load_pack<T, VEC>(h + static_cast<int64_t>(e) * a.C, r);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) r[k] = x[k];
+      }
+      if (e > 0) store_pack<T, VEC>(ho + static_cast<int64_t>(e - 1) * a.C, r);
+      if (e % a.dil == 0) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = fmaf(to_f32(wp[k * a.K + e / a.dil]), r[k], v[k]);
+      }
     }
   }
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v[k] = a.act ? silu(v[k]) : v[k];
+  for (int k = 0; k < VEC; ++k) v[k] = a.act ? silu<T>(v[k]) : v[k];
   store_pack<T, VEC>(static_cast<T*>(a.y) + b * a.C + c, v);
 }
 
@@ -431,13 +450,23 @@ int run_grad(ConvArgs a, void* dw, void* db, hipStream_t st) {
   return check_launch("short_conv_grad");
 }
 
+template <typename T, typename W, int VEC>
+void launch_step(const ConvArgs& a, hipStream_t st) {
+  const unsigned blocks = static_cast<unsigned>(cdiv(a.B * (a.C / VEC), 256));
+  if (a.dil == 1)
+    k_short_conv_step<T, W, VEC, true><<<blocks, 256, 0, st>>>(a);
+  else
+    k_short_conv_step<T, W, VEC, false><<<blocks, 256, 0, st>>>(a);
+}
+
 template <typename T, typename W>
 int run_step(const ConvArgs& a, hipStream_t st) {
+  // few channels in all: one a thread, so that more waves wait for memory at once
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
-  if (vector_ok(a, V, sizeof(T)))
-    k_short_conv_step<T, W, V><<<static_cast<unsigned>(cdiv(a.B * (a.C / V), 256)), 256, 0, st>>>(a);
+  if (a.B * a.C > 65536 && vector_ok(a, V, sizeof(T)))
+    launch_step<T, W, V>(a, st);
   else
-    k_short_conv_step<T, W, 1><<<static_cast<unsigned>(cdiv(a.B * a.C, 256)), 256, 0, st>>>(a);
+    launch_step<T, W, 1>(a, st);
   return check_launch("short_conv_step");
 }
 

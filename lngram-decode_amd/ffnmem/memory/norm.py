@@ -33,9 +33,10 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of x (fp32, bf16 or fp16,
     any strides); weight and bias ``[d]`` in x's type or fp32, or None.  Differentiable once."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, float(eps))
-    return ops.layer_norm(x, weight, bias, eps)
+    return ops.layer_norm(x, weight, bias, float(eps))
 
 
 class LayerNorm(nn.Module):

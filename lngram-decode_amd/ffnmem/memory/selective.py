@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 from lngram_hip import ops
 
 from .norm import LayerNorm
-from .short_conv import short_conv, short_conv_step
+from .short_conv import _needs_grad, short_conv, short_conv_step
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -48,7 +48,7 @@ class _SelectiveScan(torch.autograd.Function):
 
 
 def _f32(t: Optional[Tensor]) -> Optional[Tensor]:
-    return None if t is None else t.float()
+    return t if t is None or t.dtype == torch.float32 else t.float()
 
 
 def selective_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor] = None,
@@ -66,9 +66,8 @@ def selective_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Op
     positions behind them are not read and give zeros.  Returns y ``[B, T, C]`` in u's type, with
     ``return_state`` also the state after each sequence's last own token (fp32).  States and sums are fp32.
     Differentiable once, in everything but the lengths."""
-    A, D, dt_bias, state = A.float(), _f32(D), _f32(dt_bias), _f32(state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (u, dt, A, B, C, D, z, dt_bias, state)):
+    A, D, dt_bias, state = _f32(A), _f32(D), _f32(dt_bias), _f32(state)
+    if _needs_grad(u, dt, A, B, C, D, z, dt_bias, state):
         y, end = _SelectiveScan.apply(u, dt, A, B, C, D, z, dt_bias, state, lengths, bool(dt_softplus),
                                       bool(return_state))
     else:
@@ -83,10 +82,9 @@ def selective_step(state: Tensor, u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C
     ``[B, G, N]``; returns y ``[B, C]``.  ``state [B, C, N]`` (fp32, contiguous) moves on in place; with
     ``out_state`` the new one is written there and ``state`` stays (a step that may have to be taken back).
     No gradient: call it under ``torch.no_grad()``."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (state, u, dt, A, B, C, D, z, dt_bias)):
+    if _needs_grad(state, u, dt, A, B, C, D, z, dt_bias):
         raise RuntimeError("selective_step has no backward pass; call it under torch.no_grad()")
-    return ops.selective_step(state, u, dt, A.float(), B, C, _f32(D), z, _f32(dt_bias), dt_softplus, out_state)
+    return ops.selective_step(state, u, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias), dt_softplus, out_state)
 
 
 class _Linear(torch.autograd.Function):
@@ -146,7 +144,7 @@ class SelectiveSSM(nn.Module):
                 torch.zeros(batch, self.state_dim, self.d_state, dtype=torch.float32, device=w.device))
 
     def _linear(self, x: Tensor, w: nn.Linear) -> Tensor:
-        if torch.is_grad_enabled() and (x.requires_grad or w.weight.requires_grad):
+        if _needs_grad(x, w.weight):
             return _Linear.apply(x, w.weight)
         return ops.linear(x, w.weight)
 

@@ -7,10 +7,10 @@ are rejected: there is no CPU path in the product.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
+import struct
 import threading
 
 import torch
@@ -1334,33 +1334,42 @@ def ssm_scan_status(dev: torch.device) -> int:
 
 
 # ----------------------------------------------------------------------------- norm, short conv, selective scan
+# A training step or a decoded token makes these calls by the dozen, so their host side is kept short: shapes
+# are compared as they are, and the stream is asked for by its handle.
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _on(dev: torch.device):
-    """The tensors' device as the current one while a call is made on it."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _call(name: str, dev: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on the tensors' device and its current stream."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _call(name, dev, fn, *args)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = _timed(name, dev, lambda: fn(*args, stream)) if KernelTimer._active else fn(*args, stream)
+    if rc:
+        check(rc, name)
 
 
-def _float_rows(what: str, x: torch.Tensor, *weights) -> None:
+def _float_rows(what: str, x: torch.Tensor, w_dtype: torch.dtype | None, other: torch.dtype | None = None) -> None:
     """fp32, bf16 or fp16 rows with weights of one type, the rows' own or fp32."""
     if x.dtype not in _FLOATS:
         raise TypeError(f"{what}: fp32, bf16 or fp16 tensors, got {x.dtype}")
-    types = {w.dtype for w in weights if w is not None}
-    if len(types) > 1 or not types <= {x.dtype, torch.float32}:
-        raise TypeError(f"{what}: weights of one type, {x.dtype} as the rows or float32, got "
-                        f"{', '.join(str(t) for t in types)}")
+    for t in (w_dtype, other):
+        if t is not None and t != x.dtype and t != torch.float32:
+            raise TypeError(f"{what}: weights in {x.dtype} as the rows or in float32, got {t}")
+    if w_dtype is not None and other is not None and w_dtype != other:
+        raise TypeError(f"{what}: weights of one type, got {w_dtype} and {other}")
 
 
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
     """``x [..., d]`` as ``[rows, d]`` with contiguous rows, without a copy where its strides allow it."""
     d = x.shape[-1]
-    rows = x.reshape(x.numel() // d, d)
+    rows = x if x.dim() == 2 else x.reshape(x.numel() // d, d)
     return rows if rows.stride(1) == 1 or d == 1 else rows.contiguous()
 
 
 def _last_contiguous(x: torch.Tensor) -> torch.Tensor:
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
 def _near_rows(x: torch.Tensor) -> torch.Tensor:
@@ -1369,9 +1378,13 @@ def _near_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.dim() < 3 or x.stride(1) * x.element_size() <= 1 << 26 else x.contiguous()
 
 
+def _whole(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _expect(what: str, name: str, t: torch.Tensor | None, *shape) -> None:
-    if t is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {shape}")
+    if t is not None and t.shape != shape:
+        raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _lengths32(what: str, lengths: torch.Tensor | None, batch: int) -> torch.Tensor | None:
@@ -1385,8 +1398,10 @@ def _lengths32(what: str, lengths: torch.Tensor | None, batch: int) -> torch.Ten
 
 def _separate(what: str, name: str, out: torch.Tensor, src: torch.Tensor) -> None:
     """``out`` is ``src`` itself or shares no memory with it."""
-    lo, n = src.data_ptr(), src.numel() * src.element_size()
-    at = out.data_ptr()
+    if out is src:
+        return
+    lo, at = src.data_ptr(), out.data_ptr()
+    n = src.numel() * src.element_size()
     if at != lo and at < lo + n and lo < at + n:
         raise ValueError(f"{what}: {name} overlaps what it is computed from")
 
@@ -1395,24 +1410,22 @@ def layer_norm(x: torch.Tensor, w: torch.Tensor | None, b: torch.Tensor | None, 
     """Layer norm over the last dimension (``lng_layer_norm``); w, b ``[d]`` in x's type or fp32, or None.
     ``want_stats``: returns ``(y, mean, rstd)`` for :func:`layer_norm_grad`, fp32 ``[rows]``."""
     dev = _dev(x, w, b)
-    _float_rows("layer_norm", x, w, b)
+    wt = None if w is None else w.dtype
+    bt = None if b is None else b.dtype
+    _float_rows("layer_norm", x, wt, bt)
     d = x.shape[-1] if x.dim() else 0
     if d == 0:
         raise ValueError("layer_norm: the last dimension is empty")
     _expect("layer_norm", "weight", w, d)
     _expect("layer_norm", "bias", b, d)
-    rows = _as_rows(x)
-    wc, bc = (None if t is None else t.contiguous() for t in (w, b))
+    rows, wc, bc = _as_rows(x), _whole(w), _whole(b)
     n = rows.shape[0]
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     mean = rstd = None
     if want_stats:
-        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=dev)
-    wt = next((t.dtype for t in (w, b) if t is not None), x.dtype)
-    with _on(dev):
-        check(_timed("layer_norm", dev, lambda: lib().lng_layer_norm(
-            _ptr(rows), dtype_code(x.dtype), n, d, rows.stride(0), _ptr(wc), _ptr(bc), dtype_code(wt), float(eps), _ptr(y),
-            _ptr(mean), _ptr(rstd), _stream(dev))), "layer_norm")
+        mean, rstd = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+    _call("layer_norm", dev, lib().lng_layer_norm, rows.data_ptr(), _DT[x.dtype], n, d, rows.stride(0), _ptr(wc),
+          _ptr(bc), _DT[wt or bt or x.dtype], eps, y.data_ptr(), _ptr(mean), _ptr(rstd))
     return (y, mean, rstd) if want_stats else y
 
 
@@ -1422,26 +1435,28 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, m
     ``w_dtype`` (None: the weight's type)."""
     dev = _dev(dy, x, w, mean, rstd)
     d = x.shape[-1]
-    _expect("layer_norm_grad", "dy", dy, *x.shape)
+    if dy.shape != x.shape:
+        raise ValueError(f"layer_norm_grad: dy {tuple(dy.shape)}, expected {tuple(x.shape)}")
     if dy.dtype != x.dtype:
         raise TypeError(f"layer_norm_grad: dy {dy.dtype} for rows in {x.dtype}")
     wt = w_dtype or (x.dtype if w is None else w.dtype)
-    _float_rows("layer_norm_grad", x, w, torch.empty(0, dtype=wt))
-    rows, grads = _as_rows(x), _as_rows(dy)
+    _float_rows("layer_norm_grad", x, wt, None if w is None else w.dtype)
+    rows, grads, wc = _as_rows(x), _as_rows(dy), _whole(w)
     n = rows.shape[0]
-    _expect("layer_norm_grad", "mean", mean, n)
-    _expect("layer_norm_grad", "rstd", rstd, n)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _expect("layer_norm_grad", name, t, n)
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise TypeError(f"layer_norm_grad: {name} as layer_norm gave it")
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-    dw, db = (torch.empty(d, dtype=wt, device=dev) if k else None for k in want[1:])
-    ws = None
+    dw = torch.empty(d, dtype=wt, device=dev) if want[1] else None
+    db = torch.empty(d, dtype=wt, device=dev) if want[2] else None
+    ws, size = None, 0
     if want[1] or want[2]:
-        ws = torch.empty(lib().lng_layer_norm_grad_workspace_bytes(n, d), dtype=torch.uint8, device=dev)
-    wc = None if w is None else w.contiguous()
-    with _on(dev):
-        check(_timed("layer_norm_grad", dev, lambda: lib().lng_layer_norm_grad(
-            _ptr(grads), grads.stride(0), _ptr(rows), rows.stride(0), dtype_code(x.dtype), n, d, _ptr(wc), dtype_code(wt),
-            _ptr(mean), _ptr(rstd), _ptr(ws), 0 if ws is None else ws.numel(), _ptr(dx), _ptr(dw), _ptr(db),
-            _stream(dev))), "layer_norm_grad")
+        size = lib().lng_layer_norm_grad_workspace_bytes(n, d)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _call("layer_norm_grad", dev, lib().lng_layer_norm_grad, grads.data_ptr(), grads.stride(0), rows.data_ptr(),
+          rows.stride(0), _DT[x.dtype], n, d, _ptr(wc), _DT[wt], mean.data_ptr(), rstd.data_ptr(), _ptr(ws), size,
+          _ptr(dx), _ptr(dw), _ptr(db))
     return dx, dw, db
 
 
@@ -1449,19 +1464,20 @@ def _conv_check(what: str, x, w, bias, dilation: int, hist, dims: int) -> tuple:
     """``(C, K, rows of a history)`` of a short conv's checked arguments."""
     if x.dim() != dims:
         raise ValueError(f"{what}: x is {'[B, T, C]' if dims == 3 else '[B, C]'}, got {tuple(x.shape)}")
-    _float_rows(what, x, w, bias)
+    _float_rows(what, x, w.dtype, None if bias is None else bias.dtype)
     c = x.shape[-1]
     if w.dim() != 2 or w.shape[0] != c or not 1 <= w.shape[1] <= 8:
         raise ValueError(f"{what}: weight [C, K] with C = {c} and 1 to 8 taps, got {tuple(w.shape)}")
-    if int(dilation) < 1:
+    if dilation < 1:
         raise ValueError(f"{what}: dilation must be positive")
     _expect(what, "bias", bias, c)
-    back = (w.shape[1] - 1) * int(dilation)
+    k = w.shape[1]
+    back = (k - 1) * dilation
     if hist is not None:
         _expect(what, "history", hist, x.shape[0], back, c)
         if hist.dtype != x.dtype:
             raise TypeError(f"{what}: history {hist.dtype} for rows in {x.dtype}")
-    return c, w.shape[1], back
+    return c, k, back
 
 
 def short_conv(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, dilation: int = 1,
@@ -1471,18 +1487,17 @@ def short_conv(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     ``[B, (K - 1) * dilation, C]``: the rows before the first position (None: zeros); ``lengths [B]``: each
     sequence's own tokens (zeros behind them).  ``want_history``: returns ``(y, next history)``."""
     dev = _dev(x, w, bias, history, lengths)
+    dilation = int(dilation)
     c, k, back = _conv_check("short_conv", x, w, bias, dilation, history, 3)
     b, t, _ = x.shape
     n = _lengths32("short_conv", lengths, b)
-    xc, wc, bc, hc = _last_contiguous(x), _c(w), None if bias is None else bias.contiguous(),         None if history is None else history.contiguous()
+    xc, wc, bc, hc = _last_contiguous(x), _c(w), _whole(bias), _whole(history)
     y = torch.empty(b, t, c, dtype=x.dtype, device=dev)
     out = torch.empty(b, back, c, dtype=x.dtype, device=dev) if want_history else None
     if c:
-        with _on(dev):
-            check(_timed("short_conv", dev, lambda: lib().lng_short_conv(
-                _ptr(xc), dtype_code(x.dtype), b, t, c, xc.stride(0), xc.stride(1), _ptr(wc), _ptr(bc),
-                dtype_code(w.dtype), k, int(dilation), int(bool(silu)), _ptr(hc) if back else None, _ptr(n), _ptr(y),
-                _ptr(out) if back else None, _stream(dev))), "short_conv")
+        _call("short_conv", dev, lib().lng_short_conv, xc.data_ptr(), _DT[x.dtype], b, t, c, xc.stride(0), xc.stride(1),
+              wc.data_ptr(), _ptr(bc), _DT[w.dtype], k, dilation, int(silu), _ptr(hc) if back else None, _ptr(n),
+              y.data_ptr(), _ptr(out) if back else None)
     return (y, out) if want_history else y
 
 
@@ -1492,6 +1507,7 @@ def short_conv_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, bias: to
     """``(dx, dw, dbias, dhistory)`` of :func:`short_conv` (``lng_short_conv_grad``), None where not wanted;
     ``dhistory``: the gradient of the next history, or None."""
     dev = _dev(dy, x, w, bias, history, lengths, dhistory)
+    dilation = int(dilation)
     c, k, back = _conv_check("short_conv_grad", x, w, bias, dilation, history, 3)
     b, t, _ = x.shape
     _expect("short_conv_grad", "dy", dy, b, t, c)
@@ -1500,23 +1516,20 @@ def short_conv_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, bias: to
         raise TypeError(f"short_conv_grad: gradients in the rows' type {x.dtype}")
     n = _lengths32("short_conv_grad", lengths, b)
     dyc, xc, wc = _last_contiguous(dy), _last_contiguous(x), _c(w)
-    bc, hc, dhc = (None if v is None else v.contiguous() for v in (bias, history, dhistory))
+    bc, hc, dhc = _whole(bias), _whole(history), _whole(dhistory)
     dx = torch.empty(b, t, c, dtype=x.dtype, device=dev) if want[0] else None
     dw = torch.empty(c, k, dtype=w.dtype, device=dev) if want[1] else None
     db = torch.empty(c, dtype=w.dtype, device=dev) if want[2] else None
     dh = torch.empty(b, back, c, dtype=x.dtype, device=dev) if want[3] else None
-    ws = None
+    ws, size = None, 0
     if want[1] or want[2]:
-        ws = torch.empty(lib().lng_short_conv_grad_workspace_bytes(b, t, c, k, int(dilation)), dtype=torch.uint8,
-                         device=dev)
+        size = lib().lng_short_conv_grad_workspace_bytes(b, t, c, k, dilation)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
     if c:
-        with _on(dev):
-            check(_timed("short_conv_grad", dev, lambda: lib().lng_short_conv_grad(
-                _ptr(dyc), dyc.stride(0), dyc.stride(1), _ptr(xc), xc.stride(0), xc.stride(1), dtype_code(x.dtype), b, t,
-                c, _ptr(wc), _ptr(bc), dtype_code(w.dtype), k, int(dilation), int(bool(silu)),
-                _ptr(hc) if back else None, _ptr(n), _ptr(dhc) if back else None, _ptr(ws),
-                0 if ws is None else ws.numel(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(dh) if back else None,
-                _stream(dev))), "short_conv_grad")
+        _call("short_conv_grad", dev, lib().lng_short_conv_grad, dyc.data_ptr(), dyc.stride(0), dyc.stride(1),
+              xc.data_ptr(), xc.stride(0), xc.stride(1), _DT[x.dtype], b, t, c, wc.data_ptr(), _ptr(bc), _DT[w.dtype], k,
+              dilation, int(silu), _ptr(hc) if back else None, _ptr(n), _ptr(dhc) if back else None, _ptr(ws), size,
+              _ptr(dx), _ptr(dw), _ptr(db), _ptr(dh) if back else None)
     return dx, dw, db, dh
 
 
@@ -1526,31 +1539,38 @@ def short_conv_step(x: torch.Tensor, history: torch.Tensor, w: torch.Tensor, bia
     history moves on in place, or into ``out_history``."""
     out = history if out_history is None else out_history
     dev = _dev(x, history, w, bias, out)
+    dilation = int(dilation)
     c, k, back = _conv_check("short_conv_step", x, w, bias, dilation, history, 2)
-    _expect("short_conv_step", "out_history", out, x.shape[0], back, c)
+    b = x.shape[0]
+    if out is not history:
+        _expect("short_conv_step", "out_history", out, b, back, c)
+        _separate("short_conv_step", "out_history", out, history)
     if out.dtype != x.dtype or not (history.is_contiguous() and out.is_contiguous()):
         raise ValueError("short_conv_step: histories are contiguous, in the rows' type")
-    _separate("short_conv_step", "out_history", out, history)
-    xc, wc, bc = _last_contiguous(x), _c(w), None if bias is None else bias.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    xc, wc, bc = _last_contiguous(x), _c(w), _whole(bias)
+    y = torch.empty(b, c, dtype=x.dtype, device=dev)
     if c:
-        with _on(dev):
-            check(_timed("short_conv_step", dev, lambda: lib().lng_short_conv_step(
-                _ptr(xc), dtype_code(x.dtype), x.shape[0], c, xc.stride(0), _ptr(wc), _ptr(bc), dtype_code(w.dtype), k,
-                int(dilation), int(bool(silu)), _ptr(history), _ptr(out), _ptr(y), _stream(dev))), "short_conv_step")
+        _call("short_conv_step", dev, lib().lng_short_conv_step, xc.data_ptr(), _DT[x.dtype], b, c, xc.stride(0),
+              wc.data_ptr(), _ptr(bc), _DT[w.dtype], k, dilation, int(silu), history.data_ptr(), out.data_ptr(),
+              y.data_ptr())
     return y
 
 
-def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool, state, lengths, dims: int):
+# lng_selective as one packed value: a ctypes structure filled field by field takes longer than the rest of a
+# single-token call.
+_SELECTIVE = struct.Struct("2q6i5P12q9P")
+
+
+def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool, state, lengths, y, state_out, dims: int,
+                    checkpoints=None, checkpoints_in=None):
     """``(lng_selective, tensors to keep alive)`` of a selective scan's checked arguments; dims 3: ``[B, T, C]``
     tensors, 2: ``[B, C]`` (one token)."""
-    if u.dim() != dims or u.shape[-1] == 0:
-        raise ValueError(f"{what}: u is {'[B, T, C]' if dims == 3 else '[B, C]'}, got {tuple(u.shape)}")
-    lead, c = tuple(u.shape[:-1]), u.shape[-1]
-    if u.dtype not in _FLOATS or any(t is not None and t.dtype != u.dtype for t in (dt, B, C, z)):
+    lead, c = u.shape[:-1], u.shape[-1]
+    if any(t is not None and t.dtype != u.dtype for t in (dt, B, C, z)) or u.dtype not in _FLOATS:
         raise TypeError(f"{what}: u, dt, B, C and z in one type, fp32, bf16 or fp16")
-    _expect(what, "dt", dt, *lead, c)
-    _expect(what, "z", z, *lead, c)
+    if dt.shape != u.shape or (z is not None and z.shape != u.shape):
+        raise ValueError(f"{what}: dt and z {tuple(u.shape)} as u, got {tuple(dt.shape)}"
+                         f"{'' if z is None else f' and {tuple(z.shape)}'}")
     if A.dim() != 2 or A.shape[0] != c or not 1 <= A.shape[1] <= 256:
         raise ValueError(f"{what}: A is [C, N] with C = {c} and 1 to 256 states, got {tuple(A.shape)}")
     n = A.shape[1]
@@ -1566,27 +1586,27 @@ def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool,
     _expect(what, "D", D, c)
     _expect(what, "dt_bias", dt_bias, c)
     _expect(what, "state", state, lead[0], c, n)
-    if any(t is not None and t.dtype != torch.float32 for t in (A, D, dt_bias, state)):
-        raise TypeError(f"{what}: A, D, dt_bias and states are float32")
+    for t in (A, D, dt_bias, state):
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{what}: A, D, dt_bias and states are float32")
     ln = _lengths32(what, lengths, lead[0])
     u, dt, B, C = _near_rows(u), _near_rows(dt), _last_contiguous(B), _last_contiguous(C)
     z = None if z is None else _near_rows(z)
-    A, D, dt_bias, state = (None if t is None else t.contiguous() for t in (A, D, dt_bias, state))
-
-    def strides(t):
-        s = t.stride()
-        return (s[0], s[1] if dims == 3 else 0)
-
-    a = _lib.Selective(B=lead[0], T=lead[1] if dims == 3 else 1, C=c, N=n, G=g, dtype=dtype_code(u.dtype),
-                       softplus=int(bool(dt_softplus)), u=_ptr(u), dt=_ptr(dt), z=_ptr(z), Bm=_ptr(B), Cm=_ptr(C),
-                       A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias), state=_ptr(state), lengths=_ptr(ln))
-    a.u_batch, a.u_token = strides(u)
-    a.dt_batch, a.dt_token = strides(dt)
-    if z is not None:
-        a.z_batch, a.z_token = strides(z)
-    a.B_batch, a.B_token, a.B_group = *strides(B), B.stride(-2)
-    a.C_batch, a.C_token, a.C_group = *strides(C), C.stride(-2)
+    A, D, dt_bias, state = _whole(A), _whole(D), _whole(dt_bias), _whole(state)
+    us, ds, zs, bs, cs = u.stride(), dt.stride(), (0, 0) if z is None else z.stride(), B.stride(), C.stride()
+    if dims == 2:
+        us, ds, zs, bs, cs = (us[0], 0), (ds[0], 0), (zs[0], 0), (bs[0], 0, bs[1]), (cs[0], 0, cs[1])
+    at = [0 if t is None else t.data_ptr()
+          for t in (u, dt, z, B, C, A, D, dt_bias, state, ln, y, state_out, checkpoints, checkpoints_in)]
+    a = _lib.Selective.from_buffer_copy(_SELECTIVE.pack(
+        lead[0], lead[1] if dims == 3 else 1, c, n, g, _DT[u.dtype], int(bool(dt_softplus)), 0, *at[:5], *us[:2], *ds[:2],
+        *zs[:2], *bs[:3], *cs[:3], *at[5:]))
     return a, (u, dt, z, B, C, A, D, dt_bias, state, ln)
+
+
+def _selective_u(what: str, u: torch.Tensor, dims: int) -> None:
+    if u.dim() != dims or u.shape[-1] == 0:
+        raise ValueError(f"{what}: u is {'[B, T, C]' if dims == 3 else '[B, C]'}, got {tuple(u.shape)}")
 
 
 def _selective_workspace(a, grad: bool, dev: torch.device) -> torch.Tensor:
@@ -1602,22 +1622,22 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     u, dt, z ``[B, T, C]`` with A ``[C, N]`` and B, C ``[B, T, N]`` or ``[B, T, G, N]``; the checkpoints are
     what :func:`selective_scan_grad` takes."""
     dev = _dev(u, dt, A, B, C, D, z, dt_bias, state, lengths)
-    a, keep = _selective_args("selective_scan", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, 3)
+    _selective_u("selective_scan", u, 3)
+    b, t, c = u.shape
+    n = A.shape[-1] if A.dim() else 0
     y = torch.empty(u.shape, dtype=u.dtype, device=dev)
     end = ckpt = None
     if want_state:
-        if a.T == 0:
-            end = torch.zeros(a.B, a.C, a.N, device=dev) if state is None else state.clone()
-        else:
-            end = torch.empty(a.B, a.C, a.N, dtype=torch.float32, device=dev)
+        end = torch.empty(b, c, n, dtype=torch.float32, device=dev)
     if want_checkpoints:
-        ckpt = torch.empty(lib().lng_selective_checkpoints(a.B, a.T, a.C, a.N), dtype=torch.float32, device=dev)
-    a.y, a.state_out, a.checkpoints = _ptr(y), _ptr(end), _ptr(ckpt)
-    ws = _selective_workspace(a, False, dev)
-    if y.numel():
-        with _on(dev):
-            check(_timed("selective_scan", dev, lambda: lib().lng_selective_scan(
-                ctypes.byref(a), _ptr(ws), ws.numel(), _stream(dev))), "selective_scan")
+        ckpt = torch.empty(lib().lng_selective_checkpoints(b, t, c, n), dtype=torch.float32, device=dev)
+    a, keep = _selective_args("selective_scan", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, y, end, 3,
+                              ckpt)
+    if b and t:
+        ws = _selective_workspace(a, False, dev)
+        _call("selective_scan", dev, lib().lng_selective_scan, ctypes.byref(a), ws.data_ptr(), ws.numel())
+    elif want_state:                                     # no tokens: the state passes through
+        end.zero_() if state is None else end.copy_(state)
     del keep
     return y, end, ckpt
 
@@ -1629,12 +1649,16 @@ def selective_scan_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoin
     """The gradients of :func:`selective_scan` (``lng_selective_scan_grad``) by their inputs' names, given
     those of y and of the final state (None: zero)."""
     dev = _dev(dy, dstate, checkpoints, u, dt, A, B, C, D, z, dt_bias, state, lengths)
-    a, keep = _selective_args("selective_scan_grad", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, 3)
+    _selective_u("selective_scan_grad", u, 3)
+    a, keep = _selective_args("selective_scan_grad", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, None,
+                              None, 3, None, checkpoints)
     _expect("selective_scan_grad", "dy", dy, *u.shape)
     _expect("selective_scan_grad", "dstate", dstate, a.B, a.C, a.N)
     if dy.dtype != u.dtype or (dstate is not None and dstate.dtype != torch.float32):
         raise TypeError("selective_scan_grad: dy in u's type, dstate in float32")
     _expect("selective_scan_grad", "checkpoints", checkpoints, lib().lng_selective_checkpoints(a.B, a.T, a.C, a.N))
+    if checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous():
+        raise TypeError("selective_scan_grad: checkpoints as selective_scan gave them")
     f32 = torch.float32
     out = {"u": torch.empty(u.shape, dtype=u.dtype, device=dev), "dt": torch.empty(u.shape, dtype=u.dtype, device=dev),
            "A": torch.empty(A.shape, dtype=f32, device=dev), "B": torch.empty(B.shape, dtype=u.dtype, device=dev),
@@ -1651,16 +1675,13 @@ def selective_scan_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoin
         for k, v in out.items():
             v.zero_() if k != "state" or dstate is None else v.copy_(dstate)
         return out
-    dyc, dsc = _near_rows(dy), None if dstate is None else dstate.contiguous()
-    a.checkpoints_in = _ptr(checkpoints)
-    g = _lib.SelectiveGrad(dy=_ptr(dyc), dy_batch=dyc.stride(0), dy_token=dyc.stride(1), dstate_out=_ptr(dsc),
-                           du=_ptr(out["u"]), ddt=_ptr(out["dt"]), dz=_ptr(out.get("z")), dB=_ptr(out["B"]),
-                           dC=_ptr(out["C"]), dA=_ptr(out["A"]), dD=_ptr(out.get("D")),
-                           ddt_bias=_ptr(out.get("dt_bias")), dstate=_ptr(out.get("state")))
+    dyc, dsc = _near_rows(dy), _whole(dstate)
+    g = _lib.SelectiveGrad(dyc.data_ptr(), dyc.stride(0), dyc.stride(1), _ptr(dsc), _ptr(out["u"]), _ptr(out["dt"]),
+                           _ptr(out.get("z")), _ptr(out["B"]), _ptr(out["C"]), _ptr(out["A"]), _ptr(out.get("D")),
+                           _ptr(out.get("dt_bias")), _ptr(out.get("state")))
     ws = _selective_workspace(a, True, dev)
-    with _on(dev):
-        check(_timed("selective_scan_grad", dev, lambda: lib().lng_selective_scan_grad(
-            ctypes.byref(a), ctypes.byref(g), _ptr(ws), ws.numel(), _stream(dev))), "selective_scan_grad")
+    _call("selective_scan_grad", dev, lib().lng_selective_scan_grad, ctypes.byref(a), ctypes.byref(g), ws.data_ptr(),
+          ws.numel())
     del keep
     return out
 
@@ -1673,16 +1694,15 @@ def selective_step(state: torch.Tensor, u: torch.Tensor, dt: torch.Tensor, A: to
     state moves on in place, or into ``out_state``."""
     out = state if out_state is None else out_state
     dev = _dev(state, u, dt, A, B, C, D, z, dt_bias, out)
+    _selective_u("selective_step", u, 2)
     if not state.is_contiguous() or not out.is_contiguous() or out.dtype != torch.float32:
         raise ValueError("selective_step: states are contiguous float32 [B, C, N]")
-    a, keep = _selective_args("selective_step", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, None, 2)
-    _expect("selective_step", "out_state", out, a.B, a.C, a.N)
-    _separate("selective_step", "out_state", out, state)
+    if out is not state:
+        _expect("selective_step", "out_state", out, *state.shape)
+        _separate("selective_step", "out_state", out, state)
     y = torch.empty(u.shape, dtype=u.dtype, device=dev)
-    a.y, a.state_out = _ptr(y), _ptr(out)
-    with _on(dev):
-        check(_timed("selective_step", dev, lambda: lib().lng_selective_step(ctypes.byref(a), _stream(dev))),
-              "selective_step")
+    a, keep = _selective_args("selective_step", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, None, y, out, 2)
+    _call("selective_step", dev, lib().lng_selective_step, ctypes.byref(a))
     del keep
     return y
 
