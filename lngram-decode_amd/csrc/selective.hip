@@ -790,14 +790,17 @@ int waves_for(const Dims& d, bool grad) {
   return std::min(by_n, d.cbg);
 }
 
-Dims make_dims(const lng_selective& a) {
+Dims make_dims(const lng_selective& a, bool grad) {
   Dims d{};
   d.B = a.B, d.T = static_cast<int>(a.T), d.C = a.C, d.N = a.N, d.G = a.G, d.softplus = a.softplus;
   d.cbg = static_cast<int>(cdiv(a.C / a.G, 64));
   d.segs = static_cast<int>(cdiv(a.T, SEG)), d.gsegs = static_cast<int>(cdiv(a.T, GSEG));
-  // chunks: four waves for each of the 1024 SIMDs, of at least two segments
-  const int64_t units = a.B * a.G * d.cbg;
-  const int64_t want = std::min<int64_t>(cdiv(4096, std::max<int64_t>(units, 1)), std::max(1, d.segs / 2));
+  // chunks of at least four segments, for two waves on each of the 1024 SIMDs (the backward pass, whose waves
+  // wait more, four: 553 -> 511 us for a training step of 8 x 2048 x 1024); of two segments where even those
+  // leave SIMDs idle (3 x 777 x 1000: 80 -> 55 us)
+  const int64_t units = a.B * a.G * d.cbg, goal = grad ? 4096 : 2048;
+  int64_t want = std::min<int64_t>(cdiv(goal, std::max<int64_t>(units, 1)), std::max(1, d.segs / 4));
+  if (units * want < 2048) want = std::min<int64_t>(cdiv(2048, std::max<int64_t>(units, 1)), std::max(1, d.segs / 2));
   d.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1)))) * SEG;
   d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
   return d;
@@ -948,7 +951,7 @@ size_t lng_selective_workspace_bytes(int64_t B, int64_t T, int32_t C, int32_t N,
   lng_selective a{};
   a.B = B, a.T = T, a.C = C, a.N = N, a.G = G, a.dtype = LNG_F32;
   if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > MAX_N || G <= 0 || C % G) return 0;
-  return static_cast<size_t>(Space(make_dims(a), grad != 0).total) * 4;
+  return static_cast<size_t>(Space(make_dims(a, grad != 0), grad != 0).total) * 4;
 }
 
 int64_t lng_selective_checkpoints(int64_t B, int64_t T, int32_t C, int32_t N) {
@@ -961,7 +964,7 @@ int lng_selective_scan(const lng_selective* args, void* workspace, size_t worksp
   const lng_selective& a = *args;
   if (a.B == 0 || a.T == 0) return LNG_OK;
   if (!a.y) return fail(LNG_E_ARG, "selective_scan: null pointer");
-  const Dims d = make_dims(a);
+  const Dims d = make_dims(a, false);
   const Space s(d, false);
   if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)
     return fail(LNG_E_ARG, "selective_scan: the workspace is too small or not 64-byte aligned");
@@ -981,7 +984,7 @@ int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad*
     return fail(LNG_E_ARG, "selective_scan_grad: null pointer");
   if (g.dy_token < 0 || g.dy_token > (int64_t{1} << 26) / dtype_size(a.dtype))
     return fail(LNG_E_ARG, "selective_scan_grad: rows of dy are 0 to 2^26 bytes apart");
-  const Dims d = make_dims(a);
+  const Dims d = make_dims(a, true);
   const Space s(d, true);
   if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)
     return fail(LNG_E_ARG, "selective_scan_grad: the workspace is too small or not 64-byte aligned");
@@ -998,7 +1001,7 @@ int lng_selective_step(const lng_selective* args, void* stream) {
   if (a.T != 1) return fail(LNG_E_ARG, "selective_step: one token of every sequence (T = 1)");
   if (a.B == 0) return LNG_OK;
   if (!a.state || !a.state_out || !a.y) return fail(LNG_E_ARG, "selective_step: null pointer");
-  const Dims d = make_dims(a);
+  const Dims d = make_dims(a, false);
   const Ptrs p = make_ptrs(a);
   return with_type(a.dtype, [&](auto t) { return run_step<decltype(t)>(d, p, as_stream(stream)); });
 }

@@ -61,21 +61,28 @@ struct ConvArgs {
   }
 };
 
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Pack<T, N>& r, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = to_f32(r.v[i]);
+}
+
 // Row of a sequence at position pos: x, the history below 0, zeros below the history and from `end` on.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_at(const ConvArgs& a, int64_t b, int64_t pos, int64_t end, int c, float (&v)[VEC]) {
+__device__ __forceinline__ Pack<T, VEC> pack_at(const ConvArgs& a, int64_t b, int64_t pos, int64_t end, int c) {
   const T* p = nullptr;
   if (pos >= 0) {
     if (pos < end) p = static_cast<const T*>(a.x) + b * a.xb + pos * a.xt + c;
   } else if (a.hist && pos >= -a.lp()) {
     p = static_cast<const T*>(a.hist) + (b * a.lp() + a.lp() + pos) * a.C + c;
   }
-  if (p) {
-    load_pack<T, VEC>(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = 0.f;
-  }
+  Pack<T, VEC> r{};
+  if (p) r = *reinterpret_cast<const Pack<T, VEC>*>(p);
+  return r;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void load_at(const ConvArgs& a, int64_t b, int64_t pos, int64_t end, int c, float (&v)[VEC]) {
+  unpack<T, VEC>(pack_at<T, VEC>(a, b, pos, end, c), v);
 }
 
 // w[j + KM - K][i]: tap j of channel c + i, so that the last register is the tap of the position itself.
@@ -102,8 +109,9 @@ __device__ __forceinline__ void load_weights(const ConvArgs& a, int c, float (&w
 }
 
 // d silu / dv = s (1 + v (1 - s)), s = sigmoid(v)
+template <typename T>
 __device__ __forceinline__ float silu_grad(float v) {
-  const float s = sigmoid(v);
+  const float s = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-v * LOG2E)) : sigmoid(v);
   return s * fmaf(v, 1.f - s, 1.f);
 }
 
@@ -132,16 +140,29 @@ __global__ __launch_bounds__(256) void k_short_conv(ConvArgs a) {
   const int64_t n = a.len(b);
   // the registers of absent taps are skipped, not multiplied by zero: what their rows hold may be infinite
   const int skip = KT > 0 ? 0 : KM - a.K;
-  float w[KM][VEC], bias[VEC], x[TT + KM - 1][VEC];
-  // x[m]: position pos0 + (m - (KM - 1)) * dil
+  // x[m]: position pos0 + (m - (KM - 1)) * dil, kept as stored until it enters the window
+  Pack<T, VEC> x[TT + KM - 1];
+  const int64_t first = pos0 - static_cast<int64_t>(a.K - 1) * a.dil, last = pos0 + static_cast<int64_t>(TT - 1) * a.dil;
+  const bool inside = first >= 0 && last < n;  // no history, no padding: loads without a choice go out together
+  if (inside) {
+    const T* p = static_cast<const T*>(a.x) + b * a.xb + c;
 #pragma unroll
-  for (int m = 0; m < TT + KM - 1; ++m)
-    if (m >= skip) load_at<T, VEC>(a, b, pos0 + static_cast<int64_t>(m - (KM - 1)) * a.dil, n, c, x[m]);
+    for (int m = 0; m < TT + KM - 1; ++m)
+      if (m >= skip) x[m] = *reinterpret_cast<const Pack<T, VEC>*>(p + (pos0 + static_cast<int64_t>(m - (KM - 1)) * a.dil) * a.xt);
+  } else {
+#pragma unroll
+    for (int m = 0; m < TT + KM - 1; ++m)
+      if (m >= skip) x[m] = pack_at<T, VEC>(a, b, pos0 + static_cast<int64_t>(m - (KM - 1)) * a.dil, n, c);
+  }
+  float w[KM][VEC], bias[VEC], win[TT + KM - 1][VEC];
   load_weights<W, VEC, KT, KM>(a, c, w, bias);
 #pragma unroll
+  for (int m = 0; m < KM - 1; ++m) unpack<T, VEC>(x[m], win[m]);
+  T* const y = static_cast<T*>(a.y) + (b * a.T + pos0) * a.C + c;
+#pragma unroll
   for (int m = 0; m < TT; ++m) {
+    unpack<T, VEC>(x[m + KM - 1], win[m + KM - 1]);
     const int64_t pos = pos0 + static_cast<int64_t>(m) * a.dil;
-    if (pos >= a.T) break;
     float v[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) v[k] = bias[k];
@@ -149,11 +170,20 @@ __global__ __launch_bounds__(256) void k_short_conv(ConvArgs a) {
     for (int j = 0; j < KM; ++j) {
       if (j < skip) continue;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[j][k], x[m + j][k], v[k]);
+      for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[j][k], win[m + j][k], v[k]);
     }
+    if (a.act) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = pos < n ? (a.act ? silu<T>(v[k]) : v[k]) : 0.f;
-    store_pack<T, VEC>(static_cast<T*>(a.y) + (b * a.T + pos) * a.C + c, v);
+      for (int k = 0; k < VEC; ++k) v[k] = silu<T>(v[k]);
+    }
+    if (!inside) {
+      if (pos >= a.T) break;
+      if (pos >= n) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = 0.f;
+      }
+    }
+    store_pack<T, VEC>(y + static_cast<int64_t>(m) * a.dil * a.C, v);
   }
 }
 
@@ -190,64 +220,98 @@ __global__ __launch_bounds__(256) void k_short_conv_grad(ConvArgs a, int cx) {
       const int64_t q0 = tr / a.dil * TT - (a.K - 1);
       const int64_t pos0 = q0 * a.dil + tr % a.dil;
       if (pos0 >= a.T) continue;
+      // one position's dpre from the window's rows (the newest last), and its share of the weights' gradients
+      auto slope = [&](const float (&x)[KM][VEC], const float (&dy)[VEC], bool own_pos, float (&g)[VEC]) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float v = bias[k];
+#pragma unroll
+          for (int j = 0; j < KM; ++j)
+            if (j >= skip) v = fmaf(w[j][k], x[j][k], v);
+          g[k] = a.act ? dy[k] * silu_grad<T>(v) : dy[k];
+        }
+        if (own_pos) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            db[k] += g[k];
+#pragma unroll
+            for (int j = 0; j < KM; ++j)
+              if (j >= skip) dw[j][k] = fmaf(g[k], x[j][k], dw[j][k]);
+          }
+        }
+      };
+      // d ext of the row K - 1 steps back, which then has all its uses
+      auto gather = [&](const float (&dp)[KM][VEC], float (&g)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < KM; ++j) {
+          if (j >= (KT > 0 ? KT : a.K)) continue;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) g[k] = fmaf(wl[j][k], dp[KM - 1 - j][k], g[k]);
+        }
+      };
       float x[KM][VEC], dp[KM][VEC];  // the last KM rows and their dpre; the newest at KM - 1
 #pragma unroll
-      for (int j = 0; j < KM; ++j) {
+      for (int j = 0; j < KM; ++j)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) dp[j][k] = 0.f;
-        if (j > skip) load_at<T, VEC>(a, b, pos0 + static_cast<int64_t>(j - KM) * a.dil, n, c, x[j]);
-      }
-#pragma unroll 1
-      for (int m = 0; m < TT + a.K - 1; ++m) {
-        const int64_t pos = pos0 + static_cast<int64_t>(m) * a.dil;
+      auto shift = [&] {
 #pragma unroll
         for (int j = 0; j < KM - 1; ++j)
 #pragma unroll
           for (int k = 0; k < VEC; ++k) x[j][k] = x[j + 1][k], dp[j][k] = dp[j + 1][k];
+      };
+      const int64_t last = pos0 + static_cast<int64_t>(TT + a.K - 2) * a.dil;
+      if (KT > 0 && pos0 - lp >= 0 && last < n && a.dx) {
+        // neither history nor padding: every row is asked for at once
+        constexpr int XS = TT + 2 * (KM - 1), YS = TT + KM - 1;
+        Pack<T, VEC> xr[XS], yr[YS];
+        const T* const xp = static_cast<const T*>(a.x) + b * a.xb + (pos0 - lp) * a.xt + c;
+        const T* const yp = static_cast<const T*>(a.dy) + b * a.dyb + pos0 * a.dyt + c;
+#pragma unroll
+        for (int m = 0; m < XS; ++m) xr[m] = *reinterpret_cast<const Pack<T, VEC>*>(xp + static_cast<int64_t>(m) * a.dil * a.xt);
+#pragma unroll
+        for (int m = 0; m < YS; ++m) yr[m] = *reinterpret_cast<const Pack<T, VEC>*>(yp + static_cast<int64_t>(m) * a.dil * a.dyt);
+        T* const out = static_cast<T*>(a.dx) + (b * a.T + pos0) * a.C + c;
+#pragma unroll
+        for (int j = 1; j < KM; ++j) unpack<T, VEC>(xr[j - 1], x[j]);
+#pragma unroll
+        for (int m = 0; m < YS; ++m) {
+          float dy[VEC];
+          shift();
+          unpack<T, VEC>(xr[m + KM - 1], x[KM - 1]);
+          unpack<T, VEC>(yr[m], dy);
+          slope(x, dy, m < TT, dp[KM - 1]);
+          if (m >= KM - 1) {
+            float g[VEC] = {};
+            gather(dp, g);
+            store_pack<T, VEC>(out + static_cast<int64_t>(m - (KM - 1)) * a.dil * a.C, g);
+          }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < KM; ++j)
+        if (j > skip) load_at<T, VEC>(a, b, pos0 + static_cast<int64_t>(j - KM) * a.dil, n, c, x[j]);
+#pragma unroll 1
+      for (int m = 0; m < TT + a.K - 1; ++m) {
+        const int64_t pos = pos0 + static_cast<int64_t>(m) * a.dil;
+        shift();
         load_at<T, VEC>(a, b, pos, n, c, x[KM - 1]);
         if (pos >= 0 && pos < n) {
-          float g[VEC];
-          load_pack<T, VEC>(static_cast<const T*>(a.dy) + b * a.dyb + pos * a.dyt + c, g);
-          if (a.act) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              float v = bias[k];
-#pragma unroll
-              for (int j = 0; j < KM; ++j)
-                if (j >= skip) v = fmaf(w[j][k], x[j][k], v);
-              g[k] *= silu_grad(v);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) dp[KM - 1][k] = g[k];
-          if (m < TT) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              db[k] += g[k];
-#pragma unroll
-              for (int j = 0; j < KM; ++j)
-                if (j >= skip) dw[j][k] = fmaf(g[k], x[j][k], dw[j][k]);
-            }
-          }
+          float dy[VEC];
+          load_pack<T, VEC>(static_cast<const T*>(a.dy) + b * a.dyb + pos * a.dyt + c, dy);
+          slope(x, dy, m < TT, dp[KM - 1]);
         } else {
 #pragma unroll
           for (int k = 0; k < VEC; ++k) dp[KM - 1][k] = 0.f;
         }
-        // the row K - 1 steps back has all its uses: sum_j w[j] dpre[its position + (K - 1 - j) dil]
         const int64_t at = pos - lp;
         if (m >= a.K - 1 && at < a.T && (at >= 0 ? a.dx != nullptr : a.dhist != nullptr)) {
-          float g[VEC];
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) g[k] = 0.f;
+          float g[VEC] = {};
           const int64_t slot = pos - n;  // of the next history
           if (a.dhist_out && slot >= 0 && slot < lp)
             load_pack<T, VEC>(static_cast<const T*>(a.dhist_out) + (b * lp + slot) * a.C + c, g);
-#pragma unroll
-          for (int j = 0; j < KM; ++j) {
-            if (j >= a.K || at >= n) continue;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) g[k] = fmaf(wl[j][k], dp[KM - 1 - j][k], g[k]);
-          }
+          if (at < n) gather(dp, g);
           T* const out = at >= 0 ? static_cast<T*>(a.dx) + (b * a.T + at) * a.C
                                  : static_cast<T*>(a.dhist) + (b * lp + lp + at) * a.C;
           store_pack<T, VEC>(out + c, g);
@@ -304,8 +368,9 @@ __global__ __launch_bounds__(256) void k_conv_partials(const float* __restrict__
 // One new token of every sequence: a thread owns VEC channels of a sequence, so the history may move in
 // place (hist_out == hist): each of its rows is read before the thread writes the row in front of it.  NEAR:
 // without dilation the window has at most MAX_TAPS rows, which are all asked for together.
-template <typename T, typename W, int VEC, bool NEAR>
+template <typename T, typename W, int VEC, int KT, bool NEAR>
 __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
+  constexpr int KM = KT > 0 ? KT : MAX_TAPS;
   const int64_t ncv = a.C / VEC, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= a.B * ncv) return;
   const int c = static_cast<int>(i % ncv) * VEC, lp = a.lp();
@@ -315,14 +380,14 @@ __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
   float x[VEC], v[VEC];
   load_pack<T, VEC>(static_cast<const T*>(a.x) + b * a.xb + c, x);
   if constexpr (NEAR) {
-    const int skip = MAX_TAPS - a.K;  // row e of the window and its weight in registers e + skip, the token's last
-    float r[MAX_TAPS - 1][VEC], w[MAX_TAPS][VEC];
+    const int skip = KT > 0 ? 0 : KM - a.K;  // row e of the window and its weight in registers e + skip, the token's last
+    float r[KM][VEC], w[KM][VEC];
 #pragma unroll
-    for (int j = 0; j < MAX_TAPS - 1; ++j)
+    for (int j = 0; j < KM - 1; ++j)
       if (j >= skip) load_pack<T, VEC>(h + static_cast<int64_t>(j - skip) * a.C, r[j]);
-    load_weights<W, VEC, 0, MAX_TAPS>(a, c, w, v);  // v: the bias
+    load_weights<W, VEC, KT, KM>(a, c, w, v);  // v: the bias
 #pragma unroll
-    for (int j = 0; j < MAX_TAPS - 1; ++j) {
+    for (int j = 0; j < KM - 1; ++j) {
       if (j < skip) continue;
       if (j > skip) store_pack<T, VEC>(ho + static_cast<int64_t>(j - skip - 1) * a.C, r[j]);
 #pragma unroll
@@ -330,7 +395,7 @@ __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
     }
     if (lp > 0) store_pack<T, VEC>(ho + static_cast<int64_t>(lp - 1) * a.C, x);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[MAX_TAPS - 1][k], x[k], v[k]);
+    for (int k = 0; k < VEC; ++k) v[k] = fmaf(w[KM - 1][k], x[k], v[k]);
   } else {
     const W *wp = static_cast<const W*>(a.w) + static_cast<int64_t>(c) * a.K, *bp = static_cast<const W*>(a.bias);
 #pragma unroll
@@ -382,12 +447,12 @@ struct GradGrid {
   int tt, vec, cx;
   int64_t tiles, gx, gy;
   GradGrid(int64_t B, int64_t T, int C, int K, int dil, int vec_) : vec(vec_) {
-    tt = B * T / 16 * cdiv(C, vec) >= 1024 * 64 ? 16 : 4;
+    tt = B * T / 16 * cdiv(C, vec) >= 1024 * 64 ? 8 : 4;
     tiles = cdiv(cdiv(T, dil) + K - 1, tt);
     const int64_t ncv = cdiv(C, vec);
     for (cx = 1; cx < 64 && cx < ncv; cx *= 2) {}
     gx = cdiv(ncv, cx);
-    gy = std::max<int64_t>(1, std::min(cdiv(B * tiles * dil, 256 / cx), std::max<int64_t>(1, 2048 / gx)));
+    gy = std::max<int64_t>(1, std::min(cdiv(B * tiles * dil, 256 / cx), std::max<int64_t>(1, 1024 / gx)));
   }
 };
 
@@ -399,8 +464,8 @@ void launch_grad(const ConvArgs& a, const GradGrid& g, hipStream_t st) {
 
 template <typename T, typename W, int VEC, int KT>
 void grad_tile(const ConvArgs& a, const GradGrid& g, hipStream_t st) {
-  if (g.tt == 16)
-    launch_grad<T, W, VEC, KT, 16>(a, g, st);
+  if (g.tt == 8)
+    launch_grad<T, W, VEC, KT, 8>(a, g, st);
   else
     launch_grad<T, W, VEC, KT, 4>(a, g, st);
 }
@@ -453,10 +518,12 @@ int run_grad(ConvArgs a, void* dw, void* db, hipStream_t st) {
 template <typename T, typename W, int VEC>
 void launch_step(const ConvArgs& a, hipStream_t st) {
   const unsigned blocks = static_cast<unsigned>(cdiv(a.B * (a.C / VEC), 256));
-  if (a.dil == 1)
-    k_short_conv_step<T, W, VEC, true><<<blocks, 256, 0, st>>>(a);
+  if (a.dil == 1 && a.K == 4)
+    k_short_conv_step<T, W, VEC, 4, true><<<blocks, 256, 0, st>>>(a);
+  else if (a.dil == 1)
+    k_short_conv_step<T, W, VEC, 0, true><<<blocks, 256, 0, st>>>(a);
   else
-    k_short_conv_step<T, W, VEC, false><<<blocks, 256, 0, st>>>(a);
+    k_short_conv_step<T, W, VEC, 0, false><<<blocks, 256, 0, st>>>(a);
 }
 
 template <typename T, typename W>
