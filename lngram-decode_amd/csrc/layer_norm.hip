@@ -319,7 +319,8 @@ constexpr int64_t GRAD_BLOCKS = 512;  // two blocks of 8 waves per CU
 // Blocks of the backward pass, each leaving one partial row of the weight gradients.
 int64_t grad_blocks(int64_t rows, int64_t d) {
   const int64_t rpb = d <= 32 ? 128 : d <= 128 ? 32 : d <= 256 ? 16 : d <= 2048 ? 8 : 1;
-  return std::max<int64_t>(1, std::min(cdiv(rows, rpb), GRAD_BLOCKS));
+  const int64_t most = std::min(GRAD_BLOCKS, (int64_t{1} << 26) / d);  // very wide rows: partial rows of 512 MB at most
+  return std::max<int64_t>(1, std::min(cdiv(rows, rpb), most));
 }
 
 struct Rows {  // one call's rows

@@ -845,7 +845,7 @@ int check_args(const char* what, const lng_selective* a) {
       a->B * a->T > (int64_t{1} << 38) / a->C / a->N)
     return fail(LNG_E_ARG, std::string(what) + ": bad shape (1 to 256 states, groups that divide the channels)");
   const int64_t lanes = cdiv(a->C / a->G, 64) * 64 * a->G, most = int64_t{1} << 38;  // of any launch's threads
-  if (a->B * a->G * (a->T + SEG) > most / 2 / a->N || a->B * lanes * (a->T / 64 + 1) > most ||
+  if (a->B * a->G * (a->T + SEG) > most / 2 / a->N || a->B * lanes * (a->T / (2 * SEG) + 1) > most ||
       a->B * a->C > most / SEG || a->B * lanes > most / a->N)
     return fail(LNG_E_ARG, std::string(what) + ": too many tokens, groups or channels for one call");
   // a segment's rows are reached by 32-bit offsets from its first one

@@ -49,7 +49,7 @@ struct ConvArgs {
   const void *x, *w, *bias, *hist, *dy, *dhist_out;
   const int32_t* lengths;
   int64_t B, T, xb, xt, dyb, dyt, tiles;
-  int C, K, dil, act;
+  int C, K, dil, act, classes;  // classes: residue classes of t mod dil that the launch's positions fall into
   void *y, *hist_out, *dx, *dhist;
   float* partial;
 
@@ -115,13 +115,13 @@ __device__ __forceinline__ float silu_grad(float v) {
   return s * fmaf(v, 1.f - s, 1.f);
 }
 
-// Threads [0, B * tiles * dil * C / VEC): outputs; behind them B * lp * C / VEC threads copy the next history.
+// Threads [0, B * tiles * classes * C / VEC): outputs; behind them B * lp * C / VEC threads copy the next history.
 template <typename T, typename W, int VEC, int KT, int TT>
 __global__ __launch_bounds__(256) void k_short_conv(ConvArgs a) {
   constexpr int KM = KT > 0 ? KT : MAX_TAPS;
   const int64_t ncv = a.C / VEC;
   int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t n_out = a.B * a.tiles * a.dil * ncv;
+  const int64_t n_out = a.B * a.tiles * a.classes * ncv;
   if (i >= n_out) {
     i -= n_out;
     const int lp = a.lp();
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(256) void k_short_conv(ConvArgs a) {
     return;
   }
   const int c = static_cast<int>(i % ncv) * VEC;
-  const int64_t rest = i / ncv, tr = rest % (a.tiles * a.dil), b = rest / (a.tiles * a.dil);
-  const int64_t pos0 = tr / a.dil * TT * a.dil + tr % a.dil;  // first position, the others dil apart
+  const int64_t rest = i / ncv, tr = rest % (a.tiles * a.classes), b = rest / (a.tiles * a.classes);
+  const int64_t pos0 = tr / a.classes * TT * a.dil + tr % a.classes;  // first position, the others dil apart
   if (pos0 >= a.T) return;
   const int64_t n = a.len(b);
   // the registers of absent taps are skipped, not multiplied by zero: what their rows hold may be infinite
@@ -438,8 +438,9 @@ int tile_rows(const ConvArgs& a, int vec) {
 template <typename T, typename W, int VEC, int KT, int TT>
 void launch_conv(ConvArgs a, hipStream_t st) {
   a.tiles = cdiv(cdiv(a.T, a.dil), TT);
-  const int64_t rows = a.B * (a.tiles * a.dil + (a.hist_out ? (a.K - 1) * a.dil : 0));
-  const int64_t threads = rows * (a.C / VEC);
+  a.classes = static_cast<int>(std::min<int64_t>(a.dil, a.T));
+  const int64_t rows = a.B * (a.tiles * a.classes + (a.hist_out ? (a.K - 1) * a.dil : 0));
+  const int64_t threads = rows * (a.C / VEC);  // below 2^39: outputs and history rows that fit the memory
   if (threads) k_short_conv<T, W, VEC, KT, TT><<<static_cast<unsigned>(cdiv(threads, 256)), 256, 0, st>>>(a);
 }
 
@@ -544,8 +545,10 @@ int check_conv(const char* what, int dtype, int w_dtype, int64_t B, int64_t T, i
   if (w_dtype != dtype && w_dtype != LNG_F32)
     return fail(LNG_E_DTYPE, std::string(what) + ": weights in the rows' type or fp32");
   if (B < 0 || T < 0 || C <= 0 || K < 1 || K > MAX_TAPS || dil < 1 || dil > 4096 || (act != 0 && act != 1) ||
-      C > (1 << 24) || B > (int64_t{1} << 24) || T > (int64_t{1} << 31) || B * T > (int64_t{1} << 34) / C)
-    return fail(LNG_E_ARG, std::string(what) + ": bad shape (1 to 8 taps, dilation up to 4096, B * T * C up to 2^34)");
+      C > (1 << 24) || B > (int64_t{1} << 24) || T > (int64_t{1} << 31) ||
+      B * (T + int64_t{K - 1} * dil) > (int64_t{1} << 36) / C)
+    return fail(LNG_E_ARG, std::string(what) + ": bad shape (1 to 8 taps, dilation up to 4096, 2^36 elements with "
+                                               "the history)");
   return LNG_OK;
 }
 

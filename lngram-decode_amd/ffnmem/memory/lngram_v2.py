@@ -27,7 +27,7 @@ from torch import Tensor, nn
 
 from lngram_hip import ops
 
-from .norm import LayerNorm
+from .norm import LayerNorm, rows_type
 from .short_conv import short_conv
 
 
@@ -226,10 +226,14 @@ class DepthwiseCausalConv(nn.Module):
         at a position that the device holds, and a tree's windows."""
         return self.conv.bias is None and not isinstance(self.norm, LayerNorm)
 
+    def _two_kernels(self, values: Tensor, **kw):
+        return short_conv(self.norm(values), rows_type(self.conv.weight, values), rows_type(self.conv.bias, values),
+                          dilation=self.dilation, **kw)
+
     def forward(self, values: Tensor, segment_ids: Optional[Tensor] = None) -> Tensor:
         self._check(values, segment_ids)
         if not self.one_kernel:
-            return short_conv(self.norm(values), self.conv.weight, self.conv.bias, dilation=self.dilation)
+            return self._two_kernels(values)
         return ops.causal_conv(values, self.norm.weight, self.conv.weight, self.dilation, self.norm.eps,
                                residual=False)
 
@@ -249,8 +253,7 @@ class DepthwiseCausalConv(nn.Module):
                 if tuple(history.shape) != (b, d, lp):
                     raise ValueError(f"conv history shape={tuple(history.shape)}, expected {(b, d, lp)}")
                 history = history.transpose(1, 2).to(values.dtype)
-            out, rows = short_conv(self.norm(values), self.conv.weight, self.conv.bias, dilation=self.dilation,
-                                   history=history, return_history=True)
+            out, rows = self._two_kernels(values, history=history, return_history=True)
             return out, rows.transpose(1, 2).contiguous()
         if lp == 0:
             return self.forward(values), values.new_zeros(b, d, 0)

@@ -39,6 +39,14 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     return ops.layer_norm(x, weight, bias, float(eps))
 
 
+def rows_type(parameter: Optional[Tensor], rows: Tensor) -> Optional[Tensor]:
+    """A parameter as the kernels take it beside ``rows``: as it is in the rows' type or fp32, else cast to the
+    rows' type (as ``RMSNorm`` casts its weight)."""
+    if parameter is None or parameter.dtype in (rows.dtype, torch.float32):
+        return parameter
+    return parameter.to(rows.dtype)
+
+
 class LayerNorm(nn.Module):
     """``nn.LayerNorm(hidden_size, eps)``: parameters ``weight`` (ones) and ``bias`` (zeros)."""
 
@@ -52,4 +60,5 @@ class LayerNorm(nn.Module):
     def forward(self, hidden_states: Tensor) -> Tensor:
         if hidden_states.shape[-1] != self.hidden_size:
             raise ValueError(f"LayerNorm expects last dim {self.hidden_size}, got {hidden_states.shape[-1]}")
-        return layer_norm(hidden_states, self.weight, self.bias, self.eps)
+        return layer_norm(hidden_states, rows_type(self.weight, hidden_states), rows_type(self.bias, hidden_states),
+                          self.eps)

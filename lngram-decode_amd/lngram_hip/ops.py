@@ -1387,13 +1387,15 @@ def _expect(what: str, name: str, t: torch.Tensor | None, *shape) -> None:
         raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _lengths32(what: str, lengths: torch.Tensor | None, batch: int) -> torch.Tensor | None:
+def _lengths32(what: str, lengths: torch.Tensor | None, batch: int, t: int) -> torch.Tensor | None:
     if lengths is None:
         return None
     _expect(what, "lengths", lengths, batch)
-    if lengths.dtype not in (torch.int32, torch.int64):
+    if lengths.dtype == torch.int64:                     # longer than T is T, also where 32 bits would wrap
+        return lengths.clamp(0, t).to(torch.int32)
+    if lengths.dtype != torch.int32:
         raise TypeError(f"{what}: int32 or int64 lengths, got {lengths.dtype}")
-    return lengths.to(torch.int32).contiguous()
+    return lengths.contiguous()
 
 
 def _separate(what: str, name: str, out: torch.Tensor, src: torch.Tensor) -> None:
@@ -1490,7 +1492,7 @@ def short_conv(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     dilation = int(dilation)
     c, k, back = _conv_check("short_conv", x, w, bias, dilation, history, 3)
     b, t, _ = x.shape
-    n = _lengths32("short_conv", lengths, b)
+    n = _lengths32("short_conv", lengths, b, t)
     xc, wc, bc, hc = _last_contiguous(x), _c(w), _whole(bias), _whole(history)
     y = torch.empty(b, t, c, dtype=x.dtype, device=dev)
     out = torch.empty(b, back, c, dtype=x.dtype, device=dev) if want_history else None
@@ -1514,7 +1516,7 @@ def short_conv_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, bias: to
     _expect("short_conv_grad", "the next history's gradient", dhistory, b, back, c)
     if dy.dtype != x.dtype or (dhistory is not None and dhistory.dtype != x.dtype):
         raise TypeError(f"short_conv_grad: gradients in the rows' type {x.dtype}")
-    n = _lengths32("short_conv_grad", lengths, b)
+    n = _lengths32("short_conv_grad", lengths, b, t)
     dyc, xc, wc = _last_contiguous(dy), _last_contiguous(x), _c(w)
     bc, hc, dhc = _whole(bias), _whole(history), _whole(dhistory)
     dx = torch.empty(b, t, c, dtype=x.dtype, device=dev) if want[0] else None
@@ -1589,7 +1591,7 @@ def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool,
     for t in (A, D, dt_bias, state):
         if t is not None and t.dtype != torch.float32:
             raise TypeError(f"{what}: A, D, dt_bias and states are float32")
-    ln = _lengths32(what, lengths, lead[0])
+    ln = _lengths32(what, lengths, lead[0], lead[-1])
     u, dt, B, C = _near_rows(u), _near_rows(dt), _last_contiguous(B), _last_contiguous(C)
     z = None if z is None else _near_rows(z)
     A, D, dt_bias, state = _whole(A), _whole(D), _whole(dt_bias), _whole(state)

@@ -303,3 +303,17 @@ def test_refusals(dev):
     both = torch.zeros(3, 16, 4, device=dev)
     with pytest.raises(ValueError, match="overlaps"):
         selective_step(both[:2], cut[0], cut[1], s["A"], cut[2], cut[3], out_state=both[1:])
+
+
+def test_lengths_past_32_bits(dev):
+    s = _make(dev, 3, 9, 16, 4)
+    outs = [_call(dict(s, lengths=v)) for v in (torch.tensor([2 ** 32 + 2, 4, -2 ** 33], device=dev),
+                                                torch.tensor([9, 4, 0], dtype=torch.int32, device=dev))]
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+def test_rows_far_apart(dev):
+    """Sequences that lie token by token in a large buffer, and rows that overlap."""
+    s = _make(dev, 2, 40, 64, 16, dtype=BF)
+    big = torch.randn(40, 2, 64 * 300, device=dev).to(BF)
+    _check(dict(s, u=big.transpose(0, 1)[..., 128:192], dt=s["dt"].as_strided((2, 40, 64), (3, 5, 1))))

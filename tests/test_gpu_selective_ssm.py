@@ -252,6 +252,11 @@ def test_causal_conv_module(dev, norm, bias):
     assert torch.equal(torch.cat(ys, 1), whole) and hist.shape == (2, 48, 9)
     with pytest.raises(ValueError, match="conv history"):
         conv.forward_incremental(x, hist[:, :, :4])
+    half = conv.to(BF)                                  # fp32 rows beside parameters of another type
+    p = {k: mixing.d(v) for k, v in half.state_dict().items()}
+    want, _ = mixing.short_conv(_norm64(p, "norm", mixing.d(x), 1e-5), p["conv.weight"][:, 0], p.get("conv.bias"), 3, True)
+    assert om.rel_err(half(x).detach().cpu(), want) < 1e-5
+    conv = conv.to(FP)
     if norm == "LayerNorm":
         xl = x.clone().requires_grad_(True)
         leaves = [xl, *conv.parameters()]

@@ -230,3 +230,13 @@ def test_refusals(dev):
     both = torch.zeros(3, 3, 16, device=dev, dtype=BF)
     with pytest.raises(ValueError, match="overlaps"):
         short_conv_step(x[:, 0], both[:2], w, b, out_history=both[1:])
+
+
+def test_long_dilations_and_lengths_past_32_bits(dev):
+    for t in (1, 3, 40):
+        _check(_make(dev, 2, t, 24, 4, 50, BF))                       # fewer positions than residue classes
+    s = _make(dev, 3, 9, 16, 4, 1, BF)
+    far = torch.tensor([2 ** 32 + 2, 4, -2 ** 33], device=dev)        # the first is past the end, not 2
+    y = short_conv(s["x"], s["w"], s["bias"], history=s["hist"], lengths=far)
+    assert torch.equal(y, short_conv(s["x"], s["w"], s["bias"], history=s["hist"],
+                                     lengths=torch.tensor([9, 4, 0], dtype=torch.int32, device=dev)))
