@@ -22,6 +22,8 @@
 // (from zero) and total step sizes, then their start states from one short pass over the chunks, then every
 // chunk from its start.  The backward pass does the same for q, backwards, and takes the states of
 // every GSEG tokens' start from the forward pass (N / GSEG floats a (token, channel)).
+#include <type_traits>
+
 #include "common.h"
 
 namespace lng {
@@ -38,7 +40,9 @@ struct Dims {
   int64_t B;
   int T, chunk, segs, gsegs;  // chunk: tokens of a chunk, a multiple of SEG; segs, gsegs: a sequence's segments
   int C, N, G, chunks, cbg;  // cbg: channel blocks of 64 in a group
+  int np;                    // states of a tile: N, or N and zero rows up to whole sixteens
   int softplus;
+  int rows;                  // a tile's values in the order of a state a lane: fours of tokens, then states
 };
 
 struct Ptrs {
@@ -80,19 +84,26 @@ __device__ __forceinline__ int seq_len(const int32_t* lengths, int64_t b, int T)
 template <typename T>
 __global__ __launch_bounds__(256) void k_sel_tiles(Dims d, Ptrs p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t n_tiles = d.B * d.G * d.segs * SEG * d.N;
+  const int64_t n_tiles = d.B * d.G * d.segs * SEG * d.np;
   if (i < n_tiles) {
-    const int n = static_cast<int>(i % d.N), k = static_cast<int>(i / d.N % SEG);
-    const int64_t seg = i / d.N / SEG % d.segs, bg = i / d.N / SEG / d.segs, g = bg % d.G, b = bg / d.G;
+    const int n = static_cast<int>(i % d.np), k = static_cast<int>(i / d.np % SEG);
+    const int64_t seg = i / d.np / SEG % d.segs, bg = i / d.np / SEG / d.segs, g = bg % d.G, b = bg / d.G;
     const int64_t t = seg * SEG + k;
     float bv = 0.f, cv = 0.f;
-    if (t < seq_len(p.lengths, b, d.T)) {
+    if (n < d.N && t < seq_len(p.lengths, b, d.T)) {
       bv = to_f32(static_cast<const T*>(p.Bm)[b * p.Bb + t * p.Bt + g * p.Bg + n]);
       cv = to_f32(static_cast<const T*>(p.Cm)[b * p.Cb + t * p.Ct + g * p.Cg + n]);
     }
-    float* const o = p.tiles + ((bg * d.segs + seg) * d.N + n) * 2 * SEG + k;
-    o[0] = bv;
-    o[SEG] = cv;
+    float* const tile = p.tiles + (bg * d.segs + seg) * d.np * 2 * SEG;
+    if (d.rows) {
+      float* const o = tile + n / 16 * 32 * SEG + k / 4 * 64 + n % 16 * 4 + k % 4;
+      o[0] = bv;
+      o[SEG * 16] = cv;
+    } else {
+      float* const o = tile + n * 2 * SEG + k;
+      o[0] = bv;
+      o[SEG] = cv;
+    }
   } else if (i - n_tiles < static_cast<int64_t>(d.C) * d.N) {
     const int64_t j = i - n_tiles, c = j % d.C, n = j / d.C;
     p.at[j] = p.A[c * d.N + n];
@@ -313,7 +324,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
       if (p.z) fetch<T>(p.z, w.b * p.zb, p.zt, t, stop, d.C, in, zr);
   };
   Warm warm;
-  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.N * 2 * SEG; };
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.np * 2 * SEG; };
   if (w.t0 < stop) {
     warm.start(p.tiles, tile_of(w.t0), d.N, w.lane);
     read(w.t0);
@@ -341,7 +352,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
 #pragma unroll
     for (int i = 0; i < SEG; ++i) {
       if constexpr (AGG) total += s[i];
-      y[i] = dskip * x[i];
+      y[i] = p.D ? dskip * x[i] : 0.f;  // nothing of u without a skip, were it infinite
       x[i] *= s[i];
       gate[i] = 1.f;
     }
@@ -445,6 +456,182 @@ __global__ __launch_bounds__(1024) void k_sel_join(Dims d, Ptrs p) {
   }
 }
 
+// ------------------------------------------------------------------ a state a lane
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ float swap_add(bool high, float a, float b) {  // low lanes keep a's sum, high lanes b's
+  const float keep = high ? b : a, give = high ? a : b;
+  return keep + dpp_move<CTRL>(give);
+}
+// The sum over a row of 16 lanes of each of 16 values, in 45 operations: lane j of the row receives value j's.
+__device__ __forceinline__ float row_sums(float (&v)[16], int j) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = swap_add<0x128>(j & 8, v[i], v[i + 8]);  // row_ror:8
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = swap_add<0x141>(j & 4, v[i], v[i + 4]);  // row_half_mirror
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = swap_add<0x4E>(j & 2, v[i], v[i + 2]);   // quad_perm 2 3 0 1
+  return swap_add<0xB1>(j & 1, v[0], v[1]);                                   // quad_perm 1 0 3 2
+}
+
+// What the wave's lanes wrote to LDS before is what they read behind it.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <int I, int S, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  if constexpr (I < S) {
+    f(std::integral_constant<int, I>{});
+    unrolled<I + 1, S>(f);
+  }
+}
+
+// Prompts in one pass, without a cut in time: a wave holds four channels, a row of 16 lanes each, and lane j of
+// a row holds state j (and j + 16) of its channel.  What a (token, channel) needs once (step size, input, gate,
+// output) is read, made and written by lane 4 * token + channel, so that a load's neighbours are neighbours in
+// memory (token-major lanes took 1.37 us a segment instead of 1.15 with two waves a SIMD: 64 lines a load);
+// step sizes and inputs reach the rows through LDS, and a segment's 16 outputs are summed over a row's states in
+// 45 operations.  The next segment's tile and the inputs after it are asked for before this segment is run.
+// A wave needs 0.6 us a segment whatever its neighbours do, so few and short sequences are what it is for
+// (rows_serve): 1 x 64 x 2048 13 us against 45 by chunks, 16 x 128 x 1024 29 against 51.
+template <typename T, int K>
+struct RowSeg {
+  f32x4 B[K][4], C[K][4];
+  unsigned u, dt, z;
+};
+template <typename T, int K, bool CKPT>
+__global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
+  __shared__ f32x4 lds[WAVES][5][9];  // a channel's 16 step sizes and 16 inputs; the fifth row: zeros
+  const int lane = threadIdx.x & 63, r = lane >> 4, j = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned waves = blockDim.x >> 6;
+  const int cg = d.C / d.G;
+  const unsigned bpg = (cg + 4 * waves - 1) / (4 * waves), x = blockIdx.x, cb = x % (bpg * d.G);
+  const int64_t b = x / (bpg * d.G);
+  const int g = cb / bpg, in0 = ((cb % bpg) * waves + wave) * 4;
+  if (in0 >= cg) return;
+  const bool ok = in0 + r < cg;
+  const int c = g * cg + (ok ? in0 + r : cg - 1), es = sizeof(T);
+  const int64_t bg = b * d.G + g;
+  const int end = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, d.T));
+  float a[K], h[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int n = j + 16 * k;
+    const bool real = n < d.N;
+    a[k] = real ? p.A[static_cast<int64_t>(c) * d.N + n] * LOG2E : 0.f;
+    h[k] = real && p.start ? p.start[(b * d.C + c) * d.N + n] : 0.f;
+  }
+  // a token's four channels in neighbouring lanes for what a (token, channel) needs once
+  const int lt = lane >> 2, lr = lane & 3;
+  const bool lok = in0 + lr < cg;
+  const int lc = g * cg + (lok ? in0 + lr : cg - 1);
+  const float bias = p.bias ? p.bias[lc] : 0.f, dskip = p.D ? p.D[lc] : 0.f;
+  const int ou = lt * static_cast<int>(p.ut) * es + lc * es, od = lt * static_cast<int>(p.dtt) * es + lc * es;
+  // loads without a branch, so that a wait counts exactly the ones it is for: without a gate z reads u
+  const T* const zp = p.z ? static_cast<const T*>(p.z) + b * p.zb : static_cast<const T*>(p.u) + b * p.ub;
+  const int64_t zt = p.z ? p.zt : p.ut;
+  const int oz = lt * static_cast<int>(zt) * es + lc * es;
+  const int oy = lok ? (lt * d.C + lc) * es : static_cast<int>(0x80000000u);
+  float* const own_lds = reinterpret_cast<float*>(&lds[wave][0][0]) + lr * 36 + lt;
+  // lanes without a state take the zeros, so that what isn't finite in a row stays out of its sums
+  const f32x4* const row_lds = &lds[wave][j < d.N ? r : 4][0];
+  if (lane < 9) lds[wave][4][lane] = f32x4{};
+  const int last = end > 0 ? (end - 1) / SEG * SEG : 0;
+  auto read_own = [&](int t, RowSeg<T, K>& s) {
+    t = t < last ? t : last;
+    const int n = live<SEG>(t, end);
+    s.u = Rows<T>(static_cast<const T*>(p.u) + b * p.ub + t * p.ut, p.ut, n, d.C).load(ou, 0);
+    s.dt = Rows<T>(static_cast<const T*>(p.dt) + b * p.dtb + t * p.dtt, p.dtt, n, d.C).load(od, 0);
+    s.z = Rows<T>(zp + t * zt, zt, n, d.C).load(oz, 0);
+  };
+  auto read_tile = [&](int t, RowSeg<T, K>& s) {
+    t = t < last ? t : last;
+    const f32x4* const q =
+        reinterpret_cast<const f32x4*>(p.tiles + (bg * d.segs + static_cast<unsigned>(t) / SEG) * K * 32 * SEG);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.B[k][i] = q[k * 128 + i * 16 + j], s.C[k][i] = q[k * 128 + 64 + i * 16 + j];
+  };
+  auto run = [&](int t, RowSeg<T, K>& in, RowSeg<T, K>& next) {
+    unsigned ub = in.u, db = in.dt, zb = in.z;
+    asm volatile("" : "+v"(ub), "+v"(db), "+v"(zb));  // converted here, not where they are asked for
+    const bool own = t + lt < end;
+    const float u = own ? value<T>(ub) : 0.f;
+    float s = value<T>(db) + bias;
+    if (d.softplus) s = softplus(s);
+    s = own ? s : 0.f;
+    const float xs = s * u;
+    wave_order();
+    own_lds[0] = s;
+    own_lds[16] = xs;
+    wave_order();
+    read_tile(t + SEG, next);
+    read_own(t + 2 * SEG, in);
+    f32x4 ss[4], xx[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss[i] = row_lds[i], xx[i] = row_lds[4 + i];
+    __builtin_amdgcn_sched_barrier(0);
+    float v[SEG];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      unrolled<0, SEG>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (CKPT && i % GSEG == 0) {
+          const int seg = (t + i) / GSEG;
+          const Rows<float> ck(p.ckpt + (b * d.gsegs + (seg < d.gsegs ? seg : 0)) * d.N * d.C, d.C, d.N, d.C);
+          const int n = j + 16 * k;
+          ck.store(ok && n < d.N && t + i < end ? (n * d.C + c) * 4 : static_cast<int>(0x80000000u), 0, h[k]);
+        }
+        h[k] = fmaf(__builtin_amdgcn_exp2f(ss[i / 4][i % 4] * a[k]), h[k], xx[i / 4][i % 4] * in.B[k][i / 4][i % 4]);
+        if (k)
+          v[i] = j + 16 < d.N ? fmaf(in.C[k][i / 4][i % 4], h[k], v[i]) : v[i];
+        else
+          v[i] = in.C[k][i / 4][i % 4] * h[k];
+      });
+    }
+    const float sum = __builtin_bit_cast(
+        float, __builtin_amdgcn_ds_bpermute((lr * 16 + lt) * 4, __builtin_bit_cast(int, row_sums(v, j))));
+    float y = p.D ? fmaf(dskip, u, sum) : sum;
+    if (p.z) y *= silu<T>(value<T>(zb));
+    const Rows<T> out(static_cast<T*>(p.y) + (b * d.T + t) * d.C, d.C, live<SEG>(t, d.T), d.C);
+    out.store(oy, 0, own ? y : 0.f);
+  };
+  int t = 0;
+  if (end > 0) {
+    RowSeg<T, K> s0, s1;
+    read_own(0, s0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_tile(0, s0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_own(SEG, s1);
+    __builtin_amdgcn_sched_barrier(0);
+    for (;;) {
+      run(t, s0, s1);
+      t += SEG;
+      if (t > last) break;
+      run(t, s1, s0);
+      t += SEG;
+      if (t > last) break;
+    }
+  }
+  for (; t < d.T; t += SEG) {
+    const Rows<T> out(static_cast<T*>(p.y) + (b * d.T + t) * d.C, d.C, live<SEG>(t, d.T), d.C);
+    out.store(oy, 0, 0.f);
+  }
+  if (p.end && ok) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (j + 16 * k < d.N) p.end[(b * d.C + c) * d.N + j + 16 * k] = h[k];
+  }
+}
+
 // A chunk's own gradient of the state in front of it (nothing from behind) and its total step size.
 template <typename T>
 __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
@@ -460,7 +647,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
   };
   const int last = stop > w.t0 ? (stop - 1) / SEG * SEG : w.t0 - SEG;
   Warm warm;
-  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.N * 2 * SEG; };
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.np * 2 * SEG; };
   if (last >= w.t0) {
     warm.start(p.tiles, tile_of(last), d.N, w.lane);
     read(last);
@@ -503,15 +690,6 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_grad_ends(Dims d, Ptrs p) {
 // The sum over the wave's 64 lanes of each of 16 values, in 35 operations instead of 16 * 7: every round
 // halves the values that a lane carries by handing the other half to its partner.  Lane l receives the sum
 // of value l / 4.
-template <int CTRL>
-__device__ __forceinline__ float dpp_move(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
-}
-template <int CTRL>
-__device__ __forceinline__ float swap_add(bool high, float a, float b) {  // low lanes keep a's sum, high lanes b's
-  const float keep = high ? b : a, give = high ? a : b;
-  return keep + dpp_move<CTRL>(give);
-}
 // The two halves of a swap's result, added.  (Through integers of their own: a bit cast of a vector's element
 // takes the vector's first one.)
 __device__ __forceinline__ float sum_of(unsigned a, unsigned b) {
@@ -565,7 +743,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void k_sel_grad(Dims d, Ptrs p) {
   const int in = w.in<T>(), out_t = w.in<T>(true), in32 = w.in<float>();
   const Rows<float> at(p.at, d.C, N, d.C);
   Warm warm;
-  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * N * 2 * SEG + t % SEG; };
+  auto tile_of = [&](int t) { return (w.bg * d.segs + t / SEG) * d.np * 2 * SEG + t % SEG; };
   warm.start(p.tiles, tile_of(w.t1 - 1), N, w.lane);
   for (int t = (w.t1 - 1) / GSEG * GSEG; t >= w.t0; t -= GSEG) {
     const int64_t row = (w.b * d.T + t) * d.C;
@@ -639,9 +817,9 @@ __global__ __launch_bounds__(64 * WAVES, 3) void k_sel_grad(Dims d, Ptrs p) {
 #pragma unroll
         for (int i = 0; i < GSEG; ++i) {
           dD = fmaf(e[i], u[i], dD);
-          dz[i] *= fmaf(dskip, u[i], y[i]);
+          dz[i] *= p.D ? fmaf(dskip, u[i], y[i]) : y[i];
           gs[i] = fmaf(gb[i], u[i], gs[i]) * slope[i];  // d dt
-          gb[i] = fmaf(gb[i], s[i], e[i] * dskip);      // du
+          gb[i] = fmaf(gb[i], s[i], p.D ? e[i] * dskip : 0.f);      // du
         }
         if (t + GSEG > w.end) {
 #pragma unroll
@@ -790,9 +968,20 @@ int waves_for(const Dims& d, bool grad) {
   return std::min(by_n, d.cbg);
 }
 
+// Whether a state a lane serves a forward call: its time grows with a sequence's segments alone until every SIMD
+// has its waves, the chunks' with all tokens behind 30 us of their own.  Measured at 16 states, rows against
+// chunks: 1 x 64 x 2048 13 us and 45, 16 x 128 x 1024 29 and 51, 1 x 512 x 512 28 and 40, 3 x 777 x 1000 44 and 55,
+// 4 x 1024 x 2048 81 and 100, 2 x 1024 x 1024 50 and 50; 1 x 1024 x 512 50 and 46, 8 x 4096 x 256 170 and 102.
+// Far more waves pay each wave's beginning: 64 x 16 x 2048 42 and 26.  Below 9 states half of a row has nothing to
+// do (4 x 512 x 2048 with 4 states 39 by chunks), above 32 the tiles no longer fit in registers.
+bool rows_serve(const Dims& d) {
+  const int64_t lanes = d.B * d.C;
+  return lanes <= 65536 && (d.T <= 512 || (d.T <= 1024 && lanes >= 2048));
+}
+
 Dims make_dims(const lng_selective& a, bool grad) {
   Dims d{};
-  d.B = a.B, d.T = static_cast<int>(a.T), d.C = a.C, d.N = a.N, d.G = a.G, d.softplus = a.softplus;
+  d.B = a.B, d.T = static_cast<int>(a.T), d.C = a.C, d.N = a.N, d.np = a.N, d.G = a.G, d.softplus = a.softplus;
   d.cbg = static_cast<int>(cdiv(a.C / a.G, 64));
   d.segs = static_cast<int>(cdiv(a.T, SEG)), d.gsegs = static_cast<int>(cdiv(a.T, GSEG));
   // chunks of at least four segments, for two waves on each of the 1024 SIMDs (the backward pass, whose waves
@@ -803,6 +992,10 @@ Dims make_dims(const lng_selective& a, bool grad) {
   if (units * want < 2048) want = std::min<int64_t>(cdiv(2048, std::max<int64_t>(units, 1)), std::max(1, d.segs / 2));
   d.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1)))) * SEG;
   d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
+  if (!grad && d.N > 8 && d.N <= 32) {
+    d.np = static_cast<int>(cdiv(d.N, 16)) * 16;
+    d.rows = rows_serve(d);
+  }
   return d;
 }
 
@@ -815,7 +1008,7 @@ struct Space {  // workspace offsets in floats
   }
   Space(const Dims& d, bool grad) {
     const int64_t NC = int64_t{d.N} * d.C, units = d.B * d.chunks;
-    tiles = take(d.B * d.G * d.segs * SEG * 2 * d.N);
+    tiles = take(d.B * d.G * d.segs * SEG * 2 * d.np);
     at = take(NC);
     hloc = take(d.chunks > 1 ? units * NC : 0);
     ssum = take(d.chunks > 1 ? units * d.C : 0);
@@ -879,9 +1072,26 @@ void launch_join(const Dims& d, const Ptrs& p, hipStream_t st) {
 
 template <typename T>
 int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
+  if (d.rows) {
+    k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+    const int cg = d.C / d.G, waves = static_cast<int>(std::min<int64_t>(WAVES, cdiv(cg, 4)));
+    const unsigned blocks = static_cast<unsigned>(cdiv(cg, 4 * waves) * d.G * d.B);
+    auto launch = [&](auto ck) {
+      constexpr bool CK = decltype(ck)::value;
+      if (d.N <= 16)
+        k_sel_rows<T, 1, CK><<<blocks, 64 * waves, 0, st>>>(d, p);
+      else
+        k_sel_rows<T, 2, CK><<<blocks, 64 * waves, 0, st>>>(d, p);
+    };
+    if (p.ckpt)
+      launch(std::true_type{});
+    else
+      launch(std::false_type{});
+    return check_launch("selective_scan");
+  }
   const int waves = waves_for(d, false);
   const unsigned blocks = unit_blocks(d, waves);
-  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.N + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
   if (d.chunks > 1) {
     k_sel_scan<T, true><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
     launch_join<false>(d, p, st);
@@ -894,7 +1104,7 @@ template <typename T>
 int run_grad(const Dims& d, Ptrs p, const lng_selective_grad& g, hipStream_t st) {
   const int waves = waves_for(d, true);
   const unsigned blocks = unit_blocks(d, waves);
-  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.N + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
   if (d.chunks > 1) {
     k_sel_grad_ends<T><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
     launch_join<true>(d, p, st);

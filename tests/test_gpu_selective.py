@@ -92,6 +92,31 @@ def test_several_chunks(dev, b, t, c, dtype):
     _check(_make(dev, b, t, c, 16, 1, dtype))
 
 
+@pytest.mark.parametrize("b,t,c,n,g", [(1, 600, 70, 16, 1), (2, 1030, 24, 20, 2), (1, 513, 64, 12, 1),
+                                       (2, 512, 40, 9, 1), (3, 100, 33, 17, 3), (2, 48, 60, 32, 1), (1, 37, 1, 33, 1),
+                                       (3, 530, 700, 16, 1), (2, 15, 6, 24, 2)])
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_states_over_lanes_and_over_time(dev, b, t, c, n, g, dtype):
+    """Both ways to run a prompt, on each side of their rule in lengths, channels and states."""
+    _check(_make(dev, b, t, c, n, g, dtype, ragged=b > 1))
+
+
+@pytest.mark.parametrize("n", [5, 9, 12, 16, 20, 32, 40])
+@pytest.mark.parametrize("t", [20, 600])
+def test_infinite_input_stays_infinite(dev, n, t):
+    """Positive B and C: what follows an infinite input is infinite in its channel and finite in the others, and
+    nothing multiplies it by a state that isn't there."""
+    s = _make(dev, 1, t, 9, n, gate=False, plain=True, start=False)
+    s["u"] = s["u"].abs()
+    s["u"][0, 7, 4] = float("inf")
+    s["B"], s["C"] = s["B"].abs() + 0.1, s["C"].abs() + 0.1
+    s["dt"] = s["dt"] * 0.01 + 1e-3                                  # decays far from zero over all of the tokens
+    y, end = _call(s)
+    assert torch.isinf(y[0, 7:, 4]).all() and (y[0, 7:, 4] > 0).all() and torch.isinf(end[0, 4]).all()
+    rest = [i for i in range(9) if i != 4]
+    assert torch.isfinite(y[:, :, rest]).all() and torch.isfinite(y[0, :7]).all()
+
+
 @pytest.mark.parametrize("t", [5, 48, 150, 260])
 @pytest.mark.parametrize("start", [True, False])
 def test_ragged_batches(dev, t, start):
