@@ -10,6 +10,8 @@
 // once per block, and in the backward pass the weight gradients of a thread's columns stay in registers
 // over all of the block's rows: they leave as one partial row per block, summed in a fixed order by
 // k_norm_partials (no atomics: the result of a call does not vary).
+// bf16, out of the Infinity Cache where a call fits: 16384 x 1024 13 us (67 MB) forward, 19 backward (100 MB)
+// and 4 for the partial rows; 421911 x 256 78 us, 5.5 TB/s.
 #include "common.h"
 
 namespace lng {

@@ -11,7 +11,10 @@
 //   ds = u sum_n q B + sum_n q exp(s A) h[t-1] A,  dA = sum_t q exp(s A) h[t-1] s,  d dt = ds softplus'(dt)
 //
 // Bound by the vector ALU: an exponential and some five multiply-adds for every (token, channel, state), on
-// 8 bytes a (token, channel).  A lane holds one channel, so u, dt, z and y move as whole rows, and what all
+// 8 bytes a (token, channel).  An exponential and four of the others take a SIMD 25 cycles a wave, so one pass
+// over 8 x 4096 x 256 x 16 states is 21 us of all SIMDs' time and its bytes are 14 us; it takes 52, and 37 more
+// for the chunks' ends, whose waves (two a SIMD) do not cover each other's waits.  A training step of
+// 8 x 2048 x 1024 x 16: forward 105 and 67, backward 245 and 77 us, 505 with all.  A lane holds one channel, so u, dt, z and y move as whole rows, and what all
 // of a wave's channels share (B and C of a token) comes through the scalar unit: k_sel_tiles lays B and C
 // out as fp32 tiles of SEG tokens per state, and a tile's row of 2 * SEG values is one scalar load for
 // 64 * SEG state updates.  A segment of SEG tokens stays in registers (step sizes, inputs, outputs) while
@@ -21,7 +24,8 @@
 // Where batch * channels gives too few waves, the time axis is cut into chunks: the chunks' own end states
 // (from zero) and total step sizes, then their start states from one short pass over the chunks, then every
 // chunk from its start.  The backward pass does the same for q, backwards, and takes the states of
-// every GSEG tokens' start from the forward pass (N / GSEG floats a (token, channel)).
+// every GSEG tokens' start from the forward pass (N / GSEG floats a (token, channel)).  Short prompts of up to
+// 32 states are not cut: k_sel_rows gives every state a lane instead (rows_serve says when).
 #include <type_traits>
 
 #include "common.h"
@@ -262,7 +266,7 @@ struct Warm {
 
 // Scalar loads come back in any order, so a wait for one is a wait for all: it stands in front of the next
 // row's load, where what it waits for was asked for a whole row's work ago (behind that load, where the
-// compiler would put it, every row waits for memory: 75 us instead of 55 for the outputs of 8 x 4096 x 256).
+// compiler would put it, every row waits for memory: 20 us more for the outputs of 8 x 4096 x 256, now 52).
 constexpr int WAITCNT_LGKM0 = 0xC07F;  // s_waitcnt lgkmcnt(0), the other counts left open
 __device__ __forceinline__ void rows_arrived() {
   __builtin_amdgcn_sched_barrier(0);
@@ -271,8 +275,8 @@ __device__ __forceinline__ void rows_arrived() {
 }
 
 // A lane's per-state values (a state or its gradient, and the decay exponent A log2 e): the lane's columns of
-// [N][64] arrays in LDS.  They could stay in registers only with the walk over the states unrolled, and that
-// is slower: some 20 KB of code, which a wave runs through once a segment, are fetched slower than they run.
+// [N][64] arrays in LDS.  They could stay in registers only with the walk over the states unrolled for each N,
+// which is no faster (56 us against 55 for the outputs of 8 x 4096 x 256); one loop serves any N.
 struct States {
   float *v, *a;
   __device__ __forceinline__ States(float* lds, int wave, int lane, int N) {
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_scan(Dims d, Ptrs p) {
 // a chunk from behind, from the last chunk on, starting with the final state's gradient.  Block: 64 (b, n, c)
 // by up to 16 waves, each of which holds the values of JOIN neighbouring chunks in registers: their loads go
 // out together, their joint end and decay meet the other waves' in LDS, and longer sequences take another
-// round (22 us for 64 chunks one after the other, 9 with 16 loads at a time).
+// round (64 chunks of 8 x 16 x 256 states: 22 us one after the other, 9 with 16 loads at a time, 6 so).
 constexpr int JOIN = 8;
 template <bool BACK>
 __global__ __launch_bounds__(1024) void k_sel_join(Dims d, Ptrs p) {
@@ -903,7 +907,8 @@ __global__ __launch_bounds__(256) void k_sel_grad_a(Dims d, const float* __restr
 }
 
 // One new token of every sequence: LPC neighbouring lanes hold a channel, four states (16 bytes) each and a
-// round; the output is summed over the lanes.  `end` may be the state that is read.
+// round; the output is summed over the lanes.  `end` may be the state that is read.  Bound by memory, which is
+// the state read and written: 512 x 2048 x 16 134 MB in 32 us, 4.2 TB/s; 8 x 1024 x 16 3.6 us.
 template <typename T, int LPC, bool VEC>
 __global__ __launch_bounds__(256) void k_sel_step(Dims d, Ptrs p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -972,11 +977,13 @@ int waves_for(const Dims& d, bool grad) {
 // has its waves, the chunks' with all tokens behind 30 us of their own.  Measured at 16 states, rows against
 // chunks: 1 x 64 x 2048 13 us and 45, 16 x 128 x 1024 29 and 51, 1 x 512 x 512 28 and 40, 3 x 777 x 1000 44 and 55,
 // 4 x 1024 x 2048 81 and 100, 2 x 1024 x 1024 50 and 50; 1 x 1024 x 512 50 and 46, 8 x 4096 x 256 170 and 102.
-// Far more waves pay each wave's beginning: 64 x 16 x 2048 42 and 26.  Below 9 states half of a row has nothing to
-// do (4 x 512 x 2048 with 4 states 39 by chunks), above 32 the tiles no longer fit in registers.
+// Far more waves pay each wave's beginning: 64 x 16 x 2048 42 and 26.  Up to 8 states half of a row has nothing to
+// do (4 states: 1 x 256 x 512 21 and 30, 4 x 256 x 1024 23 and 30, 8 x 128 x 2048 28 and 28, 4 x 512 x 1024 34 and
+// 31); above 32 the tiles no longer fit in registers.
 bool rows_serve(const Dims& d) {
   const int64_t lanes = d.B * d.C;
-  return lanes <= 65536 && (d.T <= 512 || (d.T <= 1024 && lanes >= 2048));
+  if (d.N <= 8) return lanes <= 16384 && d.T <= 256;
+  return d.N <= 32 && lanes <= 65536 && (d.T <= 512 || (d.T <= 1024 && lanes >= 2048));
 }
 
 Dims make_dims(const lng_selective& a, bool grad) {
@@ -992,10 +999,8 @@ Dims make_dims(const lng_selective& a, bool grad) {
   if (units * want < 2048) want = std::min<int64_t>(cdiv(2048, std::max<int64_t>(units, 1)), std::max(1, d.segs / 2));
   d.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1)))) * SEG;
   d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
-  if (!grad && d.N > 8 && d.N <= 32) {
-    d.np = static_cast<int>(cdiv(d.N, 16)) * 16;
-    d.rows = rows_serve(d);
-  }
+  d.rows = !grad && rows_serve(d);
+  if (d.rows) d.np = static_cast<int>(cdiv(d.N, 16)) * 16;
   return d;
 }
 

@@ -18,6 +18,8 @@
 // The backward pass forms pre again from x (K multiply-adds) instead of reading it.  Weight gradients are
 // summed in registers over all of a thread's tiles, over a block's threads in LDS, and over blocks by
 // k_conv_partials in a fixed order.
+// bf16, 4 taps, SiLU: 8 x 4096 x 1024 33 us (134 MB, 4.1 TB/s), 3 x 777 x 1024 6.4; training of 8 x 2048 x 1024
+// 20 us forward, 35 backward (100 MB) and 4 for the partial rows.
 #include "common.h"
 
 namespace lng {
@@ -367,7 +369,8 @@ __global__ __launch_bounds__(256) void k_conv_partials(const float* __restrict__
 
 // One new token of every sequence: a thread owns VEC channels of a sequence, so the history may move in
 // place (hist_out == hist): each of its rows is read before the thread writes the row in front of it.  NEAR:
-// without dilation the window has at most MAX_TAPS rows, which are all asked for together.
+// without dilation the window has at most MAX_TAPS rows, which are all asked for together (512 x 2048: 5 us
+// instead of 12 with one row after the other).
 template <typename T, typename W, int VEC, int KT, bool NEAR>
 __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
   constexpr int KM = KT > 0 ? KT : MAX_TAPS;

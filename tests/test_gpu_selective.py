@@ -94,7 +94,8 @@ def test_several_chunks(dev, b, t, c, dtype):
 
 @pytest.mark.parametrize("b,t,c,n,g", [(1, 600, 70, 16, 1), (2, 1030, 24, 20, 2), (1, 513, 64, 12, 1),
                                        (2, 512, 40, 9, 1), (3, 100, 33, 17, 3), (2, 48, 60, 32, 1), (1, 37, 1, 33, 1),
-                                       (3, 530, 700, 16, 1), (2, 15, 6, 24, 2)])
+                                       (3, 530, 700, 16, 1), (2, 15, 6, 24, 2), (1, 300, 130, 5, 1), (2, 257, 9, 1, 1),
+                                       (2, 256, 20, 8, 4)])
 @pytest.mark.parametrize("dtype", [FP, BF])
 def test_states_over_lanes_and_over_time(dev, b, t, c, n, g, dtype):
     """Both ways to run a prompt, on each side of their rule in lengths, channels and states."""
