@@ -1013,7 +1013,8 @@ struct Space {  // workspace offsets in floats
   }
   Space(const Dims& d, bool grad) {
     const int64_t NC = int64_t{d.N} * d.C, units = d.B * d.chunks;
-    tiles = take(d.B * d.G * d.segs * SEG * 2 * d.np);
+    // room for padded tiles in either direction, so that what serves a shape's backward pass serves its forward
+    tiles = take(d.B * d.G * d.segs * SEG * 2 * (d.N <= 32 ? cdiv(d.N, 16) * 16 : d.N));
     at = take(NC);
     hloc = take(d.chunks > 1 ? units * NC : 0);
     ssum = take(d.chunks > 1 ? units * d.C : 0);
