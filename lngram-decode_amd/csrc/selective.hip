@@ -980,6 +980,7 @@ int waves_for(const Dims& d, bool grad) {
 // Far more waves pay each wave's beginning: 64 x 16 x 2048 42 and 26.  Up to 8 states half of a row has nothing to
 // do (4 states: 1 x 256 x 512 21 and 30, 4 x 256 x 1024 23 and 30, 8 x 128 x 2048 28 and 28, 4 x 512 x 1024 34 and
 // 31); above 32 the tiles no longer fit in registers.
+int rows_states(const Dims& d) { return static_cast<int>(cdiv(d.N, 16)) * 16; }  // its tiles' states
 bool rows_serve(const Dims& d) {
   const int64_t lanes = d.B * d.C;
   if (d.N <= 8) return lanes <= 16384 && d.T <= 256;
@@ -1000,7 +1001,7 @@ Dims make_dims(const lng_selective& a, bool grad) {
   d.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(d.segs, std::max<int64_t>(want, 1)))) * SEG;
   d.chunks = static_cast<int>(std::max<int64_t>(1, cdiv(a.T, d.chunk)));
   d.rows = !grad && rows_serve(d);
-  if (d.rows) d.np = static_cast<int>(cdiv(d.N, 16)) * 16;
+  if (d.rows) d.np = rows_states(d);
   return d;
 }
 
@@ -1014,7 +1015,7 @@ struct Space {  // workspace offsets in floats
   Space(const Dims& d, bool grad) {
     const int64_t NC = int64_t{d.N} * d.C, units = d.B * d.chunks;
     // room for padded tiles in either direction, so that what serves a shape's backward pass serves its forward
-    tiles = take(d.B * d.G * d.segs * SEG * 2 * (d.N <= 32 ? cdiv(d.N, 16) * 16 : d.N));
+    tiles = take(d.B * d.G * d.segs * SEG * 2 * (rows_serve(d) ? rows_states(d) : d.N));
     at = take(NC);
     hloc = take(d.chunks > 1 ? units * NC : 0);
     ssum = take(d.chunks > 1 ? units * d.C : 0);

@@ -1555,6 +1555,7 @@ def short_conv_step(x: torch.Tensor, history: torch.Tensor, w: torch.Tensor, bia
         _call("short_conv_step", dev, lib().lng_short_conv_step, xc.data_ptr(), _DT[x.dtype], b, c, xc.stride(0),
               wc.data_ptr(), _ptr(bc), _DT[w.dtype], k, dilation, int(silu), history.data_ptr(), out.data_ptr(),
               y.data_ptr())
+        torch.autograd.graph.increment_version(out)      # a graph that keeps it for a backward pass has to know
     return y
 
 
@@ -1705,6 +1706,7 @@ def selective_step(state: torch.Tensor, u: torch.Tensor, dt: torch.Tensor, A: to
     y = torch.empty(u.shape, dtype=u.dtype, device=dev)
     a, keep = _selective_args("selective_step", u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, None, y, out, 2)
     _call("selective_step", dev, lib().lng_selective_step, ctypes.byref(a))
+    torch.autograd.graph.increment_version(out)
     del keep
     return y
 

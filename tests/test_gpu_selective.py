@@ -221,6 +221,15 @@ def test_step(dev, b, c, n, g, dtype):
     within(plain, wy[:, 0], my[:, 0], 44 + n, "plain")
 
 
+def test_step_in_place_is_seen_by_a_graph_that_kept_the_state(dev):
+    s = _make(dev, 2, 4, 16, 4)
+    A = s["A"].detach().requires_grad_(True)
+    y = selective_scan(s["u"], s["dt"], A, s["B"], s["C"], state=s["state"])
+    selective_step(s["state"], s["u"][:, 0], s["dt"][:, 0], s["A"], s["B"][:, 0], s["C"][:, 0])
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.sum().backward()
+
+
 def test_step_of_strided_rows(dev):
     s = _make(dev, 4, 1, 24, 16, 1, BF)
     wide = torch.randn(4, 100, device=dev).to(BF)

@@ -168,6 +168,15 @@ def test_step(dev, b, c, k, dil, dtype, wt):
     assert torch.equal(y, want[:, 0]) and torch.equal(h, nxt)
 
 
+def test_step_in_place_is_seen_by_a_graph_that_kept_the_history(dev):
+    s = _make(dev, 2, 4, 16, 4, 1, FP)
+    w = s["w"].detach().requires_grad_(True)
+    y = short_conv(s["x"], w, s["bias"], history=s["hist"])
+    short_conv_step(s["x"][:, 0], s["hist"], s["w"], s["bias"])
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.sum().backward()
+
+
 def test_empty_batches(dev):
     s = _make(dev, 2, 4, 16, 4, 1, BF)
     y, h = short_conv(s["x"][:, :0], s["w"], s["bias"], history=s["hist"], return_history=True)
