@@ -110,7 +110,8 @@ class SelectiveSSM(nn.Module):
 
     ``forward`` takes whole sequences (differentiable), ``step`` one token of every sequence; both carry the
     same state, ``(conv history [B, K - 1, state_dim], scan state [B, state_dim, d_state])``, and leave the
-    one they are given as it was, so that taking tokens back is keeping an earlier one."""
+    one they are given as it was, so that taking tokens back is keeping an earlier one.  Weights in fp32 or
+    bf16 (a product's rows that are no multiple of 8 values wide are padded there)."""
 
     def __init__(self, d_model: int, state_dim: int = 256, d_state: int = 16, conv_kernel: int = 4,
                  dt_rank: Optional[int] = None, eps: float = 1e-5, init_std: float = 0.02, dt_min: float = 1e-3,
@@ -144,9 +145,12 @@ class SelectiveSSM(nn.Module):
                 torch.zeros(batch, self.state_dim, self.d_state, dtype=torch.float32, device=w.device))
 
     def _linear(self, x: Tensor, w: nn.Linear) -> Tensor:
-        if _needs_grad(x, w.weight):
-            return _Linear.apply(x, w.weight)
-        return ops.linear(x, w.weight)
+        weight, odd = w.weight, -x.shape[-1] % 8
+        if odd and x.dtype == torch.bfloat16:            # the bf16 product reads 16 bytes at a time
+            x, weight = nn.functional.pad(x, (0, odd)), nn.functional.pad(weight, (0, odd))
+        if _needs_grad(x, weight):
+            return _Linear.apply(x, weight)
+        return ops.linear(x, weight)
 
     def _inputs(self, emb: Tensor) -> tuple:
         return self._linear(self.norm(emb.to(self.w_in.weight.dtype)), self.w_in).chunk(2, dim=-1)

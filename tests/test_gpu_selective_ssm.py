@@ -96,6 +96,36 @@ def test_parts_and_steps_continue_a_sequence(dev, dtype, tol):
     assert om.rel_err(whole.float().cpu(), want) < tol
 
 
+@pytest.mark.parametrize("d,n", [(72, 24), (100, 30)])
+def test_bf16_training_of_odd_widths(dev, d, n):
+    """Widths and ranks that are no multiple of 8: features as fp32 weights of the same values give them, and
+    gradients of all parameters, from ragged sequences' features and both parts of the state."""
+    m = _ssm(dev, d, n, BF)
+    emb = torch.randn(2, 40, d, device=dev).to(BF)
+    own = torch.tensor([40, 7], device=dev)
+    y, (hist, scan) = m(emb, lengths=own, return_state=True)
+    assert y.dtype == BF and scan.dtype == FP and bool((y[1, 7:] == 0).all())
+    wide = SelectiveSSM(d, n).to(dev)
+    wide.load_state_dict(m.state_dict())
+    assert om.rel_err(y.detach().float().cpu(), wide(emb.float(), lengths=own).detach().cpu()) < 2e-2
+    (y.float().sum() + hist.float().sum() + scan.sum()).backward()
+    for k, p in m.named_parameters():
+        assert p.grad.shape == p.shape and p.grad.dtype == BF and bool(torch.isfinite(p.grad).all()), k
+
+
+def test_no_tokens_and_no_sequences(dev):
+    m = _ssm(dev)
+    emb = torch.randn(2, 5, 128, device=dev)
+    with torch.no_grad():
+        _, state = m(emb, return_state=True)
+        y, after = m(emb[:, :0], state=state, return_state=True)
+        assert y.shape == (2, 0, 48) and all(torch.equal(p, q) for p, q in zip(after, state))
+        assert m(emb[:0]).shape == (0, 5, 48)
+    y, after = m(emb[:, :0], state=state, return_state=True)
+    grads = torch.autograd.grad(y.sum() + after[1].sum(), list(m.parameters()), allow_unused=True)
+    assert all(g is None or bool((g == 0).all()) for g in grads)
+
+
 def test_step_replayed_from_a_graph(dev):
     m = _ssm(dev, dtype=BF)
     emb = torch.randn(4, 128, device=dev).to(BF)
