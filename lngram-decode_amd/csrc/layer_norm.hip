@@ -19,9 +19,12 @@ namespace {
 
 constexpr int VEC = 8;
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[VEC]) {
-  if constexpr (sizeof(T) == 2) {
+// V neighbouring elements: eight, aligned to 16 bytes, or one.
+template <typename T, int V>
+__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else if constexpr (sizeof(T) == 2) {
     typedef T T8 __attribute__((ext_vector_type(8)));
     const T8 r = *reinterpret_cast<const T8*>(p);
 #pragma unroll
@@ -32,9 +35,11 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[VEC]) {
     for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[VEC]) {
-  if constexpr (sizeof(T) == 2) {
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 2) {
     typedef T T8 __attribute__((ext_vector_type(8)));
     T8 r;
 #pragma unroll
@@ -70,54 +75,62 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   }
 }
 
-// A thread's columns of a row: element i of chunk j is column (lane + LPR * j) * VEC + i.
-template <typename T, int LPR, int NV>
-__device__ __forceinline__ void load_row(const T* p, int lane, int chunks, float (&v)[NV][VEC]) {
+// A thread's columns of a row: element i of chunk j is column (lane + LPR * j) * V + i.  Single elements are
+// asked for without branches (the last one again behind a row's end), so that all are on their way together.
+template <typename T, int LPR, int NV, int V>
+__device__ __forceinline__ void load_row(const T* p, int lane, int chunks, float (&v)[NV][V]) {
+  if constexpr (V == 1) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) load_v<T, V>(p + (lane + LPR * j < chunks ? lane + LPR * j : chunks - 1), v[j]);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j][0] = lane + LPR * j < chunks ? v[j][0] : 0.f;
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = lane + LPR * j;
     if (c < chunks) {
-      load8(p + c * VEC, v[j]);
+      load_v<T, V>(p + c * V, v[j]);
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = 0.f;
+      for (int i = 0; i < V; ++i) v[j][i] = 0.f;
     }
   }
 }
 
-template <typename T, typename W, int LPR, int NV>
+template <typename T, typename W, int LPR, int NV, int V>
 __global__ __launch_bounds__(256) void k_layer_norm(const T* __restrict__ x, int64_t rows, int d, int64_t xs,
                                                     const W* __restrict__ w, const W* __restrict__ b, float eps,
                                                     T* __restrict__ y, float* __restrict__ mean_out,
                                                     float* __restrict__ rstd_out) {
   constexpr int RPB = 256 / LPR;
   __shared__ float red[4];
-  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR, chunks = d / VEC;
+  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR, chunks = d / V;
   const float inv_d = 1.f / static_cast<float>(d);
-  float wv[NV][VEC], bv[NV][VEC];
+  float wv[NV][V], bv[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) wv[j][i] = 1.f, bv[j][i] = 0.f;
-  if (w) load_row<W, LPR, NV>(w, lane, chunks, wv);
-  if (b) load_row<W, LPR, NV>(b, lane, chunks, bv);
+    for (int i = 0; i < V; ++i) wv[j][i] = 1.f, bv[j][i] = 0.f;
+  if (w) load_row<W, LPR, NV, V>(w, lane, chunks, wv);
+  if (b) load_row<W, LPR, NV, V>(b, lane, chunks, bv);
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * RPB; base < rows; base += static_cast<int64_t>(gridDim.x) * RPB) {
     const bool ok = base + slot < rows;
     const int64_t row = ok ? base + slot : rows - 1;
-    float v[NV][VEC];
-    load_row<T, LPR, NV>(x + row * xs, lane, chunks, v);
+    float v[NV][V];
+    load_row<T, LPR, NV, V>(x + row * xs, lane, chunks, v);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s += v[j][i];
+      for (int i = 0; i < V; ++i) s += v[j][i];
     const float mean = row_sum<LPR>(s, red) * inv_d;
     s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (lane + LPR * j < chunks) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] -= mean, s += v[j][i] * v[j][i];
+        for (int i = 0; i < V; ++i) v[j][i] -= mean, s += v[j][i] * v[j][i];
       }
     }
     const float rstd = 1.f / sqrtf(row_sum<LPR>(s, red) * inv_d + eps);
@@ -127,8 +140,8 @@ __global__ __launch_bounds__(256) void k_layer_norm(const T* __restrict__ x, int
         const int c = lane + LPR * j;
         if (c < chunks) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * rstd * wv[j][i] + bv[j][i];
-          store8(y + row * d + c * VEC, v[j]);
+          for (int i = 0; i < V; ++i) v[j][i] = v[j][i] * rstd * wv[j][i] + bv[j][i];
+          store_v<T, V>(y + row * d + c * V, v[j]);
         }
       }
       if (lane == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
@@ -137,7 +150,7 @@ __global__ __launch_bounds__(256) void k_layer_norm(const T* __restrict__ x, int
 }
 
 // One block per row, any width and alignment: the row is read three times (the second and third from the
-// caches).  Widths past 8192 and rows that 8-element loads cannot take.
+// caches).  Widths past 8192.
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void k_layer_norm_any(const T* __restrict__ x, int64_t rows, int64_t d, int64_t xs,
                                                         const W* __restrict__ w, const W* __restrict__ b, float eps,
@@ -163,7 +176,7 @@ __global__ __launch_bounds__(256) void k_layer_norm_any(const T* __restrict__ x,
   }
 }
 
-template <typename T, typename W, int LPR, int NV, int THREADS>
+template <typename T, typename W, int LPR, int NV, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_layer_norm_grad(const T* __restrict__ dy, int64_t dys,
                                                              const T* __restrict__ x, int64_t xs, int64_t rows, int d,
                                                              const W* __restrict__ w, const float* __restrict__ mean_in,
@@ -171,27 +184,27 @@ __global__ __launch_bounds__(THREADS) void k_layer_norm_grad(const T* __restrict
                                                              float* __restrict__ partial) {
   constexpr int RPB = THREADS / LPR;
   __shared__ float red[2][THREADS / 64];
-  __shared__ float cols[RPB > 1 ? THREADS * NV * VEC : 1];
-  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR, chunks = d / VEC;
+  __shared__ float cols[RPB > 1 ? THREADS * NV * V : 1];
+  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR, chunks = d / V;
   const float inv_d = 1.f / static_cast<float>(d);
-  float wv[NV][VEC], dw[NV][VEC], db[NV][VEC];
+  float wv[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) wv[j][i] = 1.f, dw[j][i] = 0.f, db[j][i] = 0.f;
-  if (w) load_row<W, LPR, NV>(w, lane, chunks, wv);
+    for (int i = 0; i < V; ++i) wv[j][i] = 1.f, dw[j][i] = 0.f, db[j][i] = 0.f;
+  if (w) load_row<W, LPR, NV, V>(w, lane, chunks, wv);
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * RPB; base < rows; base += static_cast<int64_t>(gridDim.x) * RPB) {
     const bool ok = base + slot < rows;
     const int64_t row = ok ? base + slot : rows - 1;
     const float mean = mean_in[row], rstd = rstd_in[row];
-    float v[NV][VEC], g[NV][VEC];
-    load_row<T, LPR, NV>(x + row * xs, lane, chunks, v);
-    load_row<T, LPR, NV>(dy + row * dys, lane, chunks, g);
+    float v[NV][V], g[NV][V];
+    load_row<T, LPR, NV, V>(x + row * xs, lane, chunks, v);
+    load_row<T, LPR, NV, V>(dy + row * dys, lane, chunks, g);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
+      for (int i = 0; i < V; ++i) {
         const float xn = (v[j][i] - mean) * rstd, gy = ok ? g[j][i] : 0.f;
         dw[j][i] += gy * xn;
         db[j][i] += gy;
@@ -208,8 +221,8 @@ __global__ __launch_bounds__(THREADS) void k_layer_norm_grad(const T* __restrict
         const int c = lane + LPR * j;
         if (c < chunks) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) g[j][i] = rstd * (g[j][i] - s1 - v[j][i] * s2);
-          store8(dx + row * d + c * VEC, g[j]);
+          for (int i = 0; i < V; ++i) g[j][i] = rstd * (g[j][i] - s1 - v[j][i] * s2);
+          store_v<T, V>(dx + row * d + c * V, g[j]);
         }
       }
     }
@@ -221,16 +234,16 @@ __global__ __launch_bounds__(THREADS) void k_layer_norm_grad(const T* __restrict
     if constexpr (RPB == 1) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (lane + LPR * j < chunks) store8(out + which * d + (lane + LPR * j) * VEC, which ? db[j] : dw[j]);
+        if (lane + LPR * j < chunks) store_v<float, V>(out + which * d + (lane + LPR * j) * V, which ? db[j] : dw[j]);
     } else {
       // the block's row slots are merged in LDS, each column by one thread, in the order of the slots
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < NV; ++j) store8(cols + (slot * LPR * NV + lane + LPR * j) * VEC, which ? db[j] : dw[j]);
+      for (int j = 0; j < NV; ++j) store_v<float, V>(cols + (slot * LPR * NV + lane + LPR * j) * V, which ? db[j] : dw[j]);
       __syncthreads();
       for (int c = threadIdx.x; c < d; c += THREADS) {
         float s = 0.f;
-        for (int r = 0; r < RPB; ++r) s += cols[r * LPR * NV * VEC + c];
+        for (int r = 0; r < RPB; ++r) s += cols[r * LPR * NV * V + c];
         out[which * d + c] = s;
       }
     }
@@ -315,7 +328,7 @@ bool vector_rows(const void* p, int64_t stride, int64_t d, int es) {
   return aligned16(p) && stride * es % 16 == 0 && d % VEC == 0;
 }
 
-constexpr int64_t MAX_VEC_D = 8192;
+constexpr int64_t MAX_ROW_D = 8192;  // a row in the registers of 256 threads
 constexpr int64_t GRAD_BLOCKS = 512;  // two blocks of 8 waves per CU
 
 // Blocks of the backward pass, each leaving one partial row of the weight gradients.
@@ -334,50 +347,65 @@ struct Rows {  // one call's rows
   hipStream_t st;
 };
 
-template <typename T, typename W, int LPR, int NV>
+template <typename T, typename W, int LPR, int NV, int V>
 void launch_fwd(const Rows& r) {
   constexpr int rpb = 256 / LPR;
   const int64_t grid = std::min<int64_t>(cdiv(r.rows, rpb), 2048);
-  k_layer_norm<T, W, LPR, NV><<<static_cast<unsigned>(grid), 256, 0, r.st>>>(
+  k_layer_norm<T, W, LPR, NV, V><<<static_cast<unsigned>(grid), 256, 0, r.st>>>(
       static_cast<const T*>(r.x), r.rows, static_cast<int>(r.d), r.xs, static_cast<const W*>(r.w),
       static_cast<const W*>(r.b), r.eps, static_cast<T*>(r.y), r.mean, r.rstd);
 }
 
-template <typename T, typename W, int LPR, int NV>
+template <typename T, typename W, int LPR, int NV, int V>
 void launch_bwd(const Rows& r) {
   constexpr int threads = LPR > 64 ? LPR : 512;
-  k_layer_norm_grad<T, W, LPR, NV, threads><<<static_cast<unsigned>(grad_blocks(r.rows, r.d)), threads, 0, r.st>>>(
+  k_layer_norm_grad<T, W, LPR, NV, V, threads><<<static_cast<unsigned>(grad_blocks(r.rows, r.d)), threads, 0, r.st>>>(
       static_cast<const T*>(r.dy), r.dys, static_cast<const T*>(r.x), r.xs, r.rows, static_cast<int>(r.d),
       static_cast<const W*>(r.w), r.mean, r.rstd, static_cast<T*>(r.dx), r.partial);
 }
 
-template <typename T, typename W, bool BWD>
+// VECTOR: 8 elements a load.  Else one, for other widths or alignments: 100000 x 37 11 us, where a block a row took
+// 80, 16384 x 1001 19 and 47, the training of 100000 x 37 25 and 216.
+template <typename T, typename W, bool BWD, bool VECTOR>
 void launch_shape(const Rows& r) {
-#define LNG_NORM_SHAPE(limit, LPR, NV) \
-  if (r.d <= limit) {                  \
-    if constexpr (BWD)                 \
-      launch_bwd<T, W, LPR, NV>(r);    \
-    else                               \
-      launch_fwd<T, W, LPR, NV>(r);    \
-    return;                            \
+#define LNG_NORM_SHAPE(limit, LPR, NV, V) \
+  if (r.d <= limit) {                     \
+    if constexpr (BWD)                    \
+      launch_bwd<T, W, LPR, NV, V>(r);    \
+    else                                  \
+      launch_fwd<T, W, LPR, NV, V>(r);    \
+    return;                               \
   }
-  LNG_NORM_SHAPE(32, 4, 1)
-  LNG_NORM_SHAPE(128, 16, 1)
-  LNG_NORM_SHAPE(256, 32, 1)
-  LNG_NORM_SHAPE(512, 64, 1)
-  LNG_NORM_SHAPE(1024, 64, 2)
-  LNG_NORM_SHAPE(2048, 64, 4)
-  LNG_NORM_SHAPE(4096, 256, 2)
-  LNG_NORM_SHAPE(8192, 256, 4)
+  if constexpr (VECTOR) {
+    LNG_NORM_SHAPE(32, 4, 1, VEC)
+    LNG_NORM_SHAPE(128, 16, 1, VEC)
+    LNG_NORM_SHAPE(256, 32, 1, VEC)
+    LNG_NORM_SHAPE(512, 64, 1, VEC)
+    LNG_NORM_SHAPE(1024, 64, 2, VEC)
+    LNG_NORM_SHAPE(2048, 64, 4, VEC)
+    LNG_NORM_SHAPE(4096, 256, 2, VEC)
+    LNG_NORM_SHAPE(8192, 256, 4, VEC)
+  } else {
+    LNG_NORM_SHAPE(16, 16, 1, 1)
+    LNG_NORM_SHAPE(64, 16, 4, 1)
+    LNG_NORM_SHAPE(256, 64, 4, 1)
+    LNG_NORM_SHAPE(512, 64, 8, 1)
+    LNG_NORM_SHAPE(1024, 64, 16, 1)
+    LNG_NORM_SHAPE(2048, 256, 8, 1)
+    LNG_NORM_SHAPE(4096, 256, 16, 1)
+    LNG_NORM_SHAPE(8192, 256, 32, 1)
+  }
 #undef LNG_NORM_SHAPE
 }
 
 template <typename T, typename W>
 int run_fwd(const Rows& r) {
-  const bool vec = r.d <= MAX_VEC_D && vector_rows(r.x, r.xs, r.d, sizeof(T)) && aligned16(r.y) && aligned16(r.w) &&
+  const bool vec = vector_rows(r.x, r.xs, r.d, sizeof(T)) && aligned16(r.y) && aligned16(r.w) &&
                    aligned16(r.b);
-  if (vec)
-    launch_shape<T, W, false>(r);
+  if (r.d <= MAX_ROW_D && vec)
+    launch_shape<T, W, false, true>(r);
+  else if (r.d <= MAX_ROW_D)
+    launch_shape<T, W, false, false>(r);
   else
     k_layer_norm_any<T, W><<<static_cast<unsigned>(std::min<int64_t>(r.rows, 8192)), 256, 0, r.st>>>(
         static_cast<const T*>(r.x), r.rows, r.d, r.xs, static_cast<const W*>(r.w), static_cast<const W*>(r.b), r.eps,
@@ -387,11 +415,13 @@ int run_fwd(const Rows& r) {
 
 template <typename T, typename W>
 int run_bwd(const Rows& r) {
-  const bool vec = r.d <= MAX_VEC_D && vector_rows(r.x, r.xs, r.d, sizeof(T)) &&
+  const bool vec = vector_rows(r.x, r.xs, r.d, sizeof(T)) &&
                    vector_rows(r.dy, r.dys, r.d, sizeof(T)) && aligned16(r.dx) && aligned16(r.w);
   int64_t P = grad_blocks(r.rows, r.d);
-  if (vec) {
-    launch_shape<T, W, true>(r);
+  if (r.d <= MAX_ROW_D && vec) {
+    launch_shape<T, W, true, true>(r);
+  } else if (r.d <= MAX_ROW_D) {
+    launch_shape<T, W, true, false>(r);
   } else {
     const T *dy = static_cast<const T*>(r.dy), *x = static_cast<const T*>(r.x);
     if (r.dx) {

@@ -61,6 +61,13 @@ def test_shapes_and_types(dev, rows, d, dtype, wt):
     _check(*_make(dev, rows, d, dtype, wt, seed=rows + d))
 
 
+@pytest.mark.parametrize("d", [1, 2, 15, 17, 63, 65, 255, 257, 511, 513, 1023, 1025, 2047, 2050, 4095, 4097, 8191])
+@pytest.mark.parametrize("rows,dtype,wt", [(37, BF, FP), (70, FP, FP), (1, HF, HF)])
+def test_odd_widths(dev, d, rows, dtype, wt):
+    """Each side of the widths at which a row is held by more threads, one element a load."""
+    _check(*_make(dev, rows, d, dtype, wt, seed=rows + d))
+
+
 def test_weight_or_bias_alone(dev):
     x, w, b, dy = _make(dev, 40, 256, BF, FP)
     _check(x, w, None, dy)
