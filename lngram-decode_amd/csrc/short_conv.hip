@@ -474,26 +474,42 @@ void grad_tile(const ConvArgs& a, const GradGrid& g, hipStream_t st) {
     launch_grad<T, W, VEC, KT, 4>(a, g, st);
 }
 
+template <typename T, typename W, int V, int KT>
+void conv_tile(const ConvArgs& a, hipStream_t st) {
+  if (tile_rows(a, V) == 16)
+    launch_conv<T, W, V, KT, 16>(a, st);
+  else
+    launch_conv<T, W, V, KT, 4>(a, st);
+}
+
+// Two to four taps as compile-time counts, for single channels too (4 x 2048 x 1001 with 4 taps 14 us and its
+// training 45; 22 and 85 with eight taps of which the call's own are run).
+template <typename T, typename W, int V>
+void conv_taps(const ConvArgs& a, hipStream_t st) {
+  switch (a.K) {
+    case 2: conv_tile<T, W, V, 2>(a, st); break;
+    case 3: conv_tile<T, W, V, 3>(a, st); break;
+    case 4: conv_tile<T, W, V, 4>(a, st); break;
+    default: launch_conv<T, W, V, 0, 4>(a, st);
+  }
+}
+template <typename T, typename W, int V>
+void grad_taps(const ConvArgs& a, const GradGrid& g, hipStream_t st) {
+  switch (a.K) {
+    case 2: grad_tile<T, W, V, 2>(a, g, st); break;
+    case 3: grad_tile<T, W, V, 3>(a, g, st); break;
+    case 4: grad_tile<T, W, V, 4>(a, g, st); break;
+    default: grad_tile<T, W, V, 0>(a, g, st);
+  }
+}
+
 template <typename T, typename W>
 int run_conv(const ConvArgs& a, hipStream_t st) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
-  if (vector_ok(a, V, sizeof(T))) {
-    const bool wide = tile_rows(a, V) == 16;
-#define LNG_CONV_TAPS(k, KT)                                       \
-  if (k) {                                                         \
-    if (wide)                                                      \
-      launch_conv<T, W, V, KT, 16>(a, st);                         \
-    else                                                           \
-      launch_conv<T, W, V, KT, 4>(a, st);                          \
-  } else
-    LNG_CONV_TAPS(a.K == 2, 2)
-    LNG_CONV_TAPS(a.K == 3, 3)
-    LNG_CONV_TAPS(a.K == 4, 4)
-    launch_conv<T, W, V, 0, 4>(a, st);
-#undef LNG_CONV_TAPS
-  } else {
-    launch_conv<T, W, 1, 0, 4>(a, st);
-  }
+  if (vector_ok(a, V, sizeof(T)))
+    conv_taps<T, W, V>(a, st);
+  else
+    conv_taps<T, W, 1>(a, st);
   return check_launch("short_conv");
 }
 
@@ -502,16 +518,10 @@ int run_grad(ConvArgs a, void* dw, void* db, hipStream_t st) {
   const bool vec = vector_ok(a, 4, sizeof(T));
   const GradGrid g(a.B, a.T, a.C, a.K, a.dil, vec ? 4 : 1);
   a.tiles = g.tiles;
-  if (!vec) {
-    grad_tile<T, W, 1, 0>(a, g, st);
-  } else {
-    switch (a.K) {
-      case 2: grad_tile<T, W, 4, 2>(a, g, st); break;
-      case 3: grad_tile<T, W, 4, 3>(a, g, st); break;
-      case 4: grad_tile<T, W, 4, 4>(a, g, st); break;
-      default: grad_tile<T, W, 4, 0>(a, g, st);
-    }
-  }
+  if (vec)
+    grad_taps<T, W, 4>(a, g, st);
+  else
+    grad_taps<T, W, 1>(a, g, st);
   if (int rc = check_launch("short_conv_grad")) return rc;
   if (!a.partial) return LNG_OK;
   k_conv_partials<W><<<static_cast<unsigned>(cdiv(int64_t{a.K + 1} * a.C, 16)), 256, 0, st>>>(

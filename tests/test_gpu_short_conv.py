@@ -168,6 +168,13 @@ def test_step(dev, b, c, k, dil, dtype, wt):
     assert torch.equal(y, want[:, 0]) and torch.equal(h, nxt)
 
 
+@pytest.mark.parametrize("k,dil", [(2, 1), (3, 2), (4, 3), (5, 1)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_wide_tiles_of_odd_channels(dev, k, dil, dtype):
+    """Enough positions for the longest tiles, channel by channel, with a history and ragged ends."""
+    _check(_make(dev, 3, 1500, 501, k, dil, dtype, ragged=True), True)
+
+
 def test_step_in_place_is_seen_by_a_graph_that_kept_the_history(dev):
     s = _make(dev, 2, 4, 16, 4, 1, FP)
     w = s["w"].detach().requires_grad_(True)
