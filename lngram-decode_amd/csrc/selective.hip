@@ -25,7 +25,7 @@
 // (from zero) and total step sizes, then their start states from one short pass over the chunks, then every
 // chunk from its start.  The backward pass does the same for q, backwards, and takes the states of
 // every GSEG tokens' start from the forward pass (N / GSEG floats a (token, channel)).  Short prompts of up to
-// 32 states are not cut: k_sel_rows gives every state a lane instead (rows_serve says when).
+// 64 states are not cut: k_sel_rows gives every state a lane instead (rows_serve says when).
 #include <type_traits>
 
 #include "common.h"
@@ -496,16 +496,17 @@ __device__ __forceinline__ void unrolled(F f) {
 }
 
 // Prompts in one pass, without a cut in time: a wave holds four channels, a row of 16 lanes each, and lane j of
-// a row holds state j (and j + 16) of its channel.  What a (token, channel) needs once (step size, input, gate,
+// a row holds states j, j + 16, .. (K of them) of its channel.  What a (token, channel) needs once (step size, input, gate,
 // output) is read, made and written by lane 4 * token + channel, so that a load's neighbours are neighbours in
 // memory (token-major lanes took 1.37 us a segment instead of 1.15 with two waves a SIMD: 64 lines a load);
 // step sizes and inputs reach the rows through LDS, and a segment's 16 outputs are summed over a row's states in
 // 45 operations.  The next segment's tile and the inputs after it are asked for before this segment is run.
-// A wave needs 0.6 us a segment whatever its neighbours do, so few and short sequences are what it is for
-// (rows_serve): 1 x 64 x 2048 13 us against 45 by chunks, 16 x 128 x 1024 29 against 51.
-template <typename T, int K>
-struct RowSeg {
-  f32x4 B[K][4], C[K][4];
+// A wave needs 0.65 us a segment whatever its neighbours do (1.1 for two states a lane, 1.4 for four), so few and
+// short sequences are what it is for (rows_serve).
+struct RowTile {  // B and C of a lane's state over a segment
+  f32x4 B[4], C[4];
+};
+struct RowOwn {  // u, dt and z of a lane's (token, channel), as stored
   unsigned u, dt, z;
 };
 template <typename T, int K, bool CKPT>
@@ -547,23 +548,23 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
   const f32x4* const row_lds = &lds[wave][j < d.N ? r : 4][0];
   if (lane < 9) lds[wave][4][lane] = f32x4{};
   const int last = end > 0 ? (end - 1) / SEG * SEG : 0;
-  auto read_own = [&](int t, RowSeg<T, K>& s) {
+  auto read_own = [&](int t, RowOwn& s) {
     t = t < last ? t : last;
     const int n = live<SEG>(t, end);
     s.u = Rows<T>(static_cast<const T*>(p.u) + b * p.ub + t * p.ut, p.ut, n, d.C).load(ou, 0);
     s.dt = Rows<T>(static_cast<const T*>(p.dt) + b * p.dtb + t * p.dtt, p.dtt, n, d.C).load(od, 0);
     s.z = Rows<T>(zp + t * zt, zt, n, d.C).load(oz, 0);
   };
-  auto read_tile = [&](int t, RowSeg<T, K>& s) {
+  auto read_tile = [&](int t, int k, RowTile& s) {
     t = t < last ? t : last;
-    const f32x4* const q =
-        reinterpret_cast<const f32x4*>(p.tiles + (bg * d.segs + static_cast<unsigned>(t) / SEG) * K * 32 * SEG);
+    const f32x4* const q = reinterpret_cast<const f32x4*>(
+        p.tiles + ((bg * d.segs + static_cast<unsigned>(t) / SEG) * K + k) * 32 * SEG);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s.B[k][i] = q[k * 128 + i * 16 + j], s.C[k][i] = q[k * 128 + 64 + i * 16 + j];
+    for (int i = 0; i < 4; ++i) s.B[i] = q[i * 16 + j], s.C[i] = q[64 + i * 16 + j];
   };
-  auto run = [&](int t, RowSeg<T, K>& in, RowSeg<T, K>& next) {
+  // `even`: the tile of the lane's first state, which is there or on its way; each further state's, and at last the
+  // next segment's first, is asked for while the one before it is run, into the other of the two
+  auto run = [&](int t, RowOwn& in, RowTile& even, RowTile& odd) {
     unsigned ub = in.u, db = in.dt, zb = in.z;
     asm volatile("" : "+v"(ub), "+v"(db), "+v"(zb));  // converted here, not where they are asked for
     const bool own = t + lt < end;
@@ -576,15 +577,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
     own_lds[0] = s;
     own_lds[16] = xs;
     wave_order();
-    read_tile(t + SEG, next);
-    read_own(t + 2 * SEG, in);
     f32x4 ss[4], xx[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ss[i] = row_lds[i], xx[i] = row_lds[4 + i];
-    __builtin_amdgcn_sched_barrier(0);
     float v[SEG];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
+      const RowTile& in_k = k % 2 ? odd : even;
+      RowTile& next = k % 2 ? even : odd;
+      if (k + 1 < K)
+        read_tile(t, k + 1, next);
+      else
+        read_tile(t + SEG, 0, next);
+      if (k == 0) {
+        read_own(t + 2 * SEG, in);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss[i] = row_lds[i], xx[i] = row_lds[4 + i];
+      }
+      __builtin_amdgcn_sched_barrier(0);
       unrolled<0, SEG>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         if constexpr (CKPT && i % GSEG == 0) {
@@ -593,11 +601,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
           const int n = j + 16 * k;
           ck.store(ok && n < d.N && t + i < end ? (n * d.C + c) * 4 : static_cast<int>(0x80000000u), 0, h[k]);
         }
-        h[k] = fmaf(__builtin_amdgcn_exp2f(ss[i / 4][i % 4] * a[k]), h[k], xx[i / 4][i % 4] * in.B[k][i / 4][i % 4]);
+        h[k] = fmaf(__builtin_amdgcn_exp2f(ss[i / 4][i % 4] * a[k]), h[k], xx[i / 4][i % 4] * in_k.B[i / 4][i % 4]);
         if (k)
-          v[i] = j + 16 < d.N ? fmaf(in.C[k][i / 4][i % 4], h[k], v[i]) : v[i];
+          v[i] = j + 16 * k < d.N ? fmaf(in_k.C[i / 4][i % 4], h[k], v[i]) : v[i];
         else
-          v[i] = in.C[k][i / 4][i % 4] * h[k];
+          v[i] = in_k.C[i / 4][i % 4] * h[k];
       });
     }
     const float sum = __builtin_bit_cast(
@@ -609,18 +617,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
   };
   int t = 0;
   if (end > 0) {
-    RowSeg<T, K> s0, s1;
-    read_own(0, s0);
+    RowOwn o0, o1;
+    RowTile t0, t1;
+    read_own(0, o0);
     __builtin_amdgcn_sched_barrier(0);
-    read_tile(0, s0);
+    read_tile(0, 0, t0);
     __builtin_amdgcn_sched_barrier(0);
-    read_own(SEG, s1);
+    read_own(SEG, o1);
     __builtin_amdgcn_sched_barrier(0);
     for (;;) {
-      run(t, s0, s1);
+      run(t, o0, t0, t1);
       t += SEG;
       if (t > last) break;
-      run(t, s1, s0);
+      if constexpr (K == 1)
+        run(t, o1, t1, t0);
+      else
+        run(t, o1, t0, t1);
       t += SEG;
       if (t > last) break;
     }
@@ -973,18 +985,21 @@ int waves_for(const Dims& d, bool grad) {
   return std::min(by_n, d.cbg);
 }
 
+int rows_states(const Dims& d) { return d.N <= 16 ? 16 : d.N <= 32 ? 32 : 64; }  // of a padded tile
+
 // Whether a state a lane serves a forward call: its time grows with a sequence's segments alone until every SIMD
-// has its waves, the chunks' with all tokens behind 30 us of their own.  Measured at 16 states, rows against
-// chunks: 1 x 64 x 2048 13 us and 45, 16 x 128 x 1024 29 and 51, 1 x 512 x 512 28 and 40, 3 x 777 x 1000 44 and 55,
-// 4 x 1024 x 2048 81 and 100, 2 x 1024 x 1024 50 and 50; 1 x 1024 x 512 50 and 46, 8 x 4096 x 256 170 and 102.
-// Far more waves pay each wave's beginning: 64 x 16 x 2048 42 and 26.  Up to 8 states half of a row has nothing to
-// do (4 states: 1 x 256 x 512 21 and 30, 4 x 256 x 1024 23 and 30, 8 x 128 x 2048 28 and 28, 4 x 512 x 1024 34 and
-// 31); above 32 the tiles no longer fit in registers.
-int rows_states(const Dims& d) { return static_cast<int>(cdiv(d.N, 16)) * 16; }  // its tiles' states
+// has its waves, the chunks' with all tokens behind 30 us of their own, and with more than 32 states they have few
+// waves.  Measured, rows against chunks, us:
+//   16 states: 1 x 64 x 2048 13 and 45, 16 x 128 x 1024 29 and 51, 1 x 512 x 512 28 and 40, 3 x 777 x 1000 44 and 55,
+//     4 x 1024 x 2048 81 and 100, 2 x 1024 x 1024 50 and 50; 1 x 1024 x 512 50 and 46, 8 x 4096 x 256 170 and 102
+//   32 states: 1 x 512 x 1024 37 and 67, 8 x 1024 x 1024 110 and 164
+//   64 states: 1 x 64 x 2048 16 and 109, 1 x 512 x 512 52 and 110, 4 x 1024 x 1024 104 and 277
+//   4 states (half of a row has nothing to do): 1 x 256 x 512 21 and 30, 8 x 128 x 2048 28 and 28, 4 x 512 x 1024 34 and 31
+// Far more waves pay each wave's beginning: 64 x 16 x 2048 with 16 states 42 and 26.
 bool rows_serve(const Dims& d) {
   const int64_t lanes = d.B * d.C;
   if (d.N <= 8) return lanes <= 16384 && d.T <= 256;
-  return d.N <= 32 && lanes <= 65536 && (d.T <= 512 || (d.T <= 1024 && lanes >= 2048));
+  return d.N <= 64 && lanes <= 65536 && (d.T <= 512 || (d.T <= 1024 && (lanes >= 2048 || d.N > 32)));
 }
 
 Dims make_dims(const lng_selective& a, bool grad) {
@@ -1085,10 +1100,12 @@ int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
     const unsigned blocks = static_cast<unsigned>(cdiv(cg, 4 * waves) * d.G * d.B);
     auto launch = [&](auto ck) {
       constexpr bool CK = decltype(ck)::value;
-      if (d.N <= 16)
+      if (d.np == 16)
         k_sel_rows<T, 1, CK><<<blocks, 64 * waves, 0, st>>>(d, p);
-      else
+      else if (d.np == 32)
         k_sel_rows<T, 2, CK><<<blocks, 64 * waves, 0, st>>>(d, p);
+      else
+        k_sel_rows<T, 4, CK><<<blocks, 64 * waves, 0, st>>>(d, p);
     };
     if (p.ckpt)
       launch(std::true_type{});

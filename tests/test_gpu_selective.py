@@ -95,14 +95,15 @@ def test_several_chunks(dev, b, t, c, dtype):
 @pytest.mark.parametrize("b,t,c,n,g", [(1, 600, 70, 16, 1), (2, 1030, 24, 20, 2), (1, 513, 64, 12, 1),
                                        (2, 512, 40, 9, 1), (3, 100, 33, 17, 3), (2, 48, 60, 32, 1), (1, 37, 1, 33, 1),
                                        (3, 530, 700, 16, 1), (2, 15, 6, 24, 2), (1, 300, 130, 5, 1), (2, 257, 9, 1, 1),
-                                       (2, 256, 20, 8, 4)])
+                                       (2, 256, 20, 8, 4), (2, 1000, 30, 50, 1), (1, 1025, 20, 64, 1),
+                                       (3, 90, 33, 33, 3), (1, 1024, 8, 48, 2), (2, 33, 70, 64, 1), (1, 50, 12, 65, 1)])
 @pytest.mark.parametrize("dtype", [FP, BF])
 def test_states_over_lanes_and_over_time(dev, b, t, c, n, g, dtype):
     """Both ways to run a prompt, on each side of their rule in lengths, channels and states."""
     _check(_make(dev, b, t, c, n, g, dtype, ragged=b > 1))
 
 
-@pytest.mark.parametrize("n", [5, 9, 12, 16, 20, 32, 40])
+@pytest.mark.parametrize("n", [5, 9, 12, 16, 20, 32, 40, 60, 70])
 @pytest.mark.parametrize("t", [20, 600])
 def test_infinite_input_stays_infinite(dev, n, t):
     """Positive B and C: what follows an infinite input is infinite in its channel and finite in the others, and
