@@ -1372,10 +1372,14 @@ def _last_contiguous(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _near_rows(x: torch.Tensor) -> torch.Tensor:
-    """``[B, T, C]`` with contiguous channels and rows at most 2^26 bytes apart (the scan's row offsets)."""
-    x = _last_contiguous(x)
-    return x if x.dim() < 3 or x.stride(1) * x.element_size() <= 1 << 26 else x.contiguous()
+def _near_rows(x: torch.Tensor) -> tuple:
+    """``[B, T, C]`` (or ``[B, C]``) with contiguous channels and rows at most 2^26 bytes apart (the scan's row
+    offsets), and its strides."""
+    at = x.stride()
+    if (at[-1] != 1 and x.shape[-1] != 1) or (len(at) == 3 and at[1] * x.element_size() > 1 << 26):
+        x = x.contiguous()
+        at = x.stride()
+    return x, at
 
 
 def _whole(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -1568,42 +1572,44 @@ def _selective_args(what: str, u, dt, A, B, C, D, z, dt_bias, dt_softplus: bool,
                     checkpoints=None, checkpoints_in=None):
     """``(lng_selective, tensors to keep alive)`` of a selective scan's checked arguments; dims 3: ``[B, T, C]``
     tensors, 2: ``[B, C]`` (one token)."""
-    lead, c = u.shape[:-1], u.shape[-1]
-    if any(t is not None and t.dtype != u.dtype for t in (dt, B, C, z)) or u.dtype not in _FLOATS:
+    shape, kind = u.shape, u.dtype
+    b, c = shape[0], shape[-1]
+    t = shape[1] if dims == 3 else 1
+    if dt.dtype != kind or B.dtype != kind or C.dtype != kind or (z is not None and z.dtype != kind) or kind not in _FLOATS:
         raise TypeError(f"{what}: u, dt, B, C and z in one type, fp32, bf16 or fp16")
-    if dt.shape != u.shape or (z is not None and z.shape != u.shape):
-        raise ValueError(f"{what}: dt and z {tuple(u.shape)} as u, got {tuple(dt.shape)}"
+    if dt.shape != shape or (z is not None and z.shape != shape):
+        raise ValueError(f"{what}: dt and z {tuple(shape)} as u, got {tuple(dt.shape)}"
                          f"{'' if z is None else f' and {tuple(z.shape)}'}")
     if A.dim() != 2 or A.shape[0] != c or not 1 <= A.shape[1] <= 256:
         raise ValueError(f"{what}: A is [C, N] with C = {c} and 1 to 256 states, got {tuple(A.shape)}")
     n = A.shape[1]
-    if B.dim() == dims:
-        B = B.unsqueeze(-2)
-    if C.dim() == dims:
-        C = C.unsqueeze(-2)
-    if B.dim() != dims + 1 or B.shape[-2] == 0 or c % B.shape[-2]:
+    # B and C [.., N] are one group's
+    g = 1 if B.dim() == dims else B.shape[-2] if B.dim() == dims + 1 else 0
+    if g == 0 or c % g:
         raise ValueError(f"{what}: B and C are [.., N] or [.., G, N] with G a divisor of {c}")
-    g = B.shape[-2]
-    _expect(what, "B", B, *lead, g, n)
-    _expect(what, "C", C, *lead, g, n)
+    one, many = (*shape[:-1], n), (*shape[:-1], g, n)
+    for name, v in (("B", B), ("C", C)):
+        if v.shape != many and (g > 1 or v.shape != one):
+            raise ValueError(f"{what}: {name} {tuple(v.shape)}, expected {many if v.dim() > dims else one}")
     _expect(what, "D", D, c)
     _expect(what, "dt_bias", dt_bias, c)
-    _expect(what, "state", state, lead[0], c, n)
-    for t in (A, D, dt_bias, state):
-        if t is not None and t.dtype != torch.float32:
+    _expect(what, "state", state, b, c, n)
+    for v in (A, D, dt_bias, state):
+        if v is not None and v.dtype != torch.float32:
             raise TypeError(f"{what}: A, D, dt_bias and states are float32")
-    ln = _lengths32(what, lengths, lead[0], lead[-1])
-    u, dt, B, C = _near_rows(u), _near_rows(dt), _last_contiguous(B), _last_contiguous(C)
-    z = None if z is None else _near_rows(z)
+    ln = _lengths32(what, lengths, b, t)
+    (u, us), (dt, ds), B, C = _near_rows(u), _near_rows(dt), _last_contiguous(B), _last_contiguous(C)
+    z, zs = (None, (0, 0)) if z is None else _near_rows(z)
     A, D, dt_bias, state = _whole(A), _whole(D), _whole(dt_bias), _whole(state)
-    us, ds, zs, bs, cs = u.stride(), dt.stride(), (0, 0) if z is None else z.stride(), B.stride(), C.stride()
-    if dims == 2:
-        us, ds, zs, bs, cs = (us[0], 0), (ds[0], 0), (zs[0], 0), (bs[0], 0, bs[1]), (cs[0], 0, cs[1])
-    at = [0 if t is None else t.data_ptr()
-          for t in (u, dt, z, B, C, A, D, dt_bias, state, ln, y, state_out, checkpoints, checkpoints_in)]
+    bs, cs = B.stride(), C.stride()
+    ut, dtt, zt = (us[1], ds[1], zs[1]) if dims == 3 else (0, 0, 0)
+    bt, ct = (bs[1], cs[1]) if dims == 3 else (0, 0)
+    bg, cg = bs[-2] if B.dim() > dims else 0, cs[-2] if C.dim() > dims else 0
+    at = [0 if v is None else v.data_ptr()
+          for v in (u, dt, z, B, C, A, D, dt_bias, state, ln, y, state_out, checkpoints, checkpoints_in)]
     a = _lib.Selective.from_buffer_copy(_SELECTIVE.pack(
-        lead[0], lead[1] if dims == 3 else 1, c, n, g, _DT[u.dtype], int(bool(dt_softplus)), 0, *at[:5], *us[:2], *ds[:2],
-        *zs[:2], *bs[:3], *cs[:3], *at[5:]))
+        b, t, c, n, g, _DT[kind], 1 if dt_softplus else 0, 0, *at[:5], us[0], ut, ds[0], dtt, zs[0], zt, bs[0], bt, bg, cs[0],
+        ct, cg, *at[5:]))
     return a, (u, dt, z, B, C, A, D, dt_bias, state, ln)
 
 
@@ -1678,8 +1684,8 @@ def selective_scan_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoin
         for k, v in out.items():
             v.zero_() if k != "state" or dstate is None else v.copy_(dstate)
         return out
-    dyc, dsc = _near_rows(dy), _whole(dstate)
-    g = _lib.SelectiveGrad(dyc.data_ptr(), dyc.stride(0), dyc.stride(1), _ptr(dsc), _ptr(out["u"]), _ptr(out["dt"]),
+    (dyc, dys), dsc = _near_rows(dy), _whole(dstate)
+    g = _lib.SelectiveGrad(dyc.data_ptr(), dys[0], dys[1], _ptr(dsc), _ptr(out["u"]), _ptr(out["dt"]),
                            _ptr(out.get("z")), _ptr(out["B"]), _ptr(out["C"]), _ptr(out["A"]), _ptr(out.get("D")),
                            _ptr(out.get("dt_bias")), _ptr(out.get("state")))
     ws = _selective_workspace(a, True, dev)
