@@ -598,8 +598,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
         if constexpr (CKPT && i % GSEG == 0) {
           const int seg = (t + i) / GSEG;
           const Rows<float> ck(p.ckpt + (b * d.gsegs + (seg < d.gsegs ? seg : 0)) * d.N * d.C, d.C, d.N, d.C);
-          const int n = j + 16 * k;
-          ck.store(ok && n < d.N && t + i < end ? (n * d.C + c) * 4 : static_cast<int>(0x80000000u), 0, h[k]);
+          const int n = lt + 16 * k;  // four channels in neighbouring lanes, as the other rows are written
+          const int kept = __builtin_amdgcn_ds_bpermute((lr * 16 + lt) * 4, __builtin_bit_cast(int, h[k]));
+          ck.store(lok && n < d.N && t + i < end ? (n * d.C + lc) * 4 : static_cast<int>(0x80000000u), 0,
+                   __builtin_bit_cast(float, kept));
         }
         h[k] = fmaf(__builtin_amdgcn_exp2f(ss[i / 4][i % 4] * a[k]), h[k], xx[i / 4][i % 4] * in_k.B[i / 4][i % 4]);
         if (k)
