@@ -12,13 +12,16 @@
 //
 // Bound by the vector ALU: an exponential and some five multiply-adds for every (token, channel, state), on
 // 8 bytes a (token, channel).  An exponential and four of the others take a SIMD 25 cycles a wave, so one pass
-// over 8 x 4096 x 256 x 16 states is 21 us of all SIMDs' time and its bytes are 14 us; it takes 52, and 37 more
-// for the chunks' ends, whose waves (two a SIMD) do not cover each other's waits.  A training step of
-// 8 x 2048 x 1024 x 16: forward 105 and 67, backward 245 and 77 us, 505 with all.  A lane holds one channel, so u, dt, z and y move as whole rows, and what all
-// of a wave's channels share (B and C of a token) comes through the scalar unit: k_sel_tiles lays B and C
-// out as fp32 tiles of SEG tokens per state, and a tile's row of 2 * SEG values is one scalar load for
-// 64 * SEG state updates.  A segment of SEG tokens stays in registers (step sizes, inputs, outputs) while
-// the loop runs over the states, whose values rest in LDS in between, so every N runs in the same registers.
+// over 8 x 4096 x 256 x 16 states is 21 us of all SIMDs' time (30 with softplus, gate and conversions) and its
+// bytes are 14 us; it takes 52, and 37 more for the chunks' ends.  States kept in registers instead of LDS, or
+// tiles read from LDS instead of through the scalar unit, take the same times.  A training step of
+// 8 x 2048 x 1024 x 16: forward 105 and 67, backward 245 and 77 us, 505 with all.
+//
+// A lane holds one channel, so u, dt, z and y move as whole rows, and what all of a wave's channels share (B
+// and C of a token) comes through the scalar unit: k_sel_tiles lays B and C out as fp32 tiles of SEG tokens
+// per state, and a tile's row of 2 * SEG values is one scalar load for 64 * SEG state updates.  A segment of
+// SEG tokens stays in registers (step sizes, inputs, outputs) while the loop runs over the states, whose
+// values rest in LDS in between, so every N runs in the same registers.
 // All sums and states are fp32.
 //
 // Where batch * channels gives too few waves, the time axis is cut into chunks: the chunks' own end states
