@@ -196,7 +196,8 @@ class DepthwiseCausalConv(nn.Module):
 
     Parameters ``norm.weight`` and ``conv.weight [d, 1, K]`` as in the reference.  With RMSNorm and no bias
     the forward is one kernel (``lng_causal_conv``); with LayerNorm or a bias the norm and the conv
-    (``lng_short_conv``, up to 8 taps) are a kernel each, and with LayerNorm the pair is differentiable."""
+    (``lng_short_conv``, up to 8 taps) are a kernel each.  With LayerNorm the pair is differentiable; RMSNorm's
+    kernels have no backward pass, and its forms leave no part of a graph."""
 
     def __init__(self, hidden_size: int, kernel_size: int, dilation: int, eps: float, normalization: str = "RMSNorm",
                  bias: bool = False, zero_init: bool = True, device=None, dtype=None):
@@ -226,9 +227,15 @@ class DepthwiseCausalConv(nn.Module):
         at a position that the device holds, and a tree's windows."""
         return self.conv.bias is None and not isinstance(self.norm, LayerNorm)
 
+    @property
+    def differentiable(self) -> bool:
+        return isinstance(self.norm, LayerNorm)
+
     def _two_kernels(self, values: Tensor, **kw):
-        return short_conv(self.norm(values), rows_type(self.conv.weight, values), rows_type(self.conv.bias, values),
-                          dilation=self.dilation, **kw)
+        # behind a norm without a backward pass the conv's node would give some gradients and drop the others
+        with torch.set_grad_enabled(torch.is_grad_enabled() and self.differentiable):
+            return short_conv(self.norm(values), rows_type(self.conv.weight, values), rows_type(self.conv.bias, values),
+                              dilation=self.dilation, **kw)
 
     def forward(self, values: Tensor, segment_ids: Optional[Tensor] = None) -> Tensor:
         self._check(values, segment_ids)
@@ -272,7 +279,7 @@ class DepthwiseCausalConv(nn.Module):
         """``values + forward(values)`` (the ``_finish`` residual), in the conv's one kernel where it has one."""
         self._check(values, None)
         if not self.one_kernel:
-            return values + self.forward(values)
+            return (values if self.differentiable else values.detach()) + self.forward(values)
         return ops.causal_conv(values, self.norm.weight, self.conv.weight, self.dilation, self.norm.eps,
                                residual=True)
 
