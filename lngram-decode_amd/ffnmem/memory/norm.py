@@ -14,6 +14,8 @@ from torch.autograd.function import once_differentiable
 
 from lngram_hip import ops
 
+from .grad_mode import needs_grad
+
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
@@ -32,9 +34,9 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of x (fp32, bf16 or fp16,
-    any strides); weight and bias ``[d]`` in x's type or fp32, or None.  Differentiable once."""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    any strides); weight and bias ``[d]`` in x's type or fp32, or None.  Differentiable once,
+    in reverse mode."""
+    if needs_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return ops.layer_norm(x, weight, bias, float(eps))
 

@@ -23,8 +23,9 @@ from torch.autograd.function import once_differentiable
 
 from lngram_hip import ops
 
+from .grad_mode import needs_grad
 from .norm import LayerNorm
-from .short_conv import _needs_grad, short_conv, short_conv_step
+from .short_conv import short_conv, short_conv_step
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -65,9 +66,9 @@ def selective_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Op
     fp32 or converted to it; 1 to 256 states.  ``lengths [B]``: the sequences' own tokens in a padded batch;
     positions behind them are not read and give zeros.  Returns y ``[B, T, C]`` in u's type, with
     ``return_state`` also the state after each sequence's last own token (fp32).  States and sums are fp32.
-    Differentiable once, in everything but the lengths."""
+    Differentiable once, in reverse mode, in everything but the lengths."""
     A, D, dt_bias, state = _f32(A), _f32(D), _f32(dt_bias), _f32(state)
-    if _needs_grad(u, dt, A, B, C, D, z, dt_bias, state):
+    if needs_grad(u, dt, A, B, C, D, z, dt_bias, state):
         y, end = _SelectiveScan.apply(u, dt, A, B, C, D, z, dt_bias, state, lengths, bool(dt_softplus),
                                       bool(return_state))
     else:
@@ -82,7 +83,7 @@ def selective_step(state: Tensor, u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C
     ``[B, G, N]``; returns y ``[B, C]``.  ``state [B, C, N]`` (fp32, contiguous) moves on in place; with
     ``out_state`` the new one is written there and ``state`` stays (a step that may have to be taken back).
     No gradient: call it under ``torch.no_grad()``."""
-    if _needs_grad(state, u, dt, A, B, C, D, z, dt_bias):
+    if needs_grad(state, u, dt, A, B, C, D, z, dt_bias):
         raise RuntimeError("selective_step has no backward pass; call it under torch.no_grad()")
     return ops.selective_step(state, u, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias), dt_softplus, out_state)
 
@@ -148,7 +149,7 @@ class SelectiveSSM(nn.Module):
         weight, odd = w.weight, -x.shape[-1] % 8
         if odd and x.dtype == torch.bfloat16:            # the bf16 product reads 16 bytes at a time
             x, weight = nn.functional.pad(x, (0, odd)), nn.functional.pad(weight, (0, odd))
-        if _needs_grad(x, weight):
+        if needs_grad(x, weight):
             return _Linear.apply(x, weight)
         return ops.linear(x, weight)
 

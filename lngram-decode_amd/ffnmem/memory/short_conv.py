@@ -15,6 +15,8 @@ from torch.autograd.function import once_differentiable
 
 from lngram_hip import ops
 
+from .grad_mode import needs_grad
+
 ACTIVATIONS = ("silu", None)
 
 
@@ -38,14 +40,6 @@ class _ShortConv(torch.autograd.Function):
         return dx, dw, db, dh, None, None, None
 
 
-def _needs_grad(*tensors: Optional[Tensor]) -> bool:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
 def _weight(weight: Tensor) -> Tensor:
     """``[C, K]`` from that or from ``nn.Conv1d``'s ``[C, 1, K]``."""
     return weight.squeeze(1) if weight.dim() == 3 and weight.shape[1] == 1 else weight
@@ -67,9 +61,9 @@ def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, dilatio
     ``history [B, (K - 1) * dilation, C]`` holds the rows before the first position (None: zeros).
     ``lengths [B]`` are the sequences' own tokens in a padded batch: positions behind them are not read,
     and give zeros.  ``return_history``: also the history of the tokens that follow each sequence's last own
-    one.  Differentiable once, in x, weight, bias and history."""
+    one.  Differentiable once, in reverse mode, in x, weight, bias and history."""
     w, silu = _weight(weight), _is_silu(activation)
-    if _needs_grad(x, w, bias, history):
+    if needs_grad(x, w, bias, history):
         y, nxt = _ShortConv.apply(x, w, bias, history, lengths, int(dilation), silu)
         return (y, nxt) if return_history else y
     return ops.short_conv(x, w, bias, dilation, silu, history, lengths, return_history)
@@ -80,6 +74,6 @@ def short_conv_step(x: Tensor, history: Tensor, weight: Tensor, bias: Optional[T
     """:func:`short_conv` of one new token x ``[B, C]`` of every sequence.  ``history`` moves on by one row in
     place; with ``out_history`` the new one is written there and ``history`` stays (a step that may have to
     be taken back).  No gradient: call it under ``torch.no_grad()``."""
-    if _needs_grad(x, history, weight, bias):
+    if needs_grad(x, history, weight, bias):
         raise RuntimeError("short_conv_step has no backward pass; call it under torch.no_grad()")
     return ops.short_conv_step(x, history, _weight(weight), bias, dilation, _is_silu(activation), out_history)

@@ -46,3 +46,39 @@ def test_rmsnorm_conv_with_a_bias_keeps_no_part_of_a_graph(stand_ins):
         assert not any(t.requires_grad for t in conv.forward_incremental(x, history))
     with torch.no_grad():
         assert torch.equal(conv(x), whole) and torch.equal(conv.forward_residual(x), residual)
+
+
+def _dual(*shape):
+    return torch.autograd.forward_ad.make_dual(torch.randn(*shape), torch.randn(*shape))
+
+
+def test_forward_mode_tangents_are_refused():
+    """The operators have no forward-mode derivative.  A tangent asks for no reverse-mode graph, so it would be
+    dropped on the way to the kernel, under no_grad too."""
+    from ffnmem.memory.norm import LayerNorm, layer_norm
+    from ffnmem.memory.selective import SelectiveSSM, selective_scan, selective_step
+    from ffnmem.memory.short_conv import short_conv, short_conv_step
+
+    def r(*s):
+        return torch.randn(*s)
+
+    scan = dict(u=(1, 3, 4), dt=(1, 3, 4), A=(4, 2), B=(1, 3, 2), C=(1, 3, 2), D=(4,), z=(1, 3, 4), dt_bias=(4,),
+                state=(1, 4, 2))
+    step = dict(state=(1, 4, 2), u=(1, 4), dt=(1, 4), A=(4, 2), B=(1, 2), C=(1, 2), D=(4,), z=(1, 4), dt_bias=(4,))
+    conv = dict(x=(1, 3, 4), weight=(4, 2), bias=(4,), history=(1, 1, 4))
+    one = dict(x=(1, 4), history=(1, 1, 4), weight=(4, 2), bias=(4,))
+    norm = dict(x=(3, 4), weight=(4,), bias=(4,))
+    with torch.autograd.forward_ad.dual_level():
+        for fn, shapes in ((layer_norm, norm), (short_conv, conv), (short_conv_step, one), (selective_scan, scan),
+                           (selective_step, step)):
+            for name in shapes:
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        fn(**{k: _dual(*s) if k == name else r(*s) for k, s in shapes.items()})
+        for fn in (LayerNorm(4), DepthwiseCausalConv(4, 2, 1, 1e-5, normalization="LayerNorm"), SelectiveSSM(4, 4)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(_dual(1, 3, 4))
+        with pytest.raises(RuntimeError, match="no CPU path"):   # inside a level, without a tangent: as ever
+            layer_norm(r(3, 4), r(4))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(layer_norm, (r(3, 4),), (r(3, 4),))
