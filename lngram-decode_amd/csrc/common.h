@@ -17,6 +17,9 @@ int fail(int code, const std::string& msg);
 // Check the launch status of the kernel just enqueued.
 int check_launch(const char* what);
 
+// The threads of a launch, blocks times threads a block, are counted in 32 bits.
+constexpr int64_t MOST_THREADS = (int64_t{1} << 32) - 1;
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 // ------------------------------------------------------------------ types

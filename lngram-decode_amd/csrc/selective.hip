@@ -1064,10 +1064,6 @@ int check_args(const char* what, const lng_selective* a) {
       a->C > (1 << 20) || a->T > (int64_t{1} << 30) || a->B > (int64_t{1} << 24) ||
       a->B * a->T > (int64_t{1} << 38) / a->C / a->N)
     return fail(LNG_E_ARG, std::string(what) + ": bad shape (1 to 256 states, groups that divide the channels)");
-  const int64_t lanes = cdiv(a->C / a->G, 64) * 64 * a->G, most = int64_t{1} << 38;  // of any launch's threads
-  if (a->B * a->G * (a->T + SEG) > most / 2 / a->N || a->B * lanes * (a->T / (2 * SEG) + 1) > most ||
-      a->B * a->C > most / SEG || a->B * lanes > most / a->N)
-    return fail(LNG_E_ARG, std::string(what) + ": too many tokens, groups or channels for one call");
   // a segment's rows are reached by 32-bit offsets from its first one
   const int64_t far = (int64_t{1} << 26) / dtype_size(a->dtype);
   for (const int64_t token : {a->u_token, a->dt_token, a->z_token})
@@ -1085,8 +1081,25 @@ void place(Ptrs& p, const Space& s, void* ws) {
 }
 
 unsigned grid256(int64_t n) { return static_cast<unsigned>(cdiv(n, 256)); }
-unsigned unit_blocks(const Dims& d, int waves) {
-  return static_cast<unsigned>(cdiv(d.cbg, waves) * d.G * d.chunks * d.B);
+int64_t unit_blocks(const Dims& d, int waves) { return cdiv(d.cbg, waves) * d.G * d.chunks * d.B; }
+int64_t tile_threads(const Dims& d) { return d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N; }
+int step_lanes(const Dims& d) {  // of a channel
+  int lpc = 1;
+  while (lpc < 16 && lpc * 4 < d.N) lpc *= 2;
+  return lpc;
+}
+
+// The launches whose threads grow with the batch.  The others stay below: k_sel_rows serves 2^16 channels of all
+// sequences (rows_serve), k_sel_join runs where these give fewer than 4096 waves, k_sel_grad_a has 4 (N + 2) C threads.
+int check_threads(const char* what, int64_t threads) {
+  if (cdiv(threads, 256) * 256 <= MOST_THREADS) return LNG_OK;
+  return fail(LNG_E_ARG, std::string(what) + ": too many tokens, groups or channels for one launch; split the batch");
+}
+int check_launches(const char* what, const Dims& d, bool grad) {
+  const int waves = waves_for(d, grad);
+  int64_t most = std::max(tile_threads(d), unit_blocks(d, waves) * 64 * waves);
+  if (grad) most = std::max(most, d.B * d.G * d.T * 2 * d.N);
+  return check_threads(what, most);
 }
 
 unsigned states_lds(const Dims& d, int waves) { return waves * 2 * d.N * 64 * 4; }
@@ -1100,7 +1113,7 @@ void launch_join(const Dims& d, const Ptrs& p, hipStream_t st) {
 template <typename T>
 int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
   if (d.rows) {
-    k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+    k_sel_tiles<T><<<grid256(tile_threads(d)), 256, 0, st>>>(d, p);
     const int cg = d.C / d.G, waves = static_cast<int>(std::min<int64_t>(WAVES, cdiv(cg, 4)));
     const unsigned blocks = static_cast<unsigned>(cdiv(cg, 4 * waves) * d.G * d.B);
     auto launch = [&](auto ck) {
@@ -1119,8 +1132,8 @@ int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
     return check_launch("selective_scan");
   }
   const int waves = waves_for(d, false);
-  const unsigned blocks = unit_blocks(d, waves);
-  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+  const unsigned blocks = static_cast<unsigned>(unit_blocks(d, waves));
+  k_sel_tiles<T><<<grid256(tile_threads(d)), 256, 0, st>>>(d, p);
   if (d.chunks > 1) {
     k_sel_scan<T, true><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
     launch_join<false>(d, p, st);
@@ -1132,8 +1145,8 @@ int run_scan(const Dims& d, Ptrs p, hipStream_t st) {
 template <typename T>
 int run_grad(const Dims& d, Ptrs p, const lng_selective_grad& g, hipStream_t st) {
   const int waves = waves_for(d, true);
-  const unsigned blocks = unit_blocks(d, waves);
-  k_sel_tiles<T><<<grid256(d.B * d.G * d.segs * SEG * d.np + int64_t{d.C} * d.N), 256, 0, st>>>(d, p);
+  const unsigned blocks = static_cast<unsigned>(unit_blocks(d, waves));
+  k_sel_tiles<T><<<grid256(tile_threads(d)), 256, 0, st>>>(d, p);
   if (d.chunks > 1) {
     k_sel_grad_ends<T><<<blocks, 64 * waves, states_lds(d, waves), st>>>(d, p);
     launch_join<true>(d, p, st);
@@ -1150,8 +1163,7 @@ template <typename T>
 int run_step(const Dims& d, const Ptrs& p, hipStream_t st) {
   const bool vec = d.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.start) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(p.end) % 16 == 0 && reinterpret_cast<uintptr_t>(p.A) % 16 == 0;
-  int lpc = 1;
-  while (lpc < 16 && lpc * 4 < d.N) lpc *= 2;
+  const int lpc = step_lanes(d);
   const unsigned blocks = grid256(d.B * d.C * lpc);
 #define LNG_SEL_STEP(L)                                       \
   if (lpc == L) {                                             \
@@ -1204,6 +1216,7 @@ int lng_selective_scan(const lng_selective* args, void* workspace, size_t worksp
   if (a.B == 0 || a.T == 0) return LNG_OK;
   if (!a.y) return fail(LNG_E_ARG, "selective_scan: null pointer");
   const Dims d = make_dims(a, false);
+  if (int rc = check_launches("selective_scan", d, false)) return rc;
   const Space s(d, false);
   if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)
     return fail(LNG_E_ARG, "selective_scan: the workspace is too small or not 64-byte aligned");
@@ -1224,6 +1237,7 @@ int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad*
   if (g.dy_token < 0 || g.dy_token > (int64_t{1} << 26) / dtype_size(a.dtype))
     return fail(LNG_E_ARG, "selective_scan_grad: rows of dy are 0 to 2^26 bytes apart");
   const Dims d = make_dims(a, true);
+  if (int rc = check_launches("selective_scan_grad", d, true)) return rc;
   const Space s(d, true);
   if (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 || reinterpret_cast<uintptr_t>(workspace) % 64)
     return fail(LNG_E_ARG, "selective_scan_grad: the workspace is too small or not 64-byte aligned");
@@ -1241,6 +1255,7 @@ int lng_selective_step(const lng_selective* args, void* stream) {
   if (a.B == 0) return LNG_OK;
   if (!a.state || !a.state_out || !a.y) return fail(LNG_E_ARG, "selective_step: null pointer");
   const Dims d = make_dims(a, false);
+  if (int rc = check_threads("selective_step", d.B * d.C * step_lanes(d))) return rc;
   const Ptrs p = make_ptrs(a);
   return with_type(a.dtype, [&](auto t) { return run_step<decltype(t)>(d, p, as_stream(stream)); });
 }

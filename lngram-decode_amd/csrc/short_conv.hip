@@ -438,13 +438,19 @@ int tile_rows(const ConvArgs& a, int vec) {
   return a.B * a.T / 16 * cdiv(a.C, vec) >= 1024 * 2 * 64 ? 16 : 4;
 }
 
+int too_many(const char* what) {
+  return fail(LNG_E_ARG, std::string(what) + ": too many rows and channels for one launch; split the batch");
+}
+
 template <typename T, typename W, int VEC, int KT, int TT>
-void launch_conv(ConvArgs a, hipStream_t st) {
+int launch_conv(ConvArgs a, hipStream_t st) {
   a.tiles = cdiv(cdiv(a.T, a.dil), TT);
   a.classes = static_cast<int>(std::min<int64_t>(a.dil, a.T));
   const int64_t rows = a.B * (a.tiles * a.classes + (a.hist_out ? (a.K - 1) * a.dil : 0));
-  const int64_t threads = rows * (a.C / VEC);  // below 2^39: outputs and history rows that fit the memory
+  const int64_t threads = rows * (a.C / VEC);
+  if (cdiv(threads, 256) * 256 > MOST_THREADS) return too_many("short_conv");
   if (threads) k_short_conv<T, W, VEC, KT, TT><<<static_cast<unsigned>(cdiv(threads, 256)), 256, 0, st>>>(a);
+  return check_launch("short_conv");
 }
 
 struct GradGrid {
@@ -475,22 +481,19 @@ void grad_tile(const ConvArgs& a, const GradGrid& g, hipStream_t st) {
 }
 
 template <typename T, typename W, int V, int KT>
-void conv_tile(const ConvArgs& a, hipStream_t st) {
-  if (tile_rows(a, V) == 16)
-    launch_conv<T, W, V, KT, 16>(a, st);
-  else
-    launch_conv<T, W, V, KT, 4>(a, st);
+int conv_tile(const ConvArgs& a, hipStream_t st) {
+  return tile_rows(a, V) == 16 ? launch_conv<T, W, V, KT, 16>(a, st) : launch_conv<T, W, V, KT, 4>(a, st);
 }
 
 // Two to four taps as compile-time counts, for single channels too (4 x 2048 x 1001 with 4 taps 14 us and its
 // training 45; 22 and 85 with eight taps of which the call's own are run).
 template <typename T, typename W, int V>
-void conv_taps(const ConvArgs& a, hipStream_t st) {
+int conv_taps(const ConvArgs& a, hipStream_t st) {
   switch (a.K) {
-    case 2: conv_tile<T, W, V, 2>(a, st); break;
-    case 3: conv_tile<T, W, V, 3>(a, st); break;
-    case 4: conv_tile<T, W, V, 4>(a, st); break;
-    default: launch_conv<T, W, V, 0, 4>(a, st);
+    case 2: return conv_tile<T, W, V, 2>(a, st);
+    case 3: return conv_tile<T, W, V, 3>(a, st);
+    case 4: return conv_tile<T, W, V, 4>(a, st);
+    default: return launch_conv<T, W, V, 0, 4>(a, st);
   }
 }
 template <typename T, typename W, int V>
@@ -506,11 +509,7 @@ void grad_taps(const ConvArgs& a, const GradGrid& g, hipStream_t st) {
 template <typename T, typename W>
 int run_conv(const ConvArgs& a, hipStream_t st) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
-  if (vector_ok(a, V, sizeof(T)))
-    conv_taps<T, W, V>(a, st);
-  else
-    conv_taps<T, W, 1>(a, st);
-  return check_launch("short_conv");
+  return vector_ok(a, V, sizeof(T)) ? conv_taps<T, W, V>(a, st) : conv_taps<T, W, 1>(a, st);
 }
 
 template <typename T, typename W>
@@ -530,25 +529,24 @@ int run_grad(ConvArgs a, void* dw, void* db, hipStream_t st) {
 }
 
 template <typename T, typename W, int VEC>
-void launch_step(const ConvArgs& a, hipStream_t st) {
-  const unsigned blocks = static_cast<unsigned>(cdiv(a.B * (a.C / VEC), 256));
+int launch_step(const ConvArgs& a, hipStream_t st) {
+  const int64_t n = cdiv(a.B * (a.C / VEC), 256);
+  if (n * 256 > MOST_THREADS) return too_many("short_conv_step");
+  const unsigned blocks = static_cast<unsigned>(n);
   if (a.dil == 1 && a.K == 4)
     k_short_conv_step<T, W, VEC, 4, true><<<blocks, 256, 0, st>>>(a);
   else if (a.dil == 1)
     k_short_conv_step<T, W, VEC, 0, true><<<blocks, 256, 0, st>>>(a);
   else
     k_short_conv_step<T, W, VEC, 0, false><<<blocks, 256, 0, st>>>(a);
+  return check_launch("short_conv_step");
 }
 
 template <typename T, typename W>
 int run_step(const ConvArgs& a, hipStream_t st) {
   // few channels in all: one a thread, so that more waves wait for memory at once
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
-  if (a.B * a.C > 65536 && vector_ok(a, V, sizeof(T)))
-    launch_step<T, W, V>(a, st);
-  else
-    launch_step<T, W, 1>(a, st);
-  return check_launch("short_conv_step");
+  return a.B * a.C > 65536 && vector_ok(a, V, sizeof(T)) ? launch_step<T, W, V>(a, st) : launch_step<T, W, 1>(a, st);
 }
 
 int check_conv(const char* what, int dtype, int w_dtype, int64_t B, int64_t T, int32_t C, int32_t K, int32_t dil,

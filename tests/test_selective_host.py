@@ -108,3 +108,43 @@ def test_modules_on_the_cpu():
         SelectiveSSM(32, 16, conv_kernel=9)
     with pytest.raises(ValueError):
         SelectiveSSM(32, 16, dt_min=0.0)
+
+
+def test_launches_past_2_to_the_32_threads_are_refused():
+    """A launch's blocks times threads are counted in 32 bits: a call that any of its launches would take past them
+    is refused before the first one."""
+    lib = _lib.load()
+    ws = ctypes.c_void_p(4096)
+    grads = _lib.SelectiveGrad(dy=4096, du=4096, ddt=4096, dz=4096, dB=4096, dC=4096)
+
+    def scan(**kw):
+        return lib.lng_selective_scan(ctypes.byref(_args(**kw)), ws, 1 << 50, None)
+
+    def grad(**kw):
+        return lib.lng_selective_scan_grad(ctypes.byref(_args(checkpoints_in=4096, **kw)), ctypes.byref(grads), ws, 1 << 50,
+                                           None)
+
+    def step(**kw):
+        return lib.lng_selective_step(ctypes.byref(_args(T=1, **kw)), None)
+
+    calls = [lambda: scan(B=1 << 12, T=1 << 12, C=1, N=256),             # a value of B and C a thread
+             lambda: scan(B=1 << 12, T=1 << 12, C=16, G=16, N=16),
+             lambda: scan(B=1 << 20, T=1, C=1 << 13, N=1),               # a channel a lane
+             lambda: grad(B=1 << 12, T=1 << 11, C=1, N=256),             # dB and dC: a thread each
+             lambda: grad(B=1 << 20, T=1 << 10, C=64, N=4),
+             lambda: step(B=1 << 20, C=1 << 12, N=16),                   # four lanes a channel
+             lambda: step(B=1 << 20, C=1 << 12, N=1)]
+    for i, call in enumerate(calls):
+        assert call() == -1, i
+        assert b"split the batch" in lib.lng_last_error(), i
+
+    names = "x dtype B T C xb xt w bias wt K dil silu hist lengths y hist_out st".split()
+    ok = [P, BF, 2, 8, 16, 128, 16, P, P, BF, 4, 1, 1, P, None, P, ctypes.c_void_p(8192), None]
+    for kw in (dict(B=1, T=1 << 31, C=31, xb=0, xt=31, K=8),             # a channel a thread, four positions
+               dict(B=1 << 21, T=17, C=1501, xb=17 * 1501, xt=1501, hist_out=None),  # sixteen, in two tiles
+               dict(B=1 << 11, T=0, C=1024, K=8, dil=4096, hist=None),   # the next history alone: a thread a channel
+               dict(B=1 << 12, T=1, C=1023, K=8, dil=2048, xb=1023, xt=1023)):
+        assert lib.lng_short_conv(*[kw.get(n, v) for n, v in zip(names, ok)]) == -1, kw
+        assert b"split the batch" in lib.lng_last_error(), kw
+    assert lib.lng_short_conv_step(P, BF, 1 << 20, (1 << 12) + 1, 8192, P, P, BF, 2, 1, 1, P, P, P, None) == -1
+    assert b"split the batch" in lib.lng_last_error()
