@@ -814,7 +814,8 @@ int lng_short_conv_step(const void* x, int dtype, int64_t B, int32_t C, int64_t 
  * the other strides in elements; y contiguous.  A [C, N], D [C], dt_bias [C], states [B, C, N]: fp32,
  * contiguous.  z, D, dt_bias, state (zeros), state_out, lengths may be null.  lengths [B] int32: a
  * sequence's own tokens; what stands behind them is not read, y is zero there and state_out is the state
- * after the last own one.  1 to 256 states.  States and sums are fp32. */
+ * after the last own one.  1 to 256 states.  States and sums are fp32.  A rate A below -2e38, minus infinity
+ * too, counts as -2e38: nothing is kept of the state before a token with a step above 1e-36. */
 typedef struct lng_selective {
   int64_t B, T;
   int32_t C, N, G, dtype, softplus, reserved;

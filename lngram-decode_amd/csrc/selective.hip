@@ -80,6 +80,14 @@ __device__ __forceinline__ float softplus(float x) {
   p = fmaf(p, q, 1.f);
   return fmaf(2.f * s, p, fmaxf(x, 0.f));
 }
+
+// A decay rate without a bound (minus infinity keeps nothing of a state) as one that is still finite times log2 e:
+// the steps of zero behind a sequence's end would make a NaN of it, while it ends every own token's state as well.
+__device__ __forceinline__ float rate(float a) {
+  constexpr float LEAST = -2e38f;
+  return a < LEAST ? LEAST : a;
+}
+
 // The own tokens of sequence b (the same in every lane that asks for the same b).
 __device__ __forceinline__ int seq_len(const int32_t* lengths, int64_t b, int T) {
   if (!lengths) return T;
@@ -113,7 +121,7 @@ __global__ __launch_bounds__(256) void k_sel_tiles(Dims d, Ptrs p) {
     }
   } else if (i - n_tiles < static_cast<int64_t>(d.C) * d.N) {
     const int64_t j = i - n_tiles, c = j % d.C, n = j / d.C;
-    p.at[j] = p.A[c * d.N + n];
+    p.at[j] = rate(p.A[c * d.N + n]);
   }
 }
 
@@ -532,7 +540,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sel_rows(Dims d, Ptrs p) {
   for (int k = 0; k < K; ++k) {
     const int n = j + 16 * k;
     const bool real = n < d.N;
-    a[k] = real ? p.A[static_cast<int64_t>(c) * d.N + n] * LOG2E : 0.f;
+    a[k] = real ? rate(p.A[static_cast<int64_t>(c) * d.N + n]) * LOG2E : 0.f;
     h[k] = real && p.start ? p.start[(b * d.C + c) * d.N + n] : 0.f;
   }
   // a token's four channels in neighbouring lanes for what a (token, channel) needs once
@@ -955,7 +963,7 @@ __global__ __launch_bounds__(256) void k_sel_step(Dims d, Ptrs p) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (VEC || n0 + k < d.N) {
-        hv[k] = fmaf(__builtin_amdgcn_exp2f(s * (av[k] * LOG2E)), hv[k], x * to_f32(Bm[n0 + k]));
+        hv[k] = fmaf(__builtin_amdgcn_exp2f(s * (rate(av[k]) * LOG2E)), hv[k], x * to_f32(Bm[n0 + k]));
         y = fmaf(to_f32(Cm[n0 + k]), hv[k], y);
       }
     }

@@ -1,5 +1,6 @@
 """Layer norm, short conv and selective scan where the other tests of single calls and modules do not go: prompts
-of more than a hundred chunks, and the gradients of padded products and of the conv behind a LayerNorm."""
+of more than a hundred chunks, decay rates without a bound, and the gradients of padded products and of the conv
+behind a LayerNorm."""
 
 from __future__ import annotations
 
@@ -12,7 +13,7 @@ from ffnmem.memory.selective import SelectiveSSM
 from oracle import memory as om
 from oracle import mixing
 from tests.bounds import within
-from tests.test_gpu_selective import _check, _make
+from tests.test_gpu_selective import LEAVES, _call, _check, _make
 
 pytestmark = pytest.mark.gpu
 
@@ -24,6 +25,29 @@ BF, FP = torch.bfloat16, torch.float32
 @pytest.mark.parametrize("t", [4000, 4500, 8224])
 def test_prompts_of_many_chunks(dev, t):
     _check(_make(dev, 2, t, 8, 4, dtype=FP, ragged=True))
+
+
+@pytest.mark.parametrize("b,t,n", [(1, 17, 16), (2, 30, 20), (2, 30, 70), (3, 600, 5), (2, 600, 16), (1, 20, 40)])
+def test_decay_rates_without_a_bound(dev, b, t, n):
+    """A rate of minus infinity keeps nothing of the state before a token.  No time passes behind a sequence's end,
+    where the product of the rate and a step of zero must not be formed."""
+    s = _make(dev, b, t, 24, n, dtype=FP, ragged=b > 1)
+    s["A"][::2, ::3] = float("-inf")
+    s["A"][1::2, 1::3] = -3e38
+    y, end = _call(s)
+    v = {k: mixing.d(s[k]) for k in LEAVES}
+    kw = dict(softplus=True, lengths=None if s["lengths"] is None else s["lengths"].cpu(), **v)
+    (wy, wend), (my, mend) = mixing.selective_scan(**kw), mixing.selective_scan(mag=True, **kw)
+    within(y, wy, my, 4 * t + 40, "y")
+    within(end, wend, mend, 4 * t + 40, "state")
+    names = [k for k in LEAVES if k not in ("dt", "dt_bias")]        # whose gradient is the rate times zero
+    leaves = {k: s[k].detach().requires_grad_(True) for k in names}
+    got = dict(zip(names, torch.autograd.grad(list(_call(s, leaves)), list(leaves.values()), [s["dy"], s["dend"]])))
+    dy, dend = mixing.d(s["dy"]), mixing.d(s["dend"])
+    want, mag = mixing.selective_grad(dy, dend, **kw), mixing.selective_grad(dy, dend, mag=True, **kw)
+    sums = {"B": 24, "C": 24, "A": b * t, "D": b * t, "u": n, "z": n, "state": 0}
+    for k in names:
+        within(got[k], want[k], mag[k], 8 * t + 80 + sums[k], "d" + k)
 
 
 # ----------------------------------------------------------------------------- the modules
