@@ -163,8 +163,14 @@ class SelectiveSSM(nn.Module):
     def forward(self, emb: Tensor, state: Optional[tuple] = None, lengths: Optional[Tensor] = None,
                 return_state: bool = False):
         """Features ``[B, T, state_dim]`` of the embeddings ``[B, T, d]`` that follow ``state`` (None: the
-        sequence start); with ``return_state`` also the state after each sequence's last own token."""
+        sequence start); with ``return_state`` also the state after each sequence's last own token.  ``lengths
+        [B]``: the sequences' own tokens; what stands behind them has no part in features, state or gradients."""
         hist, scan = (None, None) if state is None else state
+        if lengths is not None and lengths.shape == emb.shape[:1] and torch.is_grad_enabled():
+            # the gradients of the norm and of the products sum over every row, those behind a sequence's end
+            # with a factor of zero: a NaN there would come through
+            behind = torch.arange(emb.shape[1], device=emb.device) >= lengths[:, None]
+            emb = emb.masked_fill(behind[..., None], 0)
         x, z = self._inputs(emb)
         u, hist = short_conv(x, self.conv.weight, self.conv.bias, history=hist, lengths=lengths, return_history=True)
         dt, bm, cm = self._selection(u)

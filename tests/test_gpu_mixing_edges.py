@@ -1,6 +1,6 @@
 """Layer norm, short conv and selective scan where the other tests of single calls and modules do not go: prompts
-of more than a hundred chunks, decay rates without a bound, and the gradients of padded products and of the conv
-behind a LayerNorm."""
+of more than a hundred chunks, decay rates without a bound, NaN in the padding of a training batch, and the
+gradients of padded products and of the conv behind a LayerNorm."""
 
 from __future__ import annotations
 
@@ -51,6 +51,25 @@ def test_decay_rates_without_a_bound(dev, b, t, n):
 
 
 # ----------------------------------------------------------------------------- the modules
+def test_padding_of_a_training_batch_is_not_read(dev):
+    """NaN embeddings behind the sequences' ends leave every gradient as it is."""
+    torch.manual_seed(0)
+    m = SelectiveSSM(32, 24).to(dev)
+    emb = torch.randn(3, 20, 32, device=dev)
+    own = torch.tensor([20, 6, 0], device=dev)
+    dy = torch.randn(3, 20, 24, device=dev)
+    runs = []
+    for fill in (0.5, float("nan")):
+        e = emb.clone()
+        e[1, 6:], e[2] = fill, fill
+        e.requires_grad_(True)
+        y, (hist, scan) = m(e, lengths=own, return_state=True)
+        g = torch.autograd.grad([y, hist, scan], [e, *m.parameters()], [dy, torch.ones_like(hist), torch.ones_like(scan)])
+        runs.append([y, hist, scan, *g])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("d,n", [(72, 24), (100, 30), (96, 32)])
 def test_products_of_odd_widths_and_their_gradients(dev, d, n):
     """The bf16 projections of ``SelectiveSSM``, padded where their rows are no multiple of 8 wide: sums of K, N and M
