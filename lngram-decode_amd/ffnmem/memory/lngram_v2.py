@@ -225,7 +225,10 @@ class DepthwiseCausalConv(nn.Module):
     def one_kernel(self) -> bool:
         """Whether the norm is part of the conv's kernel (RMSNorm, no bias): those forms also read a cache
         at a position that the device holds, and a tree's windows."""
-        return self.conv.bias is None and not isinstance(self.norm, LayerNorm)
+        # every decoded token asks: the module's dictionaries, not its attribute lookup
+        own = self._modules["conv"]._parameters
+        bias = own["bias"] if "bias" in own else self.conv.bias
+        return bias is None and not isinstance(self._modules["norm"], LayerNorm)
 
     @property
     def differentiable(self) -> bool:
@@ -540,8 +543,8 @@ class _RouteNgramMemoryBase(nn.Module):
               and self.bits_per_route == 4 and self.num_routes <= 256
               and self.readout_num_heads == 16 and self.readout_head_dim == 64
               and self.readout_num_kv_heads == 4 and self.readout_kv_proj.weight.dtype == torch.bfloat16
-              and not isinstance(self.readout_query_norm, LayerNorm)
-              and not isinstance(self.readout_memory_norm, LayerNorm)
+              and not isinstance(self._modules["readout_query_norm"], LayerNorm)
+              and not isinstance(self._modules["readout_memory_norm"], LayerNorm)
               and all(t.weight.dtype == torch.bfloat16 for t in self.tables.values()))
         if ok and tables:
             ok = all(t.weight.device.type == "cuda" for t in self.tables.values())
@@ -585,7 +588,8 @@ class _RouteNgramMemoryBase(nn.Module):
             tables = [mods["tables"]._modules[f"ngram_{n}"]._parameters["weight"] for n in self.ngrams]
         except KeyError:                                   # a parametrised weight
             return None
-        if bias is not None or any(isinstance(n, LayerNorm) for n in (*norms, conv._modules["norm"])):
+        if bias is not None or isinstance(norms[0], LayerNorm) or isinstance(norms[1], LayerNorm) or \
+                isinstance(conv._modules["norm"], LayerNorm):
             return None                                    # the norms of these launches are RMSNorms
         if len(tables) > 4 or any(x is None for x in (wq, qn, kv, mn, wo, cn, cw, *tables)):
             return None

@@ -82,3 +82,18 @@ def test_forward_mode_tangents_are_refused():
             layer_norm(r(3, 4), r(4))
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(layer_norm, (r(3, 4),), (r(3, 4),))
+
+
+def test_one_kernel_forms_of_the_conv():
+    """Which norm and bias a conv has is read as they are now: replaced and parametrised ones too."""
+    conv = DepthwiseCausalConv(4, 2, 1, 1e-5)
+    assert conv.one_kernel
+    torch.nn.utils.parametrizations.weight_norm(conv.conv)
+    assert conv.one_kernel
+    conv.conv.bias = torch.nn.Parameter(torch.zeros(4))
+    assert not conv.one_kernel
+    torch.nn.utils.parametrize.register_parametrization(conv.conv, "bias", torch.nn.Identity())
+    assert "bias" not in conv.conv._parameters and not conv.one_kernel
+    conv = DepthwiseCausalConv(4, 2, 1, 1e-5)
+    conv.norm = DepthwiseCausalConv(4, 2, 1, 1e-5, normalization="LayerNorm").norm
+    assert not conv.one_kernel
