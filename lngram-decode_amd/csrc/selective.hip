@@ -13,9 +13,10 @@
 // Bound by the vector ALU: an exponential and some five multiply-adds for every (token, channel, state), on
 // 8 bytes a (token, channel).  An exponential and four of the others take a SIMD 25 cycles a wave, so one pass
 // over 8 x 4096 x 256 x 16 states is 21 us of all SIMDs' time (30 with softplus, gate and conversions) and its
-// bytes are 14 us; it takes 52, and 37 more for the chunks' ends.  States kept in registers instead of LDS, or
-// tiles read from LDS instead of through the scalar unit, take the same times.  A training step of
-// 8 x 2048 x 1024 x 16: forward 105 and 67, backward 245 and 77 us, 505 with all.
+// bytes are 14 us; it takes 53, and 39 more for the chunks' ends (the vector unit busy 57 % of either).  States kept
+// in registers instead of LDS, or tiles read from LDS instead of through the scalar unit, take the same times.  A
+// training step of 8 x 2048 x 1024 x 16: forward 108 and 74, backward 245 (the vector unit busy 81 %) and 77 us, 503
+// with all.
 //
 // A lane holds one channel, so u, dt, z and y move as whole rows, and what all of a wave's channels share (B
 // and C of a token) comes through the scalar unit: k_sel_tiles lays B and C out as fp32 tiles of SEG tokens
@@ -277,7 +278,7 @@ struct Warm {
 
 // Scalar loads come back in any order, so a wait for one is a wait for all: it stands in front of the next
 // row's load, where what it waits for was asked for a whole row's work ago (behind that load, where the
-// compiler would put it, every row waits for memory: 20 us more for the outputs of 8 x 4096 x 256, now 52).
+// compiler would put it, every row waits for memory: 20 us more for the outputs of 8 x 4096 x 256, now 53).
 constexpr int WAITCNT_LGKM0 = 0xC07F;  // s_waitcnt lgkmcnt(0), the other counts left open
 __device__ __forceinline__ void rows_arrived() {
   __builtin_amdgcn_sched_barrier(0);
@@ -1002,13 +1003,14 @@ int rows_states(const Dims& d) { return d.N <= 16 ? 16 : d.N <= 32 ? 32 : 64; } 
 
 // Whether a state a lane serves a forward call: its time grows with a sequence's segments alone until every SIMD
 // has its waves, the chunks' with all tokens behind 30 us of their own, and with more than 32 states they have few
-// waves.  Measured, rows against chunks, us:
-//   16 states: 1 x 64 x 2048 13 and 45, 16 x 128 x 1024 29 and 51, 1 x 512 x 512 28 and 40, 3 x 777 x 1000 44 and 55,
-//     4 x 1024 x 2048 81 and 100, 2 x 1024 x 1024 50 and 50; 1 x 1024 x 512 50 and 46, 8 x 4096 x 256 170 and 102
-//   32 states: 1 x 512 x 1024 37 and 67, 8 x 1024 x 1024 110 and 164
-//   64 states: 1 x 64 x 2048 16 and 109, 1 x 512 x 512 52 and 110, 4 x 1024 x 1024 104 and 277
-//   4 states (half of a row has nothing to do): 1 x 256 x 512 21 and 30, 8 x 128 x 2048 28 and 28, 4 x 512 x 1024 34 and 31
-// Far more waves pay each wave's beginning: 64 x 16 x 2048 with 16 states 42 and 26.
+// waves.  Measured, rows against chunks, us of a call replayed from a graph (bf16, with the tiles):
+//   16 states: 1 x 64 x 2048 9 and 41, 16 x 128 x 1024 27 and 47, 1 x 512 x 512 29 and 41, 3 x 777 x 1000 44 and 59,
+//     4 x 1024 x 2048 80 and 98; 2 x 1024 x 1024 53 and 46, 1 x 1024 x 512 52 and 42, 8 x 4096 x 256 183 and 100
+//   32 states: 1 x 512 x 1024 33 and 65, 8 x 1024 x 1024 106 and 157
+//   64 states: 1 x 64 x 2048 13 and 106, 1 x 512 x 512 49 and 107, 4 x 1024 x 1024 98 and 275
+//   4 states (half of a row has nothing to do): 1 x 256 x 512 18 and 25, 8 x 128 x 2048 25 and 27, 4 x 512 x 1024 31 and 27
+// Far more waves pay each wave's beginning: 64 x 16 x 2048 with 16 states 39 and 22.  2 x 1024 x 1024 is on the rule's
+// slower side.
 bool rows_serve(const Dims& d) {
   const int64_t lanes = d.B * d.C;
   if (d.N <= 8) return lanes <= 16384 && d.T <= 256;

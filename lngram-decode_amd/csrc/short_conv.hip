@@ -18,8 +18,11 @@
 // The backward pass forms pre again from x (K multiply-adds) instead of reading it.  Weight gradients are
 // summed in registers over all of a thread's tiles, over a block's threads in LDS, and over blocks by
 // k_conv_partials in a fixed order.
-// bf16, 4 taps, SiLU: 8 x 4096 x 1024 33 us (134 MB, 4.1 TB/s), 3 x 777 x 1024 6.4; training of 8 x 2048 x 1024
-// 20 us forward, 35 backward (100 MB) and 4 for the partial rows.
+// bf16, 4 taps, SiLU: 8 x 4096 x 1024 33 us (75 MB read, 67 written, 4.4 TB/s), 3 x 777 x 1024 6.4; training of
+// 8 x 2048 x 1024 20 us forward, 35 backward and 4 for the partial rows.  The backward pass moves 77 and 39 MB, 24 us
+// of memory, and keeps the vector unit busy 47 % of its time, 17 us: a thread's 25 rows arrive before it computes, and
+// four waves a SIMD do not hide all of either.  1 and 5 to 8 taps take a row after the other (training of the same
+// size 89 us with 1 tap, 151 with 5, 225 with 8; 56 with 4).
 #include "common.h"
 
 namespace lng {
@@ -369,8 +372,8 @@ __global__ __launch_bounds__(256) void k_conv_partials(const float* __restrict__
 
 // One new token of every sequence: a thread owns VEC channels of a sequence, so the history may move in
 // place (hist_out == hist): each of its rows is read before the thread writes the row in front of it.  NEAR:
-// without dilation the window has at most MAX_TAPS rows, which are all asked for together (512 x 2048: 5 us
-// instead of 12 with one row after the other).
+// without dilation the window has at most MAX_TAPS rows, which are all asked for together (512 x 2048, 4 taps: 5 us
+// instead of 12 with one row after the other).  With dilation 3 its nine rows, one after the other, take 15.
 template <typename T, typename W, int VEC, int KT, bool NEAR>
 __global__ __launch_bounds__(256) void k_short_conv_step(ConvArgs a) {
   constexpr int KM = KT > 0 ? KT : MAX_TAPS;
