@@ -852,6 +852,53 @@ int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad*
  * state. */
 int lng_selective_step(const lng_selective* args, void* stream);
 
+/* ---------------------------------------------------------------- linear attention */
+/* Linear attention with a decay for each head, a state S [K, V] a (sequence, head):
+ *   S[t] = e^{decay[t, h]} S[t-1] + k[t] v[t]^T,   y[t] = scale S[t]^T q[t]
+ * (the recurrence of ffnmem/memory/ssm.py:58-91 with a matrix for a state).  H heads; q [B, T, Hq, K],
+ * k [B, T, Hk, K], v [B, T, Hv, V] in `dtype` (fp32, bf16 or fp16) with 1 to 128 keys and values, innermost dimension
+ * contiguous, the other strides in elements; Hq, Hk and Hv divide H, head h reads q's head h / (H / Hq), and so on.
+ * decay: log decays in fp32, heads contiguous; one a head (token_decay 0, strides 0) or one a token and head.  Below
+ * -300, minus infinity too, they count as -300: nothing is kept of the state before.  state [B, H, K, V] fp32 (null:
+ * zeros), state_out, y [B, T, H, V] contiguous.  lengths [B] int32 or null: a sequence's own tokens; what stands behind
+ * them is not read, y is zero there and state_out is the state after the last own one.  States and sums are fp32. */
+typedef struct lng_linear_attention {
+  int64_t B, T;
+  int32_t H, Hq, Hk, Hv, K, V, dtype, token_decay;
+  float scale;
+  int32_t reserved;
+  const void *q, *k, *v;
+  int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
+  const float* decay;
+  int64_t decay_batch, decay_token;
+  const float* state;
+  const int32_t* lengths;
+  void* y;
+  float* state_out;
+  float* checkpoints; /* lng_linear_attention_checkpoints() floats: written by the forward call where not null, read by
+                       * the backward call */
+} lng_linear_attention;
+/* Gradients: dy [B, T, H, V] (strided) and dstate_out [B, H, K, V] or null in; dq, dk, dv contiguous in the tensors'
+ * type and shapes, ddecay [B, T, H] (token_decay) or [H], dstate [B, H, K, V] (may be null) in fp32 out. */
+typedef struct lng_linear_attention_grad {
+  const void* dy;
+  int64_t dy_batch, dy_token, dy_head;
+  const float* dstate_out;
+  void *dq, *dk, *dv;
+  float *ddecay, *dstate;
+} lng_linear_attention_grad;
+size_t lng_linear_attention_size(void);      /* sizeof(lng_linear_attention) */
+size_t lng_linear_attention_grad_size(void); /* sizeof(lng_linear_attention_grad) */
+size_t lng_linear_attention_workspace_bytes(const lng_linear_attention* args, int grad);
+int64_t lng_linear_attention_checkpoints(int64_t B, int64_t T, int32_t H, int32_t K, int32_t V, int dtype);
+/* Prompts and training.  workspace: lng_linear_attention_workspace_bytes(.., grad 0 / 1), 64-byte aligned, its contents
+ * need not outlive the call.  Equal calls give equal bits. */
+int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace, size_t workspace_bytes, void* stream);
+int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_linear_attention_grad* grads,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+/* One new token of every sequence (T = 1; the token strides and lengths are not read): state_out may be state. */
+int lng_linear_attention_step(const lng_linear_attention* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

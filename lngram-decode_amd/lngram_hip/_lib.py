@@ -96,8 +96,29 @@ class SelectiveGrad(ctypes.Structure):
         (n, ctypes.c_void_p) for n in ("dstate_out", "du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate")]
 
 
+class LinearAttention(ctypes.Structure):
+    """``lng_linear_attention`` (include/lngram_hip.h): shapes, strides and pointers of a linear attention."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("B", "T")] + [
+        (n, ctypes.c_int32) for n in ("H", "Hq", "Hk", "Hv", "K", "V", "dtype", "token_decay")] + [
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] + [(n, ctypes.c_void_p) for n in ("q", "k", "v")] + [
+        (n, ctypes.c_int64) for n in ("q_batch", "q_token", "q_head", "k_batch", "k_token", "k_head", "v_batch",
+                                      "v_token", "v_head")] + [("decay", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("decay_batch", "decay_token")] + [
+        (n, ctypes.c_void_p) for n in ("state", "lengths", "y", "state_out", "checkpoints")]
+
+
+class LinearAttentionGrad(ctypes.Structure):
+    """``lng_linear_attention_grad`` (include/lngram_hip.h): the gradients of a linear attention."""
+
+    _fields_ = [("dy", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("dy_batch", "dy_token", "dy_head")] + [
+        (n, ctypes.c_void_p) for n in ("dstate_out", "dq", "dk", "dv", "ddecay", "dstate")]
+
+
 _PSel = ctypes.POINTER(Selective)
 _PSelG = ctypes.POINTER(SelectiveGrad)
+_PLin = ctypes.POINTER(LinearAttention)
+_PLinG = ctypes.POINTER(LinearAttentionGrad)
 
 # name -> (restype, argtypes); must cover every function declared in the header
 SIGNATURES = {
@@ -182,6 +203,13 @@ SIGNATURES = {
     "lng_selective_scan": (_int, [_PSel, _p, ctypes.c_size_t, _p]),
     "lng_selective_scan_grad": (_int, [_PSel, _PSelG, _p, ctypes.c_size_t, _p]),
     "lng_selective_step": (_int, [_PSel, _p]),
+    "lng_linear_attention_size": (ctypes.c_size_t, []),
+    "lng_linear_attention_grad_size": (ctypes.c_size_t, []),
+    "lng_linear_attention_workspace_bytes": (ctypes.c_size_t, [_PLin, _int]),
+    "lng_linear_attention_checkpoints": (_i64, [_i64, _i64, _i32, _i32, _i32, _int]),
+    "lng_linear_attention_scan": (_int, [_PLin, _p, ctypes.c_size_t, _p]),
+    "lng_linear_attention_scan_grad": (_int, [_PLin, _PLinG, _p, ctypes.c_size_t, _p]),
+    "lng_linear_attention_step": (_int, [_PLin, _p]),
     "lng_host_device_pointer": (_int, [_p, ctypes.POINTER(_p)]),
     "lng_permute_table": (_int, [_p, _p, _int, _i32, _i32, _i32, _i32, _p]),
     "lng_serving_address": (_int, [_p, _int, _i64, _i64, _i32, _i32, _i32, _p, _p]),

@@ -1717,6 +1717,141 @@ def selective_step(state: torch.Tensor, u: torch.Tensor, dt: torch.Tensor, A: to
     return y
 
 
+# lng_linear_attention as one packed value, as lng_selective is.
+_LINEAR = struct.Struct("2q8ifi3P9qP2q5P")
+
+
+def _linear_args(what: str, q, k, v, decay, scale, state, lengths, y, state_out, dims: int, checkpoints=None):
+    """``(lng_linear_attention, tensors to keep alive)`` of a linear attention's checked arguments; dims 4:
+    ``[B, T, heads, width]`` tensors, 3: ``[B, heads, width]`` (one token).  ``y`` is made where it is None."""
+    lead, kind, h, keys, values = q.shape[:-2], q.dtype, decay.shape[-1], q.shape[-1], v.shape[-1]
+    b, t = lead[0], lead[1] if dims == 4 else 1
+    if k.dtype != kind or v.dtype != kind or kind not in _FLOATS:
+        raise TypeError(f"{what}: q, k and v in one type, fp32, bf16 or fp16")
+    if k.dim() != dims or v.dim() != dims or k.shape[:-2] != lead or v.shape[:-2] != lead or k.shape[-1] != keys:
+        raise ValueError(f"{what}: q {tuple(q.shape)} with k {tuple(k.shape)} and v {tuple(v.shape)}")
+    if not 1 <= keys <= 128 or not 1 <= values <= 128:
+        raise ValueError(f"{what}: heads of 1 to 128 keys and values, got {keys} and {values}")
+    token = decay.dim() > 1
+    if decay.dtype != torch.float32 or (token and decay.shape[:-1] != lead):
+        raise ValueError(f"{what}: log decays in float32, [H] or {[*lead, 'H']}, got {decay.dtype} {tuple(decay.shape)}")
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if x.shape[-2] == 0 or h == 0 or h % x.shape[-2]:
+            raise ValueError(f"{what}: the heads of q, k and v divide the {h} of the decays, got {x.shape[-2]} of {name}")
+    _expect(what, "state", state, b, h, keys, values)
+    if state is not None and state.dtype != torch.float32:
+        raise TypeError(f"{what}: states are float32")
+    ln = _lengths32(what, lengths, b, t)
+    q, k, v, decay, state = (_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), _last_contiguous(decay),
+                             _whole(state))
+    qs, ks, vs, ds = q.stride(), k.stride(), v.stride(), decay.stride()
+    at = (lambda s: s[:3]) if dims == 4 else (lambda s: (s[0], 0, s[1]))
+    scale = keys ** -0.5 if scale is None else float(scale)
+    a = _lib.LinearAttention.from_buffer_copy(_LINEAR.pack(
+        b, t, h, q.shape[-2], k.shape[-2], v.shape[-2], keys, values, _DT[kind], int(token), scale, 0, q.data_ptr(),
+        k.data_ptr(), v.data_ptr(), *at(qs), *at(ks), *at(vs), decay.data_ptr(), ds[0] if token else 0,
+        ds[1] if token and dims == 4 else 0, _ptr(state) or 0, _ptr(ln) or 0, _ptr(y) or 0, _ptr(state_out) or 0,
+        _ptr(checkpoints) or 0))
+    return a, (q, k, v, decay, state, ln)
+
+
+def _linear_shapes(what: str, q: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, dims: int) -> None:
+    if q.dim() != dims or v.dim() != dims or decay.dim() not in (1, dims - 1):
+        raise ValueError(f"{what}: q and v are {'[B, T, heads, width]' if dims == 4 else '[B, heads, width]'} and log "
+                         f"decays [H] or one a token and head, got {tuple(q.shape)}, {tuple(v.shape)} and "
+                         f"{tuple(decay.shape)}")
+
+
+def _linear_workspace(a, grad: bool, dev: torch.device) -> torch.Tensor:
+    return torch.empty(lib().lng_linear_attention_workspace_bytes(ctypes.byref(a), int(grad)), dtype=torch.uint8,
+                       device=dev)
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, scale: float | None = None,
+                     state: torch.Tensor | None = None, lengths: torch.Tensor | None = None, want_state: bool = False,
+                     want_checkpoints: bool = False) -> tuple:
+    """``(y, final state or None, checkpoints or None)`` of linear attention (``lng_linear_attention_scan``) of
+    q ``[B, T, Hq, K]``, k ``[B, T, Hk, K]``, v ``[B, T, Hv, V]`` with log decays ``[H]`` or ``[B, T, H]`` in
+    fp32; the checkpoints are what :func:`linear_attention_grad` takes."""
+    what = "linear_attention"
+    dev = _dev(q, k, v, decay, state, lengths)
+    _linear_shapes(what, q, v, decay, 4)
+    b, t, _, keys = q.shape
+    h, values = decay.shape[-1], v.shape[-1]
+    y = torch.empty(b, t, h, values, dtype=q.dtype, device=dev)
+    end = ckpt = None
+    if want_state:
+        end = torch.empty(b, h, keys, values, dtype=torch.float32, device=dev)
+    if want_checkpoints:
+        ckpt = torch.empty(lib().lng_linear_attention_checkpoints(b, t, h, keys, values, dtype_code(q.dtype)),
+                           dtype=torch.float32, device=dev)
+    a, keep = _linear_args(what, q, k, v, decay, scale, state, lengths, y, end, 4, ckpt)
+    if b and t:
+        ws = _linear_workspace(a, False, dev)
+        _call(what, dev, lib().lng_linear_attention_scan, ctypes.byref(a), ws.data_ptr(), ws.numel())
+    elif want_state:                                     # no tokens: the state passes through
+        end.zero_() if state is None else end.copy_(state)
+    del keep
+    return y, end, ckpt
+
+
+def linear_attention_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoints: torch.Tensor, q: torch.Tensor,
+                          k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, scale: float | None,
+                          state: torch.Tensor | None, lengths: torch.Tensor | None) -> tuple:
+    """``(dq, dk, dv, ddecay, dstate or None)`` of :func:`linear_attention` (``lng_linear_attention_scan_grad``),
+    given the gradients of y and of the final state (None: zero)."""
+    what = "linear_attention_grad"
+    dev = _dev(dy, dstate, checkpoints, q, k, v, decay, state, lengths)
+    _linear_shapes(what, q, v, decay, 4)
+    a, keep = _linear_args(what, q, k, v, decay, scale, state, lengths, None, None, 4, checkpoints)
+    _expect(what, "dy", dy, a.B, a.T, a.H, a.V)
+    _expect(what, "dstate", dstate, a.B, a.H, a.K, a.V)
+    if dy.dtype != q.dtype or (dstate is not None and dstate.dtype != torch.float32):
+        raise TypeError(f"{what}: dy in q's type, dstate in float32")
+    _expect(what, "checkpoints", checkpoints, lib().lng_linear_attention_checkpoints(a.B, a.T, a.H, a.K, a.V, a.dtype))
+    if checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous():
+        raise TypeError(f"{what}: checkpoints as linear_attention gave them")
+    dq, dk, dv = (torch.empty(x.shape, dtype=q.dtype, device=dev) for x in (q, k, v))
+    dg = torch.empty(decay.shape, dtype=torch.float32, device=dev)
+    ds = None if state is None else torch.empty(a.B, a.H, a.K, a.V, dtype=torch.float32, device=dev)
+    if not (a.B and a.T):                                # no tokens: the state's gradient passes through
+        for x in (dq, dk, dv, dg):
+            x.zero_()
+        if ds is not None:
+            ds.zero_() if dstate is None else ds.copy_(dstate)
+        return dq, dk, dv, dg, ds
+    dyc, dsc = _last_contiguous(dy), _whole(dstate)
+    at = dyc.stride()
+    g = _lib.LinearAttentionGrad(dyc.data_ptr(), *at[:3], _ptr(dsc), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                 dg.data_ptr(), _ptr(ds))
+    ws = _linear_workspace(a, True, dev)
+    _call(what, dev, lib().lng_linear_attention_scan_grad, ctypes.byref(a), ctypes.byref(g), ws.data_ptr(), ws.numel())
+    del keep
+    return dq, dk, dv, dg, ds
+
+
+def linear_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+                          scale: float | None = None, out_state: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`linear_attention` of one new token of every sequence (``lng_linear_attention_step``): q ``[B, Hq, K]``,
+    k ``[B, Hk, K]``, v ``[B, Hv, V]``, log decays ``[H]`` or ``[B, H]``.  The state moves on in place, or into
+    ``out_state``."""
+    what = "linear_attention_step"
+    out = state if out_state is None else out_state
+    dev = _dev(state, q, k, v, decay, out)
+    _linear_shapes(what, q, v, decay, 3)
+    if not state.is_contiguous() or not out.is_contiguous() or out.dtype != torch.float32:
+        raise ValueError(f"{what}: states are contiguous float32 [B, H, K, V]")
+    if out is not state:
+        _expect(what, "out_state", out, *state.shape)
+        _separate(what, "out_state", out, state)
+    y = torch.empty(q.shape[0], decay.shape[-1], v.shape[-1], dtype=q.dtype, device=dev)
+    a, keep = _linear_args(what, q, k, v, decay, scale, state, None, y, out, 3)
+    _call(what, dev, lib().lng_linear_attention_step, ctypes.byref(a))
+    torch.autograd.graph.increment_version(out)
+    del keep
+    return y
+
+
 def tree_accept(parent: torch.Tensor, node_tokens: torch.Tensor, argmax: torch.Tensor, out=None):
     """Device tree acceptance -> ``(path int32 [n], path_len int32 [1], new_tokens int64 [n])``
     (valid entries: the first ``path_len``).  ``out`` = (path, path_len, new_tokens) writes into
