@@ -852,7 +852,7 @@ int lng_selective_scan_grad(const lng_selective* args, const lng_selective_grad*
  * state. */
 int lng_selective_step(const lng_selective* args, void* stream);
 
-/* ---------------------------------------------------------------- linear attention */
+/* ---------------------------------------------------------------- linear attention, group norm */
 /* Linear attention with a decay for each head, a state S [K, V] a (sequence, head):
  *   S[t] = e^{decay[t, h]} S[t-1] + k[t] v[t]^T,   y[t] = scale S[t]^T q[t]
  * (the recurrence of ffnmem/memory/ssm.py:58-91 with a matrix for a state).  H heads; q [B, T, Hq, K],
@@ -898,6 +898,22 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
                                    void* workspace, size_t workspace_bytes, void* stream);
 /* One new token of every sequence (T = 1; the token strides and lengths are not read): state_out may be state. */
 int lng_linear_attention_step(const lng_linear_attention* args, void* stream);
+
+/* Group norm with an activation, channels last: x [N, L, C] (samples x_sample, positions x_row elements apart, channels
+ * contiguous; fp32, bf16 or fp16), G groups of C / G neighbouring channels, statistics over a group's L C / G values of a
+ * sample: z = (x - mean) / sqrt(var + eps) * w + b, y = z or silu(z) (silu 1).  w, b [C] in the rows' type or fp32, each
+ * may be null (1 and 0).  y [N, L, C] contiguous; mean, rstd [N, G] fp32, or both null.  Statistics in fp32, one rounding.
+ * workspace: lng_group_norm_workspace_bytes(.., grad 0 / 1), 64-byte aligned (none needed where that is 0). */
+size_t lng_group_norm_workspace_bytes(int64_t N, int64_t L, int32_t C, int32_t G, int grad);
+int lng_group_norm(const void* x, int dtype, int64_t N, int64_t L, int32_t C, int32_t G, int64_t x_sample, int64_t x_row,
+                   const void* w, const void* b, int w_dtype, float eps, int silu, void* workspace, size_t workspace_bytes,
+                   void* y, float* mean, float* rstd, void* stream);
+/* Its backward pass from x and the statistics of the forward call: dx [N, L, C] contiguous, dw and db [C] in w_dtype, each
+ * may be null (not wanted).  Sums run in a fixed order, so equal calls give equal bits. */
+int lng_group_norm_grad(const void* dy, int64_t dy_sample, int64_t dy_row, const void* x, int64_t x_sample, int64_t x_row,
+                        int dtype, int64_t N, int64_t L, int32_t C, int32_t G, const void* w, const void* b, int w_dtype,
+                        int silu, const float* mean, const float* rstd, void* workspace, size_t workspace_bytes, void* dx,
+                        void* dw, void* db, void* stream);
 
 #ifdef __cplusplus
 }

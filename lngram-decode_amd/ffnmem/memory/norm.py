@@ -1,5 +1,6 @@
 """Layer norm with its backward pass (``nn.LayerNorm``, the LayerNorm choice of the reference's
-``build_lngram_norm``, ``ffnmem/memory/lngram_v2.py:56-71``).
+``build_lngram_norm``, ``ffnmem/memory/lngram_v2.py:56-71``), and group norm of channels-last rows with an
+activation behind it.
 
 Statistics, sums and the weights' gradients are fp32; every output is rounded once.
 """
@@ -41,6 +42,36 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     return ops.layer_norm(x, weight, bias, float(eps))
 
 
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float, silu: bool) -> Tensor:
+        y, mean, rstd = ops.group_norm(x, groups, weight, bias, eps, silu, want_stats=True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.cfg = (groups, silu)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: Tensor):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        groups, silu = ctx.cfg
+        return (*ops.group_norm_grad(dy, x, groups, weight, bias, silu, mean, rstd, ctx.needs_input_grad[:3]), None, None,
+                None)
+
+
+def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
+               activation: Optional[str] = None) -> Tensor:
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)`` of channels-last x ``[N, .., C]`` (fp32, bf16 or fp16):
+    mean and variance of each of ``groups`` groups of neighbouring channels over all positions of a sample.  Tokens
+    that are normed on their own are samples of one position, ``x [N, C]``.  weight and bias ``[C]`` in x's type or
+    fp32, or None; ``activation`` None or "silu".  Differentiable once, in reverse mode."""
+    if activation not in (None, "silu"):
+        raise ValueError(f"group norm activation must be None or 'silu', got {activation!r}")
+    if needs_grad(x, weight, bias):
+        return _GroupNorm.apply(x, weight, bias, int(groups), float(eps), activation == "silu")
+    return ops.group_norm(x, int(groups), weight, bias, float(eps), activation == "silu")
+
+
 def rows_type(parameter: Optional[Tensor], rows: Tensor) -> Optional[Tensor]:
     """A parameter as the kernels take it beside ``rows``: as it is in the rows' type or fp32, else cast to the
     rows' type (as ``RMSNorm`` casts its weight)."""
@@ -64,3 +95,24 @@ class LayerNorm(nn.Module):
             raise ValueError(f"LayerNorm expects last dim {self.hidden_size}, got {hidden_states.shape[-1]}")
         return layer_norm(hidden_states, rows_type(self.weight, hidden_states), rows_type(self.bias, hidden_states),
                           self.eps)
+
+
+class GroupNorm(nn.Module):
+    """Group norm of channels-last rows, ``nn.GroupNorm(groups, channels, eps)``'s parameters ``weight`` (ones) and
+    ``bias`` (zeros), with an activation behind it."""
+
+    def __init__(self, groups: int, channels: int, eps: float = 1e-5, activation: Optional[str] = None, device=None,
+                 dtype=None):
+        super().__init__()
+        if groups < 1 or channels % groups:
+            raise ValueError(f"groups that divide the {channels} channels, got {groups}")
+        if activation not in (None, "silu"):
+            raise ValueError(f"group norm activation must be None or 'silu', got {activation!r}")
+        self.groups, self.channels, self.eps, self.activation = int(groups), int(channels), float(eps), activation
+        self.weight = nn.Parameter(torch.ones(channels, device=device, dtype=dtype))
+        self.bias = nn.Parameter(torch.zeros(channels, device=device, dtype=dtype))
+
+    def forward(self, x: Tensor) -> Tensor:
+        if x.shape[-1] != self.channels:
+            raise ValueError(f"GroupNorm expects last dim {self.channels}, got {x.shape[-1]}")
+        return group_norm(x, self.groups, rows_type(self.weight, x), rows_type(self.bias, x), self.eps, self.activation)

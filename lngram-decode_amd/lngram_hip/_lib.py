@@ -203,6 +203,11 @@ SIGNATURES = {
     "lng_selective_scan": (_int, [_PSel, _p, ctypes.c_size_t, _p]),
     "lng_selective_scan_grad": (_int, [_PSel, _PSelG, _p, ctypes.c_size_t, _p]),
     "lng_selective_step": (_int, [_PSel, _p]),
+    "lng_group_norm_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i32, _int]),
+    "lng_group_norm": (_int, [_p, _int, _i64, _i64, _i32, _i32, _i64, _i64, _p, _p, _int, _f, _int, _p, ctypes.c_size_t,
+                              _p, _p, _p, _p]),
+    "lng_group_norm_grad": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i32, _i32, _p, _p, _int, _int, _p,
+                                   _p, _p, ctypes.c_size_t, _p, _p, _p, _p]),
     "lng_linear_attention_size": (ctypes.c_size_t, []),
     "lng_linear_attention_grad_size": (ctypes.c_size_t, []),
     "lng_linear_attention_workspace_bytes": (ctypes.c_size_t, [_PLin, _int]),

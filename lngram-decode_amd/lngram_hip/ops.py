@@ -1466,6 +1466,78 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, m
     return dx, dw, db
 
 
+def _as_samples(what: str, x: torch.Tensor, groups: int) -> tuple:
+    """``([N, L, C] view with contiguous channels, N, L, C)`` of channels-last ``x [N, .., C]``."""
+    if x.dim() < 2 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: x is [N, .., C], got {tuple(x.shape)}")
+    n, c = x.shape[0], x.shape[-1]
+    if groups < 1 or c % groups:
+        raise ValueError(f"{what}: groups that divide the {c} channels, got {groups}")
+    at = math.prod(x.shape[1:-1])
+    rows = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.reshape(n, at, c)
+    return _last_contiguous(rows), n, at, c
+
+
+def group_norm(x: torch.Tensor, groups: int, w: torch.Tensor | None, b: torch.Tensor | None, eps: float, silu: bool = False,
+               want_stats: bool = False):
+    """Group norm of channels-last x ``[N, .., C]`` over all positions of a sample, with SiLU behind it where ``silu``
+    (``lng_group_norm``); w, b ``[C]`` in x's type or fp32, or None.  ``want_stats``: returns ``(y, mean, rstd)`` for
+    :func:`group_norm_grad`, fp32 ``[N, groups]``."""
+    dev = _dev(x, w, b)
+    wt = None if w is None else w.dtype
+    bt = None if b is None else b.dtype
+    _float_rows("group_norm", x, wt, bt)
+    rows, n, at, c = _as_samples("group_norm", x, groups)
+    _expect("group_norm", "weight", w, c)
+    _expect("group_norm", "bias", b, c)
+    wc, bc = _whole(w), _whole(b)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean = rstd = ws = None
+    if want_stats:
+        mean, rstd = (torch.empty(n, groups, dtype=torch.float32, device=dev) for _ in range(2))
+    size = lib().lng_group_norm_workspace_bytes(n, at, c, groups, 0)
+    if size:
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _call("group_norm", dev, lib().lng_group_norm, rows.data_ptr(), _DT[x.dtype], n, at, c, groups, rows.stride(0),
+          rows.stride(1), _ptr(wc), _ptr(bc), _DT[wt or bt or x.dtype], eps, int(silu), _ptr(ws), size, y.data_ptr(),
+          _ptr(mean), _ptr(rstd))
+    return (y, mean, rstd) if want_stats else y
+
+
+def group_norm_grad(dy: torch.Tensor, x: torch.Tensor, groups: int, w: torch.Tensor | None, b: torch.Tensor | None,
+                    silu: bool, mean: torch.Tensor, rstd: torch.Tensor, want=(True, True, True),
+                    w_dtype: torch.dtype | None = None) -> tuple:
+    """``(dx, dw, db)`` of :func:`group_norm` (``lng_group_norm_grad``), None where not wanted; dw and db in
+    ``w_dtype`` (None: the weight's type)."""
+    what = "group_norm_grad"
+    dev = _dev(dy, x, w, b, mean, rstd)
+    if dy.shape != x.shape:
+        raise ValueError(f"{what}: dy {tuple(dy.shape)}, expected {tuple(x.shape)}")
+    if dy.dtype != x.dtype:
+        raise TypeError(f"{what}: dy {dy.dtype} for rows in {x.dtype}")
+    wt = w_dtype or next((t.dtype for t in (w, b) if t is not None), x.dtype)
+    for t in (w, b):
+        _float_rows(what, x, wt, None if t is None else t.dtype)
+    rows, n, at, c = _as_samples(what, x, groups)
+    grads = _as_samples(what, dy, groups)[0]
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _expect(what, name, t, n, groups)
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise TypeError(f"{what}: {name} as group_norm gave it")
+    _expect(what, "weight", w, c)
+    _expect(what, "bias", b, c)
+    wc, bc = _whole(w), _whole(b)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    dw = torch.empty(c, dtype=wt, device=dev) if want[1] else None
+    db = torch.empty(c, dtype=wt, device=dev) if want[2] else None
+    size = lib().lng_group_norm_workspace_bytes(n, at, c, groups, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _call(what, dev, lib().lng_group_norm_grad, grads.data_ptr(), grads.stride(0), grads.stride(1), rows.data_ptr(),
+          rows.stride(0), rows.stride(1), _DT[x.dtype], n, at, c, groups, _ptr(wc), _ptr(bc), _DT[wt], int(silu),
+          mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), size, _ptr(dx), _ptr(dw), _ptr(db))
+    return dx, dw, db
+
+
 def _conv_check(what: str, x, w, bias, dilation: int, hist, dims: int) -> tuple:
     """``(C, K, rows of a history)`` of a short conv's checked arguments."""
     if x.dim() != dims:
