@@ -878,7 +878,8 @@ typedef struct lng_linear_attention {
   float* checkpoints; /* lng_linear_attention_checkpoints() floats: written by the forward call where not null, read by
                        * the backward call */
 } lng_linear_attention;
-/* Gradients: dy [B, T, H, V] (strided) and dstate_out [B, H, K, V] or null in; dq, dk, dv contiguous in the tensors'
+/* Gradients: dy [B, T, H, V] (strided; where V is a multiple of 8, in rows of 16-byte pieces less than 2^25 bytes apart)
+ * and dstate_out [B, H, K, V] or null in; dq, dk, dv contiguous in the tensors'
  * type and shapes, ddecay [B, T, H] (token_decay) or [H], dstate [B, H, K, V] (may be null) in fp32 out. */
 typedef struct lng_linear_attention_grad {
   const void* dy;

@@ -25,7 +25,6 @@ namespace {
 
 constexpr int MAX_D = 128;  // of keys and values
 constexpr int VT = 64;      // columns of values a block takes
-constexpr int PAD = 8;      // elements behind a row in LDS
 
 // Planes: bf16 parts of an input; PREC: parts of a computed operand of a product whose result is rounded to the type.
 template <typename T>
@@ -50,7 +49,8 @@ struct Args {
   float scale;
   const void *q, *k, *v, *dy;
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, yb, yt, yh;
-  bool qvec, kvec, vvec, yvec;  // rows that 16-byte loads take
+  bool qvec, kvec, vvec, yvec;  // rows that 16-byte loads take (y: stores of four values)
+  int Kp, Vp;                   // keys and values a row of q, k, v and dy holds, zeros behind K and V
   const float* g;
   int64_t gb, gt;
   const float* start;    // [B, H, K, V] or null
@@ -87,47 +87,36 @@ __device__ __forceinline__ Unit unit_of(const Args& a, int segs, int first_seg) 
 }
 
 // ------------------------------------------------------------------ sums of log decays
-struct Sum {
-  float hi, lo;
-};
-__device__ __forceinline__ Sum add(Sum a, Sum b) {
-  const float s = a.hi + b.hi, bb = s - a.hi;
-  const float lo = ((a.hi - (s - bb)) + (b.hi - bb)) + (a.lo + b.lo);
-  const float hi = s + lo;
-  return {hi, lo - (hi - s)};
-}
-// 2^(a - b)
+// 2^(a - b) of two sums, each the sum of two floats
 __device__ __forceinline__ float exp2_gap(float ahi, float alo, float bhi, float blo) {
   return __builtin_amdgcn_exp2f((ahi - bhi) + (alo - blo));
 }
+__device__ __forceinline__ float exp2_sum(double x) {
+  const float hi = static_cast<float>(x), e = __builtin_amdgcn_exp2f(hi);
+  return fmaf(e, static_cast<float>(x - hi) * 0.69314718f, e);
+}
 // A log decay in powers of two.  Below -300 the decay is zero in fp32 whatever the rest: it counts as -300, minus
 // infinity too, so that a difference of two such sums is no NaN.
-__device__ __forceinline__ Sum log2_decay(float g) {
-  constexpr float REST = 1.92596303e-8f;  // log2 e - LOG2E
+__device__ __forceinline__ double log2_decay(float g) {
   g = g < -300.f ? -300.f : g;
-  const float p = g * LOG2E;
-  return {p, fmaf(g, REST, fmaf(g, LOG2E, -p))};
-}
-// Inclusive sums over the first n lanes' tokens
-__device__ __forceinline__ Sum scan_sum(Sum v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const Sum o{__shfl_up(v.hi, off, 64), __shfl_up(v.lo, off, 64)};
-    if (lane >= off) v = add(o, v);
-  }
-  return v;
+  return static_cast<double>(g) * 1.4426950408889634;
 }
 
 // ------------------------------------------------------------------ operands
-// x as the sum of N bf16 values; what is no finite bf16 value stands in the first part alone
+// x as the sum of N bf16 values: its first eight significant bits, the next eight, and so on, the last part rounded.
+// An fp16 value is two parts exactly, an fp32 value three.  (What is not finite comes out as NaN.)
+__device__ __forceinline__ float top(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u); }
 template <int N>
 __device__ __forceinline__ void split(float x, bf16 (&out)[N]) {
-  float r = x;
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    out[p] = static_cast<bf16>(r);
-    const float f = static_cast<float>(out[p]);
-    if (p + 1 < N) r = fabsf(f) < INFINITY ? r - f : 0.f;
+    if (p + 1 < N) {
+      const float f = top(x);
+      out[p] = __builtin_bit_cast(bf16, static_cast<uint16_t>(__builtin_bit_cast(uint32_t, f) >> 16));
+      x -= f;
+    } else {
+      out[p] = static_cast<bf16>(x);
+    }
   }
 }
 
@@ -136,12 +125,20 @@ struct Frag {
   bf16x8 p[N];
 };
 
+// two neighbouring values of an operand
 template <int N>
-__device__ __forceinline__ void put(Frag<N>& f, int i, float x) {
-  bf16 t[N];
-  split<N>(x, t);
+__device__ __forceinline__ void put2(Frag<N>& f, int i, float x, float y) {
+  u32x4* w[N];
 #pragma unroll
-  for (int p = 0; p < N; ++p) f.p[p][i] = t[p];
+  for (int p = 0; p < N; ++p) {
+    w[p] = reinterpret_cast<u32x4*>(&f.p[p]);
+    if (p + 1 < N) {
+      (*w[p])[i / 2] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
+      x -= top(x), y -= top(y);
+    } else {
+      (*w[p])[i / 2] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<bf16>(x), static_cast<bf16>(y)});
+    }
+  }
 }
 
 // acc += a . b without the products of parts that add to LIM or more
@@ -158,34 +155,63 @@ __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB
 // 4 g + 0..3 and 16 + 4 g + 0..3 with g = l / 16.  (Any order will do that both operands share; this one is that of
 // two stacked result tiles, whose rows 4 g + 0..3 a lane holds, so that results are operands as they are.)
 //
-// From LDS, rows of `stride` elements, planes `plane` elements apart.  by_row: row r0 + l % 16, index along the row.
+// Matrices stand in LDS as tiles of 16 x 16, 512 bytes each; in row r of a tile the four pieces of four values are
+// swapped by r / 4, so that 16 lanes' 8-byte pieces of one column or of four rows cover all banks once, whichever way a
+// matrix is read.  Whatever the matrix, a lane's place in a tile is one of two: the rest are constants.
+constexpr int TILE = 256;  // elements
+__device__ __forceinline__ int row_place() {  // row l % 16, piece g
+  const int lane = threadIdx.x & 63, i = lane & 15;
+  return i * 16 + (((lane >> 4) ^ (i >> 2)) << 2);
+}
+__device__ __forceinline__ int col_place() {  // row 4 g + i / 4, piece i % 4
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  return (4 * g + (i >> 2)) * 16 + (((i & 3) ^ g) << 2);
+}
+__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ bf16x4 piece(const bf16* at) { return *reinterpret_cast<const bf16x4*>(at); }
+// the transposing read: lane i of each 16-lane group gets element i % 4 of the pieces that lanes i / 4 + 4 c address
+__device__ __forceinline__ bf16x4 piece_tr(const bf16* at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(at));
+}
+// A matrix of W columns in N planes: by_row: row r0 + l % 16, index along the row from c0; by_col: column c0 + l % 16,
+// index along the rows from r0.
+template <int N, int W>
+__device__ __forceinline__ Frag<N> by_row(const bf16* s, int plane, int r0, int c0) {
+  const bf16* at = s + ((r0 / 16) * (W / 16) + c0 / 16) * TILE + row_place();
+  Frag<N> f;
+#pragma unroll
+  for (int p = 0; p < N; ++p) f.p[p] = join(piece(at + p * plane), piece(at + p * plane + TILE));
+  return f;
+}
+template <int N, int W>
+__device__ __forceinline__ Frag<N> by_col(const bf16* s, int plane, int r0, int c0) {
+  const bf16* at = s + ((r0 / 16) * (W / 16) + c0 / 16) * TILE + col_place();
+  Frag<N> f;
+#pragma unroll
+  for (int p = 0; p < N; ++p) f.p[p] = join(piece_tr(at + p * plane), piece_tr(at + p * plane + (W / 16) * TILE));
+  return f;
+}
+// A lower triangle of tiles: (it, jt) with jt <= it
+__device__ __forceinline__ constexpr int tri(int it, int jt) { return (it * (it + 1) / 2 + jt) * TILE; }
 template <int N>
-__device__ __forceinline__ Frag<N> by_row(const bf16* s, int stride, int plane, int r0, int c0) {
-  const int lane = threadIdx.x & 63;
-  const bf16* at = s + (r0 + (lane & 15)) * stride + c0 + 4 * (lane >> 4);
+__device__ __forceinline__ Frag<N> tri_by_row(const bf16* s, int plane, int it, int st) {  // columns 32 st ..
   Frag<N> f;
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    const bf16x4 a = *reinterpret_cast<const bf16x4*>(at + p * plane);
-    const bf16x4 b = *reinterpret_cast<const bf16x4*>(at + p * plane + 16);
-    f.p[p] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    const bf16* at = s + p * plane + row_place();
+    f.p[p] = join(piece(at + tri(it, 2 * st)), 2 * st + 1 <= it ? piece(at + tri(it, 2 * st + 1)) : bf16x4{});
   }
   return f;
 }
-// by_col: column c0 + l % 16, index along the rows from r0: the transposing read gives lane i of each 16-lane group
-// element i % 4 of the 8-byte chunks that lanes i / 4 + 4 c address (c = 0..3).
 template <int N>
-__device__ __forceinline__ Frag<N> by_col(const bf16* s, int stride, int plane, int r0, int c0) {
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const bf16* at = s + (r0 + 4 * g + (i >> 2)) * stride + c0 + 4 * (i & 3);
+__device__ __forceinline__ Frag<N> tri_by_col(const bf16* s, int plane, int st, int jt, int tiles) {  // rows 32 st ..
   Frag<N> f;
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-        (__attribute__((address_space(3))) bf16x4*)(at + p * plane));
-    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-        (__attribute__((address_space(3))) bf16x4*)(at + p * plane + 16 * stride));
-    f.p[p] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    const bf16* at = s + p * plane + col_place();
+    // nothing has been written to tiles that hold no token
+    f.p[p] = join(2 * st >= jt ? piece_tr(at + tri(2 * st, jt)) : bf16x4{},
+                  2 * st + 1 < tiles ? piece_tr(at + tri(2 * st + 1, jt)) : bf16x4{});
   }
   return f;
 }
@@ -193,37 +219,43 @@ template <int N>
 __device__ __forceinline__ float value(const Frag<N>& f, int i) {
   float x = 0.f;
 #pragma unroll
-  for (int p = N - 1; p >= 0; --p) x += static_cast<float>(f.p[p][i]);
+  for (int p = N - 1; p >= 0; --p) x = p == N - 1 ? static_cast<float>(f.p[p][i]) : x + static_cast<float>(f.p[p][i]);
   return x;
 }
-// Four neighbouring values of a row
+// The four values of a tile's row l % 16 from column 4 g on, as a result tile's lane holds them (transposed)
 template <int N>
-__device__ __forceinline__ void four(const bf16* at, int plane, float (&x)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = 0.f;
+__device__ __forceinline__ void four(const bf16* tile, int plane, float (&x)[4]) {
 #pragma unroll
   for (int p = N - 1; p >= 0; --p) {
-    const bf16x4 a = *reinterpret_cast<const bf16x4*>(at + p * plane);
+    const bf16x4 a = piece(tile + p * plane + row_place());
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] += static_cast<float>(a[i]);
+    for (int i = 0; i < 4; ++i) x[i] = p == N - 1 ? static_cast<float>(a[i]) : x[i] + static_cast<float>(a[i]);
   }
 }
-// a lane's four values of a result tile into row-major LDS planes
 template <int N>
-__device__ __forceinline__ void put_four(bf16* at, int plane, const float (&x)[4]) {
-  bf16 t[4][N];
+__device__ __forceinline__ void put_four(bf16* tile, int plane, const float (&x)[4]) {
+  Frag<N> f;
+  put2(f, 0, x[0], x[1]);
+  put2(f, 2, x[2], x[3]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) split<N>(x[i], t[i]);
-#pragma unroll
-  for (int p = 0; p < N; ++p) *reinterpret_cast<bf16x4*>(at + p * plane) = bf16x4{t[0][p], t[1][p], t[2][p], t[3][p]};
+  for (int p = 0; p < N; ++p)
+    *reinterpret_cast<bf16x4*>(tile + p * plane + row_place()) = __builtin_shufflevector(f.p[p], f.p[p], 0, 1, 2, 3);
+}
+// one value, by its row and column
+template <int N, int W>
+__device__ __forceinline__ float at_cell(const bf16* s, int plane, int r, int c) {
+  const int at = ((r / 16) * (W / 16) + c / 16) * TILE + (r & 15) * 16 + ((((c >> 2) ^ (r >> 2)) & 3) << 2) + (c & 3);
+  float x = 0.f;
+  for (int p = N - 1; p >= 0; --p) x += static_cast<float>(s[at + p * plane]);
+  return x;
 }
 
 // ------------------------------------------------------------------ rows from memory to LDS
+// Eight neighbouring values of a row as they are in memory, element by element where 16-byte loads do not do
 template <typename T>
-struct Eight {  // neighbouring values of a row as they are in memory
+struct Eight {
   T x[8] __attribute__((aligned(16)));
 };
-
 template <typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T* row, int c, int D, bool vec) {
   Eight<T> e;
@@ -243,39 +275,53 @@ __device__ __forceinline__ Eight<T> load_eight(const T* row, int c, int D, bool 
   return e;
 }
 
-// The rows of one tensor of a chunk, held by a block's threads: C rows of W columns
+// The rows of one tensor of a chunk, held by a block's threads: C rows of W columns.  16 neighbouring threads take eight
+// rows of half a tile, so that they write to all banks; a wave reads whole lines.
 template <typename T, int C, int W, int THREADS>
 struct Stage {
-  static constexpr int N = (C * W / 8 + THREADS - 1) / THREADS, PER = W / 8;
-  static constexpr bool WHOLE = C * W % (8 * THREADS) == 0;  // else some threads have a group less
+  static constexpr int GROUPS = C * W / 8, N = (GROUPS + THREADS - 1) / THREADS, TILES = W / 16;
+  static constexpr bool WHOLE = GROUPS % THREADS == 0;  // else some threads have a group less
   Eight<T> e[N];
-  // rows t0 .. t0 + n - 1 of the tensor; the others are zero
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int t0, int n, int c0, int D, bool vec) {
+  static __device__ __forceinline__ void place(int i, int& r, int& c) {
+    const int at = static_cast<int>(threadIdx.x) + i * THREADS;
+    r = ((at >> 1) & 7) + (at >> 4) / TILES * 8;
+    c = ((at >> 4) % TILES) * 16 + (at & 1) * 8;
+  }
+  // rows 0 .. n - 1 from `base`, `stride` bytes apart (the same in every lane), c0 their first column; else zeros
+  __device__ __forceinline__ void load(const T* base, uint32_t stride, int n, int c0, int Dp) {
+    const __amdgpu_buffer_rsrc_t rs = dev_buf(base, 0x7ffffff0u);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * THREADS, r = at / PER, c = at % PER * 8;
-      if (r < n)
-        e[i] = load_eight<T>(base + (t0 + r) * stride + c0, c, D - c0, vec);
-      else {
-        u32x4* w = reinterpret_cast<u32x4*>(&e[i]);
-        for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) w[k] = u32x4{0, 0, 0, 0};
-      }
+      int r, c;
+      place(i, r, c);
+      // an offset past the descriptor's range reads zeros
+      const uint32_t off = r < n && c0 + c < Dp ? static_cast<uint32_t>(r) * stride + (c0 + c) * sizeof(T) : 0x7ffffff0u;
+      u32x4* w = reinterpret_cast<u32x4*>(&e[i]);
+#pragma unroll
+      for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
+        w[k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16 * k, 0, 0));
     }
   }
-  __device__ __forceinline__ void store(bf16* s, int stride, int plane) const {
+  __device__ __forceinline__ void store(bf16* s, int plane) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * THREADS, r = at / PER, c = at % PER * 8;
+      int r, c;
+      place(i, r, c);
       if (!WHOLE && r >= C) continue;
-      bf16* to = s + r * stride + c;
+      bf16* tile = s + ((r / 16) * TILES + c / 16) * TILE + (r & 15) * 16;
+      const int u = (c >> 2) & 3, h = (r >> 2) & 3;
+      Frag<Traits<T>::planes> f;
       if constexpr (std::is_same<T, bf16>::value) {
-        *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(&e[i]);
+        f.p[0] = *reinterpret_cast<const bf16x8*>(&e[i]);
       } else {
-        Frag<Traits<T>::planes> f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) put(f, k, to_f32(e[i].x[k]));
+        for (int k = 0; k < 8; k += 2) put2(f, k, to_f32(e[i].x[k]), to_f32(e[i].x[k + 1]));
+      }
 #pragma unroll
-        for (int p = 0; p < Traits<T>::planes; ++p) *reinterpret_cast<bf16x8*>(to + p * plane) = f.p[p];
+      for (int p = 0; p < Traits<T>::planes; ++p) {
+        *reinterpret_cast<bf16x4*>(tile + p * plane + ((u ^ h) << 2)) = __builtin_shufflevector(f.p[p], f.p[p], 0, 1, 2, 3);
+        *reinterpret_cast<bf16x4*>(tile + p * plane + (((u + 1) ^ h) << 2)) =
+            __builtin_shufflevector(f.p[p], f.p[p], 4, 5, 6, 7);
       }
     }
   }
@@ -286,107 +332,144 @@ template <int C>
 struct Decays {
   float hi[C], lo[C], from[C], left[C];
   float whole;     // e^{G[n]}
-  Sum total;
   float pad;
+  double total;
 };
 // by one whole wave; g: this lane's token's log decay (0 behind the sequence's end)
 template <int C>
 __device__ __forceinline__ void decays(Decays<C>& d, float g, float scale) {
   const int lane = threadIdx.x & 63;
-  const Sum s = scan_sum(log2_decay(g), lane);
-  const Sum t{__shfl(s.hi, C - 1, 64), __shfl(s.lo, C - 1, 64)};
-  if (lane < C) {
-    d.hi[lane] = s.hi, d.lo[lane] = s.lo;
-    d.from[lane] = __builtin_amdgcn_exp2f(s.hi + s.lo) * scale;
-    d.left[lane] = exp2_gap(t.hi, t.lo, s.hi, s.lo);
+  double s = log2_decay(g);
+#pragma unroll
+  for (int off = 1; off < C; off *= 2) {
+    const double o = __shfl_up(s, off, 64);
+    s += lane >= off ? o : 0.;
   }
-  if (lane == 0) d.whole = __builtin_amdgcn_exp2f(t.hi + t.lo), d.total = t;
+  const double t = __shfl(s, C - 1, 64);
+  if (lane < C) {
+    const float hi = static_cast<float>(s);
+    d.hi[lane] = hi, d.lo[lane] = static_cast<float>(s - hi);
+    d.from[lane] = exp2_sum(s) * scale;
+    d.left[lane] = exp2_sum(t - s);
+  }
+  if (lane == 0) d.whole = exp2_sum(t), d.total = t;
 }
-__device__ __forceinline__ float load_decay(const Args& a, const Unit& u, int t0, int n) {
+__device__ __forceinline__ float load_decay(const float* g, int64_t stride, int n) {
   const int lane = threadIdx.x & 63;
-  return lane < n ? a.g[u.b * a.gb + (t0 + lane) * a.gt + u.h] : 0.f;
+  return lane < n ? g[lane * stride] : 0.f;
 }
 
-// four neighbouring values of a row of an output, as far as it goes
+// Reads and writes through buffer descriptors: an offset past the range reads zero and writes nothing, so that no lane
+// has to leave the others.  `base` is the same in every lane.
+constexpr uint32_t NOWHERE = 0x7ffffff0u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t from(const void* base) { return dev_buf(base, NOWHERE); }
+
+// four neighbouring values of a row of an output, as far as it goes (left > 0 in some lane at most)
 template <typename T>
-__device__ __forceinline__ void store_four(T* at, int left, bool vec, const float (&x)[4]) {
-  if (vec && left >= 4) {
-    struct alignas(4 * sizeof(T)) Four {
-      T x[4];
-    };
-    Four f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.x[i] = from_f32<T>(x[i]);
-    *reinterpret_cast<Four*>(at) = f;
+__device__ __forceinline__ void store_four(__amdgpu_buffer_rsrc_t rs, uint32_t off, int left, bool vec, const f32x4& x) {
+  if (vec) {  // whole pieces of four
+    const uint32_t at = left > 0 ? off : NOWHERE;
+    if constexpr (sizeof(T) == 4) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rs, at, 0, 0);
+    } else {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      const T4 t{from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])};
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, t), rs, at, 0, 0);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) at[i] = from_f32<T>(x[i]);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = i < left ? off + i * sizeof(T) : NOWHERE;
+      const float v = x[i];  // a bit cast of a vector's element itself comes out as element 0
+      if constexpr (sizeof(T) == 4)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rs, at, 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<T>(v)), rs, at, 0, 0);
+    }
   }
 }
 
 // ------------------------------------------------------------------ a state in a wave's registers
 // Tile t holds rows 16 t + 4 g + 0..3 (keys) of column c0 + l % 16 (values) of a [K, V] matrix
+__device__ __forceinline__ uint32_t state_place(int V, int c0) {
+  const int lane = threadIdx.x & 63, c = c0 + (lane & 15);
+  return c < V ? 4u * (4 * (lane >> 4) * V + c) : NOWHERE / 2;
+}
 template <int TK>
 __device__ __forceinline__ void load_state(f32x4 (&s)[TK], const float* m, int K, int V, int c0) {
-  const int lane = threadIdx.x & 63, c = c0 + (lane & 15), r0 = 4 * (lane >> 4);
+  const __amdgpu_buffer_rsrc_t rs = dev_buf(m, 4u * K * V);
+  const uint32_t at = state_place(V, c0);
 #pragma unroll
   for (int t = 0; t < TK; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * t + r0 + i;
-      s[t][i] = r < K && c < V ? m[r * V + c] : 0.f;
-    }
+    for (int i = 0; i < 4; ++i)
+      s[t][i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4u * (16 * t + i) * V, 0, 0));
 }
 template <int TK>
 __device__ __forceinline__ void store_state(const f32x4 (&s)[TK], float* m, int K, int V, int c0) {
-  const int lane = threadIdx.x & 63, c = c0 + (lane & 15), r0 = 4 * (lane >> 4);
+  const __amdgpu_buffer_rsrc_t rs = dev_buf(m, 4u * K * V);
+  const uint32_t at = state_place(V, c0);
 #pragma unroll
   for (int t = 0; t < TK; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 16 * t + r0 + i;
-      if (r < K && c < V) m[r * V + c] = s[t][i];
+      const float v = s[t][i];
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rs, at + 4u * (16 * t + i) * V, 0, 0);
     }
 }
 
-// S <- whole S + X^T (f Y): rows of X (sX, keys) and Y (sY, values) of a chunk, f a factor a row.  The scaled operand is
-// fp32 in three parts: the states are the results that stay in fp32.
-template <int C, int TK, int NX>
-__device__ __forceinline__ void update_state(f32x4 (&s)[TK], const bf16* sX, int xstride, int xplane, const Frag<NX> (&y)[C / 32],
+// S <- whole S + X^T (f Y): rows of X (sX, W keys) and Y (values, this wave's columns) of a chunk, f a factor a row.  The
+// scaled operand is fp32 in three parts: the states are the results that stay in fp32.
+template <int C, int TK, int W, int NX>
+__device__ __forceinline__ void update_state(f32x4 (&s)[TK], const bf16* sX, int xplane, const Frag<NX> (&y)[C / 32],
                                              const float* f, float whole) {
-  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int t = 0; t < TK; ++t) s[t] *= whole;
 #pragma unroll
   for (int st = 0; st < C / 32; ++st) {
     Frag<3> fy;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) put(fy, i, value(y[st], i) * f[32 * st + (i < 4 ? 0 : 16) + 4 * g + (i & 3)]);
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 fr = *reinterpret_cast<const f32x4*>(f + 32 * st + 16 * h + 4 * g);
 #pragma unroll
-    for (int t = 0; t < TK; ++t) mma<3>(s[t], by_col<NX>(sX, xstride, xplane, 32 * st, 16 * t), fy);
+      for (int i = 0; i < 4; i += 2)
+        put2(fy, 4 * h + i, value(y[st], 4 * h + i) * fr[i], value(y[st], 4 * h + i + 1) * fr[i + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < TK; ++t) mma<3>(s[t], by_col<NX, W>(sX, xplane, 32 * st, 16 * t), fy);
   }
+}
+// The state as the operand whose index runs over keys
+template <int TK, int N>
+__device__ __forceinline__ void state_frags(const f32x4 (&s)[TK], Frag<N> (&f)[TK / 2]) {
+#pragma unroll
+  for (int t = 0; t < TK; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) put2(f[t / 2], 4 * (t & 1) + r, s[t][r], s[t][r + 1]);
 }
 
 // ------------------------------------------------------------------ forward
 template <typename T, int DK, int NW>
 struct FwdLds {
   using Tr = Traits<T>;
-  static constexpr int C = Tr::chunk, KS = DK + PAD, VS = 16 * NW + PAD, PS = C + PAD;
-  bf16 q[Tr::planes][C][KS];
-  bf16 k[Tr::planes][C][KS];
-  bf16 v[Tr::planes][C][VS];
-  bf16 p[Tr::prec][C][PS];
+  static constexpr int C = Tr::chunk, W = 16 * NW;
+  bf16 q[Tr::planes][C * DK];
+  bf16 k[Tr::planes][C * DK];
+  bf16 v[Tr::planes][C * W];
+  bf16 p[Tr::prec][tri(C / 16, 0)];
   Decays<C> d[2];
 };
 
 // A block of NW waves takes a head's 16 NW value columns over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
 template <typename T, int DK, int NW, bool ENDS>
-__global__ __launch_bounds__(64 * NW) void k_la_fwd(Args a) {
+__global__ __launch_bounds__(64 * NW, (ENDS ? 4 : DK <= 64 ? 3 : 2) - (NW == 2 && DK > 32)) void k_la_fwd(Args a) {
   using L = FwdLds<T, DK, NW>;
   using Tr = Traits<T>;
-  constexpr int C = L::C, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, THREADS = 64 * NW;
+  constexpr int C = L::C, W = L::W, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, THREADS = 64 * NW;
+  constexpr int KP = C * DK, VP = C * W, PP = tri(C / 16, 0);  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
@@ -398,7 +481,9 @@ __global__ __launch_bounds__(64 * NW) void k_la_fwd(Args a) {
   const T* q = static_cast<const T*>(a.q) + u.b * a.qb + u.h / (a.H / a.Hq) * a.qh;
   const T* k = static_cast<const T*>(a.k) + u.b * a.kb + u.h / (a.H / a.Hk) * a.kh;
   const T* v = static_cast<const T*>(a.v) + u.b * a.vb + u.h / (a.H / a.Hv) * a.vh;
+  const float* g = a.g + u.b * a.gb + u.h;
   T* y = static_cast<T*>(a.y) + (u.b * a.T * a.H + u.h) * a.V;
+  const int yrow = a.H * a.V;
 
   f32x4 s[TK];
   if (!ENDS && a.segs > 1)
@@ -408,32 +493,37 @@ __global__ __launch_bounds__(64 * NW) void k_la_fwd(Args a) {
   else
     for (int t = 0; t < TK; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  Stage<T, C, DK, THREADS> rq, rk;
-  Stage<T, C, 16 * NW, THREADS> rv;
-  float rg = 0.f;
-  auto fetch = [&](int c) {
-    const int t0 = c * C, n = min(C, u.len - t0);
-    if (!ENDS) rq.load(q, a.qt, t0, n, 0, a.K, a.qvec);
-    rk.load(k, a.kt, t0, n, 0, a.K, a.kvec);
-    rv.load(v, a.vt, t0, n, v0, a.V, a.vvec);
-    if (w == 0) rg = load_decay(a, u, t0, n);
-  };
   const int c_end = min(c_last, (u.len + C - 1) / C);  // chunks with tokens
+  Stage<T, C, DK, THREADS> rq, rk;
+  Stage<T, C, W, THREADS> rv;
+  // one wave's: the next chunk's log decays, asked for a chunk before the rows are, so that their sums wait for nothing
+  float rg = 0.f;
+  auto fetch_decay = [&](int c) {
+    if (w == NW - 1 && c < c_end) rg = load_decay(g + int64_t{c} * C * a.gt, a.gt, min(C, u.len - c * C));
+  };
+  auto fetch = [&](int c) {
+    const int64_t t0 = int64_t{c} * C;
+    const int n = min(C, u.len - c * C);
+    if (!ENDS) rq.load(q + t0 * a.qt, static_cast<uint32_t>(a.qt * sizeof(T)), n, 0, a.Kp);
+    rk.load(k + t0 * a.kt, static_cast<uint32_t>(a.kt * sizeof(T)), n, 0, a.Kp);
+    rv.load(v + t0 * a.vt, static_cast<uint32_t>(a.vt * sizeof(T)), n, v0, a.Vp);
+  };
   if (c_first < c_end) {
+    fetch_decay(c_first);
     fetch(c_first);
-    if (!ENDS)  // the tiles above the diagonal stay zero
-      for (int i = threadIdx.x; i < static_cast<int>(sizeof(lds.p) / 16); i += THREADS)
-        reinterpret_cast<u32x4*>(&lds.p)[i] = u32x4{0, 0, 0, 0};
-    if (w == 0) decays(lds.d[c_first & 1], rg, a.scale);
+    if (w == NW - 1) decays(lds.d[c_first & 1], rg, a.scale);
+    fetch_decay(c_first + 1);
   }
-  Sum seg{0.f, 0.f};
+  double seg = 0.;
   for (int c = c_first; c < c_end; ++c) {
     const int t0 = c * C, n = min(C, u.len - t0);
     const Decays<C>& d = lds.d[c & 1];
-    if (!ENDS) rq.store(&lds.q[0][0][0], L::KS, C * L::KS);
-    rk.store(&lds.k[0][0][0], L::KS, C * L::KS);
-    rv.store(&lds.v[0][0][0], L::VS, C * L::VS);
+    if (!ENDS) rq.store(lds.q[0], KP);
+    rk.store(lds.k[0], KP);
+    rv.store(lds.v[0], VP);
     __syncthreads();
+    const float g_next = rg;
+    fetch_decay(c + 2);
     if (c + 1 < c_end) fetch(c + 1);
     if (!ENDS && a.ckpt) store_state(s, a.ckpt + (bh * a.chunks + c) * KV, a.K, a.V, vc);
 
@@ -445,77 +535,72 @@ __global__ __launch_bounds__(64 * NW) void k_la_fwd(Args a) {
         f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < DK / 32; ++st)
-          mma<3>(acc, by_row<NP>(&lds.k[0][0][0], L::KS, C * L::KS, 16 * jt, 32 * st),
-                 by_row<NP>(&lds.q[0][0][0], L::KS, C * L::KS, 16 * it, 32 * st));
+          mma<3>(acc, by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st), by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
         const int i = 16 * it + li, j0 = 16 * jt + 4 * lg;
         const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
         const float ih = d.hi[i], il = d.lo[i];
         float p[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          p[r] = j0 + r <= i ? acc[r] * exp2_gap(ih, il, jh[r], jl[r]) * a.scale : 0.f;
-        put_four<PR>(&lds.p[0][i][j0], C * L::PS, p);
+        for (int r = 0; r < 4; ++r) p[r] = acc[r] * (exp2_gap(ih, il, jh[r], jl[r]) * a.scale);
+        if (it == jt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[r] = 4 * lg + r <= li ? p[r] : 0.f;
+        put_four<PR>(lds.p[0] + idx * TILE, PP, p);
       }
       __syncthreads();
     }
-    if (w == 0 && c + 1 < c_end) decays(lds.d[(c + 1) & 1], rg, a.scale);
+    if (w == NW - 1 && c + 1 < c_end) decays(lds.d[(c + 1) & 1], g_next, a.scale);
 
     Frag<NP> fv[C / 32];
     float odd = 0.f;
 #pragma unroll
     for (int st = 0; st < C / 32; ++st) {
-      fv[st] = by_col<NP>(&lds.v[0][0][0], L::VS, C * L::VS, 32 * st, 16 * w);
+      fv[st] = by_col<NP, W>(lds.v[0], VP, 32 * st, 16 * w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) odd = fmaf(static_cast<float>(fv[st].p[0][i]), 0.f, odd);
     }
     if (!ENDS) {
       // an infinity or NaN among the values may not reach the tokens before it, with a weight of zero
       const bool careful = __ballot(!(odd == 0.f)) != 0ull;
-      Frag<PR> fs[DK / 32];
-#pragma unroll
-      for (int t = 0; t < TK; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) put(fs[t / 2], 4 * (t & 1) + r, s[t][r]);
+      Frag<PR> fs[TK / 2];
+      state_frags(s, fs);
+      const __amdgpu_buffer_rsrc_t yc = from(y + int64_t{t0} * yrow);
 #pragma unroll
       for (int it = 0; it < TI; ++it) {
         if (it >= tiles) break;
         const int i = 16 * it + li;
         f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < DK / 32; ++st)
-          mma<PR>(acc, fs[st], by_row<NP>(&lds.q[0][0][0], L::KS, C * L::KS, 16 * it, 32 * st));
+        for (int st = 0; st < DK / 32; ++st) mma<PR>(acc, fs[st], by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
         acc *= d.from[i];
         if (!careful) {
 #pragma unroll
-          for (int st = 0; st <= it / 2; ++st)
-            mma<PR>(acc, fv[st], by_row<PR>(&lds.p[0][0][0], L::PS, C * L::PS, 16 * it, 32 * st));
+          for (int st = 0; st <= it / 2; ++st) mma<PR>(acc, fv[st], tri_by_row<PR>(lds.p[0], PP, it, st));
         } else {
           for (int j = 0; j <= i; ++j) {
-            float p = 0.f, x[4];
-            for (int b = PR - 1; b >= 0; --b) p += static_cast<float>(lds.p[b][i][j]);
-            four<NP>(&lds.v[0][j][16 * w + 4 * lg], C * L::VS, x);
-            for (int r = 0; r < 4; ++r) acc[r] = fmaf(p, x[r], acc[r]);
+            const float p = at_cell<PR, 16>(lds.p[0] + tri(it, j / 16), PP, li, j & 15);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = fmaf(p, at_cell<NP, W>(lds.v[0], VP, j, 16 * w + 4 * lg + r), acc[r]);
           }
         }
-        const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
         const int col = vc + 4 * lg;
-        if (i < n) store_four(y + int64_t{t0 + i} * a.H * a.V + col, a.V - col, a.yvec, out);
+        store_four<T>(yc, static_cast<uint32_t>(i * yrow + col) * sizeof(T), i < n ? a.V - col : 0, a.yvec, acc);
       }
     }
-    update_state<C, TK, NP>(s, &lds.k[0][0][0], L::KS, C * L::KS, fv, d.left, d.whole);
-    if (ENDS && threadIdx.x == 0) seg = add(seg, d.total);
+    update_state<C, TK, DK, NP>(s, lds.k[0], KP, fv, d.left, d.whole);
+    if (ENDS && threadIdx.x == 0) seg += d.total;
     __syncthreads();
   }
   if (ENDS) {
     store_state(s, a.seg_state + (bh * a.segs + u.seg) * KV, a.K, a.V, vc);
-    if (threadIdx.x == 0 && u.vt == 0) a.seg_decay[bh * a.segs + u.seg] = seg.hi + seg.lo;
+    if (threadIdx.x == 0 && u.vt == 0) a.seg_decay[bh * a.segs + u.seg] = static_cast<float>(seg);
     return;
   }
   // positions behind the sequence's end
-  const int from = max(u.len, c_first * C), to = static_cast<int>(min(static_cast<int64_t>(c_last) * C, a.T));
-  const int cols = min(16 * NW, a.V - v0);
-  for (int64_t i = threadIdx.x; i < int64_t{to - from} * cols; i += THREADS)
-    y[(from + i / cols) * a.H * a.V + v0 + i % cols] = from_f32<T>(0.f);
+  const int start = max(u.len, c_first * C), to = static_cast<int>(min(static_cast<int64_t>(c_last) * C, a.T));
+  const int cols = min(W, a.V - v0);
+  for (int64_t i = threadIdx.x; i < int64_t{to - start} * cols; i += THREADS)
+    y[(start + i / cols) * a.H * a.V + v0 + i % cols] = from_f32<T>(0.f);
   if (a.end && u.seg == a.segs - 1) store_state(s, a.end + bh * KV, a.K, a.V, vc);
 }
 
@@ -557,20 +642,20 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 template <typename T, int DK>
 struct BwdLds {
   using Tr = Traits<T>;
-  static constexpr int C = Tr::chunk, KS = DK + PAD, VS = VT + PAD, PS = C + PAD, NR = Tr::planes > 2 ? 3 : 2;
-  bf16 q[Tr::planes][C][KS];
-  bf16 k[Tr::planes][C][KS];
-  bf16 v[Tr::planes][C][VS];
-  bf16 o[Tr::planes][C][VS];  // dy
-  bf16 p[Tr::prec][C][PS];
-  bf16 a[Tr::prec][C][PS];
-  bf16 r[NR][DK][VS];
+  static constexpr int C = Tr::chunk, NR = Tr::planes > 2 ? 3 : 2;
+  bf16 q[Tr::planes][C * DK];
+  bf16 k[Tr::planes][C * DK];
+  bf16 v[Tr::planes][C * VT];
+  bf16 o[Tr::planes][C * VT];  // dy
+  bf16 p[Tr::prec][tri(C / 16, 0)];
+  bf16 a[Tr::prec][tri(C / 16, 0)];
+  bf16 r[NR][VT * DK];         // R, rows of values
   Decays<C> d[2];
-  float row[C / 16][C];       // sums over a tile's j of P (dy.v), below the diagonal
-  float col[C / 16][C];       // over its i
-  float qs[DK / 16][C];       // q[i].(scale e^{G[i]} S_in dy[i]) over 16 keys
-  float kr[4][C];             // v[j].(e^{G[n]-G[j]} R^T k[j]) over a wave's columns
-  float sr[4];                // a wave's share of <S_in, R>
+  float row[C / 16][C];        // sums over a tile's j of P (dy.v), below the diagonal
+  float col[C / 16][C];        // over its i
+  float qs[DK / 16][C];        // q[i].(scale e^{G[i]} S_in dy[i]) over 16 keys
+  float kr[4][C];              // v[j].(e^{G[n]-G[j]} R^T k[j]) over a wave's columns
+  float sr[4];                 // a wave's share of <S_in, R>
 };
 
 constexpr int BW = 4, BTHREADS = 64 * BW;  // waves and threads of a backward block
@@ -581,14 +666,20 @@ __device__ __forceinline__ float row_sum(float v) {
   for (int m = 1; m < 16; m *= 2) v += __shfl_xor(v, m, 64);
   return v;
 }
+// Sum over the four rows of the wave, in all of them
+__device__ __forceinline__ float col_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
 
 // What the columns v0 .. v0 + 63 of the values add to the gradients; ENDS: only what the segment adds to the state's
 // gradient.
 template <typename T, int DK, bool ENDS>
-__global__ __launch_bounds__(BTHREADS) void k_la_bwd(Args a) {
+__global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bwd(Args a) {
   using L = BwdLds<T, DK>;
   using Tr = Traits<T>;
   constexpr int C = L::C, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, NR = L::NR;
+  constexpr int KP = C * DK, VP = C * VT, PP = tri(C / 16, 0), RP = VT * DK;  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
@@ -601,6 +692,7 @@ __global__ __launch_bounds__(BTHREADS) void k_la_bwd(Args a) {
   const T* k = static_cast<const T*>(a.k) + u.b * a.kb + u.h / (a.H / a.Hk) * a.kh;
   const T* v = static_cast<const T*>(a.v) + u.b * a.vb + u.h / (a.H / a.Hv) * a.vh;
   const T* dy = static_cast<const T*>(a.dy) + u.b * a.yb + u.h * a.yh;
+  const float* g = a.g + u.b * a.gb + u.h;
   const int hv = u.h * a.vts + u.vt;  // of the heads' value tiles
 
   f32x4 s[TK];  // R: rows of keys, this wave's 16 columns
@@ -611,47 +703,60 @@ __global__ __launch_bounds__(BTHREADS) void k_la_bwd(Args a) {
   else
     for (int t = 0; t < TK; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  const int c_end = min(c_last, (u.len + C - 1) / C);  // chunks with tokens
   Stage<T, C, DK, BTHREADS> rq, rk;
   Stage<T, C, VT, BTHREADS> rv, ro;
-  float rg = 0.f;
-  auto fetch = [&](int c) {
-    const int t0 = c * C, n = min(C, u.len - t0);
-    rq.load(q, a.qt, t0, n, 0, a.K, a.qvec);
-    ro.load(dy, a.yt, t0, n, v0, a.V, a.yvec);
-    if (!ENDS) {
-      rk.load(k, a.kt, t0, n, 0, a.K, a.kvec);
-      rv.load(v, a.vt, t0, n, v0, a.V, a.vvec);
-    }
-    if (w == 0) rg = load_decay(a, u, t0, n);
+  float rg = 0.f;  // one wave's: the log decays of the chunk before, asked for a chunk ahead of its rows
+  auto fetch_decay = [&](int c) {
+    if (w == BW - 1 && c >= c_first) rg = load_decay(g + int64_t{c} * C * a.gt, a.gt, min(C, u.len - c * C));
   };
-  const int c_end = min(c_last, (u.len + C - 1) / C);  // chunks with tokens
+  auto fetch = [&](int c) {
+    const int64_t t0 = int64_t{c} * C;
+    const int n = min(C, u.len - c * C);
+    rq.load(q + t0 * a.qt, static_cast<uint32_t>(a.qt * sizeof(T)), n, 0, a.Kp);
+    ro.load(dy + t0 * a.yt, static_cast<uint32_t>(a.yt * sizeof(T)), n, v0, a.Vp);
+    if (!ENDS) {
+      rk.load(k + t0 * a.kt, static_cast<uint32_t>(a.kt * sizeof(T)), n, 0, a.Kp);
+      rv.load(v + t0 * a.vt, static_cast<uint32_t>(a.vt * sizeof(T)), n, v0, a.Vp);
+    }
+  };
   if (c_first < c_end) {
+    fetch_decay(c_end - 1);
     fetch(c_end - 1);
-    if (!ENDS)  // the tiles above the diagonal stay zero
-      for (int i = threadIdx.x; i < static_cast<int>((sizeof(lds.p) + sizeof(lds.a)) / 16); i += BTHREADS)
-        reinterpret_cast<u32x4*>(&lds.p)[i] = u32x4{0, 0, 0, 0};
-    if (w == 0) decays(lds.d[(c_end - 1) & 1], rg, a.scale);
+    if (w == BW - 1) decays(lds.d[(c_end - 1) & 1], rg, a.scale);
+    fetch_decay(c_end - 2);
   }
-  Sum seg{0.f, 0.f};
+  // rows of the outputs, in elements
+  const int qrow = (a.dq32 ? a.H * a.vts : a.H) * a.K, krow = (a.dk32 ? a.H * a.vts : a.H) * a.K, vrow = a.H * a.V;
+  const int qcol = (a.dq32 ? hv : u.h) * a.K, kcol = (a.dk32 ? hv : u.h) * a.K;
+  const bool k4 = a.K % 4 == 0, v4 = a.V % 4 == 0;
+  // a lane's four values of a token's output: in the type, or in fp32 to be summed with others
+  auto emit = [&](void* out, bool f32, int64_t first, int row, int i, int col, int left, bool vec, const f32x4& x) {
+    const uint32_t at = static_cast<uint32_t>(i * row + col);
+    if (f32)
+      store_four<float>(from(static_cast<float*>(out) + first * row), at * 4, left, vec, x);
+    else
+      store_four<T>(from(static_cast<T*>(out) + first * row), at * sizeof(T), left, vec, x);
+  };
+  double seg = 0.;
   for (int c = c_end - 1; c >= c_first; --c) {
     const int t0 = c * C, n = min(C, u.len - t0), tiles = (n + 15) / 16;
+    const int64_t token = u.b * a.T + t0;
     const Decays<C>& d = lds.d[c & 1];
-    rq.store(&lds.q[0][0][0], L::KS, C * L::KS);
-    ro.store(&lds.o[0][0][0], L::VS, C * L::VS);
+    rq.store(lds.q[0], KP);
+    ro.store(lds.o[0], VP);
     if (!ENDS) {
-      rk.store(&lds.k[0][0][0], L::KS, C * L::KS);
-      rv.store(&lds.v[0][0][0], L::VS, C * L::VS);
+      rk.store(lds.k[0], KP);
+      rv.store(lds.v[0], VP);
 #pragma unroll
-      for (int t = 0; t < TK; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          bf16 x[NR];
-          split<NR>(s[t][r], x);
-#pragma unroll
-          for (int b = 0; b < NR; ++b) lds.r[b][16 * t + 4 * lg + r][16 * w + li] = x[b];
-        }
+      for (int t = 0; t < TK; ++t) {
+        const float x[4] = {s[t][0], s[t][1], s[t][2], s[t][3]};
+        put_four<NR>(lds.r[0] + (w * TK + t) * TILE, RP, x);
+      }
     }
     __syncthreads();
+    const float g_next = rg;
+    fetch_decay(c - 2);
     if (c > c_first) fetch(c - 1);
 
     if (!ENDS) {
@@ -660,12 +765,10 @@ __global__ __launch_bounds__(BTHREADS) void k_la_bwd(Args a) {
         f32x4 qk{0.f, 0.f, 0.f, 0.f}, ov{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < DK / 32; ++st)
-          mma<3>(qk, by_row<NP>(&lds.k[0][0][0], L::KS, C * L::KS, 16 * jt, 32 * st),
-                 by_row<NP>(&lds.q[0][0][0], L::KS, C * L::KS, 16 * it, 32 * st));
+          mma<3>(qk, by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st), by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
 #pragma unroll
         for (int st = 0; st < VT / 32; ++st)
-          mma<3>(ov, by_row<NP>(&lds.v[0][0][0], L::VS, C * L::VS, 16 * jt, 32 * st),
-                 by_row<NP>(&lds.o[0][0][0], L::VS, C * L::VS, 16 * it, 32 * st));
+          mma<3>(ov, by_row<NP, VT>(lds.v[0], VP, 16 * jt, 32 * st), by_row<NP, VT>(lds.o[0], VP, 16 * it, 32 * st));
         const int i = 16 * it + li, j0 = 16 * jt + 4 * lg;
         const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
         const float ih = d.hi[i], il = d.lo[i];
@@ -673,146 +776,126 @@ __global__ __launch_bounds__(BTHREADS) void k_la_bwd(Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float dec = exp2_gap(ih, il, jh[r], jl[r]) * a.scale;
-          p[r] = j0 + r <= i ? qk[r] * dec : 0.f;
-          x[r] = j0 + r <= i ? ov[r] * dec : 0.f;
-          pair[r] = j0 + r < i ? p[r] * ov[r] : 0.f;
+          p[r] = qk[r] * dec, x[r] = ov[r] * dec, pair[r] = p[r] * ov[r];
         }
-        put_four<PR>(&lds.p[0][i][j0], C * L::PS, p);
-        put_four<PR>(&lds.a[0][i][j0], C * L::PS, x);
-        float rows = (pair[0] + pair[1]) + (pair[2] + pair[3]);
-        rows += __shfl_xor(rows, 16, 64);
-        rows += __shfl_xor(rows, 32, 64);
+        if (it == jt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool on = 4 * lg + r <= li;
+            p[r] = on ? p[r] : 0.f, x[r] = on ? x[r] : 0.f, pair[r] = 4 * lg + r < li ? pair[r] : 0.f;
+          }
+        put_four<PR>(lds.p[0] + idx * TILE, PP, p);
+        put_four<PR>(lds.a[0] + idx * TILE, PP, x);
+        const float rows = col_sum((pair[0] + pair[1]) + (pair[2] + pair[3]));
         if (lg == 0) lds.row[jt][i] = rows;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float cols = row_sum(pair[r]);
-          if (li == 0) lds.col[it][j0 + r] = cols;
-        }
+        for (int r = 0; r < 4; ++r) pair[r] = row_sum(pair[r]);
+        if (li == 0) *reinterpret_cast<f32x4*>(&lds.col[it][j0]) = f32x4{pair[0], pair[1], pair[2], pair[3]};
       }
       __syncthreads();
     }
-    if (w == 0 && c > c_first) decays(lds.d[(c - 1) & 1], rg, a.scale);
+    if (w == BW - 1 && c > c_first) decays(lds.d[(c - 1) & 1], g_next, a.scale);
 
     if (!ENDS) {
       // dq and dk: tiles of 16 keys and 16 tokens, a wave's share of the keys (of the tokens, where keys are few)
       constexpr int SHARE = TK >= BW ? 1 : BW / TK, KT = TK >= BW ? TK / BW : 1, IT = TI / SHARE > 0 ? TI / SHARE : 1;
-      const float* s_in = a.ckpt + (bh * a.chunks + c) * KV;
+      const __amdgpu_buffer_rsrc_t si = dev_buf(a.ckpt + (bh * a.chunks + c) * KV, 4u * a.K * a.V);
       const int part = w % SHARE;
+      float sr = 0.f;
 #pragma unroll 1
       for (int kk = 0; kk < KT; ++kk) {
         const int kt = w / SHARE * KT + kk;
-        if (part * IT >= tiles) break;
         Frag<3> fs[VT / 32];  // S_in, rows of keys, index of values
-        const int row = 16 * kt + li;
-#pragma unroll
-        for (int st = 0; st < VT / 32; ++st)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int col = v0 + 32 * st + (i < 4 ? 0 : 16) + 4 * lg + (i & 3);
-            put(fs[st], i, row < a.K && col < a.V ? s_in[row * a.V + col] : 0.f);
-          }
         Frag<NR> fr[VT / 32];
+        const int row = 16 * kt + li;
+        float dot = 0.f;      // this wave's share of <S_in, R>
 #pragma unroll
-        for (int st = 0; st < VT / 32; ++st) fr[st] = by_row<NR>(&lds.r[0][0][0], L::VS, DK * L::VS, 16 * kt, 32 * st);
-        for (int ii = 0; ii < IT; ++ii) {
-          const int it = part * IT + ii;
-          if (it >= tiles) break;
-          const int i = 16 * it + li, key = 16 * kt + 4 * lg;
+        for (int st = 0; st < VT / 32; ++st) {
+          fr[st] = by_col<NR, DK>(lds.r[0], RP, 32 * st, 16 * kt);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = v0 + 32 * st + 16 * h + 4 * lg;
+            const uint32_t at = 4u * (row * a.V + col);
+            f32x4 x;
+            if (v4) {
+              x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(si, col < a.V ? at : NOWHERE, 0, 0));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, col + i < a.V ? at + 4 * i : NOWHERE, 0, 0));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = fmaf(x[i], value(fr[st], 4 * h + i), dot);
+            put2(fs[st], 4 * h, x[0], x[1]);
+            put2(fs[st], 4 * h + 2, x[2], x[3]);
+          }
+        }
+        if (part == 0) sr += dot;
+#pragma unroll
+        for (int ii = 0; ii < TI; ++ii) {
+          if (ii / IT != part || ii >= tiles) continue;
+          const int it = ii, i = 16 * it + li, key = 16 * kt + 4 * lg;
           f32x4 acc{0.f, 0.f, 0.f, 0.f};
           float x[4], sum = 0.f;
 #pragma unroll
-          for (int st = 0; st < VT / 32; ++st)
-            mma<3>(acc, fs[st], by_row<NP>(&lds.o[0][0][0], L::VS, C * L::VS, 16 * it, 32 * st));
+          for (int st = 0; st < VT / 32; ++st) mma<3>(acc, fs[st], by_row<NP, VT>(lds.o[0], VP, 16 * it, 32 * st));
           acc *= d.from[i];
-          four<NP>(&lds.q[0][i][key], C * L::KS, x);
+          four<NP>(lds.q[0] + (it * TK + kt) * TILE, KP, x);
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[r], sum);
-          sum += __shfl_xor(sum, 16, 64);
-          sum += __shfl_xor(sum, 32, 64);
+          sum = col_sum(sum);
           if (lg == 0) lds.qs[kt][i] = sum;
+#pragma unroll
           for (int st = 0; st <= it / 2; ++st)
-            mma<PR>(acc, by_col<NP>(&lds.k[0][0][0], L::KS, C * L::KS, 32 * st, 16 * kt),
-                    by_row<PR>(&lds.a[0][0][0], L::PS, C * L::PS, 16 * it, 32 * st));
-          const int64_t token = u.b * a.T + t0 + i;
-          if (i < n) {
-            const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
-            if (a.dq32)
-              store_four(static_cast<float*>(a.dq) + (token * a.H * a.vts + hv) * a.K + key, a.K - key, a.K % 4 == 0, out);
-            else
-              store_four(static_cast<T*>(a.dq) + (token * a.H + u.h) * a.K + key, a.K - key, a.K % 4 == 0, out);
-          }
+            mma<PR>(acc, by_col<NP, DK>(lds.k[0], KP, 32 * st, 16 * kt), tri_by_row<PR>(lds.a[0], PP, it, st));
+          emit(a.dq, a.dq32, token, qrow, i, qcol + key, i < n ? a.K - key : 0, k4, acc);
           acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int st = 0; st < VT / 32; ++st)
-            mma<NR>(acc, fr[st], by_row<NP>(&lds.v[0][0][0], L::VS, C * L::VS, 16 * it, 32 * st));
+          for (int st = 0; st < VT / 32; ++st) mma<NR>(acc, fr[st], by_row<NP, VT>(lds.v[0], VP, 16 * it, 32 * st));
           acc *= d.left[i];
-          for (int st = it / 2; st < C / 32; ++st)
-            mma<PR>(acc, by_col<NP>(&lds.q[0][0][0], L::KS, C * L::KS, 32 * st, 16 * kt),
-                    by_col<PR>(&lds.a[0][0][0], L::PS, C * L::PS, 32 * st, 16 * it));
-          if (i < n) {
-            const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
-            if (a.dk32)
-              store_four(static_cast<float*>(a.dk) + (token * a.H * a.vts + hv) * a.K + key, a.K - key, a.K % 4 == 0, out);
-            else
-              store_four(static_cast<T*>(a.dk) + (token * a.H + u.h) * a.K + key, a.K - key, a.K % 4 == 0, out);
+#pragma unroll
+          for (int st = it / 2; st < C / 32; ++st) {
+            if (2 * st >= tiles) break;  // tiles of no tokens hold nothing
+            mma<PR>(acc, by_col<NP, DK>(lds.q[0], KP, 32 * st, 16 * kt), tri_by_col<PR>(lds.a[0], PP, st, it, tiles));
           }
+          emit(a.dk, a.dk32, token, krow, i, kcol + key, i < n ? a.K - key : 0, k4, acc);
         }
       }
+      sr = wave_sum(sr);
+      if (lane == 0) lds.sr[w] = sr;
     }
-    Frag<NP> fo[C / 32];
+    Frag<NP> fo[C / 32];  // dy: this wave's columns
 #pragma unroll
-    for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP>(&lds.o[0][0][0], L::VS, C * L::VS, 32 * st, 16 * w);
+    for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP, VT>(lds.o[0], VP, 32 * st, 16 * w);
     if (!ENDS) {
       // dv: this wave's 16 columns
-      Frag<3> fs[DK / 32];
-#pragma unroll
-      for (int t = 0; t < TK; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) put(fs[t / 2], 4 * (t & 1) + r, s[t][r]);
+      Frag<3> fs[TK / 2];
+      state_frags(s, fs);
 #pragma unroll
       for (int jt = 0; jt < TI; ++jt) {
         if (jt >= tiles) break;
         const int j = 16 * jt + li;
         f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < DK / 32; ++st)
-          mma<3>(acc, fs[st], by_row<NP>(&lds.k[0][0][0], L::KS, C * L::KS, 16 * jt, 32 * st));
+        for (int st = 0; st < DK / 32; ++st) mma<3>(acc, fs[st], by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st));
         acc *= d.left[j];
         float x[4], sum = 0.f;
-        four<NP>(&lds.v[0][j][16 * w + 4 * lg], C * L::VS, x);
+        four<NP>(lds.v[0] + (jt * (VT / 16) + w) * TILE, VP, x);
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[r], sum);
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
+        sum = col_sum(sum);
         if (lg == 0) lds.kr[w][j] = sum;
 #pragma unroll
-        for (int st = jt / 2; st < C / 32; ++st)
-          mma<PR>(acc, fo[st], by_col<PR>(&lds.p[0][0][0], L::PS, C * L::PS, 32 * st, 16 * jt));
-        if (j < n) {
-          const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
-          const int col = vc + 4 * lg;
-          const int64_t token = u.b * a.T + t0 + j;
-          if (a.dv32)
-            store_four(static_cast<float*>(a.dv) + (token * a.H + u.h) * a.V + col, a.V - col, a.V % 4 == 0, out);
-          else
-            store_four(static_cast<T*>(a.dv) + (token * a.H + u.h) * a.V + col, a.V - col, a.V % 4 == 0, out);
+        for (int st = jt / 2; st < C / 32; ++st) {
+          if (2 * st >= tiles) break;
+          mma<PR>(acc, fo[st], tri_by_col<PR>(lds.p[0], PP, st, jt, tiles));
         }
+        const int col = vc + 4 * lg;
+        emit(a.dv, a.dv32, token, vrow, j, u.h * a.V + col, j < n ? a.V - col : 0, v4, acc);
       }
-      // <S_in, R> over this wave's columns
-      const float* s_in = a.ckpt + (bh * a.chunks + c) * KV;
-      float sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < TK; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * t + 4 * lg + r, col = vc + li;
-          if (row < a.K && col < a.V) sum = fmaf(s_in[row * a.V + col], s[t][r], sum);
-        }
-      sum = wave_sum(sum);
-      if (lane == 0) lds.sr[w] = sum;
     }
-    update_state<C, TK, NP>(s, &lds.q[0][0][0], L::KS, C * L::KS, fo, d.from, d.whole);
-    if (ENDS && threadIdx.x == 0) seg = add(seg, d.total);
+    update_state<C, TK, DK, NP>(s, lds.q[0], KP, fo, d.from, d.whole);
+    if (ENDS && threadIdx.x == 0) seg += d.total;
     __syncthreads();
     if (!ENDS && w == BW - 1) {
       // the decays' gradients: a lane a token
@@ -825,27 +908,27 @@ __global__ __launch_bounds__(BTHREADS) void k_la_bwd(Args a) {
       }
       double total = kept;
 #pragma unroll
-      for (int off = 1; off < 64; off *= 2) {
+      for (int off = 1; off < C; off *= 2) {
         const double x = __shfl_down(later, off, 64), y = __shfl_up(total, off, 64);
         if (lane + off < 64) later += x;
         if (lane >= off) total += y;
       }
       if (lane < n)
-        a.dg[(u.b * a.T + t0 + lane) * a.H * a.vts + hv] = static_cast<float>(
+        a.dg[(token + lane) * a.H * a.vts + hv] = static_cast<float>(
             later + (total - kept) + double(d.whole) * ((double(lds.sr[0]) + lds.sr[1]) + (double(lds.sr[2]) + lds.sr[3])));
     }
   }
   if (ENDS) {
     store_state(s, a.seg_state + (bh * a.segs + u.seg) * KV, a.K, a.V, vc);
-    if (threadIdx.x == 0 && u.vt == 0) a.seg_decay[bh * a.segs + u.seg] = seg.hi + seg.lo;
+    if (threadIdx.x == 0 && u.vt == 0) a.seg_decay[bh * a.segs + u.seg] = static_cast<float>(seg);
     return;
   }
   // positions behind the sequence's end
-  const int from = max(u.len, c_first * C), to = static_cast<int>(min(static_cast<int64_t>(c_last) * C, a.T));
+  const int start = max(u.len, c_first * C), to = static_cast<int>(min(static_cast<int64_t>(c_last) * C, a.T));
   const int cols = min(VT, a.V - v0);
   auto clear = [&](void* out, bool f32, int64_t head, int64_t heads, int d, int c0, int width) {
-    for (int64_t i = threadIdx.x; i < int64_t{to - from} * width; i += BTHREADS) {
-      const int64_t at = ((u.b * a.T + from + i / width) * heads + head) * d + c0 + i % width;
+    for (int64_t i = threadIdx.x; i < int64_t{to - start} * width; i += BTHREADS) {
+      const int64_t at = ((u.b * a.T + start + i / width) * heads + head) * d + c0 + i % width;
       if (f32)
         static_cast<float*>(out)[at] = 0.f;
       else
@@ -898,6 +981,25 @@ __global__ __launch_bounds__(64) void k_la_column_ends(const float* part, int bl
   if (threadIdx.x == 0) out[h] = static_cast<float>(s);
 }
 
+// ------------------------------------------------------------------ rows for 16-byte loads
+// [B, T, heads, D] -> [B, T, heads, Dp] in neighbouring rows, zeros behind D: what rows of other widths, addresses or
+// distances go through first
+template <typename T>
+__global__ __launch_bounds__(256) void k_la_pack(const T* x, int64_t batch, int64_t token, int64_t head, int64_t tokens, int heads,
+                                                 int D, int Dp, int64_t groups, T* out) {
+  const int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x;
+  if (i >= groups) return;
+  const int per = Dp / 8, c = static_cast<int>(i % per) * 8;
+  int64_t r = i / per;
+  const int h = static_cast<int>(r % heads);
+  r /= heads;
+  const T* row = x + r / tokens * batch + r % tokens * token + h * head;
+  const Eight<T> e = load_eight<T>(row, c, D, false);
+#pragma unroll
+  for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
+    reinterpret_cast<u32x4*>(out + i * 8)[k] = reinterpret_cast<const u32x4*>(&e)[k];
+}
+
 // ------------------------------------------------------------------ one token
 // A wave takes 64 value columns of a head: lane l four of them, and of the keys every fourth part.  All of a lane's
 // state is asked for at once; the state is read and written where it stands, so that it may move on in place.
@@ -937,8 +1039,7 @@ __global__ __launch_bounds__(256) void k_la_step(Args a, int64_t waves) {
       }
     }
   }
-  const Sum d = log2_decay(g);
-  const float e = __builtin_amdgcn_exp2f(d.hi), decay = fmaf(e, d.lo * 0.69314718f, e);
+  const float decay = exp2_sum(log2_decay(g));
   f32x4 y{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < 8 * NB; ++n) {
@@ -964,16 +1065,26 @@ __global__ __launch_bounds__(256) void k_la_step(Args a, int64_t waves) {
     y[i] += __shfl_xor(y[i], 16, 64);
     y[i] += __shfl_xor(y[i], 32, 64);
   }
-  const float out[4] = {y[0] * a.scale, y[1] * a.scale, y[2] * a.scale, y[3] * a.scale};
-  if (lg == 0) store_four(static_cast<T*>(a.y) + bh * a.V + c, a.V - c, VEC, out);
+  if (lg) return;
+  T* out = static_cast<T*>(a.y) + bh * a.V + c;
+  if constexpr (VEC) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    y *= a.scale;
+    if (c < a.V) *reinterpret_cast<T4*>(out) = T4{from_f32<T>(y[0]), from_f32<T>(y[1]), from_f32<T>(y[2]), from_f32<T>(y[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < a.V) out[i] = from_f32<T>(y[i] * a.scale);
+  }
 }
 
 // ------------------------------------------------------------------ host
 int chunk_of(int dtype) { return dtype == LNG_BF16 ? Traits<bf16>::chunk : Traits<float>::chunk; }
 
+// Rows in 16-byte pieces, a chunk's within 32-bit offsets
 bool vector_rows(const void* p, int es, int64_t batch, int64_t token, int64_t head, int d) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && batch * es % 16 == 0 && token * es % 16 == 0 && head * es % 16 == 0 &&
-         d % 8 == 0;
+         d % 8 == 0 && token >= 0 && token * es < (int64_t{1} << 25);
 }
 
 // Blocks that a launch should have: a segment more costs the keys and values (the queries and dy) of all but one
@@ -992,6 +1103,7 @@ Args make_args(const lng_linear_attention& l, bool grad) {
   a.g = l.decay, a.gb = l.decay_batch, a.gt = l.decay_token;
   a.start = l.state, a.lengths = l.lengths, a.y = l.y, a.end = l.state_out, a.ckpt = l.checkpoints;
   a.yvec = a.V % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * es) == 0;
+  a.Kp = static_cast<int>(cdiv(a.K, 8)) * 8, a.Vp = static_cast<int>(cdiv(a.V, 8)) * 8;
   a.vts = static_cast<int>(cdiv(a.V, VT));
   a.chunks = static_cast<int>(cdiv(a.T, chunk_of(l.dtype)));
   const int64_t units = a.B * a.H * a.vts, want = grad ? BWD_BLOCKS : FWD_BLOCKS;
@@ -1003,16 +1115,21 @@ Args make_args(const lng_linear_attention& l, bool grad) {
 
 // floats of the workspace
 struct Space {
-  int64_t seg_state = 0, seg_decay = 0, dq = 0, dk = 0, dv = 0, dg = 0, cols = 0, total = 0;
+  int64_t seg_state = 0, seg_decay = 0, q = 0, k = 0, v = 0, dy = 0, dq = 0, dk = 0, dv = 0, dg = 0, cols = 0, total = 0;
   int64_t col_blocks = 0;
-  Space(const Args& a, bool grad, bool token_decay) {
+  Space(const Args& a, int es, bool grad, bool token_decay) {
     auto take = [&](int64_t n) {
       const int64_t at = total;
       total += cdiv(n, 16) * 16;
       return at;
     };
     if (a.segs > 1) seg_state = take(a.B * a.H * a.segs * a.K * a.V), seg_decay = take(a.B * a.H * a.segs);
+    auto rows_of = [&](int heads, int width) { return take(cdiv(a.B * a.T * heads * width * es, 4)); };
+    if (!a.qvec) q = rows_of(a.Hq, a.Kp);
+    if (!a.kvec) k = rows_of(a.Hk, a.Kp);
+    if (!a.vvec) v = rows_of(a.Hv, a.Vp);
     if (!grad) return;
+    if (a.V % 8) dy = rows_of(a.H, a.Vp);
     const int64_t rows = a.B * a.T, hv = int64_t{a.H} * a.vts;
     if (hv > a.Hq) dq = take(rows * hv * a.K);
     if (hv > a.Hk) dk = take(rows * hv * a.K);
@@ -1029,7 +1146,7 @@ int check_args(const char* what, const lng_linear_attention* l) {
     return fail(LNG_E_DTYPE, std::string(what) + ": fp32, bf16 or fp16 tensors");
   if (l->K < 1 || l->K > MAX_D || l->V < 1 || l->V > MAX_D)
     return fail(LNG_E_ARG, std::string(what) + ": heads of 1 to 128 keys and values");
-  if (l->H < 1 || l->H > (1 << 16) || l->Hq < 1 || l->Hk < 1 || l->Hv < 1 || l->H % l->Hq || l->H % l->Hk || l->H % l->Hv)
+  if (l->H < 1 || l->H > (1 << 14) || l->Hq < 1 || l->Hk < 1 || l->Hv < 1 || l->H % l->Hq || l->H % l->Hk || l->H % l->Hv)
     return fail(LNG_E_ARG, std::string(what) + ": the heads of q, k and v divide those of the decays");
   if (l->B < 0 || l->T < 0 || l->B > (int64_t{1} << 24) || l->T > (int64_t{1} << 30) ||
       l->B * l->T > (int64_t{1} << 40) / l->H / MAX_D)
@@ -1059,6 +1176,27 @@ template <bool BACK>
 int run_join(const Args& a, hipStream_t st) {
   k_la_join<BACK><<<static_cast<unsigned>(a.B * a.H * cdiv(int64_t{a.K} * a.V, 256)), 256, 0, st>>>(a);
   return check_launch("linear_attention");
+}
+
+// A tensor's rows into the workspace; from there on they are the tensor
+template <typename T>
+int pack(const void*& x, int64_t& batch, int64_t& token, int64_t& head, int64_t B, int64_t tokens, int heads, int D, int Dp,
+         float* to, hipStream_t st) {
+  const int64_t groups = B * tokens * heads * (Dp / 8);
+  k_la_pack<T><<<static_cast<unsigned>(cdiv(groups, 256)), 256, 0, st>>>(static_cast<const T*>(x), batch, token, head, tokens,
+                                                                       heads, D, Dp, groups, reinterpret_cast<T*>(to));
+  x = to, head = Dp, token = int64_t{heads} * Dp, batch = tokens * token;
+  return check_launch("linear_attention");
+}
+template <typename T>
+int pack_inputs(Args& a, const Space& s, float* ws, hipStream_t st) {
+  if (!a.qvec)
+    if (int rc = pack<T>(a.q, a.qb, a.qt, a.qh, a.B, a.T, a.Hq, a.K, a.Kp, ws + s.q, st)) return rc;
+  if (!a.kvec)
+    if (int rc = pack<T>(a.k, a.kb, a.kt, a.kh, a.B, a.T, a.Hk, a.K, a.Kp, ws + s.k, st)) return rc;
+  if (!a.vvec)
+    if (int rc = pack<T>(a.v, a.vb, a.vt, a.vh, a.B, a.T, a.Hv, a.V, a.Vp, ws + s.v, st)) return rc;
+  return LNG_OK;
 }
 
 template <typename T, int DK, int NW>
@@ -1125,7 +1263,7 @@ size_t lng_linear_attention_grad_size(void) { return sizeof(lng_linear_attention
 size_t lng_linear_attention_workspace_bytes(const lng_linear_attention* args, int grad) {
   if (check_args("linear_attention_workspace_bytes", args) || args->B == 0 || args->T == 0) return 0;
   const Args a = make_args(*args, grad != 0);
-  return static_cast<size_t>(Space(a, grad != 0, args->token_decay != 0).total) * 4;
+  return static_cast<size_t>(Space(a, dtype_size(args->dtype), grad != 0, args->token_decay != 0).total) * 4;
 }
 
 int64_t lng_linear_attention_checkpoints(int64_t B, int64_t T, int32_t H, int32_t K, int32_t V, int dtype) {
@@ -1139,7 +1277,7 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
   if (args->B == 0 || args->T == 0) return LNG_OK;
   if (!args->y) return fail(LNG_E_ARG, "linear_attention: null pointer");
   Args a = make_args(*args, false);
-  const Space s(a, false, args->token_decay != 0);
+  const Space s(a, dtype_size(args->dtype), false, args->token_decay != 0);
   if (s.total && (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 ||
                   reinterpret_cast<uintptr_t>(workspace) % 64))
     return fail(LNG_E_ARG, "linear_attention: the workspace is too small or not 64-byte aligned");
@@ -1148,6 +1286,7 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
   float* const ws = static_cast<float*>(workspace);
   a.seg_state = ws + s.seg_state, a.seg_decay = ws + s.seg_decay;
   return with_type(args->dtype, [&](auto t) {
+    if (int rc = pack_inputs<decltype(t)>(a, s, ws, as_stream(stream))) return rc;
     return with_keys(a.K, [&](auto dk) {
       using T = decltype(t);
       constexpr int DK = decltype(dk)::value;
@@ -1167,18 +1306,20 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
     return fail(LNG_E_ARG, "linear_attention_grad: null pointer");
   Args a = make_args(*args, true);
   const bool token = args->token_decay != 0;
-  const Space s(a, true, token);
+  const int es = dtype_size(args->dtype);
+  const Space s(a, es, true, token);
   if (s.total && (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 ||
                   reinterpret_cast<uintptr_t>(workspace) % 64))
     return fail(LNG_E_ARG, "linear_attention_grad: the workspace is too small or not 64-byte aligned");
   const int64_t rows = a.B * a.T, hv = int64_t{a.H} * a.vts;
   if (int rc = check_threads(what, a.B * a.H * std::max<int64_t>(a.vts * a.segs, cdiv(int64_t{a.K} * a.V, 256)), 256))
     return rc;
+  a.dy = g.dy, a.yb = g.dy_batch, a.yt = g.dy_token, a.yh = g.dy_head;
+  if (a.V % 8 == 0 && !vector_rows(a.dy, es, a.yb, a.yt, a.yh, a.V))
+    return fail(LNG_E_ARG, "linear_attention_grad: rows of dy in 16-byte pieces, less than 2^25 bytes apart");
   if (int rc = check_threads(what, cdiv(rows * a.H * std::max(a.K, a.V), 256), 256)) return rc;
   float* const ws = static_cast<float*>(workspace);
   a.seg_state = ws + s.seg_state, a.seg_decay = ws + s.seg_decay;
-  a.dy = g.dy, a.yb = g.dy_batch, a.yt = g.dy_token, a.yh = g.dy_head;
-  a.yvec = vector_rows(a.dy, dtype_size(args->dtype), a.yb, a.yt, a.yh, a.V);
   a.dend = g.dstate_out, a.dstart = g.dstate;
   a.dq32 = hv > a.Hq, a.dk32 = hv > a.Hk, a.dv32 = a.H > a.Hv;
   a.dq = a.dq32 ? ws + s.dq : g.dq, a.dk = a.dk32 ? ws + s.dk : g.dk, a.dv = a.dv32 ? ws + s.dv : g.dv;
@@ -1187,6 +1328,9 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
   hipStream_t st = as_stream(stream);
   return with_type(args->dtype, [&](auto t) {
     using T = decltype(t);
+    if (int rc = pack_inputs<T>(a, s, ws, st)) return rc;
+    if (a.V % 8)
+      if (int rc = pack<T>(a.dy, a.yb, a.yt, a.yh, a.B, a.T, a.H, a.V, a.Vp, ws + s.dy, st)) return rc;
     if (int rc = with_keys(a.K, [&](auto dk) { return run_bwd<T, decltype(dk)::value>(a, st); })) return rc;
     if (a.dq32)
       if (int rc = run_shared<T>(ws + s.dq, rows, a.Hq, static_cast<int>(hv / a.Hq), a.K, static_cast<T*>(g.dq), st)) return rc;

@@ -1893,7 +1893,10 @@ def linear_attention_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpo
             ds.zero_() if dstate is None else ds.copy_(dstate)
         return dq, dk, dv, dg, ds
     dyc, dsc = _last_contiguous(dy), _whole(dstate)
-    at = dyc.stride()
+    at, size = dyc.stride(), dyc.element_size()
+    if a.V % 8 == 0 and (dyc.data_ptr() % 16 or any(n * size % 16 for n in at[:3]) or at[1] * size >= 1 << 25):
+        dyc = _c(dyc.contiguous())                       # read in 16-byte pieces
+        at = dyc.stride()
     g = _lib.LinearAttentionGrad(dyc.data_ptr(), *at[:3], _ptr(dsc), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                  dg.data_ptr(), _ptr(ds))
     ws = _linear_workspace(a, True, dev)
