@@ -151,6 +151,38 @@ __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB
       if (i + j < LIM) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
 
+// The same for n results that do not wait for each other: acc[k] += a(k) . b(k)
+template <int LIM, int NA, int NB, int N>
+__device__ __forceinline__ void mma_n(f32x4 (&acc)[N], const Frag<NA> (&a)[N], const Frag<NB>& b) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j < LIM)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k].p[i], b.p[j], acc[k], 0, 0, 0);
+}
+template <int LIM, int NA, int NB, int N>
+__device__ __forceinline__ void mma_n(f32x4 (&acc)[N], const Frag<NA>& a, const Frag<NB> (&b)[N]) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j < LIM)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b[k].p[j], acc[k], 0, 0, 0);
+}
+template <int LIM, int NA, int NB, int N>
+__device__ __forceinline__ void mma_n(f32x4 (&acc)[N], const Frag<NA> (&a)[N], const Frag<NB> (&b)[N]) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j < LIM)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k].p[i], b[k].p[j], acc[k], 0, 0, 0);
+}
+
 // Lane l of a 16 x 16 x 32 product: row (column) l % 16 of an operand, and of its 32 products' index the values
 // 4 g + 0..3 and 16 + 4 g + 0..3 with g = l / 16.  (Any order will do that both operands share; this one is that of
 // two stacked result tiles, whose rows 4 g + 0..3 a lane holds, so that results are operands as they are.)
@@ -194,7 +226,7 @@ __device__ __forceinline__ Frag<N> by_col(const bf16* s, int plane, int r0, int 
 // A lower triangle of tiles: (it, jt) with jt <= it
 __device__ __forceinline__ constexpr int tri(int it, int jt) { return (it * (it + 1) / 2 + jt) * TILE; }
 template <int N>
-__device__ __forceinline__ Frag<N> tri_by_row(const bf16* s, int plane, int it, int st) {  // columns 32 st ..
+__device__ __forceinline__ Frag<N> tri_by_row(const bf16* s, int plane, int it, int st) {  // columns 32 st ..; 2 st <= it
   Frag<N> f;
 #pragma unroll
   for (int p = 0; p < N; ++p) {
@@ -204,14 +236,12 @@ __device__ __forceinline__ Frag<N> tri_by_row(const bf16* s, int plane, int it, 
   return f;
 }
 template <int N>
-__device__ __forceinline__ Frag<N> tri_by_col(const bf16* s, int plane, int st, int jt, int tiles) {  // rows 32 st ..
+__device__ __forceinline__ Frag<N> tri_by_col(const bf16* s, int plane, int st, int jt) {  // rows 32 st ..; jt <= 2 st + 1
   Frag<N> f;
 #pragma unroll
   for (int p = 0; p < N; ++p) {
     const bf16* at = s + p * plane + col_place();
-    // nothing has been written to tiles that hold no token
-    f.p[p] = join(2 * st >= jt ? piece_tr(at + tri(2 * st, jt)) : bf16x4{},
-                  2 * st + 1 < tiles ? piece_tr(at + tri(2 * st + 1, jt)) : bf16x4{});
+    f.p[p] = join(2 * st >= jt ? piece_tr(at + tri(2 * st, jt)) : bf16x4{}, piece_tr(at + tri(2 * st + 1, jt)));
   }
   return f;
 }
@@ -241,15 +271,6 @@ __device__ __forceinline__ void put_four(bf16* tile, int plane, const float (&x)
   for (int p = 0; p < N; ++p)
     *reinterpret_cast<bf16x4*>(tile + p * plane + row_place()) = __builtin_shufflevector(f.p[p], f.p[p], 0, 1, 2, 3);
 }
-// one value, by its row and column
-template <int N, int W>
-__device__ __forceinline__ float at_cell(const bf16* s, int plane, int r, int c) {
-  const int at = ((r / 16) * (W / 16) + c / 16) * TILE + (r & 15) * 16 + ((((c >> 2) ^ (r >> 2)) & 3) << 2) + (c & 3);
-  float x = 0.f;
-  for (int p = N - 1; p >= 0; --p) x += static_cast<float>(s[at + p * plane]);
-  return x;
-}
-
 // ------------------------------------------------------------------ rows from memory to LDS
 // Eight neighbouring values of a row as they are in memory, element by element where 16-byte loads do not do
 template <typename T>
@@ -365,9 +386,9 @@ constexpr uint32_t NOWHERE = 0x7ffffff0u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t from(const void* base) { return dev_buf(base, NOWHERE); }
 
 // four neighbouring values of a row of an output, as far as it goes (left > 0 in some lane at most)
-template <typename T>
-__device__ __forceinline__ void store_four(__amdgpu_buffer_rsrc_t rs, uint32_t off, int left, bool vec, const f32x4& x) {
-  if (vec) {  // whole pieces of four
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void store_four(__amdgpu_buffer_rsrc_t rs, uint32_t off, int left, const f32x4& x) {
+  if constexpr (VECTOR) {  // whole pieces of four
     const uint32_t at = left > 0 ? off : NOWHERE;
     if constexpr (sizeof(T) == 4) {
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rs, at, 0, 0);
@@ -437,8 +458,10 @@ __device__ __forceinline__ void update_state(f32x4 (&s)[TK], const bf16* sX, int
       for (int i = 0; i < 4; i += 2)
         put2(fy, 4 * h + i, value(y[st], 4 * h + i) * fr[i], value(y[st], 4 * h + i + 1) * fr[i + 1]);
     }
+    Frag<NX> fx[TK];
 #pragma unroll
-    for (int t = 0; t < TK; ++t) mma<3>(s[t], by_col<NX, W>(sX, xplane, 32 * st, 16 * t), fy);
+    for (int t = 0; t < TK; ++t) fx[t] = by_col<NX, W>(sX, xplane, 32 * st, 16 * t);
+    mma_n<3>(s, fx, fy);
   }
 }
 // The state as the operand whose index runs over keys
@@ -465,14 +488,15 @@ struct FwdLds {
 // A block of NW waves takes a head's 16 NW value columns over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
 template <typename T, int DK, int NW, bool ENDS>
-__global__ __launch_bounds__(64 * NW, (ENDS ? 4 : DK <= 64 ? 3 : 2) - (NW == 2 && DK > 32)) void k_la_fwd(Args a) {
+__global__ __launch_bounds__(64 * NW, (DK <= 64 ? (ENDS ? 4 : 3) : (ENDS ? 3 : 2)) - (NW == 2 && DK > 32)) void k_la_fwd(Args a) {
   using L = FwdLds<T, DK, NW>;
   using Tr = Traits<T>;
   constexpr int C = L::C, W = L::W, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, THREADS = 64 * NW;
   constexpr int KP = C * DK, VP = C * W, PP = tri(C / 16, 0);  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar arithmetic
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Unit u = unit_of(a, ENDS ? a.segs - 1 : a.segs, 0);
   const int c_first = u.seg * a.seg_chunks, c_last = min(c_first + a.seg_chunks, a.chunks);
   const int v0 = u.vt * VT, vc = v0 + 16 * w;  // the block's and the wave's first column
@@ -498,15 +522,18 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? 4 : DK <= 64 ? 3 : 2) - (NW == 2 &
   Stage<T, C, W, THREADS> rv;
   // one wave's: the next chunk's log decays, asked for a chunk before the rows are, so that their sums wait for nothing
   float rg = 0.f;
+  g += int64_t{c_first} * C * a.gt, q += int64_t{c_first} * C * a.qt;
+  k += int64_t{c_first} * C * a.kt, v += int64_t{c_first} * C * a.vt;
   auto fetch_decay = [&](int c) {
-    if (w == NW - 1 && c < c_end) rg = load_decay(g + int64_t{c} * C * a.gt, a.gt, min(C, u.len - c * C));
+    if (w == NW - 1 && c < c_end) rg = load_decay(g, a.gt, min(C, u.len - c * C));
+    g += C * a.gt;
   };
   auto fetch = [&](int c) {
-    const int64_t t0 = int64_t{c} * C;
     const int n = min(C, u.len - c * C);
-    if (!ENDS) rq.load(q + t0 * a.qt, static_cast<uint32_t>(a.qt * sizeof(T)), n, 0, a.Kp);
-    rk.load(k + t0 * a.kt, static_cast<uint32_t>(a.kt * sizeof(T)), n, 0, a.Kp);
-    rv.load(v + t0 * a.vt, static_cast<uint32_t>(a.vt * sizeof(T)), n, v0, a.Vp);
+    if (!ENDS) rq.load(q, static_cast<uint32_t>(a.qt) * sizeof(T), n, 0, a.Kp);
+    rk.load(k, static_cast<uint32_t>(a.kt) * sizeof(T), n, 0, a.Kp);
+    rv.load(v, static_cast<uint32_t>(a.vt) * sizeof(T), n, v0, a.Vp);
+    q += C * a.qt, k += C * a.kt, v += C * a.vt;
   };
   if (c_first < c_end) {
     fetch_decay(c_first);
@@ -527,26 +554,45 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? 4 : DK <= 64 ? 3 : 2) - (NW == 2 &
     if (c + 1 < c_end) fetch(c + 1);
     if (!ENDS && a.ckpt) store_state(s, a.ckpt + (bh * a.chunks + c) * KV, a.K, a.V, vc);
 
-    const int tiles = (n + 15) / 16;
     if (!ENDS) {
-      // the scores' tiles on and below the diagonal, transposed: column i, rows j
-      for (int idx = w; idx < tiles * (tiles + 1) / 2; idx += NW) {
-        const int it = idx >= 6 ? 3 : idx >= 3 ? 2 : idx >= 1 ? 1 : 0, jt = idx - it * (it + 1) / 2;
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+      // the scores' tiles on and below the diagonal, transposed: column i, rows j.  A wave's tiles do not wait for each
+      // other; one too many is done twice.
+      auto scores = [&](auto count, int first, int all) {
+        constexpr int N = decltype(count)::value;
+        f32x4 acc[N];
+        int it[N], idx[N];
 #pragma unroll
-        for (int st = 0; st < DK / 32; ++st)
-          mma<3>(acc, by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st), by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
-        const int i = 16 * it + li, j0 = 16 * jt + 4 * lg;
-        const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
-        const float ih = d.hi[i], il = d.lo[i];
-        float p[4];
+        for (int k = 0; k < N; ++k) {
+          idx[k] = first + k * NW < all ? first + k * NW : first;
+          it[k] = idx[k] >= 6 ? 3 : idx[k] >= 3 ? 2 : idx[k] >= 1 ? 1 : 0;
+          acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = acc[r] * (exp2_gap(ih, il, jh[r], jl[r]) * a.scale);
-        if (it == jt)
+        for (int st = 0; st < DK / 32; ++st) {
+          Frag<NP> fk[N], fq[N];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[r] = 4 * lg + r <= li ? p[r] : 0.f;
-        put_four<PR>(lds.p[0] + idx * TILE, PP, p);
-      }
+          for (int k = 0; k < N; ++k) {
+            fk[k] = by_row<NP, DK>(lds.k[0], KP, 16 * (idx[k] - it[k] * (it[k] + 1) / 2), 32 * st);
+            fq[k] = by_row<NP, DK>(lds.q[0], KP, 16 * it[k], 32 * st);
+          }
+          mma_n<3>(acc, fk, fq);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int jt = idx[k] - it[k] * (it[k] + 1) / 2, i = 16 * it[k] + li, j0 = 16 * jt + 4 * lg;
+          const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
+          const float ih = d.hi[i], il = d.lo[i];
+          float p[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[r] = acc[k][r] * (exp2_gap(ih, il, jh[r], jl[r]) * a.scale);
+            p[r] = j0 + r <= i ? p[r] : 0.f;
+          }
+          put_four<PR>(lds.p[0] + idx[k] * TILE, PP, p);
+        }
+      };
+      constexpr int ALL = TI * (TI + 1) / 2, EACH = (ALL + NW - 1) / NW;
+      scores(std::integral_constant<int, EACH>{}, w < ALL ? w : 0, ALL);
       __syncthreads();
     }
     if (w == NW - 1 && c + 1 < c_end) decays(lds.d[(c + 1) & 1], g_next, a.scale);
@@ -559,35 +605,77 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? 4 : DK <= 64 ? 3 : 2) - (NW == 2 &
 #pragma unroll
       for (int i = 0; i < 8; ++i) odd = fmaf(static_cast<float>(fv[st].p[0][i]), 0.f, odd);
     }
+    // A weight of zero would carry an infinity or NaN among the values to the tokens before it.  It counts as zero in the
+    // products, and what follows it in its column becomes NaN.
+    int bad = C;  // the first such token of column l % 16
+    const bool careful = __ballot(!(odd == 0.f)) != 0ull;
+    if (careful) {
+#pragma unroll
+      for (int st = 0; st < C / 32; ++st)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = static_cast<float>(fv[st].p[0][i]);
+          if (!(fabsf(f) < INFINITY)) {
+            bad = min(bad, 32 * st + (i < 4 ? 0 : 16) + 4 * lg + (i & 3));
+#pragma unroll
+            for (int p = 0; p < NP; ++p) fv[st].p[p][i] = static_cast<bf16>(0.f);
+          }
+        }
+      bad = min(bad, __shfl_xor(bad, 16, 64));
+      bad = min(bad, __shfl_xor(bad, 32, 64));
+    }
     if (!ENDS) {
-      // an infinity or NaN among the values may not reach the tokens before it, with a weight of zero
-      const bool careful = __ballot(!(odd == 0.f)) != 0ull;
       Frag<PR> fs[TK / 2];
       state_frags(s, fs);
       const __amdgpu_buffer_rsrc_t yc = from(y + int64_t{t0} * yrow);
+      const int col = vc + 4 * lg;
+      auto outputs = [&](auto count, int first) {
+        constexpr int N = decltype(count)::value;
+        f32x4 acc[N];
+        Frag<NP> fq[N];
 #pragma unroll
-      for (int it = 0; it < TI; ++it) {
-        if (it >= tiles) break;
-        const int i = 16 * it + li;
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < N; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < DK / 32; ++st) mma<PR>(acc, fs[st], by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
-        acc *= d.from[i];
-        if (!careful) {
+        for (int st = 0; st < DK / 32; ++st) {
 #pragma unroll
-          for (int st = 0; st <= it / 2; ++st) mma<PR>(acc, fv[st], tri_by_row<PR>(lds.p[0], PP, it, st));
+          for (int k = 0; k < N; ++k) fq[k] = by_row<NP, DK>(lds.q[0], KP, 16 * (first + k), 32 * st);
+          mma_n<PR>(acc, fs[st], fq);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] *= d.from[16 * (first + k) + li];
+#pragma unroll
+        for (int st = 0; st < C / 32; ++st)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (2 * st <= first + k) mma<PR>(acc[k], fv[st], tri_by_row<PR>(lds.p[0], PP, first + k, st));
+        if (careful)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int from_here = __shfl(bad, 4 * lg + r, 64);
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k][r] = 16 * (first + k) + li >= from_here ? NAN : acc[k][r];
+          }
+        if (a.yvec) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const int i = 16 * (first + k) + li;
+            store_four<T, true>(yc, static_cast<uint32_t>(i * yrow + col) * sizeof(T), i < n ? a.V - col : 0, acc[k]);
+          }
         } else {
-          for (int j = 0; j <= i; ++j) {
-            const float p = at_cell<PR, 16>(lds.p[0] + tri(it, j / 16), PP, li, j & 15);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r] = fmaf(p, at_cell<NP, W>(lds.v[0], VP, j, 16 * w + 4 * lg + r), acc[r]);
+          for (int k = 0; k < N; ++k) {
+            const int i = 16 * (first + k) + li;
+            store_four<T, false>(yc, static_cast<uint32_t>(i * yrow + col) * sizeof(T), i < n ? a.V - col : 0, acc[k]);
           }
         }
-        const int col = vc + 4 * lg;
-        store_four<T>(yc, static_cast<uint32_t>(i * yrow + col) * sizeof(T), i < n ? a.V - col : 0, a.yvec, acc);
-      }
+      };
+      outputs(std::integral_constant<int, TI>{}, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
     update_state<C, TK, DK, NP>(s, lds.k[0], KP, fv, d.left, d.whole);
+    if (careful && bad < C)
+#pragma unroll
+      for (int t = 0; t < TK; ++t) s[t] = f32x4{NAN, NAN, NAN, NAN};
     if (ENDS && threadIdx.x == 0) seg += d.total;
     __syncthreads();
   }
@@ -675,14 +763,15 @@ __device__ __forceinline__ float col_sum(float v) {
 // What the columns v0 .. v0 + 63 of the values add to the gradients; ENDS: only what the segment adds to the state's
 // gradient.
 template <typename T, int DK, bool ENDS>
-__global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bwd(Args a) {
+__global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1)) void k_la_bwd(Args a) {
   using L = BwdLds<T, DK>;
   using Tr = Traits<T>;
   constexpr int C = L::C, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, NR = L::NR;
   constexpr int KP = C * DK, VP = C * VT, PP = tri(C / 16, 0), RP = VT * DK;  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar arithmetic
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Unit u = unit_of(a, ENDS ? a.segs - 1 : a.segs, ENDS ? 1 : 0);
   const int c_first = u.seg * a.seg_chunks, c_last = min(c_first + a.seg_chunks, a.chunks);
   const int v0 = u.vt * VT, vc = v0 + 16 * w;
@@ -707,18 +796,21 @@ __global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bw
   Stage<T, C, DK, BTHREADS> rq, rk;
   Stage<T, C, VT, BTHREADS> rv, ro;
   float rg = 0.f;  // one wave's: the log decays of the chunk before, asked for a chunk ahead of its rows
+  g += int64_t{c_end - 1} * C * a.gt, q += int64_t{c_end - 1} * C * a.qt, dy += int64_t{c_end - 1} * C * a.yt;
+  k += int64_t{c_end - 1} * C * a.kt, v += int64_t{c_end - 1} * C * a.vt;
   auto fetch_decay = [&](int c) {
-    if (w == BW - 1 && c >= c_first) rg = load_decay(g + int64_t{c} * C * a.gt, a.gt, min(C, u.len - c * C));
+    if (w == BW - 1 && c >= c_first) rg = load_decay(g, a.gt, min(C, u.len - c * C));
+    g -= C * a.gt;
   };
   auto fetch = [&](int c) {
-    const int64_t t0 = int64_t{c} * C;
     const int n = min(C, u.len - c * C);
-    rq.load(q + t0 * a.qt, static_cast<uint32_t>(a.qt * sizeof(T)), n, 0, a.Kp);
-    ro.load(dy + t0 * a.yt, static_cast<uint32_t>(a.yt * sizeof(T)), n, v0, a.Vp);
+    rq.load(q, static_cast<uint32_t>(a.qt) * sizeof(T), n, 0, a.Kp);
+    ro.load(dy, static_cast<uint32_t>(a.yt) * sizeof(T), n, v0, a.Vp);
     if (!ENDS) {
-      rk.load(k + t0 * a.kt, static_cast<uint32_t>(a.kt * sizeof(T)), n, 0, a.Kp);
-      rv.load(v + t0 * a.vt, static_cast<uint32_t>(a.vt * sizeof(T)), n, v0, a.Vp);
+      rk.load(k, static_cast<uint32_t>(a.kt) * sizeof(T), n, 0, a.Kp);
+      rv.load(v, static_cast<uint32_t>(a.vt) * sizeof(T), n, v0, a.Vp);
     }
+    q -= C * a.qt, dy -= C * a.yt, k -= C * a.kt, v -= C * a.vt;
   };
   if (c_first < c_end) {
     fetch_decay(c_end - 1);
@@ -733,14 +825,17 @@ __global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bw
   // a lane's four values of a token's output: in the type, or in fp32 to be summed with others
   auto emit = [&](void* out, bool f32, int64_t first, int row, int i, int col, int left, bool vec, const f32x4& x) {
     const uint32_t at = static_cast<uint32_t>(i * row + col);
-    if (f32)
-      store_four<float>(from(static_cast<float*>(out) + first * row), at * 4, left, vec, x);
-    else
-      store_four<T>(from(static_cast<T*>(out) + first * row), at * sizeof(T), left, vec, x);
+    if (f32) {
+      const __amdgpu_buffer_rsrc_t rs = from(static_cast<float*>(out) + first * row);
+      vec ? store_four<float, true>(rs, at * 4, left, x) : store_four<float, false>(rs, at * 4, left, x);
+    } else {
+      const __amdgpu_buffer_rsrc_t rs = from(static_cast<T*>(out) + first * row);
+      vec ? store_four<T, true>(rs, at * sizeof(T), left, x) : store_four<T, false>(rs, at * sizeof(T), left, x);
+    }
   };
   double seg = 0.;
   for (int c = c_end - 1; c >= c_first; --c) {
-    const int t0 = c * C, n = min(C, u.len - t0), tiles = (n + 15) / 16;
+    const int t0 = c * C, n = min(C, u.len - t0);
     const int64_t token = u.b * a.T + t0;
     const Decays<C>& d = lds.d[c & 1];
     rq.store(lds.q[0], KP);
@@ -760,38 +855,59 @@ __global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bw
     if (c > c_first) fetch(c - 1);
 
     if (!ENDS) {
-      for (int idx = w; idx < tiles * (tiles + 1) / 2; idx += BW) {
-        const int it = idx >= 6 ? 3 : idx >= 3 ? 2 : idx >= 1 ? 1 : 0, jt = idx - it * (it + 1) / 2;
-        f32x4 qk{0.f, 0.f, 0.f, 0.f}, ov{0.f, 0.f, 0.f, 0.f};
+      auto scores = [&](auto count, int first, int all) {
+        constexpr int N = decltype(count)::value;
+        f32x4 qk[N], ov[N];
+        int it[N], jt[N], idx[N];
 #pragma unroll
-        for (int st = 0; st < DK / 32; ++st)
-          mma<3>(qk, by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st), by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
-#pragma unroll
-        for (int st = 0; st < VT / 32; ++st)
-          mma<3>(ov, by_row<NP, VT>(lds.v[0], VP, 16 * jt, 32 * st), by_row<NP, VT>(lds.o[0], VP, 16 * it, 32 * st));
-        const int i = 16 * it + li, j0 = 16 * jt + 4 * lg;
-        const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
-        const float ih = d.hi[i], il = d.lo[i];
-        float p[4], x[4], pair[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float dec = exp2_gap(ih, il, jh[r], jl[r]) * a.scale;
-          p[r] = qk[r] * dec, x[r] = ov[r] * dec, pair[r] = p[r] * ov[r];
+        for (int k = 0; k < N; ++k) {
+          idx[k] = first + k * BW < all ? first + k * BW : first;
+          it[k] = idx[k] >= 6 ? 3 : idx[k] >= 3 ? 2 : idx[k] >= 1 ? 1 : 0, jt[k] = idx[k] - it[k] * (it[k] + 1) / 2;
+          qk[k] = ov[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        if (it == jt)
+        Frag<NP> fj[N], fi[N];
+#pragma unroll
+        for (int st = 0; st < DK / 32; ++st) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            fj[k] = by_row<NP, DK>(lds.k[0], KP, 16 * jt[k], 32 * st);
+            fi[k] = by_row<NP, DK>(lds.q[0], KP, 16 * it[k], 32 * st);
+          }
+          mma_n<3>(qk, fj, fi);
+        }
+#pragma unroll
+        for (int st = 0; st < VT / 32; ++st) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            fj[k] = by_row<NP, VT>(lds.v[0], VP, 16 * jt[k], 32 * st);
+            fi[k] = by_row<NP, VT>(lds.o[0], VP, 16 * it[k], 32 * st);
+          }
+          mma_n<3>(ov, fj, fi);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int i = 16 * it[k] + li, j0 = 16 * jt[k] + 4 * lg;
+          const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
+          const float ih = d.hi[i], il = d.lo[i];
+          float p[4], x[4], pair[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const bool on = 4 * lg + r <= li;
-            p[r] = on ? p[r] : 0.f, x[r] = on ? x[r] : 0.f, pair[r] = 4 * lg + r < li ? pair[r] : 0.f;
+            const float dec = exp2_gap(ih, il, jh[r], jl[r]) * a.scale;
+            p[r] = j0 + r <= i ? qk[k][r] * dec : 0.f;
+            x[r] = j0 + r <= i ? ov[k][r] * dec : 0.f;
+            pair[r] = j0 + r < i ? p[r] * ov[k][r] : 0.f;
           }
-        put_four<PR>(lds.p[0] + idx * TILE, PP, p);
-        put_four<PR>(lds.a[0] + idx * TILE, PP, x);
-        const float rows = col_sum((pair[0] + pair[1]) + (pair[2] + pair[3]));
-        if (lg == 0) lds.row[jt][i] = rows;
+          put_four<PR>(lds.p[0] + idx[k] * TILE, PP, p);
+          put_four<PR>(lds.a[0] + idx[k] * TILE, PP, x);
+          const float rows = col_sum((pair[0] + pair[1]) + (pair[2] + pair[3]));
+          if (lg == 0) lds.row[jt[k]][i] = rows;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) pair[r] = row_sum(pair[r]);
-        if (li == 0) *reinterpret_cast<f32x4*>(&lds.col[it][j0]) = f32x4{pair[0], pair[1], pair[2], pair[3]};
-      }
+          for (int r = 0; r < 4; ++r) pair[r] = row_sum(pair[r]);
+          if (li == 0) *reinterpret_cast<f32x4*>(&lds.col[it[k]][j0]) = f32x4{pair[0], pair[1], pair[2], pair[3]};
+        }
+      };
+      constexpr int ALL = TI * (TI + 1) / 2, EACH = (ALL + BW - 1) / BW;
+      scores(std::integral_constant<int, EACH>{}, w < ALL ? w : 0, ALL);
       __syncthreads();
     }
     if (w == BW - 1 && c > c_first) decays(lds.d[(c - 1) & 1], g_next, a.scale);
@@ -831,39 +947,74 @@ __global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bw
           }
         }
         if (part == 0) sr += dot;
+        const int key = 16 * kt + 4 * lg;
+        auto tokens = [&](auto count, int first) {  // the tiles of tokens from `first` on
+          constexpr int N = decltype(count)::value;
+          f32x4 acc[N];
+          Frag<NP> fi[N];
 #pragma unroll
-        for (int ii = 0; ii < TI; ++ii) {
-          if (ii / IT != part || ii >= tiles) continue;
-          const int it = ii, i = 16 * it + li, key = 16 * kt + 4 * lg;
-          f32x4 acc{0.f, 0.f, 0.f, 0.f};
-          float x[4], sum = 0.f;
+          for (int m = 0; m < N; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int st = 0; st < VT / 32; ++st) mma<3>(acc, fs[st], by_row<NP, VT>(lds.o[0], VP, 16 * it, 32 * st));
-          acc *= d.from[i];
-          four<NP>(lds.q[0] + (it * TK + kt) * TILE, KP, x);
+          for (int st = 0; st < VT / 32; ++st) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[r], sum);
-          sum = col_sum(sum);
-          if (lg == 0) lds.qs[kt][i] = sum;
-#pragma unroll
-          for (int st = 0; st <= it / 2; ++st)
-            mma<PR>(acc, by_col<NP, DK>(lds.k[0], KP, 32 * st, 16 * kt), tri_by_row<PR>(lds.a[0], PP, it, st));
-          emit(a.dq, a.dq32, token, qrow, i, qcol + key, i < n ? a.K - key : 0, k4, acc);
-          acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int st = 0; st < VT / 32; ++st) mma<NR>(acc, fr[st], by_row<NP, VT>(lds.v[0], VP, 16 * it, 32 * st));
-          acc *= d.left[i];
-#pragma unroll
-          for (int st = it / 2; st < C / 32; ++st) {
-            if (2 * st >= tiles) break;  // tiles of no tokens hold nothing
-            mma<PR>(acc, by_col<NP, DK>(lds.q[0], KP, 32 * st, 16 * kt), tri_by_col<PR>(lds.a[0], PP, st, it, tiles));
+            for (int m = 0; m < N; ++m) fi[m] = by_row<NP, VT>(lds.o[0], VP, 16 * (first + m), 32 * st);
+            mma_n<3>(acc, fs[st], fi);
           }
-          emit(a.dk, a.dk32, token, krow, i, kcol + key, i < n ? a.K - key : 0, k4, acc);
-        }
+#pragma unroll
+          for (int m = 0; m < N; ++m) {
+            const int i = 16 * (first + m) + li;
+            float x[4], sum = 0.f;
+            acc[m] *= d.from[i];
+            four<NP>(lds.q[0] + ((first + m) * TK + kt) * TILE, KP, x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[m][r], sum);
+            sum = col_sum(sum);
+            if (lg == 0) lds.qs[kt][i] = sum;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int st = 0; st < C / 32; ++st) {
+            if (2 * st > first + N - 1) continue;
+            const Frag<NP> fk = by_col<NP, DK>(lds.k[0], KP, 32 * st, 16 * kt);
+#pragma unroll
+            for (int m = 0; m < N; ++m)
+              if (2 * st <= first + m) mma<PR>(acc[m], fk, tri_by_row<PR>(lds.a[0], PP, first + m, st));
+          }
+#pragma unroll
+          for (int m = 0; m < N; ++m) {
+            const int i = 16 * (first + m) + li;
+            emit(a.dq, a.dq32, token, qrow, i, qcol + key, i < n ? a.K - key : 0, k4, acc[m]);
+            acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int st = 0; st < VT / 32; ++st) {
+#pragma unroll
+            for (int m = 0; m < N; ++m) fi[m] = by_row<NP, VT>(lds.v[0], VP, 16 * (first + m), 32 * st);
+            mma_n<NR>(acc, fr[st], fi);
+          }
+#pragma unroll
+          for (int m = 0; m < N; ++m) acc[m] *= d.left[16 * (first + m) + li];
+#pragma unroll
+          for (int st = 0; st < C / 32; ++st) {
+            const Frag<NP> fq = by_col<NP, DK>(lds.q[0], KP, 32 * st, 16 * kt);
+#pragma unroll
+            for (int m = 0; m < N; ++m)
+              if (2 * st + 1 >= first + m)
+                mma<PR>(acc[m], fq, tri_by_col<PR>(lds.a[0], PP, st, first + m));
+          }
+#pragma unroll
+          for (int m = 0; m < N; ++m) {
+            const int i = 16 * (first + m) + li;
+            emit(a.dk, a.dk32, token, krow, i, kcol + key, i < n ? a.K - key : 0, k4, acc[m]);
+          }
+        };
+        SHARE == 1 ? tokens(std::integral_constant<int, IT>{}, 0) : tokens(std::integral_constant<int, IT>{}, part * IT);
       }
       sr = wave_sum(sr);
       if (lane == 0) lds.sr[w] = sr;
     }
+    __builtin_amdgcn_sched_barrier(0);
     Frag<NP> fo[C / 32];  // dy: this wave's columns
 #pragma unroll
     for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP, VT>(lds.o[0], VP, 32 * st, 16 * w);
@@ -871,29 +1022,45 @@ __global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bw
       // dv: this wave's 16 columns
       Frag<3> fs[TK / 2];
       state_frags(s, fs);
+      const int col = vc + 4 * lg;
+      auto values = [&](auto count, int first) {
+        constexpr int N = decltype(count)::value;
+        f32x4 acc[N];
+        Frag<NP> fj[N];
 #pragma unroll
-      for (int jt = 0; jt < TI; ++jt) {
-        if (jt >= tiles) break;
-        const int j = 16 * jt + li;
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < N; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < DK / 32; ++st) mma<3>(acc, fs[st], by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st));
-        acc *= d.left[j];
-        float x[4], sum = 0.f;
-        four<NP>(lds.v[0] + (jt * (VT / 16) + w) * TILE, VP, x);
+        for (int st = 0; st < DK / 32; ++st) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[r], sum);
-        sum = col_sum(sum);
-        if (lg == 0) lds.kr[w][j] = sum;
-#pragma unroll
-        for (int st = jt / 2; st < C / 32; ++st) {
-          if (2 * st >= tiles) break;
-          mma<PR>(acc, fo[st], tri_by_col<PR>(lds.p[0], PP, st, jt, tiles));
+          for (int m = 0; m < N; ++m) fj[m] = by_row<NP, DK>(lds.k[0], KP, 16 * (first + m), 32 * st);
+          mma_n<3>(acc, fs[st], fj);
         }
-        const int col = vc + 4 * lg;
-        emit(a.dv, a.dv32, token, vrow, j, u.h * a.V + col, j < n ? a.V - col : 0, v4, acc);
-      }
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+          const int j = 16 * (first + m) + li;
+          float x[4], sum = 0.f;
+          acc[m] *= d.left[j];
+          four<NP>(lds.v[0] + ((first + m) * (VT / 16) + w) * TILE, VP, x);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[m][r], sum);
+          sum = col_sum(sum);
+          if (lg == 0) lds.kr[w][j] = sum;
+        }
+#pragma unroll
+        for (int st = 0; st < C / 32; ++st)
+#pragma unroll
+          for (int m = 0; m < N; ++m)
+            if (2 * st + 1 >= first + m)
+              mma<PR>(acc[m], fo[st], tri_by_col<PR>(lds.p[0], PP, st, first + m));
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+          const int j = 16 * (first + m) + li;
+          emit(a.dv, a.dv32, token, vrow, j, u.h * a.V + col, j < n ? a.V - col : 0, v4, acc[m]);
+        }
+      };
+      values(std::integral_constant<int, TI>{}, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
     update_state<C, TK, DK, NP>(s, lds.q[0], KP, fo, d.from, d.whole);
     if (ENDS && threadIdx.x == 0) seg += d.total;
     __syncthreads();
@@ -902,7 +1069,7 @@ __global__ __launch_bounds__(BTHREADS, ENDS ? 4 : DK <= 64 ? 2 : 1) void k_la_bw
       double later = 0., kept = 0.;  // what is summed from t on, and before t
       if (lane < n) {
         for (int t = 0; t <= lane / 16; ++t) later += lds.row[t][lane];
-        for (int t = lane / 16; t < tiles; ++t) later -= lds.col[t][lane];
+        for (int t = lane / 16; t < TI; ++t) later -= lds.col[t][lane];
         for (int t = 0; t < TK; ++t) later += lds.qs[t][lane];
         for (int t = 0; t < BW; ++t) kept += lds.kr[t][lane];
       }
