@@ -10,8 +10,9 @@
 //   norm holds its rows; a lane keeps the same channels of the same group from sample to sample, so that weights are
 //   read, and their gradients added up, in registers.
 // - samples that a block's registers hold: threads over positions and channels, statistics through LDS, one pass.
-// - larger ones: blocks over ranges of positions leave (mean, sum of squares around it) of their values, which the
-//   second pass joins, each block for itself; it finds part of what the first one read in the caches.
+// - larger ones: blocks over ranges of positions leave (mean, sum of squares around it) of their values, a small launch
+//   joins them, and the second pass finds part of what the first one read in the caches.  (Joined by every block of the
+//   second pass for itself they took longer than the launch: 8 x 4096 x 320 in 16 groups' loads and sums a block.)
 // The variance is always formed around a mean, never as a difference of squares.  Sums are fp32 in a fixed order: no
 // atomics, equal calls give equal bits.
 #include "common.h"
@@ -23,7 +24,7 @@ namespace {
 
 constexpr int VEC = 8;
 constexpr int MAX_ROW = 8192;           // channels of a group held by a block's threads
-constexpr int MOST_CHUNKS = 256;        // a sample's ranges of positions: every block of the second pass joins them
+constexpr int MOST_CHUNKS = 1024;       // a sample's ranges of positions
 
 struct Gn {
   const void *x, *dy, *w, *b;
@@ -75,6 +76,30 @@ __device__ __forceinline__ float weight(const void* w, int dt, int64_t i, float 
   if (dt == LNG_BF16) return to_f32(static_cast<const bf16*>(w)[i]);
   return to_f32(static_cast<const _Float16*>(w)[i]);
 }
+// V neighbouring weights, 16 bytes at a time where they allow it; `none` where there are none
+template <int V>
+__device__ __forceinline__ void weights(const void* w, int dt, int64_t i, float none, float (&v)[V]) {
+  if constexpr (V > 1) {
+    if (w && reinterpret_cast<uintptr_t>(w) % 16 == 0) {
+      if (dt == LNG_F32) {
+        const Raw<float, V> r = load_raw<float, V>(static_cast<const float*>(w) + i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = r.v[k];
+      } else if (dt == LNG_BF16) {
+        const Raw<bf16, V> r = load_raw<bf16, V>(static_cast<const bf16*>(w) + i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = to_f32(r.v[k]);
+      } else {
+        const Raw<_Float16, V> r = load_raw<_Float16, V>(static_cast<const _Float16*>(w) + i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = to_f32(r.v[k]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = weight(w, dt, i + k, none);
+}
 // dy silu'(z)
 __device__ __forceinline__ float slope(float dy, float z) {
   const float s = sigmoid(z);
@@ -108,16 +133,24 @@ struct Slots {
   __host__ __device__ Slots(int G, int slots) : gs(G < slots ? G : slots), per(slots / gs), slabs((G + gs - 1) / gs) {}
 };
 
+// A lane's part of a group as it is in memory: the next one is asked for before this one is worked on
 template <typename T, int LPR, int NV, int V>
-__device__ __forceinline__ void load_group(const T* p, int lane, int vecs, float (&v)[NV][V]) {
+struct Held {
+  Raw<T, V> r[NV];
+  __device__ __forceinline__ void load(const T* p, int lane, int vecs) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = lane + LPR * j;
-    const Raw<T, V> r = load_raw<T, V>(p + (c < vecs ? c : 0) * V);  // no branch: all of them on their way together
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[j][i] = c < vecs ? to_f32(r.v[i]) : 0.f;
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + LPR * j;
+      r[j] = load_raw<T, V>(p + (c < vecs ? c : 0) * V);  // no branch: all of them on their way together
+    }
   }
-}
+  __device__ __forceinline__ void values(int lane, int vecs, float (&v)[NV][V]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = lane + LPR * j < vecs ? to_f32(r[j].v[i]) : 0.f;
+  }
+};
 
 template <typename T, int LPR, int NV, int V>
 __global__ __launch_bounds__(256) void k_gn_rows(Gn a) {
@@ -127,20 +160,22 @@ __global__ __launch_bounds__(256) void k_gn_rows(Gn a) {
   const int64_t first = int64_t{blockIdx.x} / sl.slabs * sl.per + slot / sl.gs;
   const int64_t step = int64_t{gridDim.x} / sl.slabs * sl.per;
   const int g = static_cast<int>(blockIdx.x % sl.slabs) * sl.gs + slot % sl.gs;
-  if (slot >= sl.per * sl.gs || g >= a.G) return;  // LPR > 64 has one slot: nobody leaves a barrier behind
+  if (slot >= sl.per * sl.gs || g >= a.G || first >= a.N) return;  // LPR > 64 has one slot: nobody leaves a barrier behind
   const float inv = 1.f / static_cast<float>(a.cg);
+  const T* x = static_cast<const T*>(a.x) + int64_t{g} * a.cg;
+  Held<T, LPR, NV, V> next;
+  next.load(x + first * a.xs, lane, vecs);
   float wv[NV][V], bv[NV][V];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (lane + LPR * j) * V + i;
-      wv[j][i] = c < a.cg ? weight(a.w, a.wdt, int64_t{g} * a.cg + c, 1.f) : 0.f;
-      bv[j][i] = c < a.cg ? weight(a.b, a.wdt, int64_t{g} * a.cg + c, 0.f) : 0.f;
-    }
+  for (int j = 0; j < NV; ++j) {
+    const int c = lane + LPR * j < vecs ? (lane + LPR * j) * V : 0;
+    weights<V>(a.w, a.wdt, int64_t{g} * a.cg + c, 1.f, wv[j]);
+    weights<V>(a.b, a.wdt, int64_t{g} * a.cg + c, 0.f, bv[j]);
+  }
   for (int64_t n = first; n < a.N; n += step) {
     float v[NV][V];
-    load_group<T, LPR, NV, V>(static_cast<const T*>(a.x) + n * a.xs + int64_t{g} * a.cg, lane, vecs, v);
+    next.values(lane, vecs, v);
+    if (n + step < a.N) next.load(x + (n + step) * a.xs, lane, vecs);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -180,23 +215,30 @@ __global__ __launch_bounds__(256) void k_gn_rows_grad(Gn a) {
   const int64_t first = int64_t{blockIdx.x} / sl.slabs * sl.per + slot / sl.gs;
   const int64_t step = int64_t{gridDim.x} / sl.slabs * sl.per;
   const int g = static_cast<int>(blockIdx.x % sl.slabs) * sl.gs + slot % sl.gs;
-  const bool on = slot < sl.per * sl.gs && g < a.G;
+  const bool on = slot < sl.per * sl.gs && g < a.G && first < a.N;
   const float inv = 1.f / static_cast<float>(a.cg);
+  const T *x = static_cast<const T*>(a.x) + int64_t{g} * a.cg, *dy = static_cast<const T*>(a.dy) + int64_t{g} * a.cg;
   float wv[NV][V], bv[NV][V], dw[NV][V], db[NV][V];
+  Held<T, LPR, NV, V> nx, nd;
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t n) {
+    nx.load(x + n * a.xs, lane, vecs), nd.load(dy + n * a.dys, lane, vecs);
+    nmean = a.mean[n * a.G + g], nrstd = a.rstd[n * a.G + g];
+  };
+  if (on) fetch(first);
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    const int c = lane + LPR * j < vecs ? (lane + LPR * j) * V : 0, gc = on ? g : 0;
+    weights<V>(a.w, a.wdt, int64_t{gc} * a.cg + c, 1.f, wv[j]);
+    weights<V>(a.b, a.wdt, int64_t{gc} * a.cg + c, 0.f, bv[j]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (lane + LPR * j) * V + i;
-      wv[j][i] = on && c < a.cg ? weight(a.w, a.wdt, int64_t{g} * a.cg + c, 1.f) : 0.f;
-      bv[j][i] = on && c < a.cg ? weight(a.b, a.wdt, int64_t{g} * a.cg + c, 0.f) : 0.f;
-      dw[j][i] = db[j][i] = 0.f;
-    }
+    for (int i = 0; i < V; ++i) dw[j][i] = db[j][i] = 0.f;
+  }
   for (int64_t n = on ? first : a.N; n < a.N; n += step) {
     float v[NV][V], h[NV][V];
-    load_group<T, LPR, NV, V>(static_cast<const T*>(a.x) + n * a.xs + int64_t{g} * a.cg, lane, vecs, v);
-    load_group<T, LPR, NV, V>(static_cast<const T*>(a.dy) + n * a.dys + int64_t{g} * a.cg, lane, vecs, h);
-    const float mean = a.mean[n * a.G + g], rstd = a.rstd[n * a.G + g];
+    nx.values(lane, vecs, v), nd.values(lane, vecs, h);  // dy is zero behind the group's end
+    const float mean = nmean, rstd = nrstd;
+    if (n + step < a.N) fetch(n + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -205,7 +247,7 @@ __global__ __launch_bounds__(256) void k_gn_rows_grad(Gn a) {
         v[j][i] = (v[j][i] - mean) * rstd;
         const float dz = a.act ? slope(h[j][i], fmaf(v[j][i], wv[j][i], bv[j][i])) : h[j][i];
         dw[j][i] = fmaf(dz, v[j][i], dw[j][i]), db[j][i] += dz;
-        h[j][i] = dz * wv[j][i];  // zero behind the group's end, where w is
+        h[j][i] = dz * wv[j][i];
         s1 += h[j][i], s2 = fmaf(h[j][i], v[j][i], s2);
       }
     s1 = row_sum<LPR>(s1, red) * inv;
@@ -251,6 +293,16 @@ __global__ __launch_bounds__(256) void k_gn_rows_grad(Gn a) {
 }
 
 // ------------------------------------------------------------------ blocks over positions and channels
+// A block's slab, range of positions and sample
+struct Place {
+  int slab, chunk;
+  int64_t n;
+  __device__ explicit Place(const Gn& a) {
+    const uint32_t slabs = a.slabs, chunks = a.chunks, u = blockIdx.x / slabs;
+    slab = blockIdx.x - u * slabs, n = u / chunks, chunk = u - static_cast<uint32_t>(n) * chunks;
+  }
+};
+
 // A thread has V neighbouring channels of a slab and every RL-th position.
 template <int V>
 struct Tile {
@@ -265,8 +317,12 @@ struct Tile {
     RL = 256 / CV, cv = static_cast<int>(threadIdx.x) % CV, rl = static_cast<int>(threadIdx.x) / CV, on = rl < RL;
     g0 = c0 / a.cg, groups = (c0 + width - 1) / a.cg - g0 + 1;
     c = c0 + cv * V;
+    int g = c / a.cg, rest = c - g * a.cg;  // one division: they are slow
 #pragma unroll
-    for (int i = 0; i < V; ++i) gk[i] = (c + i) / a.cg - g0;
+    for (int i = 0; i < V; ++i) {
+      gk[i] = g - g0;
+      if (++rest == a.cg) rest = 0, ++g;
+    }
   }
   // channels of group gi within the slab: [from, to)
   __device__ int from(const Gn& a, int gi) const { return max((g0 + gi) * a.cg - c0, 0); }
@@ -275,38 +331,51 @@ struct Tile {
 
 template <int V>
 struct TileLds {
-  float red[256 * V];    // a value a (position lane, channel)
-  float chan[256 * V];   // a channel's sum
-  float mean[256 * V], m2[256 * V];  // of a group (or sums of two kinds)
-  float rmean[256 * V], rm2[256 * V];
+  alignas(16) float one[256 * V], two[256 * V];    // values a (position lane, channel), of two kinds
+  float mean[256 * V], m2[256 * V];    // of a group: mean and sum of squares around it (or sums of two kinds)
 };
 
-// Sums of a thread's values by channel, into lds.chan
+// V neighbouring floats into LDS, 16 bytes at a time (one by one they would meet on the same banks)
 template <int V>
-__device__ __forceinline__ void channel_sums(TileLds<V>& lds, const Tile<V>& t, const float (&v)[V]) {
-  __syncthreads();
-  if (t.on)
+__device__ __forceinline__ void put_row(float* at, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *at = v[0];
+  } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) lds.red[t.rl * t.width + t.cv * V + i] = v[i];
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<f32x4*>(at + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  }
+}
+
+// Two values a (position, channel), summed over the positions: into lds.one and lds.two by channel
+template <int V>
+__device__ __forceinline__ void channel_sums(TileLds<V>& lds, const Tile<V>& t, const float (&x)[V], const float (&y)[V]) {
+  __syncthreads();
+  if (t.on) {
+    put_row<V>(&lds.one[t.rl * t.width + t.cv * V], x);
+    put_row<V>(&lds.two[t.rl * t.width + t.cv * V], y);
+  }
   __syncthreads();
   for (int c = threadIdx.x; c < t.width; c += 256) {
-    float s = 0.f;
-    for (int r = 0; r < t.RL; ++r) s += lds.red[r * t.width + c];
-    lds.chan[c] = s;
+    float s = lds.one[c], u = lds.two[c];
+#pragma unroll 8
+    for (int r = 1; r < t.RL; ++r) s += lds.one[r * t.width + c], u += lds.two[r * t.width + c];
+    lds.one[c] = s, lds.two[c] = u;  // this thread's column
   }
   __syncthreads();
 }
-// f(group, sum of lds.chan over the group's channels in the slab, times w where given), by one thread each
+// f(group, sums of lds.one and lds.two over the group's channels in the slab, times w), by one thread each
 template <int V, typename F>
-__device__ __forceinline__ void group_sums(const TileLds<V>& lds, const Tile<V>& t, const Gn& a, bool weighted, F f) {
+__device__ __forceinline__ void group_sums(const TileLds<V>& lds, const Tile<V>& t, const Gn& a, F f) {
   const int lg = a.cg >= 256 ? 64 : 16, lane = threadIdx.x % lg;
   for (int gi = threadIdx.x / lg; gi < t.groups; gi += 256 / lg) {
-    float s = 0.f;
+    float s = 0.f, u = 0.f;
     const int to = t.to(a, gi);
-    for (int c = t.from(a, gi) + lane; c < to; c += lg)
-      s += weighted ? lds.chan[c] * weight(a.w, a.wdt, t.c0 + c, 1.f) : lds.chan[c];
-    for (int m = lg / 2; m; m >>= 1) s += __shfl_xor(s, m);
-    if (lane == 0) f(gi, s);
+    for (int c = t.from(a, gi) + lane; c < to; c += lg) {
+      const float w = weight(a.w, a.wdt, t.c0 + c, 1.f);
+      s = fmaf(lds.one[c], w, s), u = fmaf(lds.two[c], w, u);
+    }
+    for (int m = lg / 2; m; m >>= 1) s += __shfl_xor(s, m), u += __shfl_xor(u, m);
+    if (lane == 0) f(gi, s, u);
   }
 }
 
@@ -324,34 +393,54 @@ __device__ __forceinline__ void load_tile(Raw<T, V> (&v)[R], const T* x, int64_t
   }
 }
 
-// Mean and sum of squares around it of the groups in a tile of `rows` positions: lds.mean, lds.m2
+// Mean and sum of squares around it of the groups in a tile of positions: lds.mean, lds.m2.  Each thread forms both of its
+// positions of a channel, a group's lanes join them: one exchange for the two steps.
 template <typename T, int V, int R>
 __device__ __forceinline__ void tile_stats(TileLds<V>& lds, const Tile<V>& t, const Gn& a, const Raw<T, V> (&v)[R], int64_t l0,
                                            int64_t l1) {
-  const float rows = static_cast<float>(l1 - l0);
-  float s[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    s[k] = 0.f;
-#pragma unroll
-    for (int i = 0; i < R; ++i) s[k] += to_f32(v[i].v[k]);
-  }
-  channel_sums(lds, t, s);
-  group_sums(lds, t, a, false,
-             [&](int gi, float x) { lds.mean[gi] = x / (rows * static_cast<float>(t.to(a, gi) - t.from(a, gi))); });
+  const int rows = static_cast<int>(l1 - l0);
+  const int all = rows / t.RL, more = rows - all * t.RL;  // position lane r has `all` of them, the first `more` one more
+  const int mine = all + (t.rl < more);
+  const float inv = mine ? 1.f / static_cast<float>(mine) : 0.f;
   __syncthreads();
+  if (t.on) {
+    float m[V], q[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const float m = lds.mean[t.gk[k]];
-    s[k] = 0.f;
+    for (int k = 0; k < V; ++k) {
+      m[k] = q[k] = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float d = to_f32(v[i].v[k]) - m;
-      if (l0 + t.rl + int64_t{i} * t.RL < l1) s[k] = fmaf(d, d, s[k]);
+      for (int i = 0; i < R; ++i) m[k] += to_f32(v[i].v[k]);
+      m[k] *= inv;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float d = to_f32(v[i].v[k]) - m[k];
+        q[k] = i < mine ? fmaf(d, d, q[k]) : q[k];
+      }
     }
+    put_row<V>(&lds.one[t.rl * t.width + t.cv * V], m);
+    put_row<V>(&lds.two[t.rl * t.width + t.cv * V], q);
   }
-  channel_sums(lds, t, s);
-  group_sums(lds, t, a, false, [&](int gi, float x) { lds.m2[gi] = x; });
+  __syncthreads();
+  const int lg = a.cg >= 256 ? 64 : 16, lane = threadIdx.x % lg, used = min(t.RL, rows);
+  for (int gi = threadIdx.x / lg; gi < t.groups; gi += 256 / lg) {
+    const int c0 = t.from(a, gi), c1 = t.to(a, gi);
+    const float count = static_cast<float>(rows) * static_cast<float>(c1 - c0);
+    float m = 0.f, q = 0.f;
+    for (int c = c0 + lane; c < c1; c += lg)
+#pragma unroll 8
+      for (int r = 0; r < used; ++r) m = fmaf(lds.one[r * t.width + c], static_cast<float>(all + (r < more)), m);
+
+    for (int k = lg / 2; k; k >>= 1) m += __shfl_xor(m, k);
+    m /= count;
+    for (int c = c0 + lane; c < c1; c += lg)
+#pragma unroll 8
+      for (int r = 0; r < used; ++r) {
+        const float d = lds.one[r * t.width + c] - m;
+        q += fmaf(d * d, static_cast<float>(all + (r < more)), lds.two[r * t.width + c]);
+      }
+    for (int k = lg / 2; k; k >>= 1) q += __shfl_xor(q, k);
+    if (lane == 0) lds.mean[gi] = m, lds.m2[gi] = q;
+  }
   __syncthreads();
 }
 
@@ -360,10 +449,10 @@ struct Weights {
   float w[V], b[V];
   __device__ Weights(const Gn& a, const Tile<V>& t) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[i] = t.on ? weight(a.w, a.wdt, t.c + i, 1.f) : 0.f;
-      b[i] = t.on ? weight(a.b, a.wdt, t.c + i, 0.f) : 0.f;
-    }
+    for (int i = 0; i < V; ++i) w[i] = b[i] = 0.f;
+    if (!t.on) return;
+    weights<V>(a.w, a.wdt, t.c, 1.f, w);
+    weights<V>(a.b, a.wdt, t.c, 0.f, b);
   }
 };
 
@@ -410,33 +499,28 @@ __global__ __launch_bounds__(256) void k_gn_samples(Gn a) {
 template <typename T, int V, int R>
 __global__ __launch_bounds__(256) void k_gn_stats(Gn a) {
   __shared__ TileLds<V> lds;
-  int64_t u = blockIdx.x;
-  const Tile<V> t(a, static_cast<int>(u % a.slabs));
-  u /= a.slabs;
-  const int chunk = static_cast<int>(u % a.chunks);
-  const int64_t n = u / a.chunks, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
+  const Place at(a);
+  const Tile<V> t(a, at.slab);
+  const int chunk = at.chunk;
+  const int64_t n = at.n, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
+  float* to = a.stats + ((n * a.chunks + chunk) * a.slabs + at.slab) * a.G * 2;
   for (int64_t l = l0; l < l1; l += int64_t{R} * t.RL) {
     const int64_t e = min(l + int64_t{R} * t.RL, l1);
     Raw<T, V> v[R];
     load_tile(v, static_cast<const T*>(a.x) + n * a.xs, a.xl, t, l, e);
     tile_stats(lds, t, a, v, l, e);
     const float before = static_cast<float>(l - l0), rows = static_cast<float>(e - l);
-    for (int gi = threadIdx.x; gi < t.groups; gi += 256) {  // joined with the tiles before
+    for (int gi = threadIdx.x; gi < t.groups; gi += 256) {  // joined with the tiles before, which this thread wrote
+      float* own = to + 2 * (t.g0 + gi);
       const float width = static_cast<float>(t.to(a, gi) - t.from(a, gi));
       if (l == l0) {
-        lds.rmean[gi] = lds.mean[gi], lds.rm2[gi] = lds.m2[gi];
+        own[0] = lds.mean[gi], own[1] = lds.m2[gi];
       } else {
-        const float d = lds.mean[gi] - lds.rmean[gi], part = rows / (before + rows);
-        lds.rmean[gi] = fmaf(d, part, lds.rmean[gi]);
-        lds.rm2[gi] += fmaf(d * d, before * part * width, lds.m2[gi]);
+        const float d = lds.mean[gi] - own[0], part = rows / (before + rows);
+        own[0] = fmaf(d, part, own[0]);
+        own[1] += fmaf(d * d, before * part * width, lds.m2[gi]);
       }
     }
-    __syncthreads();
-  }
-  float* to = a.stats + ((n * a.chunks + chunk) * a.slabs + blockIdx.x % a.slabs) * a.G * 2;
-  for (int gi = threadIdx.x; gi < t.groups; gi += 256) {
-    to[2 * (t.g0 + gi)] = lds.rmean[gi];
-    to[2 * (t.g0 + gi) + 1] = lds.rm2[gi];
   }
 }
 
@@ -445,60 +529,96 @@ __device__ __forceinline__ float chunk_size(const Gn& a, int64_t i) {
   return static_cast<float>(min(a.chunk_rows, a.L - i * a.chunk_rows));
 }
 // The slabs that hold channels of group g: [first, last]
-__device__ __forceinline__ int first_slab(const Gn& a, int g) { return static_cast<int>(int64_t{g} * a.cg / a.slab); }
-__device__ __forceinline__ int last_slab(const Gn& a, int g) {
-  return static_cast<int>((int64_t{g + 1} * a.cg - 1) / a.slab);
-}
+__device__ __forceinline__ int first_slab(const Gn& a, int g) { return a.slabs == 1 ? 0 : g * a.cg / a.slab; }
+__device__ __forceinline__ int last_slab(const Gn& a, int g) { return a.slabs == 1 ? 0 : ((g + 1) * a.cg - 1) / a.slab; }
 __device__ __forceinline__ float slab_part(const Gn& a, int g, int s) {  // channels of group g in slab s
-  const int64_t from = max(int64_t{g} * a.cg, int64_t{s} * a.slab), to = min(int64_t{g + 1} * a.cg, int64_t{s + 1} * a.slab);
-  return static_cast<float>(to - from);
+  return static_cast<float>(min((g + 1) * a.cg, (s + 1) * a.slab) - max(g * a.cg, s * a.slab));
 }
 
-// The second pass: the ranges' statistics joined, then every value
-template <typename T, int V>
-__global__ __launch_bounds__(256) void k_gn_apply(Gn a) {
-  __shared__ TileLds<V> lds;
-  int64_t u = blockIdx.x;
-  const Tile<V> t(a, static_cast<int>(u % a.slabs));
-  u /= a.slabs;
-  const int chunk = static_cast<int>(u % a.chunks);
-  const int64_t n = u / a.chunks, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
-  const float count = static_cast<float>(a.L) * static_cast<float>(a.cg);
+template <int V>
+__device__ __forceinline__ void load_stats(const Gn& a, const Tile<V>& t, int64_t n, float (&mean)[V], float (&rstd)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    mean[k] = t.on ? a.mean[n * a.G + t.g0 + t.gk[k]] : 0.f;
+    rstd[k] = t.on ? a.rstd[n * a.G + t.g0 + t.gk[k]] : 0.f;
+  }
+}
+
+// Between the passes: 16 lanes join a group's ranges.  Statistics become mean and rstd; GRAD: sums of h and h xn become
+// their means over the group, in the place of its first range.
+template <bool GRAD>
+__global__ __launch_bounds__(256) void k_gn_join(Gn a, int64_t pairs) {
+  const int64_t i = int64_t{blockIdx.x} * 16 + threadIdx.x / 16;
+  if (i >= pairs) return;
   const int lane = threadIdx.x & 15;
-  for (int gi = threadIdx.x >> 4; gi < t.groups; gi += 16) {
-    const int g = t.g0 + gi, s0 = first_slab(a, g), ns = last_slab(a, g) - s0 + 1;
-    const float* from = a.stats + (n * a.chunks * a.slabs * a.G + g) * 2;
-    float m = 0.f, m2 = 0.f;
-    for (int i = lane; i < a.chunks * ns; i += 16) {
-      const int ch = i / ns, sb = s0 + i % ns;
-      m = fmaf(from[(int64_t{ch} * a.slabs + sb) * a.G * 2], chunk_size(a, ch) * slab_part(a, g, sb) / count, m);
+  const int64_t n = i / a.G;
+  const int g = static_cast<int>(i - n * a.G), s0 = first_slab(a, g), ns = last_slab(a, g) - s0 + 1, parts = a.chunks * ns;
+  float2* const at = reinterpret_cast<float2*>(a.stats) + (n * a.chunks * a.slabs + s0) * a.G + g;
+  const float count = static_cast<float>(a.L) * static_cast<float>(a.cg);
+  const float full = static_cast<float>(a.chunk_rows), last = chunk_size(a, a.chunks - 1);
+  auto part = [&](int k, float& size) {
+    const int ch = ns == 1 ? k : k / ns, sb = k - ch * ns;
+    size = (ch + 1 < a.chunks ? full : last) * (ns == 1 ? static_cast<float>(a.cg) : slab_part(a, g, s0 + sb));
+    return at[(int64_t{ch} * a.slabs + sb) * a.G];
+  };
+  float one = 0.f, two = 0.f, size;
+  if constexpr (GRAD) {
+#pragma unroll 8
+    for (int k = lane; k < parts; k += 16) {
+      const float2 p = part(k, size);
+      one += p.x, two += p.y;
+    }
+  } else {
+#pragma unroll 8
+    for (int k = lane; k < parts; k += 16) {
+      const float2 p = part(k, size);
+      one = fmaf(p.x, size / count, one);
     }
 #pragma unroll
-    for (int k = 8; k; k >>= 1) m += __shfl_xor(m, k);
-    for (int i = lane; i < a.chunks * ns; i += 16) {
-      const int ch = i / ns, sb = s0 + i % ns;
-      const float* p = from + (int64_t{ch} * a.slabs + sb) * a.G * 2;
-      const float d = p[0] - m;
-      m2 += fmaf(d * d, chunk_size(a, ch) * slab_part(a, g, sb), p[1]);
-    }
-#pragma unroll
-    for (int k = 8; k; k >>= 1) m2 += __shfl_xor(m2, k);
-    if (lane == 0) {
-      const float rstd = 1.f / sqrtf(m2 / count + a.eps);
-      lds.mean[gi] = m, lds.m2[gi] = rstd;
-      if (a.mean && chunk == 0) a.mean[n * a.G + g] = m, a.rstd[n * a.G + g] = rstd;
+    for (int k = 8; k; k >>= 1) one += __shfl_xor(one, k);
+#pragma unroll 8
+    for (int k = lane; k < parts; k += 16) {
+      const float2 p = part(k, size);
+      two += fmaf((p.x - one) * (p.x - one), size, p.y);
     }
   }
-  __syncthreads();
+#pragma unroll
+  for (int k = 8; k; k >>= 1) {
+    if (GRAD) one += __shfl_xor(one, k);
+    two += __shfl_xor(two, k);
+  }
+  if (lane) return;
+  if (GRAD)
+    *at = float2{one / count, two / count};
+  else
+    a.mean[i] = one, a.rstd[i] = 1.f / sqrtf(two / count + a.eps);
+}
+
+// The second pass
+template <typename T, int V, int R>
+__global__ __launch_bounds__(256) void k_gn_apply(Gn a) {
+  const Place at(a);
+  const Tile<V> t(a, at.slab);
   if (!t.on) return;
+  const int64_t n = at.n, l0 = at.chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
+  const T* x = static_cast<const T*>(a.x) + n * a.xs;
+  Raw<T, V> v[R];
+  load_tile(v, x, a.xl, t, l0, l1);
   const Weights<T, V> wt(a, t);
   float mean[V], rstd[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) mean[k] = lds.mean[t.gk[k]], rstd[k] = lds.m2[t.gk[k]];
-  const T* x = static_cast<const T*>(a.x) + n * a.xs + t.c;
+  load_stats(a, t, n, mean, rstd);
   T* y = static_cast<T*>(a.y) + n * a.L * a.C + t.c;
-#pragma unroll 4
-  for (int64_t l = l0 + t.rl; l < l1; l += t.RL) write_row<T, V>(a, wt, load_raw<T, V>(x + l * a.xl), mean, rstd, y + l * a.C);
+  for (int64_t l = l0; l < l1; l += int64_t{R} * t.RL) {
+    Raw<T, V> now[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) now[i] = v[i];
+    if (l + int64_t{R} * t.RL < l1) load_tile(v, x, a.xl, t, l + int64_t{R} * t.RL, l1);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t row = l + t.rl + int64_t{i} * t.RL;
+      if (row < l1) write_row<T, V>(a, wt, now[i], mean, rstd, y + row * a.C);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ their backward pass
@@ -523,15 +643,6 @@ __device__ __forceinline__ void write_dx(const Weights<T, V>& wt, const GradRow<
   for (int k = 0; k < V; ++k) out[k] = rstd[k] * (r.dz[k] * wt.w[k] - s1[k] - r.xn[k] * s2[k]);
   store_raw<T, V>(dx, out);
 }
-template <int V>
-__device__ __forceinline__ void load_stats(const Gn& a, const Tile<V>& t, int64_t n, float (&mean)[V], float (&rstd)[V]) {
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    mean[k] = t.on ? a.mean[n * a.G + t.g0 + t.gk[k]] : 0.f;
-    rstd[k] = t.on ? a.rstd[n * a.G + t.g0 + t.gk[k]] : 0.f;
-  }
-}
-
 // Samples that the registers hold; a block's samples leave one partial row of dw and db
 template <typename T, int V, int R>
 __global__ __launch_bounds__(256) void k_gn_samples_grad(Gn a) {
@@ -559,10 +670,8 @@ __global__ __launch_bounds__(256) void k_gn_samples_grad(Gn a) {
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) dw[k] += sa[k], db[k] += sb[k];
-    channel_sums(lds, t, sb);
-    group_sums(lds, t, a, true, [&](int gi, float s) { lds.mean[gi] = s * inv; });
-    channel_sums(lds, t, sa);
-    group_sums(lds, t, a, true, [&](int gi, float s) { lds.m2[gi] = s * inv; });
+    channel_sums(lds, t, sb, sa);
+    group_sums(lds, t, a, [&](int gi, float s, float u) { lds.mean[gi] = s * inv, lds.m2[gi] = u * inv; });
     __syncthreads();
     float s1[V], s2[V];
 #pragma unroll
@@ -577,22 +686,18 @@ __global__ __launch_bounds__(256) void k_gn_samples_grad(Gn a) {
   }
   if (!a.cols) return;
   float* to = a.cols + int64_t{blockIdx.x} / a.slabs * 2 * a.C + t.c0;
-  channel_sums(lds, t, dw);
-  for (int c = threadIdx.x; c < t.width; c += 256) to[c] = lds.chan[c];
-  channel_sums(lds, t, db);
-  for (int c = threadIdx.x; c < t.width; c += 256) to[a.C + c] = lds.chan[c];
+  channel_sums(lds, t, dw, db);
+  for (int c = threadIdx.x; c < t.width; c += 256) to[c] = lds.one[c], to[a.C + c] = lds.two[c];
 }
 
 // A range of positions of a slab: sums of dz xn and dz by channel into a partial row, times w by group into stats
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_gn_grad_sums(Gn a) {
   __shared__ TileLds<V> lds;
-  int64_t u = blockIdx.x;
-  const int slab = static_cast<int>(u % a.slabs);
+  const Place at(a);
+  const int slab = at.slab, chunk = at.chunk;
   const Tile<V> t(a, slab);
-  u /= a.slabs;
-  const int chunk = static_cast<int>(u % a.chunks);
-  const int64_t n = u / a.chunks, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
+  const int64_t n = at.n, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
   const Weights<T, V> wt(a, t);
   float mean[V], rstd[V], sa[V], sb[V];
   load_stats(a, t, n, mean, rstd);
@@ -608,49 +713,46 @@ __global__ __launch_bounds__(256) void k_gn_grad_sums(Gn a) {
     }
   float* to = a.cols + (n * a.chunks + chunk) * 2 * a.C + t.c0;
   float* groups = a.stats + ((n * a.chunks + chunk) * a.slabs + slab) * a.G * 2;
-  channel_sums(lds, t, sa);
-  for (int c = threadIdx.x; c < t.width; c += 256) to[c] = lds.chan[c];
-  group_sums(lds, t, a, true, [&](int gi, float s) { groups[2 * (t.g0 + gi) + 1] = s; });
-  channel_sums(lds, t, sb);
-  for (int c = threadIdx.x; c < t.width; c += 256) to[a.C + c] = lds.chan[c];
-  group_sums(lds, t, a, true, [&](int gi, float s) { groups[2 * (t.g0 + gi)] = s; });
+  channel_sums(lds, t, sa, sb);
+  for (int c = threadIdx.x; c < t.width; c += 256) to[c] = lds.one[c], to[a.C + c] = lds.two[c];
+  group_sums(lds, t, a, [&](int gi, float s, float u) { groups[2 * (t.g0 + gi) + 1] = s, groups[2 * (t.g0 + gi)] = u; });
 }
 
-template <typename T, int V>
+template <typename T, int V, int R>
 __global__ __launch_bounds__(256) void k_gn_grad_apply(Gn a) {
-  __shared__ TileLds<V> lds;
-  int64_t u = blockIdx.x;
-  const Tile<V> t(a, static_cast<int>(u % a.slabs));
-  u /= a.slabs;
-  const int chunk = static_cast<int>(u % a.chunks);
-  const int64_t n = u / a.chunks, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
-  const float inv = 1.f / (static_cast<float>(a.L) * static_cast<float>(a.cg));
-  const int lane = threadIdx.x & 15;
-  for (int gi = threadIdx.x >> 4; gi < t.groups; gi += 16) {
-    const int g = t.g0 + gi, s0 = first_slab(a, g), ns = last_slab(a, g) - s0 + 1;
-    const float* from = a.stats + (n * a.chunks * a.slabs * a.G + g) * 2;
-    float s1 = 0.f, s2 = 0.f;
-    for (int i = lane; i < a.chunks * ns; i += 16) {
-      const float* p = from + (int64_t{i / ns} * a.slabs + s0 + i % ns) * a.G * 2;
-      s1 += p[0], s2 += p[1];
-    }
-#pragma unroll
-    for (int k = 8; k; k >>= 1) s1 += __shfl_xor(s1, k), s2 += __shfl_xor(s2, k);
-    if (lane == 0) lds.mean[gi] = s1 * inv, lds.m2[gi] = s2 * inv;
-  }
-  __syncthreads();
+  const Place at(a);
+  const Tile<V> t(a, at.slab);
   if (!t.on) return;
+  const int64_t n = at.n, l0 = at.chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
+  const T *px = static_cast<const T*>(a.x) + n * a.xs, *pd = static_cast<const T*>(a.dy) + n * a.dys;
+  Raw<T, V> x[R], dy[R];
+  load_tile(x, px, a.xl, t, l0, l1);
+  load_tile(dy, pd, a.dyl, t, l0, l1);
   const Weights<T, V> wt(a, t);
   float mean[V], rstd[V], s1[V], s2[V];
   load_stats(a, t, n, mean, rstd);
 #pragma unroll
-  for (int k = 0; k < V; ++k) s1[k] = lds.mean[t.gk[k]], s2[k] = lds.m2[t.gk[k]];
-  const T *x = static_cast<const T*>(a.x) + n * a.xs + t.c, *dy = static_cast<const T*>(a.dy) + n * a.dys + t.c;
+  for (int k = 0; k < V; ++k) {
+    const int g = t.g0 + t.gk[k];
+    const float2 s = reinterpret_cast<const float2*>(a.stats)[(n * a.chunks * a.slabs + first_slab(a, g)) * a.G + g];
+    s1[k] = s.x, s2[k] = s.y;
+  }
   T* dx = static_cast<T*>(a.dx) + n * a.L * a.C + t.c;
-#pragma unroll 4
-  for (int64_t l = l0 + t.rl; l < l1; l += t.RL) {
-    const GradRow<T, V> r(a, wt, load_raw<T, V>(x + l * a.xl), load_raw<T, V>(dy + l * a.dyl), mean, rstd);
-    write_dx<T, V>(wt, r, rstd, s1, s2, dx + l * a.C);
+  for (int64_t l = l0; l < l1; l += int64_t{R} * t.RL) {
+    Raw<T, V> nx[R], nd[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) nx[i] = x[i], nd[i] = dy[i];
+    if (l + int64_t{R} * t.RL < l1) {
+      load_tile(x, px, a.xl, t, l + int64_t{R} * t.RL, l1);
+      load_tile(dy, pd, a.dyl, t, l + int64_t{R} * t.RL, l1);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t row = l + t.rl + int64_t{i} * t.RL;
+      if (row >= l1) continue;
+      const GradRow<T, V> r(a, wt, nx[i], nd[i], mean, rstd);
+      write_dx<T, V>(wt, r, rstd, s1, s2, dx + row * a.C);
+    }
   }
 }
 
@@ -693,6 +795,7 @@ struct Plan {
   int64_t blocks;
   int64_t P;           // partial rows of the weights' gradients
   int64_t stats, cols; // floats of the workspace
+  int64_t own;         // where among the first are mean and rstd
 };
 
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -741,6 +844,7 @@ Plan make_plan(Gn& a, bool vec, bool grad) {
       a.chunks = static_cast<int>(cdiv(L, a.chunk_rows));
       p.blocks = N * a.chunks * a.slabs, p.P = N * a.chunks;
       p.stats = N * a.chunks * a.slabs * a.G * 2;
+      if (!grad) p.own = cdiv(p.stats, 16) * 16, p.stats = p.own + 2 * N * a.G;  // mean and rstd, where the caller wants none
     }
   }
   p.cols = grad ? p.P * 2 * a.C : 0;
@@ -789,6 +893,12 @@ int run_rows(const Gn& a, const Plan& p, hipStream_t st) {
   return fail(LNG_E_ARG, "group_norm: bad shape");
 }
 
+template <bool GRAD>
+int run_join(const Gn& a, hipStream_t st) {
+  k_gn_join<GRAD><<<static_cast<unsigned>(cdiv(a.N * a.G, 16)), 256, 0, st>>>(a, a.N * a.G);
+  return check_launch("group_norm");
+}
+
 template <typename T, int V>
 int run_fwd(const Gn& a, const Plan& p, hipStream_t st) {
   const unsigned blocks = static_cast<unsigned>(p.blocks);
@@ -798,7 +908,8 @@ int run_fwd(const Gn& a, const Plan& p, hipStream_t st) {
   }
   k_gn_stats<T, V, FWD_R><<<blocks, 256, 0, st>>>(a);
   if (int rc = check_launch("group_norm")) return rc;
-  k_gn_apply<T, V><<<blocks, 256, 0, st>>>(a);
+  if (int rc = run_join<false>(a, st)) return rc;
+  k_gn_apply<T, V, 2><<<blocks, 256, 0, st>>>(a);
   return check_launch("group_norm");
 }
 
@@ -812,7 +923,8 @@ int run_bwd(const Gn& a, const Plan& p, hipStream_t st) {
   k_gn_grad_sums<T, V><<<blocks, 256, 0, st>>>(a);
   if (int rc = check_launch("group_norm_grad")) return rc;
   if (!a.dx) return LNG_OK;
-  k_gn_grad_apply<T, V><<<blocks, 256, 0, st>>>(a);
+  if (int rc = run_join<true>(a, st)) return rc;
+  k_gn_grad_apply<T, V, 2><<<blocks, 256, 0, st>>>(a);
   return check_launch("group_norm_grad");
 }
 
@@ -891,6 +1003,7 @@ int lng_group_norm(const void* x, int dtype, int64_t N, int64_t L, int32_t C, in
   if (space_of(p) && (!workspace || !aligned(workspace, 64) || workspace_bytes < static_cast<size_t>(space_of(p)) * 4))
     return fail(LNG_E_ARG, "group_norm: the workspace is too small or not 64-byte aligned");
   a.stats = static_cast<float*>(workspace);
+  if (p.form == Form::passes && !mean) a.mean = a.stats + p.own, a.rstd = a.mean + N * G;
   return dispatch(dtype, a, p, false, as_stream(stream));
 }
 

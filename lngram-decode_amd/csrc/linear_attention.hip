@@ -1254,11 +1254,13 @@ bool vector_rows(const void* p, int es, int64_t batch, int64_t token, int64_t he
          d % 8 == 0 && token >= 0 && token * es < (int64_t{1} << 25);
 }
 
-// Blocks that a launch should have: a segment more costs the keys and values (the queries and dy) of all but one
-// segment a second time.
-constexpr int64_t FWD_BLOCKS = 1024, BWD_BLOCKS = 512;
+// Blocks that a launch should have, two for each CU: a segment more costs the keys and values (the queries and dy) of all
+// but one segment a second time.  8 x 4096 x 16 x 64 in 128, 256, 384, 512, 768, 1024 blocks: 200, 154, 127, 108, 111,
+// 126 us; 1 x 16384 x 16 x 128 in 256, 512, 768, 1024: 209, 149, 163, 161; the training of 8 x 2048 x 16 x 64 with its
+// backward pass in 128, 256, 512, 768: 458, 330, 257, 308.
+constexpr int64_t BLOCKS = 512;
 
-Args make_args(const lng_linear_attention& l, bool grad) {
+Args make_args(const lng_linear_attention& l) {
   Args a{};
   a.B = l.B, a.T = l.T, a.H = l.H, a.Hq = l.Hq, a.Hk = l.Hk, a.Hv = l.Hv, a.K = l.K, a.V = l.V, a.scale = l.scale;
   a.q = l.q, a.k = l.k, a.v = l.v;
@@ -1273,8 +1275,8 @@ Args make_args(const lng_linear_attention& l, bool grad) {
   a.Kp = static_cast<int>(cdiv(a.K, 8)) * 8, a.Vp = static_cast<int>(cdiv(a.V, 8)) * 8;
   a.vts = static_cast<int>(cdiv(a.V, VT));
   a.chunks = static_cast<int>(cdiv(a.T, chunk_of(l.dtype)));
-  const int64_t units = a.B * a.H * a.vts, want = grad ? BWD_BLOCKS : FWD_BLOCKS;
-  int64_t segs = units * 2 > want ? 1 : std::min<int64_t>(cdiv(want, std::max<int64_t>(units, 1)), cdiv(a.chunks, 2));
+  const int64_t units = std::max<int64_t>(1, a.B * a.H * a.vts);
+  const int64_t segs = std::min<int64_t>((BLOCKS + units / 2) / units, cdiv(a.chunks, 2));
   a.seg_chunks = static_cast<int>(cdiv(a.chunks, std::max<int64_t>(segs, 1)));
   a.segs = a.seg_chunks ? static_cast<int>(cdiv(a.chunks, a.seg_chunks)) : 1;
   return a;
@@ -1429,7 +1431,7 @@ size_t lng_linear_attention_grad_size(void) { return sizeof(lng_linear_attention
 
 size_t lng_linear_attention_workspace_bytes(const lng_linear_attention* args, int grad) {
   if (check_args("linear_attention_workspace_bytes", args) || args->B == 0 || args->T == 0) return 0;
-  const Args a = make_args(*args, grad != 0);
+  const Args a = make_args(*args);
   return static_cast<size_t>(Space(a, dtype_size(args->dtype), grad != 0, args->token_decay != 0).total) * 4;
 }
 
@@ -1443,7 +1445,7 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
   if (int rc = check_args(what, args)) return rc;
   if (args->B == 0 || args->T == 0) return LNG_OK;
   if (!args->y) return fail(LNG_E_ARG, "linear_attention: null pointer");
-  Args a = make_args(*args, false);
+  Args a = make_args(*args);
   const Space s(a, dtype_size(args->dtype), false, args->token_decay != 0);
   if (s.total && (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 ||
                   reinterpret_cast<uintptr_t>(workspace) % 64))
@@ -1471,7 +1473,7 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
   if (args->B == 0 || args->T == 0) return fail(LNG_E_ARG, "linear_attention_grad: no tokens");
   if (!args->checkpoints || !g.dy || !g.dq || !g.dk || !g.dv || !g.ddecay)
     return fail(LNG_E_ARG, "linear_attention_grad: null pointer");
-  Args a = make_args(*args, true);
+  Args a = make_args(*args);
   const bool token = args->token_decay != 0;
   const int es = dtype_size(args->dtype);
   const Space s(a, es, true, token);
@@ -1522,7 +1524,7 @@ int lng_linear_attention_step(const lng_linear_attention* args, void* stream) {
   if (args->T != 1) return fail(LNG_E_ARG, "linear_attention_step: one token of every sequence (T = 1)");
   if (args->B == 0) return LNG_OK;
   if (!args->state || !args->state_out || !args->y) return fail(LNG_E_ARG, "linear_attention_step: null pointer");
-  const Args a = make_args(*args, false);
+  const Args a = make_args(*args);
   const int64_t waves = a.B * a.H * a.vts, blocks = cdiv(waves, 4);
   if (int rc = check_threads(what, blocks, 256)) return rc;
   const bool vec = a.yvec && reinterpret_cast<uintptr_t>(a.start) % 16 == 0 && reinterpret_cast<uintptr_t>(a.end) % 16 == 0;
