@@ -23,19 +23,20 @@ from .grad_mode import needs_grad
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, decay, state, lengths, scale, want_state: bool):
-        y, end, ckpt = ops.linear_attention(q, k, v, decay, scale, state, lengths, want_state, True)
-        ctx.save_for_backward(ckpt, q, k, v, decay, state, lengths)
-        ctx.scale = scale
+        # what the backward pass can be spared is done here: it runs on autograd's own thread, whose host work is slow
+        y, end, _, ctx.plan, tensors = ops.linear_attention_plan(q, k, v, decay, scale, state, lengths, want_state, True)
+        ctx.save_for_backward(*tensors)
         ctx.set_materialize_grads(False)
         return y, end
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dend):
-        ckpt, q, k, v, decay, state, lengths = ctx.saved_tensors
+        tensors = ctx.saved_tensors
         if dy is None:
+            _, q, _, v, decay, _, _ = tensors
             dy = q.new_zeros(1).expand(*q.shape[:2], decay.shape[-1], v.shape[-1])
-        grads = ops.linear_attention_grad(dy, dend, ckpt, q, k, v, decay, ctx.scale, state, lengths)
+        grads = ops.linear_attention_back(ctx.plan, tensors, dy, dend)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
 

@@ -45,18 +45,15 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float, silu: bool) -> Tensor:
-        y, mean, rstd = ops.group_norm(x, groups, weight, bias, eps, silu, want_stats=True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.cfg = (groups, silu)
+        # what the backward pass can be spared is done here: it runs on autograd's own thread, whose host work is slow
+        y, stats, ctx.plan, tensors = ops.group_norm_plan(x, groups, weight, bias, eps, silu, True)
+        ctx.save_for_backward(*tensors, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy: Tensor):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        groups, silu = ctx.cfg
-        return (*ops.group_norm_grad(dy, x, groups, weight, bias, silu, mean, rstd, ctx.needs_input_grad[:3]), None, None,
-                None)
+        return (*ops.group_norm_back(ctx.plan, ctx.saved_tensors, dy, ctx.needs_input_grad), None, None, None)
 
 
 def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,

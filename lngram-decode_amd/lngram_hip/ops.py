@@ -1468,49 +1468,75 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, m
 
 def _as_samples(what: str, x: torch.Tensor, groups: int) -> tuple:
     """``([N, L, C] view with contiguous channels, N, L, C)`` of channels-last ``x [N, .., C]``."""
-    if x.dim() < 2 or x.shape[-1] == 0:
-        raise ValueError(f"{what}: x is [N, .., C], got {tuple(x.shape)}")
-    n, c = x.shape[0], x.shape[-1]
+    shape = x.shape
+    if len(shape) < 2 or shape[-1] == 0:
+        raise ValueError(f"{what}: x is [N, .., C], got {tuple(shape)}")
+    n, c = shape[0], shape[-1]
     if groups < 1 or c % groups:
         raise ValueError(f"{what}: groups that divide the {c} channels, got {groups}")
-    at = math.prod(x.shape[1:-1])
-    rows = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.reshape(n, at, c)
-    return _last_contiguous(rows), n, at, c
+    if len(shape) == 2:
+        return _last_contiguous(x), n, 1, c
+    at = math.prod(shape[1:-1])
+    return _last_contiguous(x if len(shape) == 3 else x.reshape(n, at, c)), n, at, c
+
+
+def _sample_strides(rows: torch.Tensor) -> tuple:
+    """Distances of samples and of positions (of one position: the row's own width)."""
+    at = rows.stride()
+    return at[:2] if len(at) == 3 else (at[0], rows.shape[1])
+
+
+@functools.lru_cache(maxsize=256)
+def _group_norm_workspace(n: int, at: int, c: int, groups: int, grad: bool) -> int:
+    return lib().lng_group_norm_workspace_bytes(n, at, c, groups, int(grad))
 
 
 def group_norm(x: torch.Tensor, groups: int, w: torch.Tensor | None, b: torch.Tensor | None, eps: float, silu: bool = False,
                want_stats: bool = False):
     """Group norm of channels-last x ``[N, .., C]`` over all positions of a sample, with SiLU behind it where ``silu``
-    (``lng_group_norm``); w, b ``[C]`` in x's type or fp32, or None.  ``want_stats``: returns ``(y, mean, rstd)`` for
-    :func:`group_norm_grad`, fp32 ``[N, groups]``."""
+    (``lng_group_norm``); w, b ``[C]`` in x's type or fp32, or None.  ``want_stats``: returns ``(y, stats)`` for
+    :func:`group_norm_grad`, mean and rstd as fp32 ``[2, N, groups]``."""
+    y, stats, _, _ = group_norm_plan(x, groups, w, b, eps, silu, want_stats)
+    return (y, stats) if want_stats else y
+
+
+def group_norm_plan(x, groups: int, w, b, eps: float, silu: bool, want_stats: bool) -> tuple:
+    """:func:`group_norm`, and what its backward pass goes by: ``(y, stats, plan, tensors)`` for
+    :func:`group_norm_back`, which checks nothing again.  The tensors (rows, weight, bias) have to be the caller's to
+    keep until then."""
+    what = "group_norm"
     dev = _dev(x, w, b)
     wt = None if w is None else w.dtype
     bt = None if b is None else b.dtype
-    _float_rows("group_norm", x, wt, bt)
-    rows, n, at, c = _as_samples("group_norm", x, groups)
-    _expect("group_norm", "weight", w, c)
-    _expect("group_norm", "bias", b, c)
-    wc, bc = _whole(w), _whole(b)
+    _float_rows(what, x, wt, bt)
+    rows, n, at, c = _as_samples(what, x, groups)
+    _expect(what, "weight", w, c)
+    _expect(what, "bias", b, c)
+    w, b = _whole(w), _whole(b)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean = rstd = ws = None
+    stats = ws = None
+    mean = rstd = None
     if want_stats:
-        mean, rstd = (torch.empty(n, groups, dtype=torch.float32, device=dev) for _ in range(2))
-    size = lib().lng_group_norm_workspace_bytes(n, at, c, groups, 0)
+        stats = torch.empty((2, n, groups), dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n * groups
+    size = _group_norm_workspace(n, at, c, groups, False)
     if size:
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    _call("group_norm", dev, lib().lng_group_norm, rows.data_ptr(), _DT[x.dtype], n, at, c, groups, rows.stride(0),
-          rows.stride(1), _ptr(wc), _ptr(bc), _DT[wt or bt or x.dtype], eps, int(silu), _ptr(ws), size, y.data_ptr(),
-          _ptr(mean), _ptr(rstd))
-    return (y, mean, rstd) if want_stats else y
+    xs, xl = _sample_strides(rows)
+    wt = wt or bt or x.dtype
+    if x.numel():
+        _call(what, dev, lib().lng_group_norm, rows.data_ptr(), _DT[x.dtype], n, at, c, groups, xs, xl, _ptr(w), _ptr(b),
+              _DT[wt], eps, int(silu), _ptr(ws), size, y.data_ptr(), mean, rstd)
+    return y, stats, (dev, x.shape, x.dtype, n, at, c, groups, wt, int(silu)), (rows, w, b)
 
 
 def group_norm_grad(dy: torch.Tensor, x: torch.Tensor, groups: int, w: torch.Tensor | None, b: torch.Tensor | None,
-                    silu: bool, mean: torch.Tensor, rstd: torch.Tensor, want=(True, True, True),
-                    w_dtype: torch.dtype | None = None) -> tuple:
+                    silu: bool, stats: torch.Tensor, want=(True, True, True), w_dtype: torch.dtype | None = None) -> tuple:
     """``(dx, dw, db)`` of :func:`group_norm` (``lng_group_norm_grad``), None where not wanted; dw and db in
     ``w_dtype`` (None: the weight's type)."""
     what = "group_norm_grad"
-    dev = _dev(dy, x, w, b, mean, rstd)
+    dev = _dev(dy, x, w, b, stats)
     if dy.shape != x.shape:
         raise ValueError(f"{what}: dy {tuple(dy.shape)}, expected {tuple(x.shape)}")
     if dy.dtype != x.dtype:
@@ -1519,22 +1545,36 @@ def group_norm_grad(dy: torch.Tensor, x: torch.Tensor, groups: int, w: torch.Ten
     for t in (w, b):
         _float_rows(what, x, wt, None if t is None else t.dtype)
     rows, n, at, c = _as_samples(what, x, groups)
-    grads = _as_samples(what, dy, groups)[0]
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _expect(what, name, t, n, groups)
-        if t.dtype != torch.float32 or not t.is_contiguous():
-            raise TypeError(f"{what}: {name} as group_norm gave it")
+    _expect(what, "stats", stats, 2, n, groups)
+    if stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise TypeError(f"{what}: stats as group_norm gave them")
     _expect(what, "weight", w, c)
     _expect(what, "bias", b, c)
-    wc, bc = _whole(w), _whole(b)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    return group_norm_back((dev, x.shape, x.dtype, n, at, c, groups, wt, int(silu)),
+                           (rows, _whole(w), _whole(b), stats), dy, want)
+
+
+def group_norm_back(plan: tuple, tensors, dy: torch.Tensor, want) -> tuple:
+    """:func:`group_norm_grad` by the plan of :func:`group_norm_plan`.  The tensors may have been moved since (saved-tensor
+    hooks): their addresses and strides are taken anew."""
+    dev, shape, kind, n, at, c, groups, wt, silu = plan
+    rows, w, b, stats = tensors
+    rows, w, b = _last_contiguous(rows), _whole(w), _whole(b)
+    xs, xl = _sample_strides(rows)
+    dx = torch.empty(shape, dtype=kind, device=dev) if want[0] else None
     dw = torch.empty(c, dtype=wt, device=dev) if want[1] else None
     db = torch.empty(c, dtype=wt, device=dev) if want[2] else None
-    size = lib().lng_group_norm_workspace_bytes(n, at, c, groups, 1)
+    if dy.is_contiguous():
+        ds, dl = at * c, c
+    else:
+        dy = _as_samples("group_norm_grad", dy, groups)[0]
+        ds, dl = _sample_strides(dy)
+    size = _group_norm_workspace(n, at, c, groups, True)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    _call(what, dev, lib().lng_group_norm_grad, grads.data_ptr(), grads.stride(0), grads.stride(1), rows.data_ptr(),
-          rows.stride(0), rows.stride(1), _DT[x.dtype], n, at, c, groups, _ptr(wc), _ptr(bc), _DT[wt], int(silu),
-          mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), size, _ptr(dx), _ptr(dw), _ptr(db))
+    mean = stats.data_ptr()
+    _call("group_norm_grad", dev, lib().lng_group_norm_grad, dy.data_ptr(), ds, dl, rows.data_ptr(), xs, xl, _DT[kind], n, at, c,
+          groups, _ptr(w), _ptr(b), _DT[wt], silu, mean, mean + 4 * n * groups, ws.data_ptr(), size, _ptr(dx), _ptr(dw),
+          _ptr(db))
     return dx, dw, db
 
 
@@ -1794,49 +1834,69 @@ _LINEAR = struct.Struct("2q8ifi3P9qP2q5P")
 
 
 def _linear_args(what: str, q, k, v, decay, scale, state, lengths, y, state_out, dims: int, checkpoints=None):
-    """``(lng_linear_attention, tensors to keep alive)`` of a linear attention's checked arguments; dims 4:
-    ``[B, T, heads, width]`` tensors, 3: ``[B, heads, width]`` (one token).  ``y`` is made where it is None."""
-    lead, kind, h, keys, values = q.shape[:-2], q.dtype, decay.shape[-1], q.shape[-1], v.shape[-1]
-    b, t = lead[0], lead[1] if dims == 4 else 1
+    """``(lng_linear_attention, (q, k, v, decay, state, lengths), shapes)`` of a linear attention's checked arguments,
+    the tensors as the kernels read them; dims 4: ``[B, T, heads, width]`` tensors, 3: ``[B, heads, width]`` (one token)."""
+    qs, ks, vs, gs, kind = q.shape, k.shape, v.shape, decay.shape, q.dtype
+    lead, h, keys, values, hq, hk, hv = qs[:-2], gs[-1], qs[-1], vs[-1], qs[-2], ks[-2], vs[-2]
     if k.dtype != kind or v.dtype != kind or kind not in _FLOATS:
         raise TypeError(f"{what}: q, k and v in one type, fp32, bf16 or fp16")
-    if k.dim() != dims or v.dim() != dims or k.shape[:-2] != lead or v.shape[:-2] != lead or k.shape[-1] != keys:
-        raise ValueError(f"{what}: q {tuple(q.shape)} with k {tuple(k.shape)} and v {tuple(v.shape)}")
+    if ks[:-2] != lead or vs[:-2] != lead or ks[-1] != keys:
+        raise ValueError(f"{what}: q {tuple(qs)} with k {tuple(ks)} and v {tuple(vs)}")
     if not 1 <= keys <= 128 or not 1 <= values <= 128:
         raise ValueError(f"{what}: heads of 1 to 128 keys and values, got {keys} and {values}")
-    token = decay.dim() > 1
-    if decay.dtype != torch.float32 or (token and decay.shape[:-1] != lead):
-        raise ValueError(f"{what}: log decays in float32, [H] or {[*lead, 'H']}, got {decay.dtype} {tuple(decay.shape)}")
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        if x.shape[-2] == 0 or h == 0 or h % x.shape[-2]:
-            raise ValueError(f"{what}: the heads of q, k and v divide the {h} of the decays, got {x.shape[-2]} of {name}")
-    _expect(what, "state", state, b, h, keys, values)
-    if state is not None and state.dtype != torch.float32:
-        raise TypeError(f"{what}: states are float32")
+    token = len(gs) > 1
+    if decay.dtype != torch.float32 or (token and gs[:-1] != lead):
+        raise ValueError(f"{what}: log decays in float32, [H] or {[*lead, 'H']}, got {decay.dtype} {tuple(gs)}")
+    if h == 0 or hq == 0 or hk == 0 or hv == 0 or h % hq or h % hk or h % hv:
+        raise ValueError(f"{what}: the heads of q, k and v divide the {h} of the decays, got {hq}, {hk} and {hv}")
+    b, t = lead[0], lead[1] if dims == 4 else 1
+    if state is not None:
+        _expect(what, "state", state, b, h, keys, values)
+        if state.dtype != torch.float32:
+            raise TypeError(f"{what}: states are float32")
     ln = _lengths32(what, lengths, b, t)
-    q, k, v, decay, state = (_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), _last_contiguous(decay),
-                             _whole(state))
-    qs, ks, vs, ds = q.stride(), k.stride(), v.stride(), decay.stride()
-    at = (lambda s: s[:3]) if dims == 4 else (lambda s: (s[0], 0, s[1]))
     scale = keys ** -0.5 if scale is None else float(scale)
-    a = _lib.LinearAttention.from_buffer_copy(_LINEAR.pack(
-        b, t, h, q.shape[-2], k.shape[-2], v.shape[-2], keys, values, _DT[kind], int(token), scale, 0, q.data_ptr(),
-        k.data_ptr(), v.data_ptr(), *at(qs), *at(ks), *at(vs), decay.data_ptr(), ds[0] if token else 0,
-        ds[1] if token and dims == 4 else 0, _ptr(state) or 0, _ptr(ln) or 0, _ptr(y) or 0, _ptr(state_out) or 0,
-        _ptr(checkpoints) or 0))
-    return a, (q, k, v, decay, state, ln)
+    shapes = (b, t, h, hq, hk, hv, keys, values, _DT[kind], token, scale, 0)
+    tensors = (q, k, v, decay, state, ln)
+    a, keep = _linear_pack(shapes, tensors, y, state_out, checkpoints, dims)
+    return a, keep, shapes
 
 
-def _linear_shapes(what: str, q: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, dims: int) -> None:
-    if q.dim() != dims or v.dim() != dims or decay.dim() not in (1, dims - 1):
-        raise ValueError(f"{what}: q and v are {'[B, T, heads, width]' if dims == 4 else '[B, heads, width]'} and log "
-                         f"decays [H] or one a token and head, got {tuple(q.shape)}, {tuple(v.shape)} and "
-                         f"{tuple(decay.shape)}")
+def _linear_pack(shapes: tuple, tensors: tuple, y, state_out, checkpoints, dims: int) -> tuple:
+    """``(lng_linear_attention, tensors as the kernels read them)`` of checked arguments."""
+    q, k, v, decay, state, ln = tensors
+    (q, qs), (k, ks), (v, vs), (decay, gs) = _strided(q), _strided(k), _strided(v), _strided(decay)
+    token = shapes[9]
+    if dims == 4:
+        strides = (*qs[:3], *ks[:3], *vs[:3])
+        ds = gs[:2] if token else (0, 0)
+    else:
+        strides = (qs[0], 0, qs[1], ks[0], 0, ks[1], vs[0], 0, vs[1])
+        ds = (gs[0], 0) if token else (0, 0)
+    state = _whole(state)
+    return _lib.LinearAttention.from_buffer_copy(_LINEAR.pack(
+        *shapes, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, decay.data_ptr(), *ds,
+        *(0 if x is None else x.data_ptr() for x in (state, ln, y, state_out, checkpoints)))), (q, k, v, decay, state, ln)
 
 
-def _linear_workspace(a, grad: bool, dev: torch.device) -> torch.Tensor:
-    return torch.empty(lib().lng_linear_attention_workspace_bytes(ctypes.byref(a), int(grad)), dtype=torch.uint8,
-                       device=dev)
+def _strided(x: torch.Tensor) -> tuple:
+    """A tensor whose last dimension is contiguous, and its strides."""
+    at = x.stride()
+    if at[-1] != 1 and x.shape[-1] != 1:
+        x = x.contiguous()
+        at = x.stride()
+    return x, at
+
+
+def _linear_shapes(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, dims: int) -> None:
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims or decay.dim() not in (1, dims - 1):
+        raise ValueError(f"{what}: q, k and v are {'[B, T, heads, width]' if dims == 4 else '[B, heads, width]'} and log "
+                         f"decays [H] or one a token and head, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} "
+                         f"and {tuple(decay.shape)}")
+
+
+def _linear_workspace(a, grad: bool) -> int:
+    return lib().lng_linear_attention_workspace_bytes(ctypes.byref(a), int(grad))
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, scale: float | None = None,
@@ -1845,26 +1905,33 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     """``(y, final state or None, checkpoints or None)`` of linear attention (``lng_linear_attention_scan``) of
     q ``[B, T, Hq, K]``, k ``[B, T, Hk, K]``, v ``[B, T, Hv, V]`` with log decays ``[H]`` or ``[B, T, H]`` in
     fp32; the checkpoints are what :func:`linear_attention_grad` takes."""
+    return linear_attention_plan(q, k, v, decay, scale, state, lengths, want_state, want_checkpoints)[:3]
+
+
+def linear_attention_plan(q, k, v, decay, scale, state, lengths, want_state: bool, want_checkpoints: bool) -> tuple:
+    """:func:`linear_attention`, and what its backward pass goes by: ``(y, state, checkpoints, plan, tensors)`` for
+    :func:`linear_attention_back`, which checks nothing again.  The tensors (checkpoints, q, k, v, decays, state and
+    lengths) have to be the caller's to keep until then."""
     what = "linear_attention"
     dev = _dev(q, k, v, decay, state, lengths)
-    _linear_shapes(what, q, v, decay, 4)
+    _linear_shapes(what, q, k, v, decay, 4)
     b, t, _, keys = q.shape
     h, values = decay.shape[-1], v.shape[-1]
-    y = torch.empty(b, t, h, values, dtype=q.dtype, device=dev)
+    y = torch.empty((b, t, h, values), dtype=q.dtype, device=dev)
     end = ckpt = None
     if want_state:
-        end = torch.empty(b, h, keys, values, dtype=torch.float32, device=dev)
+        end = torch.empty((b, h, keys, values), dtype=torch.float32, device=dev)
     if want_checkpoints:
         ckpt = torch.empty(lib().lng_linear_attention_checkpoints(b, t, h, keys, values, dtype_code(q.dtype)),
                            dtype=torch.float32, device=dev)
-    a, keep = _linear_args(what, q, k, v, decay, scale, state, lengths, y, end, 4, ckpt)
+    a, keep, shapes = _linear_args(what, q, k, v, decay, scale, state, lengths, y, end, 4, ckpt)
     if b and t:
-        ws = _linear_workspace(a, False, dev)
-        _call(what, dev, lib().lng_linear_attention_scan, ctypes.byref(a), ws.data_ptr(), ws.numel())
+        size = _linear_workspace(a, False)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        _call(what, dev, lib().lng_linear_attention_scan, ctypes.byref(a), _ptr(ws), size)
     elif want_state:                                     # no tokens: the state passes through
         end.zero_() if state is None else end.copy_(state)
-    del keep
-    return y, end, ckpt
+    return y, end, ckpt, (shapes, dev), (ckpt, *keep)
 
 
 def linear_attention_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpoints: torch.Tensor, q: torch.Tensor,
@@ -1874,8 +1941,8 @@ def linear_attention_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpo
     given the gradients of y and of the final state (None: zero)."""
     what = "linear_attention_grad"
     dev = _dev(dy, dstate, checkpoints, q, k, v, decay, state, lengths)
-    _linear_shapes(what, q, v, decay, 4)
-    a, keep = _linear_args(what, q, k, v, decay, scale, state, lengths, None, None, 4, checkpoints)
+    _linear_shapes(what, q, k, v, decay, 4)
+    a, keep, shapes = _linear_args(what, q, k, v, decay, scale, state, lengths, None, None, 4, checkpoints)
     _expect(what, "dy", dy, a.B, a.T, a.H, a.V)
     _expect(what, "dstate", dstate, a.B, a.H, a.K, a.V)
     if dy.dtype != q.dtype or (dstate is not None and dstate.dtype != torch.float32):
@@ -1883,24 +1950,35 @@ def linear_attention_grad(dy: torch.Tensor, dstate: torch.Tensor | None, checkpo
     _expect(what, "checkpoints", checkpoints, lib().lng_linear_attention_checkpoints(a.B, a.T, a.H, a.K, a.V, a.dtype))
     if checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous():
         raise TypeError(f"{what}: checkpoints as linear_attention gave them")
-    dq, dk, dv = (torch.empty(x.shape, dtype=q.dtype, device=dev) for x in (q, k, v))
-    dg = torch.empty(decay.shape, dtype=torch.float32, device=dev)
-    ds = None if state is None else torch.empty(a.B, a.H, a.K, a.V, dtype=torch.float32, device=dev)
+    return linear_attention_back((shapes, dev), (checkpoints, *keep), dy, dstate)
+
+
+def linear_attention_back(plan: tuple, tensors, dy: torch.Tensor, dstate: torch.Tensor | None) -> tuple:
+    """:func:`linear_attention_grad` by the plan of :func:`linear_attention_plan`.  The tensors may have been moved since
+    (saved-tensor hooks): their addresses and strides are taken anew."""
+    what = "linear_attention_grad"
+    shapes, dev = plan
+    a, keep = _linear_pack(shapes, tensors[1:], None, None, tensors[0], 4)
+    _, q, k, v, decay, state, _ = tensors
+    dq, dk, dv, dg = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v, decay))
+    ds = None if state is None else torch.empty(state.shape, dtype=torch.float32, device=dev)
     if not (a.B and a.T):                                # no tokens: the state's gradient passes through
         for x in (dq, dk, dv, dg):
             x.zero_()
         if ds is not None:
             ds.zero_() if dstate is None else ds.copy_(dstate)
         return dq, dk, dv, dg, ds
-    dyc, dsc = _last_contiguous(dy), _whole(dstate)
-    at, size = dyc.stride(), dyc.element_size()
-    if a.V % 8 == 0 and (dyc.data_ptr() % 16 or any(n * size % 16 for n in at[:3]) or at[1] * size >= 1 << 25):
-        dyc = _c(dyc.contiguous())                       # read in 16-byte pieces
-        at = dyc.stride()
-    g = _lib.LinearAttentionGrad(dyc.data_ptr(), *at[:3], _ptr(dsc), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    (dy, at), dstate = _strided(dy), _whole(dstate)
+    es = 4 if a.dtype == F32 else 2
+    if a.V % 8 == 0 and (dy.data_ptr() % 16 or at[0] * es % 16 or at[1] * es % 16 or at[2] * es % 16
+                         or at[1] * es >= 1 << 25):
+        dy = _c(dy.contiguous())                         # read in 16-byte pieces
+        at = dy.stride()
+    g = _lib.LinearAttentionGrad(dy.data_ptr(), *at[:3], _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                  dg.data_ptr(), _ptr(ds))
-    ws = _linear_workspace(a, True, dev)
-    _call(what, dev, lib().lng_linear_attention_scan_grad, ctypes.byref(a), ctypes.byref(g), ws.data_ptr(), ws.numel())
+    size = _linear_workspace(a, True)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call(what, dev, lib().lng_linear_attention_scan_grad, ctypes.byref(a), ctypes.byref(g), _ptr(ws), size)
     del keep
     return dq, dk, dv, dg, ds
 
@@ -1913,14 +1991,14 @@ def linear_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     what = "linear_attention_step"
     out = state if out_state is None else out_state
     dev = _dev(state, q, k, v, decay, out)
-    _linear_shapes(what, q, v, decay, 3)
+    _linear_shapes(what, q, k, v, decay, 3)
     if not state.is_contiguous() or not out.is_contiguous() or out.dtype != torch.float32:
         raise ValueError(f"{what}: states are contiguous float32 [B, H, K, V]")
     if out is not state:
         _expect(what, "out_state", out, *state.shape)
         _separate(what, "out_state", out, state)
-    y = torch.empty(q.shape[0], decay.shape[-1], v.shape[-1], dtype=q.dtype, device=dev)
-    a, keep = _linear_args(what, q, k, v, decay, scale, state, None, y, out, 3)
+    y = torch.empty((q.shape[0], decay.shape[-1], v.shape[-1]), dtype=q.dtype, device=dev)
+    a, keep, _ = _linear_args(what, q, k, v, decay, scale, state, None, y, out, 3)
     _call(what, dev, lib().lng_linear_attention_step, ctypes.byref(a))
     torch.autograd.graph.increment_version(out)
     del keep

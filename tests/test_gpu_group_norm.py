@@ -187,6 +187,22 @@ def test_equal_calls_other_stream_and_graph(dev):
             assert all(torch.equal(p, q) for p, q in zip(out, ref)), rep
 
 
+def test_saved_tensors_that_move(dev):
+    """What a graph keeps may come back elsewhere and in another layout (offloaded activations)."""
+    wide = torch.randn(3, 40, 200, device=dev)
+    for x in (wide[..., 3:67], wide[:, 0, 8:72]):
+        _, w, b, dy = _make(dev, tuple(x.shape), FP, FP)
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        with torch.autograd.graph.save_on_cpu():
+            y = group_norm(leaves[0], 4, leaves[1], leaves[2], activation="silu")
+        # rows of another address are read in other pieces and summed in another order: within the bounds of any call
+        xd, wd, bd, gd = (to64(t) for t in (x, w, b, dy))
+        args = (gd, xd, 4, wd, bd, 1e-5, True)
+        for got, want, mag, k in zip(torch.autograd.grad(y, leaves, dy), oa.group_norm_grad(*args),
+                                     oa.group_norm_grad(*args, mag=True), (2 * K, K + 120, K + 120)):
+            within(got, want, mag, k)
+
+
 def test_module_and_refusals(dev):
     m = GroupNorm(4, 32, activation="silu").to(dev)
     x = torch.randn(3, 5, 32, device=dev)

@@ -346,6 +346,20 @@ def test_two_captured_calls_keep_apart(dev):
         assert all(torch.equal(p, q) for o, w in zip(outs, want) for p, q in zip(o, w))
 
 
+def test_saved_tensors_that_move(dev):
+    """What a graph keeps may come back elsewhere and in another layout (offloaded activations)."""
+    s = _make(dev, 2, 90, 4, 32, 32, hk=2, dtype=BF)
+    wide = torch.randn(2, 90, 300, device=dev).to(BF)
+    s.update(q=wide[..., 8:136].unflatten(-1, (4, 32)), k=wide[..., 137:201].unflatten(-1, (2, 32)))
+    leaves = {k: s[k].detach().requires_grad_(True) for k in LEAVES}
+    want = torch.autograd.grad(_call(s, leaves), list(leaves.values()), [s["dy"], s["dend"]])
+    with torch.autograd.graph.save_on_cpu():
+        out = _call(s, leaves)
+    junk = [torch.full_like(wide, float("nan")) for _ in range(8)]
+    got = torch.autograd.grad(out, list(leaves.values()), [s["dy"], s["dend"]])
+    assert all(torch.equal(p, q) for p, q in zip(got, want)) and len(junk) == 8
+
+
 def test_refusals(dev):
     s = _make(dev, 2, 6, 4, 16, 8, hk=2, hv=2, dtype=BF)
     z = lambda *n, dt=BF: torch.zeros(*n, device=dev, dtype=dt)  # noqa: E731
