@@ -1000,7 +1000,8 @@ int lng_group_norm(const void* x, int dtype, int64_t N, int64_t L, int32_t C, in
   const int es = dtype_size(dtype);
   const Plan p = make_plan(a, C % VEC == 0 && vector_rows(x, x_sample, x_row, N, L, es) && aligned(y, 16), false);
   if (int rc = check_blocks(what, p)) return rc;
-  if (space_of(p) && (!workspace || !aligned(workspace, 64) || workspace_bytes < static_cast<size_t>(space_of(p)) * 4))
+  const size_t need = lng_group_norm_workspace_bytes(N, L, C, G, 0);
+  if (need && (!workspace || !aligned(workspace, 64) || workspace_bytes < need))
     return fail(LNG_E_ARG, "group_norm: the workspace is too small or not 64-byte aligned");
   a.stats = static_cast<float*>(workspace);
   if (p.form == Form::passes && !mean) a.mean = a.stats + p.own, a.rstd = a.mean + N * G;
@@ -1029,7 +1030,7 @@ int lng_group_norm_grad(const void* dy, int64_t dy_sample, int64_t dy_row, const
   const Plan p = make_plan(a, C % VEC == 0 && vector_rows(x, x_sample, x_row, N, L, es) &&
                                   vector_rows(dy, dy_sample, dy_row, N, L, es) && aligned(dx, 16), true);
   if (int rc = check_blocks(what, p)) return rc;
-  if (!workspace || !aligned(workspace, 64) || workspace_bytes < static_cast<size_t>(space_of(p)) * 4)
+  if (!workspace || !aligned(workspace, 64) || workspace_bytes < lng_group_norm_workspace_bytes(N, L, C, G, 1))
     return fail(LNG_E_ARG, "group_norm_grad: the workspace is too small or not 64-byte aligned");
   a.stats = static_cast<float*>(workspace);
   a.cols = cols || p.form == Form::passes ? a.stats + cdiv(p.stats, 16) * 16 : nullptr;

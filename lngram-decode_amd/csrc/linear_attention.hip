@@ -1330,6 +1330,18 @@ int check_threads(const char* what, int64_t blocks, int threads) {
   return fail(LNG_E_ARG, std::string(what) + ": too many sequences, heads or tokens for one launch; split the batch");
 }
 
+// Every launch of a call, before its first
+int check_launches(const char* what, const Args& a, bool grad) {
+  const int64_t rows = a.B * a.T;
+  int64_t most = a.B * a.H * std::max<int64_t>(int64_t{a.vts} * a.segs, cdiv(int64_t{a.K} * a.V, 256));
+  auto packed = [&](bool vec, int heads, int width) {
+    if (!vec) most = std::max(most, cdiv(rows * heads * (width / 8), 256));
+  };
+  packed(a.qvec, a.Hq, a.Kp), packed(a.kvec, a.Hk, a.Kp), packed(a.vvec, a.Hv, a.Vp);
+  if (grad) packed(a.V % 8 == 0, a.H, a.Vp), most = std::max(most, cdiv(rows * a.H * std::max(a.K, a.V), 256));
+  return check_threads(what, most, 256);
+}
+
 template <typename F>
 int launch(F* kernel, unsigned blocks, unsigned threads, size_t lds, hipStream_t st, const Args& a, const char* what) {
   if (lds > 64 * 1024) {
@@ -1450,8 +1462,7 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
   if (s.total && (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 ||
                   reinterpret_cast<uintptr_t>(workspace) % 64))
     return fail(LNG_E_ARG, "linear_attention: the workspace is too small or not 64-byte aligned");
-  if (int rc = check_threads(what, a.B * a.H * std::max<int64_t>(a.vts * a.segs, cdiv(int64_t{a.K} * a.V, 256)), 256))
-    return rc;
+  if (int rc = check_launches(what, a, false)) return rc;
   float* const ws = static_cast<float*>(workspace);
   a.seg_state = ws + s.seg_state, a.seg_decay = ws + s.seg_decay;
   return with_type(args->dtype, [&](auto t) {
@@ -1481,12 +1492,10 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
                   reinterpret_cast<uintptr_t>(workspace) % 64))
     return fail(LNG_E_ARG, "linear_attention_grad: the workspace is too small or not 64-byte aligned");
   const int64_t rows = a.B * a.T, hv = int64_t{a.H} * a.vts;
-  if (int rc = check_threads(what, a.B * a.H * std::max<int64_t>(a.vts * a.segs, cdiv(int64_t{a.K} * a.V, 256)), 256))
-    return rc;
+  if (int rc = check_launches(what, a, true)) return rc;
   a.dy = g.dy, a.yb = g.dy_batch, a.yt = g.dy_token, a.yh = g.dy_head;
   if (a.V % 8 == 0 && !vector_rows(a.dy, es, a.yb, a.yt, a.yh, a.V))
     return fail(LNG_E_ARG, "linear_attention_grad: rows of dy in 16-byte pieces, less than 2^25 bytes apart");
-  if (int rc = check_threads(what, cdiv(rows * a.H * std::max(a.K, a.V), 256), 256)) return rc;
   float* const ws = static_cast<float*>(workspace);
   a.seg_state = ws + s.seg_state, a.seg_decay = ws + s.seg_decay;
   a.dend = g.dstate_out, a.dstart = g.dstate;

@@ -105,6 +105,25 @@ class _Linear(torch.autograd.Function):
                 torch.mm(d2.t(), x2) if ctx.needs_input_grad[1] else None)
 
 
+def project(x: Tensor, w: nn.Linear) -> Tensor:
+    """``x . w^T``, differentiable; rows of a width that the bf16 product does not read are padded."""
+    weight, odd = w.weight, -x.shape[-1] % 8
+    if odd and x.dtype == torch.bfloat16:                # it reads 16 bytes at a time
+        x, weight = nn.functional.pad(x, (0, odd)), nn.functional.pad(weight, (0, odd))
+    if needs_grad(x, weight):
+        return _Linear.apply(x, weight)
+    return ops.linear(x, weight)
+
+
+def own_rows(emb: Tensor, lengths: Optional[Tensor]) -> Tensor:
+    """A training batch with zeros behind its sequences: the gradients of norms and products sum over every row, those
+    behind a sequence's end with a factor of zero, and a NaN there would come through."""
+    if lengths is None or lengths.shape != emb.shape[:1] or not torch.is_grad_enabled():
+        return emb
+    behind = torch.arange(emb.shape[1], device=emb.device) >= lengths[:, None]
+    return emb.masked_fill(behind[..., None], 0)
+
+
 class SelectiveSSM(nn.Module):
     """Selective SSM whose output is the token router's SSM context: ``state_dim`` features a token, as
     ``DiagonalSSM``'s, from ``d_state`` states a feature.
@@ -145,20 +164,12 @@ class SelectiveSSM(nn.Module):
         return (w.new_zeros(batch, self.conv_kernel - 1, self.state_dim),
                 torch.zeros(batch, self.state_dim, self.d_state, dtype=torch.float32, device=w.device))
 
-    def _linear(self, x: Tensor, w: nn.Linear) -> Tensor:
-        weight, odd = w.weight, -x.shape[-1] % 8
-        if odd and x.dtype == torch.bfloat16:            # the bf16 product reads 16 bytes at a time
-            x, weight = nn.functional.pad(x, (0, odd)), nn.functional.pad(weight, (0, odd))
-        if needs_grad(x, weight):
-            return _Linear.apply(x, weight)
-        return ops.linear(x, weight)
-
     def _inputs(self, emb: Tensor) -> tuple:
-        return self._linear(self.norm(emb.to(self.w_in.weight.dtype)), self.w_in).chunk(2, dim=-1)
+        return project(self.norm(emb.to(self.w_in.weight.dtype)), self.w_in).chunk(2, dim=-1)
 
     def _selection(self, u: Tensor) -> tuple:
-        low, bm, cm = self._linear(u, self.w_x).split((self.dt_rank, self.d_state, self.d_state), dim=-1)
-        return self._linear(low, self.w_dt), bm, cm
+        low, bm, cm = project(u, self.w_x).split((self.dt_rank, self.d_state, self.d_state), dim=-1)
+        return project(low, self.w_dt), bm, cm
 
     def forward(self, emb: Tensor, state: Optional[tuple] = None, lengths: Optional[Tensor] = None,
                 return_state: bool = False):
@@ -166,12 +177,7 @@ class SelectiveSSM(nn.Module):
         sequence start); with ``return_state`` also the state after each sequence's last own token.  ``lengths
         [B]``: the sequences' own tokens; what stands behind them has no part in features, state or gradients."""
         hist, scan = (None, None) if state is None else state
-        if lengths is not None and lengths.shape == emb.shape[:1] and torch.is_grad_enabled():
-            # the gradients of the norm and of the products sum over every row, those behind a sequence's end
-            # with a factor of zero: a NaN there would come through
-            behind = torch.arange(emb.shape[1], device=emb.device) >= lengths[:, None]
-            emb = emb.masked_fill(behind[..., None], 0)
-        x, z = self._inputs(emb)
+        x, z = self._inputs(own_rows(emb, lengths))
         u, hist = short_conv(x, self.conv.weight, self.conv.bias, history=hist, lengths=lengths, return_history=True)
         dt, bm, cm = self._selection(u)
         out = selective_scan(u, dt, -torch.exp(self.A_log.float()), bm, cm, D=self.D, z=z, dt_bias=self.dt_bias,
