@@ -385,6 +385,13 @@ __device__ __forceinline__ float load_decay(const float* g, int64_t stride, int 
 constexpr uint32_t NOWHERE = 0x7ffffff0u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t from(const void* base) { return dev_buf(base, NOWHERE); }
 
+// A value that is formed anew where it is used: the places of results, the same in every chunk, would take dozens of
+// registers through the whole loop, and spilling others costs a wait for all stores on their way.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // four neighbouring values of a row of an output, as far as it goes (left > 0 in some lane at most)
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void store_four(__amdgpu_buffer_rsrc_t rs, uint32_t off, int left, const f32x4& x) {
@@ -488,7 +495,7 @@ struct FwdLds {
 // A block of NW waves takes a head's 16 NW value columns over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
 template <typename T, int DK, int NW, bool ENDS>
-__global__ __launch_bounds__(64 * NW, (DK <= 64 ? (ENDS ? 4 : 3) : (ENDS ? 3 : 2)) - (NW == 2 && DK > 32)) void k_la_fwd(Args a) {
+__global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : DK == 128 && NW == 2 ? 1 : 2) void k_la_fwd(Args a) {
   using L = FwdLds<T, DK, NW>;
   using Tr = Traits<T>;
   constexpr int C = L::C, W = L::W, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, THREADS = 64 * NW;
@@ -628,7 +635,7 @@ __global__ __launch_bounds__(64 * NW, (DK <= 64 ? (ENDS ? 4 : 3) : (ENDS ? 3 : 2
       Frag<PR> fs[TK / 2];
       state_frags(s, fs);
       const __amdgpu_buffer_rsrc_t yc = from(y + int64_t{t0} * yrow);
-      const int col = vc + 4 * lg;
+      const int col = anew(vc + 4 * lg);
       auto outputs = [&](auto count, int first) {
         constexpr int N = decltype(count)::value;
         f32x4 acc[N];
@@ -824,14 +831,12 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
   const bool k4 = a.K % 4 == 0, v4 = a.V % 4 == 0;
   // a lane's four values of a token's output: in the type, or in fp32 to be summed with others
   auto emit = [&](void* out, bool f32, int64_t first, int row, int i, int col, int left, bool vec, const f32x4& x) {
-    const uint32_t at = static_cast<uint32_t>(i * row + col);
-    if (f32) {
-      const __amdgpu_buffer_rsrc_t rs = from(static_cast<float*>(out) + first * row);
-      vec ? store_four<float, true>(rs, at * 4, left, x) : store_four<float, false>(rs, at * 4, left, x);
-    } else {
-      const __amdgpu_buffer_rsrc_t rs = from(static_cast<T*>(out) + first * row);
-      vec ? store_four<T, true>(rs, at * sizeof(T), left, x) : store_four<T, false>(rs, at * sizeof(T), left, x);
-    }
+    const uint32_t es = f32 ? 4 : sizeof(T), at = static_cast<uint32_t>(i * row + col) * es;
+    const __amdgpu_buffer_rsrc_t rs = from(static_cast<char*>(out) + first * row * es);
+    if (f32)
+      vec ? store_four<float, true>(rs, at, left, x) : store_four<float, false>(rs, at, left, x);
+    else
+      vec ? store_four<T, true>(rs, at, left, x) : store_four<T, false>(rs, at, left, x);
   };
   double seg = 0.;
   for (int c = c_end - 1; c >= c_first; --c) {
@@ -907,7 +912,11 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
         }
       };
       constexpr int ALL = TI * (TI + 1) / 2, EACH = (ALL + BW - 1) / BW;
-      scores(std::integral_constant<int, EACH>{}, w < ALL ? w : 0, ALL);
+#pragma unroll 1
+      for (int k = 0; k < EACH; ++k) {
+        const int idx = w + k * BW;
+        if (idx < ALL) scores(std::integral_constant<int, 1>{}, idx, idx + 1);
+      }
       __syncthreads();
     }
     if (w == BW - 1 && c > c_first) decays(lds.d[(c - 1) & 1], g_next, a.scale);
@@ -947,7 +956,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
           }
         }
         if (part == 0) sr += dot;
-        const int key = 16 * kt + 4 * lg;
+        const int key = anew(16 * kt + 4 * lg);
         auto tokens = [&](auto count, int first) {  // the tiles of tokens from `first` on
           constexpr int N = decltype(count)::value;
           f32x4 acc[N];
@@ -1022,7 +1031,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
       // dv: this wave's 16 columns
       Frag<3> fs[TK / 2];
       state_frags(s, fs);
-      const int col = vc + 4 * lg;
+      const int col = anew(vc + 4 * lg);
       auto values = [&](auto count, int first) {
         constexpr int N = decltype(count)::value;
         f32x4 acc[N];
