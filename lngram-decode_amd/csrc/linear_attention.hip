@@ -485,11 +485,11 @@ template <typename T, int DK, int NW>
 struct FwdLds {
   using Tr = Traits<T>;
   static constexpr int C = Tr::chunk, W = 16 * NW;
-  bf16 q[Tr::planes][C * DK];
   bf16 k[Tr::planes][C * DK];
   bf16 v[Tr::planes][C * W];
-  bf16 p[Tr::prec][tri(C / 16, 0)];
   Decays<C> d[2];
+  bf16 q[Tr::planes][C * DK];  // from here on: not for a segment's ends
+  bf16 p[Tr::prec][tri(C / 16, 0)];
 };
 
 // A block of NW waves takes a head's 16 NW value columns over a segment of chunks; a wave holds 16 columns of the
@@ -708,12 +708,25 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
   if (e >= KV) return;
   const float* from = BACK ? a.dend : a.start;
   float s = from ? from[bh * KV + e] : 0.f;
-  for (int i = 0; i < a.segs; ++i) {
-    const int seg = BACK ? a.segs - 1 - i : i;
-    float* at = a.seg_state + (bh * a.segs + seg) * KV + e;
-    const float add = i + 1 < a.segs ? *at : 0.f;
-    *at = s;
-    if (i + 1 < a.segs) s = fmaf(s, __builtin_amdgcn_exp2f(a.seg_decay[bh * a.segs + seg]), add);
+  // eight segments' terms asked for at once: the loads do not wait for each other
+  constexpr int N = 8;
+  for (int first = 0; first < a.segs; first += N) {
+    float* at[N];
+    float add[N], decay[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = min(first + n, a.segs - 1), seg = BACK ? a.segs - 1 - i : i;
+      at[n] = a.seg_state + (bh * a.segs + seg) * KV + e;
+      const bool has = i + 1 < a.segs;  // the last one's end is nobody's start
+      add[n] = has ? *at[n] : 0.f;
+      decay[n] = has ? a.seg_decay[bh * a.segs + seg] : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (first + n < a.segs) {
+        *at[n] = s;
+        s = fmaf(s, __builtin_amdgcn_exp2f(decay[n]), add[n]);
+      }
   }
 }
 
@@ -739,13 +752,13 @@ struct BwdLds {
   using Tr = Traits<T>;
   static constexpr int C = Tr::chunk, NR = Tr::planes > 2 ? 3 : 2;
   bf16 q[Tr::planes][C * DK];
-  bf16 k[Tr::planes][C * DK];
-  bf16 v[Tr::planes][C * VT];
   bf16 o[Tr::planes][C * VT];  // dy
+  Decays<C> d[2];
+  bf16 k[Tr::planes][C * DK];  // from here on: not for a segment's ends
+  bf16 v[Tr::planes][C * VT];
   bf16 p[Tr::prec][tri(C / 16, 0)];
   bf16 a[Tr::prec][tri(C / 16, 0)];
-  bf16 r[NR][VT * DK];         // R, rows of values
-  Decays<C> d[2];
+  bf16 r[NR][VT * DK];         // R, rows of values: its parts in dk
   float row[C / 16][C];        // sums over a tile's j of P (dy.v), below the diagonal
   float col[C / 16][C];        // over its i
   float qs[DK / 16][C];        // q[i].(scale e^{G[i]} S_in dy[i]) over 16 keys
@@ -922,18 +935,26 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
     if (w == BW - 1 && c > c_first) decays(lds.d[(c - 1) & 1], g_next, a.scale);
 
     if (!ENDS) {
+      // <S_in, R> of this wave's columns, in 32 bits: as the state lies in registers
+      f32x4 in[TK];
+      float sr = 0.f;
+      load_state(in, a.ckpt + (bh * a.chunks + c) * KV, a.K, a.V, vc);
+#pragma unroll
+      for (int t = 0; t < TK; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sr = fmaf(in[t][r], s[t][r], sr);
+      sr = wave_sum(sr);
+      if (lane == 0) lds.sr[w] = sr;
       // dq and dk: tiles of 16 keys and 16 tokens, a wave's share of the keys (of the tokens, where keys are few)
       constexpr int SHARE = TK >= BW ? 1 : BW / TK, KT = TK >= BW ? TK / BW : 1, IT = TI / SHARE > 0 ? TI / SHARE : 1;
       const __amdgpu_buffer_rsrc_t si = dev_buf(a.ckpt + (bh * a.chunks + c) * KV, 4u * a.K * a.V);
       const int part = w % SHARE;
-      float sr = 0.f;
 #pragma unroll 1
       for (int kk = 0; kk < KT; ++kk) {
         const int kt = w / SHARE * KT + kk;
         Frag<3> fs[VT / 32];  // S_in, rows of keys, index of values
         Frag<NR> fr[VT / 32];
         const int row = 16 * kt + li;
-        float dot = 0.f;      // this wave's share of <S_in, R>
 #pragma unroll
         for (int st = 0; st < VT / 32; ++st) {
           fr[st] = by_col<NR, DK>(lds.r[0], RP, 32 * st, 16 * kt);
@@ -949,13 +970,10 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
               for (int i = 0; i < 4; ++i)
                 x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, col + i < a.V ? at + 4 * i : NOWHERE, 0, 0));
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dot = fmaf(x[i], value(fr[st], 4 * h + i), dot);
             put2(fs[st], 4 * h, x[0], x[1]);
             put2(fs[st], 4 * h + 2, x[2], x[3]);
           }
         }
-        if (part == 0) sr += dot;
         const int key = anew(16 * kt + 4 * lg);
         auto tokens = [&](auto count, int first) {  // the tiles of tokens from `first` on
           constexpr int N = decltype(count)::value;
@@ -1020,8 +1038,6 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
         };
         SHARE == 1 ? tokens(std::integral_constant<int, IT>{}, 0) : tokens(std::integral_constant<int, IT>{}, part * IT);
       }
-      sr = wave_sum(sr);
-      if (lane == 0) lds.sr[w] = sr;
     }
     __builtin_amdgcn_sched_barrier(0);
     Frag<NP> fo[C / 32];  // dy: this wave's columns
@@ -1391,12 +1407,13 @@ int pack_inputs(Args& a, const Space& s, float* ws, hipStream_t st) {
 
 template <typename T, int DK, int NW>
 int run_fwd(const Args& a, hipStream_t st) {
-  constexpr size_t lds = sizeof(FwdLds<T, DK, NW>);
+  using L = FwdLds<T, DK, NW>;
+  constexpr size_t lds = sizeof(L);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
   const int64_t units = a.B * a.H * a.vts;
   if (a.segs > 1) {
-    if (int rc = launch(&k_la_fwd<T, DK, NW, true>, static_cast<unsigned>(units * (a.segs - 1)), 64 * NW, lds, st, a,
-                        "linear_attention"))
+    if (int rc = launch(&k_la_fwd<T, DK, NW, true>, static_cast<unsigned>(units * (a.segs - 1)), 64 * NW,
+                        offsetof(L, q), st, a, "linear_attention"))
       return rc;
     if (int rc = run_join<false>(a, st)) return rc;
   }
@@ -1406,12 +1423,13 @@ int run_fwd(const Args& a, hipStream_t st) {
 
 template <typename T, int DK>
 int run_bwd(const Args& a, hipStream_t st) {
-  constexpr size_t lds = sizeof(BwdLds<T, DK>);
+  using L = BwdLds<T, DK>;
+  constexpr size_t lds = sizeof(L);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
   const int64_t units = a.B * a.H * a.vts;
   if (a.segs > 1) {
-    if (int rc = launch(&k_la_bwd<T, DK, true>, static_cast<unsigned>(units * (a.segs - 1)), BTHREADS, lds, st, a,
-                        "linear_attention_grad"))
+    if (int rc = launch(&k_la_bwd<T, DK, true>, static_cast<unsigned>(units * (a.segs - 1)), BTHREADS,
+                        offsetof(L, k), st, a, "linear_attention_grad"))
       return rc;
     if (int rc = run_join<true>(a, st)) return rc;
   }

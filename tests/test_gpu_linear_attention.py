@@ -133,6 +133,25 @@ def test_decays_of_all_sizes(dev, dtype):
     _check(dict(s, decay=torch.full((4,), 0.05, device=dev)))
 
 
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (32, 128), (128, 48)])
+def test_decay_gradients_keep_the_states_digits(dev, dtype, dk, dv):
+    """States and their gradients that outweigh the tokens, all of one sign: a decay's gradient is then their product
+    to within the roundings of fp32.  A lane adds 4 to 32 products, a wave 64 lanes' in 6 steps, then 4 waves' and up to
+    2 tiles': 41; a chunk's step of either state rounds three times, over 7 chunks each: 42.  In 16 bits, where two parts
+    of a state would be short of up to 2^-15 of it, that shows."""
+    s = _make(dev, 2, 200, 2, dk, dv, dtype=dtype, rate=1e-3)
+    for n in ("q", "k", "v", "dy"):
+        s[n] = (s[n] * 2.0 ** -10).to(dtype)
+    for n in ("state", "dend"):
+        s[n] = 1 + s[n].abs()
+    decay = s["decay"].detach().requires_grad_(True)
+    _, end = _call(s, {"decay": decay})
+    got, = torch.autograd.grad(end, decay, s["dend"])
+    want = oa.linear_attention_grad(torch.zeros_like(to64(s["dy"])), to64(s["dend"]), **_exact(s))["decay"]
+    assert float(((to64(got) - want) / want).abs().max()) <= 84 * 2.0 ** -24
+
+
 def test_a_scale_of_ones_own(dev):
     _check(dict(_make(dev, 2, 70, 2, 32, 32, dtype=BF), scale=0.37))
 
