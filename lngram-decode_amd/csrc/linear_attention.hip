@@ -24,7 +24,7 @@ namespace lng {
 namespace {
 
 constexpr int MAX_D = 128;  // of keys and values
-constexpr int VT = 64;      // columns of values a block takes
+constexpr int VT = 64;      // columns of values a block of four waves takes
 
 // Planes: bf16 parts of an input; PREC: parts of a computed operand of a product whose result is rounded to the type.
 template <typename T>
@@ -75,7 +75,9 @@ struct Unit {  // one block's work
 };
 
 __device__ __forceinline__ Unit unit_of(const Args& a, int segs, int first_seg) {
-  int64_t u = blockIdx.x;
+  // Blocks go to the eight XCDs in turn: each is given neighbouring units, whose heads share keys and values in its L2.
+  const uint32_t each = gridDim.x / 8, more = gridDim.x % 8, xcd = blockIdx.x % 8;
+  int64_t u = xcd * each + min(xcd, more) + blockIdx.x / 8;
   Unit r;
   r.vt = static_cast<int>(u % a.vts), u /= a.vts;
   r.h = static_cast<int>(u % a.H), u /= a.H;
@@ -492,10 +494,10 @@ struct FwdLds {
   bf16 p[Tr::prec][tri(C / 16, 0)];
 };
 
-// A block of NW waves takes a head's 16 NW value columns over a segment of chunks; a wave holds 16 columns of the
+// A block of NW waves takes a head's values, up to 16 NW columns, over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
 template <typename T, int DK, int NW, bool ENDS>
-__global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : DK == 128 && NW == 2 ? 1 : 2) void k_la_fwd(Args a) {
+__global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) void k_la_fwd(Args a) {
   using L = FwdLds<T, DK, NW>;
   using Tr = Traits<T>;
   constexpr int C = L::C, W = L::W, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, THREADS = 64 * NW;
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : DK 
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Unit u = unit_of(a, ENDS ? a.segs - 1 : a.segs, 0);
   const int c_first = u.seg * a.seg_chunks, c_last = min(c_first + a.seg_chunks, a.chunks);
-  const int v0 = u.vt * VT, vc = v0 + 16 * w;  // the block's and the wave's first column
+  const int vc = 16 * w;  // the wave's first column
   const int64_t bh = u.b * a.H + u.h;
   const int64_t KV = int64_t{a.K} * a.V;
   const T* q = static_cast<const T*>(a.q) + u.b * a.qb + u.h / (a.H / a.Hq) * a.qh;
@@ -539,7 +541,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : DK 
     const int n = min(C, u.len - c * C);
     if (!ENDS) rq.load(q, static_cast<uint32_t>(a.qt) * sizeof(T), n, 0, a.Kp);
     rk.load(k, static_cast<uint32_t>(a.kt) * sizeof(T), n, 0, a.Kp);
-    rv.load(v, static_cast<uint32_t>(a.vt) * sizeof(T), n, v0, a.Vp);
+    rv.load(v, static_cast<uint32_t>(a.vt) * sizeof(T), n, 0, a.Vp);
     q += C * a.qt, k += C * a.kt, v += C * a.vt;
   };
   if (c_first < c_end) {
@@ -688,14 +690,14 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : DK 
   }
   if (ENDS) {
     store_state(s, a.seg_state + (bh * a.segs + u.seg) * KV, a.K, a.V, vc);
-    if (threadIdx.x == 0 && u.vt == 0) a.seg_decay[bh * a.segs + u.seg] = static_cast<float>(seg);
+    if (threadIdx.x == 0) a.seg_decay[bh * a.segs + u.seg] = static_cast<float>(seg);
     return;
   }
   // positions behind the sequence's end
   const int start = max(u.len, c_first * C), to = static_cast<int>(min(static_cast<int64_t>(c_last) * C, a.T));
-  const int cols = min(W, a.V - v0);
+  const int cols = a.V;
   for (int64_t i = threadIdx.x; i < int64_t{to - start} * cols; i += THREADS)
-    y[(start + i / cols) * a.H * a.V + v0 + i % cols] = from_f32<T>(0.f);
+    y[(start + i / cols) * a.H * a.V + i % cols] = from_f32<T>(0.f);
   if (a.end && u.seg == a.segs - 1) store_state(s, a.end + bh * KV, a.K, a.V, vc);
 }
 
@@ -1279,10 +1281,11 @@ bool vector_rows(const void* p, int es, int64_t batch, int64_t token, int64_t he
          d % 8 == 0 && token >= 0 && token * es < (int64_t{1} << 25);
 }
 
-// Blocks that a launch should have, two for each CU: a segment more costs the keys and values (the queries and dy) of all
-// but one segment a second time.  8 x 4096 x 16 x 64 in 128, 256, 384, 512, 768, 1024 blocks: 200, 154, 127, 108, 111,
-// 126 us; 1 x 16384 x 16 x 128 in 256, 512, 768, 1024: 209, 149, 163, 161; the training of 8 x 2048 x 16 x 64 with its
-// backward pass in 128, 256, 512, 768: 458, 330, 257, 308.
+// Blocks of four waves that a launch should have, two for each CU (of eight, one): a segment more costs the keys and
+// values (the queries and dy) of all but one segment a second time.  8 x 4096 x 16 x 64 in 128, 256, 384, 512, 768, 1024
+// blocks: 179, 144, 120, 104, 118, 116 us; 1 x 16384 x 16 x 128 in 256, 384, 512, 768, 1024: 220, 161, 126, 169, 143; the
+// training of 8 x 2048 x 16 x 64 with its backward pass in 128, 256, 384, 512, 768: 421, 285, 235, 210, 253.  Segments of
+// one chunk gain nothing: 3 x 777 x 6 x 40 from one chunk, two, three, four on: 26, 26, 30, 35 us.
 constexpr int64_t BLOCKS = 512;
 
 Args make_args(const lng_linear_attention& l) {
@@ -1406,11 +1409,13 @@ int pack_inputs(Args& a, const Space& s, float* ws, hipStream_t st) {
 }
 
 template <typename T, int DK, int NW>
-int run_fwd(const Args& a, hipStream_t st) {
+int run_fwd(const Args& args, hipStream_t st) {
   using L = FwdLds<T, DK, NW>;
   constexpr size_t lds = sizeof(L);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
-  const int64_t units = a.B * a.H * a.vts;
+  Args a = args;
+  a.vts = 1;  // a block takes all columns
+  const int64_t units = a.B * a.H;
   if (a.segs > 1) {
     if (int rc = launch(&k_la_fwd<T, DK, NW, true>, static_cast<unsigned>(units * (a.segs - 1)), 64 * NW,
                         offsetof(L, q), st, a, "linear_attention"))
@@ -1497,7 +1502,10 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
     return with_keys(a.K, [&](auto dk) {
       using T = decltype(t);
       constexpr int DK = decltype(dk)::value;
-      return a.V <= 32 ? run_fwd<T, DK, 2>(a, as_stream(stream)) : run_fwd<T, DK, 4>(a, as_stream(stream));
+      // Eight waves compute the scores of 128 columns once, and twice if they are blocks of four.  1 x 8192 tokens, 16
+      // heads of 64 keys and 128 values, bf16: 55 us and 58, of 128 keys 71 and 80, in fp32 99 and 101, 144 and 153.  Up to
+      // 64 columns they would leave half of the waves without work: 57 and 39.
+      return a.V <= 64 ? run_fwd<T, DK, 4>(a, as_stream(stream)) : run_fwd<T, DK, 8>(a, as_stream(stream));
     });
   });
 }
