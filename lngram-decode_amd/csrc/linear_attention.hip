@@ -494,6 +494,10 @@ struct FwdLds {
   bf16 p[Tr::prec][tri(C / 16, 0)];
 };
 
+// What bounds it: at 8 x 4096 x 16 x 64 (bf16) 73 us for 281 MB, 3.8 TB/s; at 1 x 16384 x 16 x 128 92 us with the vector unit
+// busy for 40 % and the matrix unit for 24 %: waits, at the two waves a SIMD that 220 to 250 registers allow (three spill).
+// The segments' ends: 34 us for 102 MB, and 44 us.
+//
 // A block of NW waves takes a head's values, up to 16 NW columns, over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
 template <typename T, int DK, int NW, bool ENDS>
@@ -749,6 +753,10 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 // One pass from the last chunk to the first reads q, k, v and dy once, and the states before the chunks, which the
 // forward pass kept.  Everything is linear in the value columns: a block takes up to 64 of them, and dq, dk and dg of
 // several such tiles are summed afterwards, as the gradients of shared heads are.
+//
+// 8 x 2048 x 16 x 64, bf16: 109 us for 313 MB; the vector unit is busy for 32 %, the matrix unit for 13 %: waits, at two waves
+// a SIMD.  (The scores' tiles one by one: side by side their registers spill, and a spill waits for the stores in flight,
+// 146 us.)  128 keys leave one wave a SIMD: 4 x 2048 x 16 x 128, both passes, 516 us.
 template <typename T, int DK>
 struct BwdLds {
   using Tr = Traits<T>;
@@ -792,7 +800,8 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
   constexpr int KP = C * DK, VP = C * VT, PP = tri(C / 16, 0), RP = VT * DK;  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar arithmetic
+  // scalar: transposing reads need all lanes, which a branch on a wave's number in a vector register does not promise
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Unit u = unit_of(a, ENDS ? a.segs - 1 : a.segs, ENDS ? 1 : 0);
   const int c_first = u.seg * a.seg_chunks, c_last = min(c_first + a.seg_chunks, a.chunks);
@@ -1196,7 +1205,8 @@ __global__ __launch_bounds__(256) void k_la_pack(const T* x, int64_t batch, int6
 
 // ------------------------------------------------------------------ one token
 // A wave takes 64 value columns of a head: lane l four of them, and of the keys every fourth part.  All of a lane's
-// state is asked for at once; the state is read and written where it stands, so that it may move on in place.
+// state is asked for at once; the state is read and written where it stands, so that it may move on in place.  512 x 16 x
+// 64 x 64, bf16 rows: 57 us for 273 MB, 4.8 TB/s.
 template <typename T, int NB, bool VEC>
 __global__ __launch_bounds__(256) void k_la_step(Args a, int64_t waves) {
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
