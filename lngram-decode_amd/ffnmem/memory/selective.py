@@ -164,12 +164,14 @@ class SelectiveSSM(nn.Module):
         return (w.new_zeros(batch, self.conv_kernel - 1, self.state_dim),
                 torch.zeros(batch, self.state_dim, self.d_state, dtype=torch.float32, device=w.device))
 
+    _linear = staticmethod(project)
+
     def _inputs(self, emb: Tensor) -> tuple:
-        return project(self.norm(emb.to(self.w_in.weight.dtype)), self.w_in).chunk(2, dim=-1)
+        return self._linear(self.norm(emb.to(self.w_in.weight.dtype)), self.w_in).chunk(2, dim=-1)
 
     def _selection(self, u: Tensor) -> tuple:
-        low, bm, cm = project(u, self.w_x).split((self.dt_rank, self.d_state, self.d_state), dim=-1)
-        return project(low, self.w_dt), bm, cm
+        low, bm, cm = self._linear(u, self.w_x).split((self.dt_rank, self.d_state, self.d_state), dim=-1)
+        return self._linear(low, self.w_dt), bm, cm
 
     def forward(self, emb: Tensor, state: Optional[tuple] = None, lengths: Optional[Tensor] = None,
                 return_state: bool = False):
