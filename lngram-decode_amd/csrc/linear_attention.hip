@@ -24,7 +24,7 @@ namespace lng {
 namespace {
 
 constexpr int MAX_D = 128;  // of keys and values
-constexpr int VT = 64;      // columns of values a block of four waves takes
+constexpr int VT = 64;      // columns of values that four waves take
 
 // Planes: bf16 parts of an input; PREC: parts of a computed operand of a product whose result is rounded to the type.
 template <typename T>
@@ -429,7 +429,7 @@ __device__ __forceinline__ uint32_t state_place(int V, int c0) {
 template <int TK>
 __device__ __forceinline__ void load_state(f32x4 (&s)[TK], const float* m, int K, int V, int c0) {
   const __amdgpu_buffer_rsrc_t rs = dev_buf(m, 4u * K * V);
-  const uint32_t at = state_place(V, c0);
+  const uint32_t at = anew(state_place(V, c0));
 #pragma unroll
   for (int t = 0; t < TK; ++t)
 #pragma unroll
@@ -439,7 +439,7 @@ __device__ __forceinline__ void load_state(f32x4 (&s)[TK], const float* m, int K
 template <int TK>
 __device__ __forceinline__ void store_state(const f32x4 (&s)[TK], float* m, int K, int V, int c0) {
   const __amdgpu_buffer_rsrc_t rs = dev_buf(m, 4u * K * V);
-  const uint32_t at = state_place(V, c0);
+  const uint32_t at = anew(state_place(V, c0));
 #pragma unroll
   for (int t = 0; t < TK; ++t)
 #pragma unroll
@@ -751,32 +751,30 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 // q.dq - k.dk, takes large terms from each other along the whole sequence; this one only within a chunk.
 //
 // One pass from the last chunk to the first reads q, k, v and dy once, and the states before the chunks, which the
-// forward pass kept.  Everything is linear in the value columns: a block takes up to 64 of them, and dq, dk and dg of
+// forward pass kept.  Everything is linear in the value columns: a block takes 16 BW of them, and dq, dk and dg of
 // several such tiles are summed afterwards, as the gradients of shared heads are.
 //
 // 8 x 2048 x 16 x 64, bf16: 109 us for 313 MB; the vector unit is busy for 32 %, the matrix unit for 13 %: waits, at two waves
-// a SIMD.  (The scores' tiles one by one: side by side their registers spill, and a spill waits for the stores in flight,
-// 146 us.)  128 keys leave one wave a SIMD: 4 x 2048 x 16 x 128, both passes, 516 us.
-template <typename T, int DK>
+// a SIMD.  Registers decide: the scores' tiles go one by one and operands are split where they are used, since a spill waits
+// for the stores in flight (146 us).
+template <typename T, int DK, int BW>
 struct BwdLds {
   using Tr = Traits<T>;
-  static constexpr int C = Tr::chunk, NR = Tr::planes > 2 ? 3 : 2;
+  static constexpr int C = Tr::chunk, W = 16 * BW, NR = Tr::planes > 2 ? 3 : 2;
   bf16 q[Tr::planes][C * DK];
-  bf16 o[Tr::planes][C * VT];  // dy
+  bf16 o[Tr::planes][C * W];  // dy
   Decays<C> d[2];
   bf16 k[Tr::planes][C * DK];  // from here on: not for a segment's ends
-  bf16 v[Tr::planes][C * VT];
+  bf16 v[Tr::planes][C * W];
   bf16 p[Tr::prec][tri(C / 16, 0)];
   bf16 a[Tr::prec][tri(C / 16, 0)];
-  bf16 r[NR][VT * DK];         // R, rows of values: its parts in dk
+  bf16 r[NR][W * DK];         // R, rows of values: its parts in dk
   float row[C / 16][C];        // sums over a tile's j of P (dy.v), below the diagonal
   float col[C / 16][C];        // over its i
   float qs[DK / 16][C];        // q[i].(scale e^{G[i]} S_in dy[i]) over 16 keys
-  float kr[4][C];              // v[j].(e^{G[n]-G[j]} R^T k[j]) over a wave's columns
-  float sr[4];                 // a wave's share of <S_in, R>
+  float kr[BW][C];             // v[j].(e^{G[n]-G[j]} R^T k[j]) over a wave's columns
+  float sr[BW];                // a wave's share of <S_in, R>
 };
-
-constexpr int BW = 4, BTHREADS = 64 * BW;  // waves and threads of a backward block
 
 // Sum over the 16 lanes of a row of the wave, in all of them
 __device__ __forceinline__ float row_sum(float v) {
@@ -790,14 +788,14 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// What the columns v0 .. v0 + 63 of the values add to the gradients; ENDS: only what the segment adds to the state's
+// What a block's 16 BW columns of the values add to the gradients; ENDS: only what the segment adds to the state's
 // gradient.
-template <typename T, int DK, bool ENDS>
-__global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1)) void k_la_bwd(Args a) {
-  using L = BwdLds<T, DK>;
+template <typename T, int DK, int BW, bool ENDS>
+__global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1)) void k_la_bwd(Args a) {
+  using L = BwdLds<T, DK, BW>;
   using Tr = Traits<T>;
-  constexpr int C = L::C, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, NR = L::NR;
-  constexpr int KP = C * DK, VP = C * VT, PP = tri(C / 16, 0), RP = VT * DK;  // elements of a plane
+  constexpr int C = L::C, W = L::W, BTHREADS = 64 * BW, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, NR = L::NR;
+  constexpr int KP = C * DK, VP = C * W, PP = tri(C / 16, 0), RP = W * DK;  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
   // scalar: transposing reads need all lanes, which a branch on a wave's number in a vector register does not promise
@@ -805,7 +803,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Unit u = unit_of(a, ENDS ? a.segs - 1 : a.segs, ENDS ? 1 : 0);
   const int c_first = u.seg * a.seg_chunks, c_last = min(c_first + a.seg_chunks, a.chunks);
-  const int v0 = u.vt * VT, vc = v0 + 16 * w;
+  const int v0 = u.vt * W, vc = v0 + 16 * w;
   const int64_t bh = u.b * a.H + u.h;
   const int64_t KV = int64_t{a.K} * a.V;
   const T* q = static_cast<const T*>(a.q) + u.b * a.qb + u.h / (a.H / a.Hq) * a.qh;
@@ -825,7 +823,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
 
   const int c_end = min(c_last, (u.len + C - 1) / C);  // chunks with tokens
   Stage<T, C, DK, BTHREADS> rq, rk;
-  Stage<T, C, VT, BTHREADS> rv, ro;
+  Stage<T, C, W, BTHREADS> rv, ro;
   float rg = 0.f;  // one wave's: the log decays of the chunk before, asked for a chunk ahead of its rows
   g += int64_t{c_end - 1} * C * a.gt, q += int64_t{c_end - 1} * C * a.qt, dy += int64_t{c_end - 1} * C * a.yt;
   k += int64_t{c_end - 1} * C * a.kt, v += int64_t{c_end - 1} * C * a.vt;
@@ -905,11 +903,11 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
           mma_n<3>(qk, fj, fi);
         }
 #pragma unroll
-        for (int st = 0; st < VT / 32; ++st) {
+        for (int st = 0; st < W / 32; ++st) {
 #pragma unroll
           for (int k = 0; k < N; ++k) {
-            fj[k] = by_row<NP, VT>(lds.v[0], VP, 16 * jt[k], 32 * st);
-            fi[k] = by_row<NP, VT>(lds.o[0], VP, 16 * it[k], 32 * st);
+            fj[k] = by_row<NP, W>(lds.v[0], VP, 16 * jt[k], 32 * st);
+            fi[k] = by_row<NP, W>(lds.o[0], VP, 16 * it[k], 32 * st);
           }
           mma_n<3>(ov, fj, fi);
         }
@@ -956,6 +954,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
         for (int r = 0; r < 4; ++r) sr = fmaf(in[t][r], s[t][r], sr);
       sr = wave_sum(sr);
       if (lane == 0) lds.sr[w] = sr;
+      __builtin_amdgcn_sched_barrier(0);
       // dq and dk: tiles of 16 keys and 16 tokens, a wave's share of the keys (of the tokens, where keys are few)
       constexpr int SHARE = TK >= BW ? 1 : BW / TK, KT = TK >= BW ? TK / BW : 1, IT = TI / SHARE > 0 ? TI / SHARE : 1;
       const __amdgpu_buffer_rsrc_t si = dev_buf(a.ckpt + (bh * a.chunks + c) * KV, 4u * a.K * a.V);
@@ -963,28 +962,22 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
 #pragma unroll 1
       for (int kk = 0; kk < KT; ++kk) {
         const int kt = w / SHARE * KT + kk;
-        Frag<3> fs[VT / 32];  // S_in, rows of keys, index of values
-        Frag<NR> fr[VT / 32];
+        f32x4 in[W / 32][2];  // S_in, rows of keys, index of values
         const int row = 16 * kt + li;
 #pragma unroll
-        for (int st = 0; st < VT / 32; ++st) {
-          fr[st] = by_col<NR, DK>(lds.r[0], RP, 32 * st, 16 * kt);
+        for (int st = 0; st < W / 32; ++st)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int col = v0 + 32 * st + 16 * h + 4 * lg;
             const uint32_t at = 4u * (row * a.V + col);
-            f32x4 x;
             if (v4) {
-              x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(si, col < a.V ? at : NOWHERE, 0, 0));
+              in[st][h] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(si, col < a.V ? at : NOWHERE, 0, 0));
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, col + i < a.V ? at + 4 * i : NOWHERE, 0, 0));
+                in[st][h][i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, col + i < a.V ? at + 4 * i : NOWHERE, 0, 0));
             }
-            put2(fs[st], 4 * h, x[0], x[1]);
-            put2(fs[st], 4 * h + 2, x[2], x[3]);
           }
-        }
         const int key = anew(16 * kt + 4 * lg);
         auto tokens = [&](auto count, int first) {  // the tiles of tokens from `first` on
           constexpr int N = decltype(count)::value;
@@ -993,10 +986,18 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
 #pragma unroll
           for (int m = 0; m < N; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int st = 0; st < VT / 32; ++st) {
+          for (int st = 0; st < W / 32; ++st) {
 #pragma unroll
-            for (int m = 0; m < N; ++m) fi[m] = by_row<NP, VT>(lds.o[0], VP, 16 * (first + m), 32 * st);
-            mma_n<3>(acc, fs[st], fi);
+            for (int m = 0; m < N; ++m) fi[m] = by_row<NP, W>(lds.o[0], VP, 16 * (first + m), 32 * st);
+            Frag<3> fs;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x[4] = {in[st][h][0], in[st][h][1], in[st][h][2], in[st][h][3]};
+              put2(fs, 4 * h, x[0], x[1]);
+              put2(fs, 4 * h + 2, x[2], x[3]);
+            }
+            mma_n<3>(acc, fs, fi);
+            if (DK > 64) __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
           }
 #pragma unroll
           for (int m = 0; m < N; ++m) {
@@ -1026,10 +1027,10 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int st = 0; st < VT / 32; ++st) {
+          for (int st = 0; st < W / 32; ++st) {
 #pragma unroll
-            for (int m = 0; m < N; ++m) fi[m] = by_row<NP, VT>(lds.v[0], VP, 16 * (first + m), 32 * st);
-            mma_n<NR>(acc, fr[st], fi);
+            for (int m = 0; m < N; ++m) fi[m] = by_row<NP, W>(lds.v[0], VP, 16 * (first + m), 32 * st);
+            mma_n<NR>(acc, by_col<NR, DK>(lds.r[0], RP, 32 * st, 16 * kt), fi);
           }
 #pragma unroll
           for (int m = 0; m < N; ++m) acc[m] *= d.left[16 * (first + m) + li];
@@ -1047,17 +1048,15 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
             emit(a.dk, a.dk32, token, krow, i, kcol + key, i < n ? a.K - key : 0, k4, acc[m]);
           }
         };
-        SHARE == 1 ? tokens(std::integral_constant<int, IT>{}, 0) : tokens(std::integral_constant<int, IT>{}, part * IT);
+        if (part * IT < TI) tokens(std::integral_constant<int, IT>{}, SHARE == 1 ? 0 : part * IT);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     Frag<NP> fo[C / 32];  // dy: this wave's columns
 #pragma unroll
-    for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP, VT>(lds.o[0], VP, 32 * st, 16 * w);
+    for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP, W>(lds.o[0], VP, 32 * st, 16 * w);
     if (!ENDS) {
       // dv: this wave's 16 columns
-      Frag<3> fs[TK / 2];
-      state_frags(s, fs);
       const int col = anew(vc + 4 * lg);
       auto values = [&](auto count, int first) {
         constexpr int N = decltype(count)::value;
@@ -1069,14 +1068,19 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
         for (int st = 0; st < DK / 32; ++st) {
 #pragma unroll
           for (int m = 0; m < N; ++m) fj[m] = by_row<NP, DK>(lds.k[0], KP, 16 * (first + m), 32 * st);
-          mma_n<3>(acc, fs[st], fj);
+          Frag<3> fs;  // R, index of keys
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) put2(fs, 4 * t + r, s[2 * st + t][r], s[2 * st + t][r + 1]);
+          mma_n<3>(acc, fs, fj);
         }
 #pragma unroll
         for (int m = 0; m < N; ++m) {
           const int j = 16 * (first + m) + li;
           float x[4], sum = 0.f;
           acc[m] *= d.left[j];
-          four<NP>(lds.v[0] + ((first + m) * (VT / 16) + w) * TILE, VP, x);
+          four<NP>(lds.v[0] + ((first + m) * (W / 16) + w) * TILE, VP, x);
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[m][r], sum);
           sum = col_sum(sum);
@@ -1102,7 +1106,8 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
     __syncthreads();
     if (!ENDS && w == BW - 1) {
       // the decays' gradients: a lane a token
-      double later = 0., kept = 0.;  // what is summed from t on, and before t
+      double later = 0., kept = 0., sr = 0.;  // what is summed from t on, before t, and for all
+      for (int t = 0; t < BW; ++t) sr += lds.sr[t];
       if (lane < n) {
         for (int t = 0; t <= lane / 16; ++t) later += lds.row[t][lane];
         for (int t = lane / 16; t < TI; ++t) later -= lds.col[t][lane];
@@ -1118,7 +1123,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
       }
       if (lane < n)
         a.dg[(token + lane) * a.H * a.vts + hv] = static_cast<float>(
-            later + (total - kept) + double(d.whole) * ((double(lds.sr[0]) + lds.sr[1]) + (double(lds.sr[2]) + lds.sr[3])));
+            later + (total - kept) + double(d.whole) * sr);
     }
   }
   if (ENDS) {
@@ -1128,7 +1133,7 @@ __global__ __launch_bounds__(BTHREADS, DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1
   }
   // positions behind the sequence's end
   const int start = max(u.len, c_first * C), to = static_cast<int>(min(static_cast<int64_t>(c_last) * C, a.T));
-  const int cols = min(VT, a.V - v0);
+  const int cols = min(W, a.V - v0);
   auto clear = [&](void* out, bool f32, int64_t head, int64_t heads, int d, int c0, int width) {
     for (int64_t i = threadIdx.x; i < int64_t{to - start} * width; i += BTHREADS) {
       const int64_t at = ((u.b * a.T + start + i / width) * heads + head) * d + c0 + i % width;
@@ -1298,7 +1303,7 @@ bool vector_rows(const void* p, int es, int64_t batch, int64_t token, int64_t he
 // one chunk gain nothing: 3 x 777 x 6 x 40 from one chunk, two, three, four on: 26, 26, 30, 35 us.
 constexpr int64_t BLOCKS = 512;
 
-Args make_args(const lng_linear_attention& l) {
+Args make_args(const lng_linear_attention& l, bool grad) {
   Args a{};
   a.B = l.B, a.T = l.T, a.H = l.H, a.Hq = l.Hq, a.Hk = l.Hk, a.Hv = l.Hv, a.K = l.K, a.V = l.V, a.scale = l.scale;
   a.q = l.q, a.k = l.k, a.v = l.v;
@@ -1311,9 +1316,9 @@ Args make_args(const lng_linear_attention& l) {
   a.start = l.state, a.lengths = l.lengths, a.y = l.y, a.end = l.state_out, a.ckpt = l.checkpoints;
   a.yvec = a.V % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * es) == 0;
   a.Kp = static_cast<int>(cdiv(a.K, 8)) * 8, a.Vp = static_cast<int>(cdiv(a.V, 8)) * 8;
-  a.vts = static_cast<int>(cdiv(a.V, VT));
+  a.vts = grad && l.dtype != LNG_F32 ? 1 : static_cast<int>(cdiv(a.V, VT));  // blocks of value columns
   a.chunks = static_cast<int>(cdiv(a.T, chunk_of(l.dtype)));
-  const int64_t units = std::max<int64_t>(1, a.B * a.H * a.vts);
+  const int64_t units = std::max<int64_t>(1, a.B * a.H * cdiv(a.V, VT));
   const int64_t segs = std::min<int64_t>((BLOCKS + units / 2) / units, cdiv(a.chunks, 2));
   a.seg_chunks = static_cast<int>(cdiv(a.chunks, std::max<int64_t>(segs, 1)));
   a.segs = a.seg_chunks ? static_cast<int>(cdiv(a.chunks, a.seg_chunks)) : 1;
@@ -1371,7 +1376,7 @@ int check_threads(const char* what, int64_t blocks, int threads) {
 // Every launch of a call, before its first
 int check_launches(const char* what, const Args& a, bool grad) {
   const int64_t rows = a.B * a.T;
-  int64_t most = a.B * a.H * std::max<int64_t>(int64_t{a.vts} * a.segs, cdiv(int64_t{a.K} * a.V, 256));
+  int64_t most = a.B * a.H * std::max<int64_t>(cdiv(a.V, VT) * a.segs, cdiv(int64_t{a.K} * a.V, 256));
   auto packed = [&](bool vec, int heads, int width) {
     if (!vec) most = std::max(most, cdiv(rows * heads * (width / 8), 256));
   };
@@ -1436,19 +1441,19 @@ int run_fwd(const Args& args, hipStream_t st) {
                 "linear_attention");
 }
 
-template <typename T, int DK>
+template <typename T, int DK, int BW>
 int run_bwd(const Args& a, hipStream_t st) {
-  using L = BwdLds<T, DK>;
+  using L = BwdLds<T, DK, BW>;
   constexpr size_t lds = sizeof(L);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
   const int64_t units = a.B * a.H * a.vts;
   if (a.segs > 1) {
-    if (int rc = launch(&k_la_bwd<T, DK, true>, static_cast<unsigned>(units * (a.segs - 1)), BTHREADS,
+    if (int rc = launch(&k_la_bwd<T, DK, BW, true>, static_cast<unsigned>(units * (a.segs - 1)), 64 * BW,
                         offsetof(L, k), st, a, "linear_attention_grad"))
       return rc;
     if (int rc = run_join<true>(a, st)) return rc;
   }
-  return launch(&k_la_bwd<T, DK, false>, static_cast<unsigned>(units * a.segs), BTHREADS, lds, st, a,
+  return launch(&k_la_bwd<T, DK, BW, false>, static_cast<unsigned>(units * a.segs), 64 * BW, lds, st, a,
                 "linear_attention_grad");
 }
 
@@ -1485,7 +1490,7 @@ size_t lng_linear_attention_grad_size(void) { return sizeof(lng_linear_attention
 
 size_t lng_linear_attention_workspace_bytes(const lng_linear_attention* args, int grad) {
   if (check_args("linear_attention_workspace_bytes", args) || args->B == 0 || args->T == 0) return 0;
-  const Args a = make_args(*args);
+  const Args a = make_args(*args, grad != 0);
   return static_cast<size_t>(Space(a, dtype_size(args->dtype), grad != 0, args->token_decay != 0).total) * 4;
 }
 
@@ -1499,7 +1504,7 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
   if (int rc = check_args(what, args)) return rc;
   if (args->B == 0 || args->T == 0) return LNG_OK;
   if (!args->y) return fail(LNG_E_ARG, "linear_attention: null pointer");
-  Args a = make_args(*args);
+  Args a = make_args(*args, false);
   const Space s(a, dtype_size(args->dtype), false, args->token_decay != 0);
   if (s.total && (!workspace || workspace_bytes < static_cast<size_t>(s.total) * 4 ||
                   reinterpret_cast<uintptr_t>(workspace) % 64))
@@ -1529,7 +1534,7 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
   if (args->B == 0 || args->T == 0) return fail(LNG_E_ARG, "linear_attention_grad: no tokens");
   if (!args->checkpoints || !g.dy || !g.dq || !g.dk || !g.dv || !g.ddecay)
     return fail(LNG_E_ARG, "linear_attention_grad: null pointer");
-  Args a = make_args(*args);
+  Args a = make_args(*args, true);
   const bool token = args->token_decay != 0;
   const int es = dtype_size(args->dtype);
   const Space s(a, es, true, token);
@@ -1554,7 +1559,16 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
     if (int rc = pack_inputs<T>(a, s, ws, st)) return rc;
     if (a.V % 8)
       if (int rc = pack<T>(a.dy, a.yb, a.yt, a.yh, a.B, a.T, a.H, a.V, a.Vp, ws + s.dy, st)) return rc;
-    if (int rc = with_keys(a.K, [&](auto dk) { return run_bwd<T, decltype(dk)::value>(a, st); })) return rc;
+    if (int rc = with_keys(a.K, [&](auto dk) {
+          constexpr int DK = decltype(dk)::value;
+          // Eight waves for 128 columns spare partial results of dq and dk, and a second product of q and k.  4 x 2048 x 16,
+          // bf16, both passes: 32 keys and 128 values 159 us and 190, 64 193 and 277, 128 289 and 519; fp16, 128: 410
+          // and 681.  In fp32 three parts of everything do not fit into LDS.
+          if constexpr (!std::is_same_v<T, float>)
+            if (a.V > VT) return run_bwd<T, DK, 8>(a, st);
+          return run_bwd<T, DK, 4>(a, st);
+        }))
+      return rc;
     if (a.dq32)
       if (int rc = run_shared<T>(ws + s.dq, rows, a.Hq, static_cast<int>(hv / a.Hq), a.K, static_cast<T*>(g.dq), st)) return rc;
     if (a.dk32)
@@ -1578,7 +1592,7 @@ int lng_linear_attention_step(const lng_linear_attention* args, void* stream) {
   if (args->T != 1) return fail(LNG_E_ARG, "linear_attention_step: one token of every sequence (T = 1)");
   if (args->B == 0) return LNG_OK;
   if (!args->state || !args->state_out || !args->y) return fail(LNG_E_ARG, "linear_attention_step: null pointer");
-  const Args a = make_args(*args);
+  const Args a = make_args(*args, false);
   const int64_t waves = a.B * a.H * a.vts, blocks = cdiv(waves, 4);
   if (int rc = check_threads(what, blocks, 256)) return rc;
   const bool vec = a.yvec && reinterpret_cast<uintptr_t>(a.start) % 16 == 0 && reinterpret_cast<uintptr_t>(a.end) % 16 == 0;

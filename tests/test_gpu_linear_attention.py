@@ -91,6 +91,13 @@ def test_shapes_and_types(dev, b, t, h, dk, dv, dtype):
     _check(_make(dev, b, t, h, dk, dv, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("dk,dv", [(32, 128), (7, 80), (64, 128), (48, 65), (128, 128)])
+def test_more_than_64_values(dev, dtype, dk, dv):
+    """Blocks of eight waves, in several segments, with shared heads and ends inside of them."""
+    _check(_make(dev, 2, 330, 4, dk, dv, 2, 4, 2, dtype, ragged=True))
+
+
 @pytest.mark.parametrize("h,hq,hk,hv", [(4, 4, 1, 1), (4, 2, 4, 2), (6, 1, 2, 3), (4, 1, 1, 4), (2, 2, 1, 2)])
 @pytest.mark.parametrize("dtype,dk,dv", [(FP, 24, 40), (BF, 64, 128)])
 @pytest.mark.parametrize("token", [True, False])
