@@ -494,9 +494,9 @@ struct FwdLds {
   bf16 p[Tr::prec][tri(C / 16, 0)];
 };
 
-// What bounds it: at 8 x 4096 x 16 x 64 (bf16) 73 us for 281 MB, 3.8 TB/s; at 1 x 16384 x 16 x 128 92 us with the vector unit
-// busy for 40 % and the matrix unit for 24 %: waits, at the two waves a SIMD that 220 to 250 registers allow (three spill).
-// The segments' ends: 34 us for 102 MB, and 44 us.
+// What bounds it: at 8 x 4096 x 16 x 64 (bf16) 75 us for 281 MB, 3.8 TB/s; at 1 x 16384 x 16 x 128 94 us with the vector unit
+// busy for 38 % and the matrix unit for 24 %: waits, at two waves a SIMD (more segments cost more than a third wave gains).
+// The segments' ends: 34 us for 102 MB, and 45 us.
 //
 // A block of NW waves takes a head's values, up to 16 NW columns, over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
@@ -754,7 +754,7 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 // forward pass kept.  Everything is linear in the value columns: a block takes 16 BW of them, and dq, dk and dg of
 // several such tiles are summed afterwards, as the gradients of shared heads are.
 //
-// 8 x 2048 x 16 x 64, bf16: 109 us for 313 MB; the vector unit is busy for 32 %, the matrix unit for 13 %: waits, at two waves
+// 8 x 2048 x 16 x 64, bf16: 111 us for 313 MB; the vector unit is busy for 33 %, the matrix unit for 13 %: waits, at two waves
 // a SIMD.  Registers decide: the scores' tiles go one by one and operands are split where they are used, since a spill waits
 // for the stores in flight (146 us).
 template <typename T, int DK, int BW>
