@@ -26,20 +26,24 @@ namespace {
 constexpr int MAX_D = 128;  // of keys and values
 constexpr int VT = 64;      // columns of values that four waves take
 
-// Planes: bf16 parts of an input; PREC: parts of a computed operand of a product whose result is rounded to the type.
+// Planes: bf16 parts of an input.  What is computed (scores, states, their gradients) enters products in PARTS whatever the
+// type, so that a 16-bit result is what fp32 sums give, rounded once.  Two parts are short of up to 2^-16 of a value, which
+// turns the rounding of one bf16 result in a thousand (1.2e-4 of the norm instead of 3e-5); they would take 115 us instead of
+// 126 at 8 x 4096 x 16 x 64, bf16, and 209 instead of 222 in the training of 8 x 2048 x 16 x 64.
+constexpr int PARTS = 3;
 template <typename T>
 struct Traits;
 template <>
 struct Traits<bf16> {
-  static constexpr int planes = 1, prec = 2, chunk = 64;
+  static constexpr int planes = 1, chunk = 64;
 };
 template <>
 struct Traits<_Float16> {
-  static constexpr int planes = 2, prec = 2, chunk = 32;
+  static constexpr int planes = 2, chunk = 32;
 };
 template <>
 struct Traits<float> {
-  static constexpr int planes = 3, prec = 3, chunk = 32;
+  static constexpr int planes = 3, chunk = 32;
 };
 
 // ------------------------------------------------------------------ arguments
@@ -108,19 +112,6 @@ __device__ __forceinline__ double log2_decay(float g) {
 // x as the sum of N bf16 values: its first eight significant bits, the next eight, and so on, the last part rounded.
 // An fp16 value is two parts exactly, an fp32 value three.  (What is not finite comes out as NaN.)
 __device__ __forceinline__ float top(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u); }
-template <int N>
-__device__ __forceinline__ void split(float x, bf16 (&out)[N]) {
-#pragma unroll
-  for (int p = 0; p < N; ++p) {
-    if (p + 1 < N) {
-      const float f = top(x);
-      out[p] = __builtin_bit_cast(bf16, static_cast<uint16_t>(__builtin_bit_cast(uint32_t, f) >> 16));
-      x -= f;
-    } else {
-      out[p] = static_cast<bf16>(x);
-    }
-  }
-}
 
 template <int N>
 struct Frag {
@@ -143,44 +134,44 @@ __device__ __forceinline__ void put2(Frag<N>& f, int i, float x, float y) {
   }
 }
 
-// acc += a . b without the products of parts that add to LIM or more
-template <int LIM, int NA, int NB>
+// acc += a . b without the products of the smallest parts
+template <int NA, int NB>
 __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB>& b) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-      if (i + j < LIM) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
+      if (i + j < PARTS) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
 
 // The same for n results that do not wait for each other: acc[k] += a(k) . b(k)
-template <int LIM, int NA, int NB, int N>
+template <int NA, int NB, int N>
 __device__ __forceinline__ void mma_n(f32x4 (&acc)[N], const Frag<NA> (&a)[N], const Frag<NB>& b) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-      if (i + j < LIM)
+      if (i + j < PARTS)
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k].p[i], b.p[j], acc[k], 0, 0, 0);
 }
-template <int LIM, int NA, int NB, int N>
+template <int NA, int NB, int N>
 __device__ __forceinline__ void mma_n(f32x4 (&acc)[N], const Frag<NA>& a, const Frag<NB> (&b)[N]) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-      if (i + j < LIM)
+      if (i + j < PARTS)
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b[k].p[j], acc[k], 0, 0, 0);
 }
-template <int LIM, int NA, int NB, int N>
+template <int NA, int NB, int N>
 __device__ __forceinline__ void mma_n(f32x4 (&acc)[N], const Frag<NA> (&a)[N], const Frag<NB> (&b)[N]) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-      if (i + j < LIM)
+      if (i + j < PARTS)
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k].p[i], b[k].p[j], acc[k], 0, 0, 0);
 }
@@ -449,6 +440,18 @@ __device__ __forceinline__ void store_state(const f32x4 (&s)[TK], float* m, int 
     }
 }
 
+// A state's tile in LDS, which a lane writes four keys of a value and reads four values of a key: key r's row stands at
+// place 4 (r % 4) + r / 4, its four pieces of four swapped by r % 4, so that both take all banks once.
+__device__ __forceinline__ void put_state(float* tile, const f32x4& s) {
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tile[(4 * i + lg) * 16 + (((li >> 2) ^ i) << 2) + (li & 3)] = s[i];
+}
+__device__ __forceinline__ f32x4 get_state(const float* tile) {
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  return *reinterpret_cast<const f32x4*>(tile + (4 * (li & 3) + (li >> 2)) * 16 + ((lg ^ (li & 3)) << 2));
+}
+
 // S <- whole S + X^T (f Y): rows of X (sX, W keys) and Y (values, this wave's columns) of a chunk, f a factor a row.  The
 // scaled operand is fp32 in three parts: the states are the results that stay in fp32.
 template <int C, int TK, int W, int NX>
@@ -459,7 +462,7 @@ __device__ __forceinline__ void update_state(f32x4 (&s)[TK], const bf16* sX, int
   for (int t = 0; t < TK; ++t) s[t] *= whole;
 #pragma unroll
   for (int st = 0; st < C / 32; ++st) {
-    Frag<3> fy;
+    Frag<PARTS> fy;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const f32x4 fr = *reinterpret_cast<const f32x4*>(f + 32 * st + 16 * h + 4 * g);
@@ -470,7 +473,7 @@ __device__ __forceinline__ void update_state(f32x4 (&s)[TK], const bf16* sX, int
     Frag<NX> fx[TK];
 #pragma unroll
     for (int t = 0; t < TK; ++t) fx[t] = by_col<NX, W>(sX, xplane, 32 * st, 16 * t);
-    mma_n<3>(s, fx, fy);
+    mma_n(s, fx, fy);
   }
 }
 // The state as the operand whose index runs over keys
@@ -491,7 +494,7 @@ struct FwdLds {
   bf16 v[Tr::planes][C * W];
   Decays<C> d[2];
   bf16 q[Tr::planes][C * DK];  // from here on: not for a segment's ends
-  bf16 p[Tr::prec][tri(C / 16, 0)];
+  bf16 p[PARTS][tri(C / 16, 0)];
 };
 
 // What bounds it: at 8 x 4096 x 16 x 64 (bf16) 75 us for 281 MB, 3.8 TB/s; at 1 x 16384 x 16 x 128 94 us with the vector unit
@@ -504,7 +507,7 @@ template <typename T, int DK, int NW, bool ENDS>
 __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) void k_la_fwd(Args a) {
   using L = FwdLds<T, DK, NW>;
   using Tr = Traits<T>;
-  constexpr int C = L::C, W = L::W, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, THREADS = 64 * NW;
+  constexpr int C = L::C, W = L::W, TK = DK / 16, TI = C / 16, NP = Tr::planes, THREADS = 64 * NW;
   constexpr int KP = C * DK, VP = C * W, PP = tri(C / 16, 0);  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
@@ -588,7 +591,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) 
             fk[k] = by_row<NP, DK>(lds.k[0], KP, 16 * (idx[k] - it[k] * (it[k] + 1) / 2), 32 * st);
             fq[k] = by_row<NP, DK>(lds.q[0], KP, 16 * it[k], 32 * st);
           }
-          mma_n<3>(acc, fk, fq);
+          mma_n(acc, fk, fq);
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
@@ -601,7 +604,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) 
             p[r] = acc[k][r] * (exp2_gap(ih, il, jh[r], jl[r]) * a.scale);
             p[r] = j0 + r <= i ? p[r] : 0.f;
           }
-          put_four<PR>(lds.p[0] + idx[k] * TILE, PP, p);
+          put_four<PARTS>(lds.p[0] + idx[k] * TILE, PP, p);
         }
       };
       constexpr int ALL = TI * (TI + 1) / 2, EACH = (ALL + NW - 1) / NW;
@@ -638,7 +641,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) 
       bad = min(bad, __shfl_xor(bad, 32, 64));
     }
     if (!ENDS) {
-      Frag<PR> fs[TK / 2];
+      Frag<PARTS> fs[TK / 2];
       state_frags(s, fs);
       const __amdgpu_buffer_rsrc_t yc = from(y + int64_t{t0} * yrow);
       const int col = anew(vc + 4 * lg);
@@ -652,7 +655,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) 
         for (int st = 0; st < DK / 32; ++st) {
 #pragma unroll
           for (int k = 0; k < N; ++k) fq[k] = by_row<NP, DK>(lds.q[0], KP, 16 * (first + k), 32 * st);
-          mma_n<PR>(acc, fs[st], fq);
+          mma_n(acc, fs[st], fq);
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] *= d.from[16 * (first + k) + li];
@@ -660,7 +663,7 @@ __global__ __launch_bounds__(64 * NW, ENDS && NW == 4 ? (DK <= 64 ? 4 : 3) : 2) 
         for (int st = 0; st < C / 32; ++st)
 #pragma unroll
           for (int k = 0; k < N; ++k)
-            if (2 * st <= first + k) mma<PR>(acc[k], fv[st], tri_by_row<PR>(lds.p[0], PP, first + k, st));
+            if (2 * st <= first + k) mma(acc[k], fv[st], tri_by_row<PARTS>(lds.p[0], PP, first + k, st));
         if (careful)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -752,7 +755,8 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 //
 // One pass from the last chunk to the first reads q, k, v and dy once, and the states before the chunks, which the
 // forward pass kept.  Everything is linear in the value columns: a block takes 16 BW of them, and dq, dk and dg of
-// several such tiles are summed afterwards, as the gradients of shared heads are.
+// several such tiles are summed afterwards, as the gradients of shared heads are.  P and A take the same place in LDS, one
+// after the other, A in registers meanwhile: three parts of both and R would leave room for one block a CU.
 //
 // 8 x 2048 x 16 x 64, bf16: 111 us for 313 MB; the vector unit is busy for 33 %, the matrix unit for 13 %: waits, at two waves
 // a SIMD.  Registers decide: the scores' tiles go one by one and operands are split where they are used, since a spill waits
@@ -760,15 +764,14 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 template <typename T, int DK, int BW>
 struct BwdLds {
   using Tr = Traits<T>;
-  static constexpr int C = Tr::chunk, W = 16 * BW, NR = Tr::planes > 2 ? 3 : 2;
+  static constexpr int C = Tr::chunk, W = 16 * BW;
   bf16 q[Tr::planes][C * DK];
   bf16 o[Tr::planes][C * W];  // dy
   Decays<C> d[2];
   bf16 k[Tr::planes][C * DK];  // from here on: not for a segment's ends
   bf16 v[Tr::planes][C * W];
-  bf16 p[Tr::prec][tri(C / 16, 0)];
-  bf16 a[Tr::prec][tri(C / 16, 0)];
-  bf16 r[NR][W * DK];         // R, rows of values: its parts in dk
+  bf16 p[PARTS][tri(C / 16, 0)];  // P for dv, then A for dq and dk
+  float r[W * DK];             // R for dk: tiles of 16 values and 16 keys
   float row[C / 16][C];        // sums over a tile's j of P (dy.v), below the diagonal
   float col[C / 16][C];        // over its i
   float qs[DK / 16][C];        // q[i].(scale e^{G[i]} S_in dy[i]) over 16 keys
@@ -794,8 +797,8 @@ template <typename T, int DK, int BW, bool ENDS>
 __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : (ENDS ? 3 : 1)) void k_la_bwd(Args a) {
   using L = BwdLds<T, DK, BW>;
   using Tr = Traits<T>;
-  constexpr int C = L::C, W = L::W, BTHREADS = 64 * BW, TK = DK / 16, TI = C / 16, NP = Tr::planes, PR = Tr::prec, NR = L::NR;
-  constexpr int KP = C * DK, VP = C * W, PP = tri(C / 16, 0), RP = W * DK;  // elements of a plane
+  constexpr int C = L::C, W = L::W, BTHREADS = 64 * BW, TK = DK / 16, TI = C / 16, NP = Tr::planes;
+  constexpr int KP = C * DK, VP = C * W, PP = tri(C / 16, 0);  // elements of a plane
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   L& lds = *reinterpret_cast<L*>(lds_raw);
   // scalar: transposing reads need all lanes, which a branch on a wave's number in a vector register does not promise
@@ -871,73 +874,47 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
       rk.store(lds.k[0], KP);
       rv.store(lds.v[0], VP);
 #pragma unroll
-      for (int t = 0; t < TK; ++t) {
-        const float x[4] = {s[t][0], s[t][1], s[t][2], s[t][3]};
-        put_four<NR>(lds.r[0] + (w * TK + t) * TILE, RP, x);
-      }
+      for (int t = 0; t < TK; ++t) put_state(lds.r + (w * TK + t) * TILE, s[t]);
     }
     __syncthreads();
     const float g_next = rg;
     fetch_decay(c - 2);
     if (c > c_first) fetch(c - 1);
 
+    constexpr int ALL = TI * (TI + 1) / 2, EACH = (ALL + BW - 1) / BW;
+    float held[EACH][4];  // this wave's tiles of A: they take the place of P's when dv has been formed
     if (!ENDS) {
-      auto scores = [&](auto count, int first, int all) {
-        constexpr int N = decltype(count)::value;
-        f32x4 qk[N], ov[N];
-        int it[N], jt[N], idx[N];
+      // a wave's tiles one after the other: side by side their operands would spill
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          idx[k] = first + k * BW < all ? first + k * BW : first;
-          it[k] = idx[k] >= 6 ? 3 : idx[k] >= 3 ? 2 : idx[k] >= 1 ? 1 : 0, jt[k] = idx[k] - it[k] * (it[k] + 1) / 2;
-          qk[k] = ov[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        Frag<NP> fj[N], fi[N];
-#pragma unroll
-        for (int st = 0; st < DK / 32; ++st) {
-#pragma unroll
-          for (int k = 0; k < N; ++k) {
-            fj[k] = by_row<NP, DK>(lds.k[0], KP, 16 * jt[k], 32 * st);
-            fi[k] = by_row<NP, DK>(lds.q[0], KP, 16 * it[k], 32 * st);
-          }
-          mma_n<3>(qk, fj, fi);
-        }
-#pragma unroll
-        for (int st = 0; st < W / 32; ++st) {
-#pragma unroll
-          for (int k = 0; k < N; ++k) {
-            fj[k] = by_row<NP, W>(lds.v[0], VP, 16 * jt[k], 32 * st);
-            fi[k] = by_row<NP, W>(lds.o[0], VP, 16 * it[k], 32 * st);
-          }
-          mma_n<3>(ov, fj, fi);
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int i = 16 * it[k] + li, j0 = 16 * jt[k] + 4 * lg;
-          const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
-          const float ih = d.hi[i], il = d.lo[i];
-          float p[4], x[4], pair[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float dec = exp2_gap(ih, il, jh[r], jl[r]) * a.scale;
-            p[r] = j0 + r <= i ? qk[k][r] * dec : 0.f;
-            x[r] = j0 + r <= i ? ov[k][r] * dec : 0.f;
-            pair[r] = j0 + r < i ? p[r] * ov[k][r] : 0.f;
-          }
-          put_four<PR>(lds.p[0] + idx[k] * TILE, PP, p);
-          put_four<PR>(lds.a[0] + idx[k] * TILE, PP, x);
-          const float rows = col_sum((pair[0] + pair[1]) + (pair[2] + pair[3]));
-          if (lg == 0) lds.row[jt[k]][i] = rows;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) pair[r] = row_sum(pair[r]);
-          if (li == 0) *reinterpret_cast<f32x4*>(&lds.col[it[k]][j0]) = f32x4{pair[0], pair[1], pair[2], pair[3]};
-        }
-      };
-      constexpr int ALL = TI * (TI + 1) / 2, EACH = (ALL + BW - 1) / BW;
-#pragma unroll 1
       for (int k = 0; k < EACH; ++k) {
         const int idx = w + k * BW;
-        if (idx < ALL) scores(std::integral_constant<int, 1>{}, idx, idx + 1);
+        if (idx >= ALL) continue;
+        const int it = idx >= 6 ? 3 : idx >= 3 ? 2 : idx >= 1 ? 1 : 0, jt = idx - it * (it + 1) / 2;
+        f32x4 qk{0.f, 0.f, 0.f, 0.f}, ov{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < DK / 32; ++st)
+          mma(qk, by_row<NP, DK>(lds.k[0], KP, 16 * jt, 32 * st), by_row<NP, DK>(lds.q[0], KP, 16 * it, 32 * st));
+#pragma unroll
+        for (int st = 0; st < W / 32; ++st)
+          mma(ov, by_row<NP, W>(lds.v[0], VP, 16 * jt, 32 * st), by_row<NP, W>(lds.o[0], VP, 16 * it, 32 * st));
+        const int i = 16 * it + li, j0 = 16 * jt + 4 * lg;
+        const f32x4 jh = *reinterpret_cast<const f32x4*>(&d.hi[j0]), jl = *reinterpret_cast<const f32x4*>(&d.lo[j0]);
+        const float ih = d.hi[i], il = d.lo[i];
+        float p[4], pair[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float dec = exp2_gap(ih, il, jh[r], jl[r]) * a.scale;
+          p[r] = j0 + r <= i ? qk[r] * dec : 0.f;
+          held[k][r] = j0 + r <= i ? ov[r] * dec : 0.f;
+          pair[r] = j0 + r < i ? p[r] * ov[r] : 0.f;
+        }
+        put_four<PARTS>(lds.p[0] + idx * TILE, PP, p);
+        const float rows = col_sum((pair[0] + pair[1]) + (pair[2] + pair[3]));
+        if (lg == 0) lds.row[jt][i] = rows;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pair[r] = row_sum(pair[r]);
+        if (li == 0) *reinterpret_cast<f32x4*>(&lds.col[it][j0]) = f32x4{pair[0], pair[1], pair[2], pair[3]};
+        __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
     }
@@ -954,6 +931,68 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
         for (int r = 0; r < 4; ++r) sr = fmaf(in[t][r], s[t][r], sr);
       sr = wave_sum(sr);
       if (lane == 0) lds.sr[w] = sr;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    Frag<NP> fo[C / 32];  // dy: this wave's columns
+#pragma unroll
+    for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP, W>(lds.o[0], VP, 32 * st, 16 * w);
+    if (!ENDS) {
+      // dv: this wave's 16 columns
+      const int col = anew(vc + 4 * lg);
+      auto values = [&](auto count, int first) {
+        constexpr int N = decltype(count)::value;
+        f32x4 acc[N];
+        Frag<NP> fj[N];
+#pragma unroll
+        for (int m = 0; m < N; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < DK / 32; ++st) {
+#pragma unroll
+          for (int m = 0; m < N; ++m) fj[m] = by_row<NP, DK>(lds.k[0], KP, 16 * (first + m), 32 * st);
+          Frag<PARTS> fs;  // R, index of keys
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) put2(fs, 4 * t + r, s[2 * st + t][r], s[2 * st + t][r + 1]);
+          mma_n(acc, fs, fj);
+        }
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+          const int j = 16 * (first + m) + li;
+          float x[4], sum = 0.f;
+          acc[m] *= d.left[j];
+          four<NP>(lds.v[0] + ((first + m) * (W / 16) + w) * TILE, VP, x);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[m][r], sum);
+          sum = col_sum(sum);
+          if (lg == 0) lds.kr[w][j] = sum;
+        }
+#pragma unroll
+        for (int st = 0; st < C / 32; ++st)
+#pragma unroll
+          for (int m = 0; m < N; ++m)
+            if (2 * st + 1 >= first + m)
+              mma(acc[m], fo[st], tri_by_col<PARTS>(lds.p[0], PP, st, first + m));
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+          const int j = 16 * (first + m) + li;
+          emit(a.dv, a.dv32, token, vrow, j, u.h * a.V + col, j < n ? a.V - col : 0, v4, acc[m]);
+        }
+      };
+      values(std::integral_constant<int, TI>{}, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!ENDS) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < EACH; ++k)
+        if (w + k * BW < ALL) put_four<PARTS>(lds.p[0] + (w + k * BW) * TILE, PP, held[k]);
+    }
+    update_state<C, TK, DK, NP>(s, lds.q[0], KP, fo, d.from, d.whole);
+    if (ENDS && threadIdx.x == 0) seg += d.total;
+    if (!ENDS) {
+      __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
       // dq and dk: tiles of 16 keys and 16 tokens, a wave's share of the keys (of the tokens, where keys are few)
       constexpr int SHARE = TK >= BW ? 1 : BW / TK, KT = TK >= BW ? TK / BW : 1, IT = TI / SHARE > 0 ? TI / SHARE : 1;
@@ -989,14 +1028,14 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
           for (int st = 0; st < W / 32; ++st) {
 #pragma unroll
             for (int m = 0; m < N; ++m) fi[m] = by_row<NP, W>(lds.o[0], VP, 16 * (first + m), 32 * st);
-            Frag<3> fs;
+            Frag<PARTS> fs;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float x[4] = {in[st][h][0], in[st][h][1], in[st][h][2], in[st][h][3]};
               put2(fs, 4 * h, x[0], x[1]);
               put2(fs, 4 * h + 2, x[2], x[3]);
             }
-            mma_n<3>(acc, fs, fi);
+            mma_n(acc, fs, fi);
             if (DK > 64) __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
           }
 #pragma unroll
@@ -1017,7 +1056,7 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
             const Frag<NP> fk = by_col<NP, DK>(lds.k[0], KP, 32 * st, 16 * kt);
 #pragma unroll
             for (int m = 0; m < N; ++m)
-              if (2 * st <= first + m) mma<PR>(acc[m], fk, tri_by_row<PR>(lds.a[0], PP, first + m, st));
+              if (2 * st <= first + m) mma(acc[m], fk, tri_by_row<PARTS>(lds.p[0], PP, first + m, st));
           }
 #pragma unroll
           for (int m = 0; m < N; ++m) {
@@ -1030,7 +1069,11 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
           for (int st = 0; st < W / 32; ++st) {
 #pragma unroll
             for (int m = 0; m < N; ++m) fi[m] = by_row<NP, W>(lds.v[0], VP, 16 * (first + m), 32 * st);
-            mma_n<NR>(acc, by_col<NR, DK>(lds.r[0], RP, 32 * st, 16 * kt), fi);
+            const f32x4 r0 = get_state(lds.r + (2 * st * TK + kt) * TILE), r1 = get_state(lds.r + ((2 * st + 1) * TK + kt) * TILE);
+            Frag<PARTS> fr;  // R, index of values
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) put2(fr, r, r0[r], r0[r + 1]), put2(fr, 4 + r, r1[r], r1[r + 1]);
+            mma_n(acc, fr, fi);
           }
 #pragma unroll
           for (int m = 0; m < N; ++m) acc[m] *= d.left[16 * (first + m) + li];
@@ -1040,7 +1083,7 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
 #pragma unroll
             for (int m = 0; m < N; ++m)
               if (2 * st + 1 >= first + m)
-                mma<PR>(acc[m], fq, tri_by_col<PR>(lds.a[0], PP, st, first + m));
+                mma(acc[m], fq, tri_by_col<PARTS>(lds.p[0], PP, st, first + m));
           }
 #pragma unroll
           for (int m = 0; m < N; ++m) {
@@ -1051,58 +1094,6 @@ __global__ __launch_bounds__(64 * BW, BW == 8 ? 2 : DK <= 64 ? (ENDS ? 4 : 2) : 
         if (part * IT < TI) tokens(std::integral_constant<int, IT>{}, SHARE == 1 ? 0 : part * IT);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    Frag<NP> fo[C / 32];  // dy: this wave's columns
-#pragma unroll
-    for (int st = 0; st < C / 32; ++st) fo[st] = by_col<NP, W>(lds.o[0], VP, 32 * st, 16 * w);
-    if (!ENDS) {
-      // dv: this wave's 16 columns
-      const int col = anew(vc + 4 * lg);
-      auto values = [&](auto count, int first) {
-        constexpr int N = decltype(count)::value;
-        f32x4 acc[N];
-        Frag<NP> fj[N];
-#pragma unroll
-        for (int m = 0; m < N; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = 0; st < DK / 32; ++st) {
-#pragma unroll
-          for (int m = 0; m < N; ++m) fj[m] = by_row<NP, DK>(lds.k[0], KP, 16 * (first + m), 32 * st);
-          Frag<3> fs;  // R, index of keys
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; r += 2) put2(fs, 4 * t + r, s[2 * st + t][r], s[2 * st + t][r + 1]);
-          mma_n<3>(acc, fs, fj);
-        }
-#pragma unroll
-        for (int m = 0; m < N; ++m) {
-          const int j = 16 * (first + m) + li;
-          float x[4], sum = 0.f;
-          acc[m] *= d.left[j];
-          four<NP>(lds.v[0] + ((first + m) * (W / 16) + w) * TILE, VP, x);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sum = fmaf(x[r], acc[m][r], sum);
-          sum = col_sum(sum);
-          if (lg == 0) lds.kr[w][j] = sum;
-        }
-#pragma unroll
-        for (int st = 0; st < C / 32; ++st)
-#pragma unroll
-          for (int m = 0; m < N; ++m)
-            if (2 * st + 1 >= first + m)
-              mma<PR>(acc[m], fo[st], tri_by_col<PR>(lds.p[0], PP, st, first + m));
-#pragma unroll
-        for (int m = 0; m < N; ++m) {
-          const int j = 16 * (first + m) + li;
-          emit(a.dv, a.dv32, token, vrow, j, u.h * a.V + col, j < n ? a.V - col : 0, v4, acc[m]);
-        }
-      };
-      values(std::integral_constant<int, TI>{}, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    update_state<C, TK, DK, NP>(s, lds.q[0], KP, fo, d.from, d.whole);
-    if (ENDS && threadIdx.x == 0) seg += d.total;
     __syncthreads();
     if (!ENDS && w == BW - 1) {
       // the decays' gradients: a lane a token
