@@ -63,3 +63,28 @@ def test_whole_numbers_come_out_exactly(dev, dtype, dk, dv, swap, t):
     for p, w, m, u, name in zip(got, want, mag, units, ("y", "state", "dq", "dk", "dv", "dstate")):
         assert float(m.max()) / u < 2 ** 24, name          # the premise
         assert torch.equal(p.detach().cpu(), w.float().to(p.dtype)), (name, float((to64(p) - w).abs().max()))
+
+
+def _run(dev, dtype, b, t, h, dk, dv, make, rate, scale=None):
+    gen = torch.Generator().manual_seed(t + dk)
+    q, k, v, dy = (make(b, t, h, n, generator=gen).to(dtype).to(dev) for n in (dk, dk, dv, dv))
+    g = (-rate * torch.rand(b, t, h, generator=gen)).to(dev)
+    state, dend = (make(b, h, dk, dv, generator=gen).to(dev) for _ in range(2))
+    leaves = [x.requires_grad_(True) for x in (q, k, v, g, state)]
+    y, end = linear_attention(q, k, v, g, scale=scale, state=state, return_state=True)
+    got = [y, end, *torch.autograd.grad([y, end], leaves, [dy, dend])]
+    args = dict(q=to64(q), k=to64(k), v=to64(v), g=to64(g), scale=scale or dk ** -0.5, state=to64(state))
+    grads = oa.linear_attention_grad(to64(dy), to64(dend), **args)
+    want = [*oa.linear_attention(**args), *(grads[n] for n in ("q", "k", "v", "decay", "state"))]
+    return zip(("y", "end", "dq", "dk", "dv", "ddecay", "dstate"), got, want)
+
+
+@pytest.mark.parametrize("b,t,h,dk,dv", [(2, 32, 4, 64, 64), (2, 33, 4, 32, 32), (1, 300, 2, 128, 128)])
+def test_fp32_results_are_off_to_either_side(dev, b, t, h, dk, dv):
+    """Values of one sign, no decays, a scale of one.  Sums are rounded to nearest and what is left out of a product is of
+    either sign: the mean of thousands of results is that of the exact ones to within less than half of half a step.
+    Parts that are cut off leave out 2 * 2^-8 * 2^-16 of a product times the means of two uniform values relative to
+    theirs, about 0.7 each: one half step for every product on a result's way."""
+    for name, got, want in _run(dev, FP, b, t, h, dk, dv, lambda *s, generator: 1 + torch.rand(*s, generator=generator), 0.0, 1.0):
+        off = float(((to64(got) - want) / want).mean()) * 2 ** 24
+        assert abs(off) <= 0.4, (name, off)
