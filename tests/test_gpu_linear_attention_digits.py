@@ -79,6 +79,31 @@ def _run(dev, dtype, b, t, h, dk, dv, make, rate, scale=None):
     return zip(("y", "end", "dq", "dk", "dv", "ddecay", "dstate"), got, want)
 
 
+LONG = [(2, 333, 4, 64, 64, 0.05), (1, 600, 2, 128, 128, 0.05), (2, 200, 2, 32, 96, 1.0), (3, 31, 2, 40, 72, 0.5)]
+
+
+@pytest.mark.parametrize("b,t,h,dk,dv,rate", LONG)
+def test_fp32_results_are_within_a_few_roundings(dev, b, t, h, dk, dv, rate):
+    """Norm by norm: a result's rounding errors are of either sign, so that some hundred additions to it (six products of
+    parts for every 32 terms, a step of the state for every chunk) are off by some ten half steps together, and two such
+    sums on its way by 2^-24 * 17 = 1e-6.  Operands of two parts, 2^-17 each, would be off by 8e-6."""
+    for name, got, want in _run(dev, FP, b, t, h, dk, dv, torch.randn, rate):
+        err = float((to64(got) - want).norm() / want.norm())
+        assert err <= 1e-6, (name, err)
+
+
+@pytest.mark.parametrize("b,t,h,dk,dv,rate", LONG)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_16_bit_results_are_fp32_ones_rounded_once(dev, dtype, b, t, h, dk, dv, rate):
+    """A value that is off by d before its rounding comes out a step s away from the exact value's rounding with
+    probability d / s.  With s <= eps |y| the squares add up to eps * sum(d |y|) <= eps |d| |y|: where the norm error d is
+    that of fp32 sums, 1e-6, results are within sqrt(1e-6 eps) of the exactly rounded ones."""
+    for name, got, want in _run(dev, dtype, b, t, h, dk, dv, torch.randn, rate):
+        if got.dtype == dtype:
+            err = float((to64(got) - want.to(dtype).double()).norm() / want.norm())
+            assert err <= (1e-6 * torch.finfo(dtype).eps) ** 0.5, (name, err)
+
+
 @pytest.mark.parametrize("b,t,h,dk,dv", [(2, 32, 4, 64, 64), (2, 33, 4, 32, 32), (1, 300, 2, 128, 128)])
 def test_fp32_results_are_off_to_either_side(dev, b, t, h, dk, dv):
     """Values of one sign, no decays, a scale of one.  Sums are rounded to nearest and what is left out of a product is of
