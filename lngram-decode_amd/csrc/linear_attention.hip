@@ -1288,8 +1288,11 @@ __global__ __launch_bounds__(256) void k_la_step(Args a, int64_t waves) {
 // ------------------------------------------------------------------ host
 int chunk_of(int dtype) { return dtype == LNG_BF16 ? Traits<bf16>::chunk : Traits<float>::chunk; }
 
-// Rows in 16-byte pieces, a chunk's within 32-bit offsets
-bool vector_rows(const void* p, int es, int64_t batch, int64_t token, int64_t head, int d) {
+// Rows in 16-byte pieces, a chunk's within 32-bit offsets; a distance of what there is one of does not count.
+bool vector_rows(const void* p, int es, const Args& a, int heads, int64_t batch, int64_t token, int64_t head, int d) {
+  if (a.B == 1) batch = 0;
+  if (a.T == 1) token = 0;
+  if (heads == 1) head = 0;
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && batch * es % 16 == 0 && token * es % 16 == 0 && head * es % 16 == 0 &&
          d % 8 == 0 && token >= 0 && token * es < (int64_t{1} << 25);
 }
@@ -1308,8 +1311,8 @@ Args make_args(const lng_linear_attention& l, bool grad) {
   a.qb = l.q_batch, a.qt = l.q_token, a.qh = l.q_head, a.kb = l.k_batch, a.kt = l.k_token, a.kh = l.k_head;
   a.vb = l.v_batch, a.vt = l.v_token, a.vh = l.v_head;
   const int es = dtype_size(l.dtype);
-  a.qvec = vector_rows(a.q, es, a.qb, a.qt, a.qh, a.K), a.kvec = vector_rows(a.k, es, a.kb, a.kt, a.kh, a.K);
-  a.vvec = vector_rows(a.v, es, a.vb, a.vt, a.vh, a.V);
+  a.qvec = vector_rows(a.q, es, a, a.Hq, a.qb, a.qt, a.qh, a.K), a.kvec = vector_rows(a.k, es, a, a.Hk, a.kb, a.kt, a.kh, a.K);
+  a.vvec = vector_rows(a.v, es, a, a.Hv, a.vb, a.vt, a.vh, a.V);
   a.g = l.decay, a.gb = l.decay_batch, a.gt = l.decay_token;
   a.start = l.state, a.lengths = l.lengths, a.y = l.y, a.end = l.state_out, a.ckpt = l.checkpoints;
   a.yvec = a.V % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * es) == 0;
@@ -1542,7 +1545,7 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
   const int64_t rows = a.B * a.T, hv = int64_t{a.H} * a.vts;
   if (int rc = check_launches(what, a, true)) return rc;
   a.dy = g.dy, a.yb = g.dy_batch, a.yt = g.dy_token, a.yh = g.dy_head;
-  if (a.V % 8 == 0 && !vector_rows(a.dy, es, a.yb, a.yt, a.yh, a.V))
+  if (a.V % 8 == 0 && !vector_rows(a.dy, es, a, a.H, a.yb, a.yt, a.yh, a.V))
     return fail(LNG_E_ARG, "linear_attention_grad: rows of dy in 16-byte pieces, less than 2^25 bytes apart");
   float* const ws = static_cast<float*>(workspace);
   a.seg_state = ws + s.seg_state, a.seg_decay = ws + s.seg_decay;

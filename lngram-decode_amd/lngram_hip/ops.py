@@ -1969,6 +1969,7 @@ def linear_attention_back(plan: tuple, tensors, dy: torch.Tensor, dstate: torch.
             ds.zero_() if dstate is None else ds.copy_(dstate)
         return dq, dk, dv, dg, ds
     (dy, at), dstate = _strided(dy), _whole(dstate)
+    at = [0 if n == 1 else s for n, s in zip(dy.shape, at)]   # the distance of a single one is no distance
     es = 4 if a.dtype == F32 else 2
     if a.V % 8 == 0 and (dy.data_ptr() % 16 or at[0] * es % 16 or at[1] * es % 16 or at[2] * es % 16
                          or at[1] * es >= 1 << 25):
