@@ -900,9 +900,10 @@ int run_rows(const Gn& a, const Plan& p, hipStream_t st) {
   return fail(LNG_E_ARG, "group_norm: bad shape");
 }
 
+int64_t join_blocks(const Gn& a) { return cdiv(a.N * a.G, 16); }
 template <bool GRAD>
 int run_join(const Gn& a, hipStream_t st) {
-  k_gn_join<GRAD><<<static_cast<unsigned>(cdiv(a.N * a.G, 16)), 256, 0, st>>>(a, a.N * a.G);
+  k_gn_join<GRAD><<<static_cast<unsigned>(join_blocks(a)), 256, 0, st>>>(a, a.N * a.G);
   return check_launch("group_norm");
 }
 
@@ -959,9 +960,10 @@ int check_args(const char* what, int dtype, int w_dtype, int64_t N, int64_t L, i
   return LNG_OK;
 }
 
-// Blocks past 2^32 threads: more samples and slabs of channels than one launch counts
-int check_blocks(const char* what, const Plan& p) {
-  if (p.blocks * 256 <= MOST_THREADS) return LNG_OK;
+// Blocks past 2^32 threads: more samples and slabs of channels than one launch counts, or more groups than the one between
+// the passes
+int check_blocks(const char* what, const Gn& a, const Plan& p) {
+  if (std::max(p.blocks, p.form == Form::passes ? join_blocks(a) : 0) * 256 <= MOST_THREADS) return LNG_OK;
   return fail(LNG_E_ARG, std::string(what) + ": too many samples or channels for one launch; split the batch");
 }
 
@@ -1006,7 +1008,7 @@ int lng_group_norm(const void* x, int dtype, int64_t N, int64_t L, int32_t C, in
   a.y = y, a.mean = mean, a.rstd = rstd;
   const int es = dtype_size(dtype);
   const Plan p = make_plan(a, C % VEC == 0 && vector_rows(x, x_sample, x_row, N, L, es) && aligned(y, 16), false);
-  if (int rc = check_blocks(what, p)) return rc;
+  if (int rc = check_blocks(what, a, p)) return rc;
   const size_t need = lng_group_norm_workspace_bytes(N, L, C, G, 0);
   if (need && (!workspace || !aligned(workspace, 64) || workspace_bytes < need))
     return fail(LNG_E_ARG, "group_norm: the workspace is too small or not 64-byte aligned");
@@ -1036,7 +1038,7 @@ int lng_group_norm_grad(const void* dy, int64_t dy_sample, int64_t dy_row, const
   const int es = dtype_size(dtype);
   const Plan p = make_plan(a, C % VEC == 0 && vector_rows(x, x_sample, x_row, N, L, es) &&
                                   vector_rows(dy, dy_sample, dy_row, N, L, es) && aligned(dx, 16), true);
-  if (int rc = check_blocks(what, p)) return rc;
+  if (int rc = check_blocks(what, a, p)) return rc;
   if (!workspace || !aligned(workspace, 64) || workspace_bytes < lng_group_norm_workspace_bytes(N, L, C, G, 1))
     return fail(LNG_E_ARG, "group_norm_grad: the workspace is too small or not 64-byte aligned");
   a.stats = static_cast<float*>(workspace);

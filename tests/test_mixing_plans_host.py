@@ -32,3 +32,21 @@ def test_distances_of_single_ones_cost_no_copy():
         for n in "qkv":
             assert size(_attention(b, t, h, **{f"{n}_{name}": 3}), 0) == 0, (n, name)
         assert size(_attention(2, 64, 4, **{f"q_{name}": 3}), 0) > 0
+
+
+def _norm(n, at, c, groups, dtype=BF):
+    lib = _lib.load()
+    return lib.lng_group_norm(P, dtype, n, at, c, groups, at * c, c, P, P, FP, 1e-5, 1, P, 1 << 50, P, P, P, None)
+
+
+def _norm_grad(n, at, c, groups, dtype=BF):
+    lib = _lib.load()
+    return lib.lng_group_norm_grad(P, at * c, c, P, at * c, c, dtype, n, at, c, groups, P, P, FP, 1, P, P, P, 1 << 50, P, P, P, None)
+
+
+def test_group_norms_of_more_groups_than_a_launch_counts():
+    """Sixteen threads a group join its ranges of positions: 2^28 groups are 2^32 threads, where the passes' own launches
+    are far from it.  Refused before the first launch."""
+    for call in (_norm, _norm_grad):
+        for n, at, c, groups in ((1 << 18, 9, 2048, 2048), (1 << 17, 9, 2048, 2048), (1 << 24, 300, 64, 16)):
+            assert call(n, at, c, groups) == -1 and b"split the batch" in _lib.load().lng_last_error(), (call, n, at, c, groups)
