@@ -32,7 +32,7 @@ struct Gn {
   const void *x, *dy, *w, *b;
   void *y, *dx;
   float *mean, *rstd;   // [N, G]
-  float* stats;         // [N, parts, G, 2]
+  float* stats;         // [N, chunks, G + slabs, 2]: group g's part of slab s at g + s (a slab's first group may be shared)
   float* cols;          // [P, 2, C] partial gradients of w and b
   int64_t N, L, xs, xl, dys, dyl;
   int C, G, cg, wdt;
@@ -41,6 +41,7 @@ struct Gn {
   // blocks over positions and channels
   int slab, slabs, chunks;
   int64_t chunk_rows;
+  __host__ __device__ int64_t parts() const { return int64_t{G} + slabs; }  // of a chunk: a place for each group and boundary
 };
 
 template <typename T, int V>
@@ -505,7 +506,7 @@ __global__ __launch_bounds__(256) void k_gn_stats(Gn a) {
   const Tile<V> t(a, at.slab);
   const int chunk = at.chunk;
   const int64_t n = at.n, l0 = chunk * a.chunk_rows, l1 = min(l0 + a.chunk_rows, a.L);
-  float* to = a.stats + ((n * a.chunks + chunk) * a.slabs + at.slab) * a.G * 2;
+  float* to = a.stats + ((n * a.chunks + chunk) * a.parts() + at.slab) * 2;
   for (int64_t l = l0; l < l1; l += int64_t{R} * t.RL) {
     const int64_t e = min(l + int64_t{R} * t.RL, l1);
     Raw<T, V> v[R];
@@ -555,13 +556,13 @@ __global__ __launch_bounds__(256) void k_gn_join(Gn a, int64_t pairs) {
   const int lane = threadIdx.x & 15;
   const int64_t n = i / a.G;
   const int g = static_cast<int>(i - n * a.G), s0 = first_slab(a, g), ns = last_slab(a, g) - s0 + 1, parts = a.chunks * ns;
-  float2* const at = reinterpret_cast<float2*>(a.stats) + (n * a.chunks * a.slabs + s0) * a.G + g;
+  float2* const at = reinterpret_cast<float2*>(a.stats) + n * a.chunks * a.parts() + s0 + g;
   const float count = static_cast<float>(a.L) * static_cast<float>(a.cg);
   const float full = static_cast<float>(a.chunk_rows), last = chunk_size(a, a.chunks - 1);
   auto part = [&](int k, float& size) {
     const int ch = ns == 1 ? k : k / ns, sb = k - ch * ns;
     size = (ch + 1 < a.chunks ? full : last) * (ns == 1 ? static_cast<float>(a.cg) : slab_part(a, g, s0 + sb));
-    return at[(int64_t{ch} * a.slabs + sb) * a.G];
+    return at[ch * a.parts() + sb];
   };
   float one = 0.f, two = 0.f, size;
   if constexpr (GRAD) {
@@ -714,7 +715,7 @@ __global__ __launch_bounds__(256) void k_gn_grad_sums(Gn a) {
       for (int k = 0; k < V; ++k) sa[k] = fmaf(r.dz[k], r.xn[k], sa[k]), sb[k] += r.dz[k];
     }
   float* to = a.cols + (n * a.chunks + chunk) * 2 * a.C + t.c0;
-  float* groups = a.stats + ((n * a.chunks + chunk) * a.slabs + slab) * a.G * 2;
+  float* groups = a.stats + ((n * a.chunks + chunk) * a.parts() + slab) * 2;
   channel_sums(lds, t, sa, sb);
   for (int c = threadIdx.x; c < t.width; c += 256) to[c] = lds.one[c], to[a.C + c] = lds.two[c];
   group_sums(lds, t, a, [&](int gi, float s, float u) { groups[2 * (t.g0 + gi) + 1] = s, groups[2 * (t.g0 + gi)] = u; });
@@ -736,7 +737,7 @@ __global__ __launch_bounds__(256) void k_gn_grad_apply(Gn a) {
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int g = t.g0 + t.gk[k];
-    const float2 s = reinterpret_cast<const float2*>(a.stats)[(n * a.chunks * a.slabs + first_slab(a, g)) * a.G + g];
+    const float2 s = reinterpret_cast<const float2*>(a.stats)[n * a.chunks * a.parts() + first_slab(a, g) + g];
     s1[k] = s.x, s2[k] = s.y;
   }
   T* dx = static_cast<T*>(a.dx) + n * a.L * a.C + t.c;
@@ -850,7 +851,7 @@ Plan make_plan(Gn& a, bool vec, bool grad) {
       a.chunk_rows = cdiv(tiles, want) * tile;
       a.chunks = static_cast<int>(cdiv(L, a.chunk_rows));
       p.blocks = N * a.chunks * a.slabs, p.P = N * a.chunks;
-      p.stats = N * a.chunks * a.slabs * a.G * 2;
+      p.stats = N * a.chunks * a.parts() * 2;
       if (!grad) p.own = cdiv(p.stats, 16) * 16, p.stats = p.own + 2 * N * a.G;  // mean and rstd, where the caller wants none
     }
   }

@@ -50,3 +50,14 @@ def test_group_norms_of_more_groups_than_a_launch_counts():
     for call in (_norm, _norm_grad):
         for n, at, c, groups in ((1 << 18, 9, 2048, 2048), (1 << 17, 9, 2048, 2048), (1 << 24, 300, 64, 16)):
             assert call(n, at, c, groups) == -1 and b"split the batch" in _lib.load().lng_last_error(), (call, n, at, c, groups)
+
+
+def test_group_norm_workspaces_go_by_the_groups():
+    """A range of positions leaves two numbers a group, and two more a slab of channels, whose ends may share a group: the
+    workspace stays below the rows and the statistics that the call reads and writes anyway."""
+    size = _lib.load().lng_group_norm_workspace_bytes
+    for n, at, c, groups in ((1 << 17, 9, 2048, 2048), (1, 100, 65536, 65536), (1, 100, 65536, 4096), (3, 50, 30000, 10000),
+                             (2, 40, 5001, 1667), (1, 5000, 8192, 2048)):
+        rows, stats = 2 * n * at * c, 8 * n * groups       # bf16 rows; mean and rstd
+        assert 0 < size(n, at, c, groups, 0) <= 2 * rows + stats, (n, at, c, groups)
+        assert size(n, at, c, groups, 1) <= 4 * rows + 8 * n * c, (n, at, c, groups)
