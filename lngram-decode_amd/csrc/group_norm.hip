@@ -13,8 +13,8 @@
 // - samples that a block's registers hold: threads over positions and channels, statistics through LDS, one pass.
 // - larger ones: blocks over ranges of positions leave (mean, sum of squares around it) of their values, a small launch
 //   joins them, and the second pass finds part of what the first one read in the caches.  8 x 4096 x 320 in 32 groups: 11 +
-//   6 + 11 us, 3.8 TB/s in the two passes.  (Joined by every block of the
-//   second pass for itself they took longer than the launch: 8 x 4096 x 320 in 16 groups' loads and sums a block.)
+//   6 + 11 us, 1.9 TB/s in the first pass, 4.0 in the second.  (Joined by every block of the second pass for itself they
+//   took longer than the launch.)
 // The variance is always formed around a mean, never as a difference of squares.  Sums are fp32 in a fixed order: no
 // atomics, equal calls give equal bits.
 #include "common.h"
@@ -852,8 +852,9 @@ Plan make_plan(Gn& a, bool vec, bool grad) {
     a.slabs = static_cast<int>(cdiv(a.C, a.slab));
     const int64_t rl = 256 / (std::min(a.slab, a.C) / V);
     if (a.slab % a.cg == 0 && L <= rl * (grad ? BWD_R : FWD_R)) {
-      // one pass and one launch: 64 x 64 x 256 in 8 groups 12 us, in two passes 18; 2048 x 64 x 256 50 and 46, the training of
-      // 2048 x 32 x 256 83 and 85
+      // One pass and one launch: 64 x 64 x 256 in 8 groups 18 us and in two passes 19, 512 x 64 x 256 19 and 24, the training of
+      // 64 x 32 x 256 26 and 34, of 512 x 32 x 256 32 and 42, of 2048 x 32 x 256 90 and 90.  Where there are samples for several
+      // rounds of blocks the first pass' loads hide the launches: 2048 x 64 x 256 54 and 49.  That is given away.
       p.form = Form::samples;
       const int64_t bx = std::min<int64_t>(N, std::max<int64_t>(1, (grad ? 1024 : 4096) / a.slabs));
       p.blocks = bx * a.slabs, p.P = bx;

@@ -28,8 +28,13 @@ constexpr int VT = 64;      // columns of values that four waves take
 
 // Planes: bf16 parts of an input.  What is computed (scores, states, their gradients) enters products in PARTS whatever the
 // type, so that a 16-bit result is what fp32 sums give, rounded once.  Two parts are short of up to 2^-16 of a value, which
-// turns the rounding of one bf16 result in a thousand (1.2e-4 of the norm instead of 3e-5); they would take 115 us instead of
-// 126 at 8 x 4096 x 16 x 64, bf16, and 209 instead of 222 in the training of 8 x 2048 x 16 x 64.
+// turns the rounding of one bf16 result in a thousand (1.2e-4 of the norm instead of 3e-5); they would take 107 us instead of
+// 114 at 8 x 4096 x 16 x 64, bf16, and 200 instead of 214 in the training of 8 x 2048 x 16 x 64.
+//
+// Chunk: tokens of one.  bf16 in chunks of 64 and of 32: 8 x 4096 x 16 x 64 127 us and 139, its training 404 and 461, 4 x
+// 2048 x 16 x 128 86 and 101, 284 and 365, 64 x 40 x 16 x 64 19 and 18.  fp16 in chunks of 32 and of 64: 170 and 173, 543 and
+// 634, 125 and 111, 20 and 25; fp32 217 and 283, 707 and 1104.  Chunks of 64 tokens with 128 keys and values fit into LDS in
+// neither direction in fp32, and not in the backward one in fp16.
 constexpr int PARTS = 3;
 template <typename T>
 struct Traits;
@@ -113,7 +118,7 @@ __device__ __forceinline__ double log2_decay(float g) {
 // that the largest finite values stay finite.  ROUND: the others are rounded, so that the products that are left out (second
 // part times third: 2^-23 of the whole at most) are of either sign and add up to nothing.  Cut off as well they all have the
 // whole's sign: an fp32 product is short of 2^-24 of it on average, y and the gradients of 1.4 * 2^-24 of themselves instead of
-// 0.1, in up to 1 % less time.  Against bf16 values, one part each, nothing is left out.  (What is not finite comes out as NaN.)
+// 0.1, in 1 to 4 % less time.  Against bf16 values, one part each, nothing is left out.  (What is not finite comes out as NaN.)
 template <int PLANES>
 constexpr bool NEAREST = PLANES > 1;  // by the parts of the other operand, which is an input
 __device__ __forceinline__ float top(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u); }
@@ -504,9 +509,9 @@ struct FwdLds {
   bf16 p[PARTS][tri(C / 16, 0)];
 };
 
-// What bounds it: at 8 x 4096 x 16 x 64 (bf16) 75 us for 281 MB, 3.8 TB/s; at 1 x 16384 x 16 x 128 94 us with the vector unit
-// busy for 38 % and the matrix unit for 24 %: waits, at two waves a SIMD (more segments cost more than a third wave gains).
-// The segments' ends: 34 us for 102 MB, and 45 us.
+// What bounds it: at 8 x 4096 x 16 x 64 (bf16) 84 us for 281 MB, 3.3 TB/s, and at 1 x 16384 x 16 x 128 103 us, with the vector
+// unit busy for 43 % and the matrix unit for 19 and 27 %: waits, at two waves a SIMD (more segments cost more than a third wave
+// gains).  The segments' ends: 34 us for 109 MB, and 45 us for 49 MB.
 //
 // A block of NW waves takes a head's values, up to 16 NW columns, over a segment of chunks; a wave holds 16 columns of the
 // state.  ENDS: only what the segment adds to the state, into seg_state, with its decay.
@@ -765,9 +770,9 @@ __global__ __launch_bounds__(256) void k_la_join(Args a) {
 // several such tiles are summed afterwards, as the gradients of shared heads are.  P and A take the same place in LDS, one
 // after the other, A in registers meanwhile: three parts of both and R would leave room for one block a CU.
 //
-// 8 x 2048 x 16 x 64, bf16: 111 us for 313 MB; the vector unit is busy for 33 %, the matrix unit for 13 %: waits, at two waves
+// 8 x 2048 x 16 x 64, bf16: 117 us for 313 MB; the vector unit is busy for 35 %, the matrix unit for 15 %: waits, at two waves
 // a SIMD.  Registers decide: the scores' tiles go one by one and operands are split where they are used, since a spill waits
-// for the stores in flight (146 us).
+// for the stores in flight (a third more time).
 template <typename T, int DK, int BW>
 struct BwdLds {
   using Tr = Traits<T>;
@@ -1299,9 +1304,9 @@ bool vector_rows(const void* p, int es, const Args& a, int heads, int64_t batch,
 
 // Blocks of four waves that a launch should have, two for each CU (of eight, one): a segment more costs the keys and
 // values (the queries and dy) of all but one segment a second time.  8 x 4096 x 16 x 64 in 128, 256, 384, 512, 768, 1024
-// blocks: 179, 144, 120, 104, 118, 116 us; 1 x 16384 x 16 x 128 in 256, 384, 512, 768, 1024: 220, 161, 126, 169, 143; the
-// training of 8 x 2048 x 16 x 64 with its backward pass in 128, 256, 384, 512, 768: 421, 285, 235, 210, 253.  Segments of
-// one chunk gain nothing: 3 x 777 x 6 x 40 from one chunk, two, three, four on: 26, 26, 30, 35 us.
+// blocks: 213, 162, 133, 114, 107, 113 us; 1 x 16384 x 16 x 128 in 256, 384, 512, 768, 1024: 234, 174, 139, 182, 151; the
+// training of 8 x 2048 x 16 x 64 with its backward pass in 128, 256, 384, 512, 768: 451, 299, 247, 214, 242.  Segments of
+// one chunk gain nothing: 3 x 777 x 6 x 40 from one chunk, two, three, four on: 28, 29, 33, 37 us.
 constexpr int64_t BLOCKS = 512;
 
 Args make_args(const lng_linear_attention& l, bool grad) {
@@ -1519,8 +1524,8 @@ int lng_linear_attention_scan(const lng_linear_attention* args, void* workspace,
       using T = decltype(t);
       constexpr int DK = decltype(dk)::value;
       // Eight waves compute the scores of 128 columns once, and twice if they are blocks of four.  1 x 8192 tokens, 16
-      // heads of 64 keys and 128 values, bf16: 55 us and 58, of 128 keys 71 and 80, in fp32 99 and 101, 144 and 153.  Up to
-      // 64 columns they would leave half of the waves without work: 57 and 39.
+      // heads of 64 keys and 128 values, bf16: 63 us and 67, of 128 keys 82 and 90, in fp32 108 and 110, 152 and 161.  Up to
+      // 64 columns they would leave half of the waves without work: 64 and 46.
       return a.V <= 64 ? run_fwd<T, DK, 4>(a, as_stream(stream)) : run_fwd<T, DK, 8>(a, as_stream(stream));
     });
   });
@@ -1563,8 +1568,8 @@ int lng_linear_attention_scan_grad(const lng_linear_attention* args, const lng_l
     if (int rc = with_keys(a.K, [&](auto dk) {
           constexpr int DK = decltype(dk)::value;
           // Eight waves for 128 columns spare partial results of dq and dk, and a second product of q and k.  4 x 2048 x 16,
-          // bf16, both passes: 32 keys and 128 values 159 us and 190, 64 193 and 277, 128 289 and 519; fp16, 128: 410
-          // and 681.  In fp32 three parts of everything do not fit into LDS.
+          // bf16, both passes: 32 keys and 128 values 164 us and 194, 64 199 and 278, 128 288 and 545; fp16, 128: 425
+          // and 693.  In fp32 three parts of 128 keys and of 128 values do not fit into LDS.
           if constexpr (!std::is_same_v<T, float>)
             if (a.V > VT) return run_bwd<T, DK, 8>(a, st);
           return run_bwd<T, DK, 4>(a, st);
