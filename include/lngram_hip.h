@@ -879,8 +879,8 @@ typedef struct lng_linear_attention {
                        * the backward call */
 } lng_linear_attention;
 /* Gradients: dy [B, T, H, V] (strided; where V is a multiple of 8, in rows of 16-byte pieces less than 2^25 bytes apart)
- * and dstate_out [B, H, K, V] or null in; dq, dk, dv contiguous in the tensors'
- * type and shapes, ddecay [B, T, H] (token_decay) or [H], dstate [B, H, K, V] (may be null) in fp32 out. */
+ * and dstate_out [B, H, K, V] or null in (distances of a single sequence, token or head are not looked at); dq, dk, dv
+ * contiguous in the tensors' type and shapes, ddecay [B, T, H] (token_decay) or [H], dstate [B, H, K, V] (may be null) in fp32 out. */
 typedef struct lng_linear_attention_grad {
   const void* dy;
   int64_t dy_batch, dy_token, dy_head;

@@ -113,3 +113,18 @@ def test_fp32_results_are_off_to_either_side(dev, b, t, h, dk, dv):
     for name, got, want in _run(dev, FP, b, t, h, dk, dv, lambda *s, generator: 1 + torch.rand(*s, generator=generator), 0.0, 1.0):
         off = float(((to64(got) - want) / want).mean()) * 2 ** 24
         assert abs(off) <= 0.4, (name, off)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_the_largest_finite_values_stay_finite(dev, dtype):
+    """The type's lowest value among the values, with keys that leave the results in range."""
+    gen = torch.Generator().manual_seed(5)
+    q, k = (torch.randn(1, 90, 2, 32, generator=gen).to(dtype).to(dev) * 2.0 ** -7 for _ in range(2))
+    v = torch.full((1, 90, 2, 48), torch.finfo(dtype).min).to(dtype).to(dev)
+    g = -0.1 * torch.ones(2, device=dev)
+    y, end = linear_attention(q, k, v, g, scale=1.0, return_state=True)
+    want = oa.linear_attention(to64(q), to64(k), to64(v), to64(g), 1.0)
+    for got, w in zip((y, end), want):
+        assert torch.isfinite(got).all()
+        err = float(((to64(got) - w) * 2.0 ** -100).norm() / (w * 2.0 ** -100).norm())
+        assert err <= (1e-6 if got.dtype == FP else torch.finfo(dtype).eps / 2), err
